@@ -7,7 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int32, c_size_t, c_void_p, POINTER, Structure
+from ctypes import (c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p, POINTER,
+                    Structure)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfastlstm_b200.so")
 
@@ -26,12 +27,28 @@ FLAG_TEST_NO_ARRIVE = 4   # test hook: no CTA signals step completion (every wai
 OK = 0
 E_WAIT_TIMEOUT = 6
 E_TOO_LARGE = 8
+E_TOKEN = 9
 
 
 class Desc(Structure):
     _fields_ = [("dtype", c_int32), ("seq_len", c_int32), ("batch", c_int32),
                 ("input_size", c_int32), ("hidden_size", c_int32), ("flags", c_int32),
                 ("wait_limit_us", c_int32), ("reserved", c_int32)]
+
+
+class EmbedDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("token_bits", c_int32), ("n0", c_int64), ("n1", c_int64), ("token_stride", c_int64 * 2),
+                ("vocab", c_int64), ("width", c_int64), ("row_stride", c_int64 * 2), ("padding", c_int64), ("scale", c_float)]
+
+
+class DropoutDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("shared", c_int32), ("n0", c_int64), ("n1", c_int64), ("cols", c_int64),
+                ("stride", c_int64 * 2), ("p", c_double), ("seed", c_uint64), ("offset", c_uint64)]
+
+
+class ScoreDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("token_bits", c_int32), ("n0", c_int64), ("n1", c_int64), ("token_stride", c_int64 * 2),
+                ("vocab", c_int64), ("logits_stride", c_int64 * 2), ("ignore", c_int64), ("top", c_int32), ("temperature", c_float)]
 
 
 # name -> (restype, argtypes); every symbol include/fastlstm_b200.h declares
@@ -65,6 +82,12 @@ SIGNATURES = {
     "blstm_fwd_recurrence_static": (c_int, [DP, P, P, P, P, P]),
     "blstm_static_scratch_capacity": (c_size_t, []),
     "blstm_static_scratch_status": (c_int, [POINTER(c_int32), P]),
+    "blstm_embedding": (c_int, [POINTER(EmbedDesc), P, P, P, P]),
+    "blstm_embedding_grad_workspace": (c_size_t, [POINTER(EmbedDesc)]),
+    "blstm_embedding_grad": (c_int, [POINTER(EmbedDesc), P, P, P, P, c_size_t, P]),
+    "blstm_dropout": (c_int, [POINTER(DropoutDesc), P, P, P, P]),
+    "blstm_token_log_probs": (c_int, [POINTER(ScoreDesc)] + [P] * 8),
+    "blstm_token_log_probs_grad": (c_int, [POINTER(ScoreDesc)] + [P] * 12),
 }
 
 _lib = None

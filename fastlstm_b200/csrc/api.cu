@@ -11,6 +11,7 @@
 #include "f32_gemm.cuh"
 #include "f32_cluster.cuh"
 #include "generic.cuh"
+#include "language.cuh"
 #include "sm100.cuh"
 #include "step.cuh"
 
@@ -116,6 +117,7 @@ size_t control_bytes(const blstm_desc& d, int phase) {
 
 // What the calling thread's launches tell the host through, or null (blstm_set_mailbox).
 static thread_local int* g_mailbox = nullptr;
+int* current_mailbox() { return g_mailbox; }
 
 struct BeginParams {
   uint4* ws;
@@ -198,6 +200,7 @@ const char* blstm_strerror(int code) {
     case BLSTM_E_WAIT_TIMEOUT: return "device-side wait ran out (peer CTA never arrived)";
     case BLSTM_E_ARCH: return "device is not sm_100 (B200)";
     case BLSTM_E_TOO_LARGE: return "request exceeds the fixed capacity of this entry point";
+    case BLSTM_E_TOKEN: return "token outside of the vocabulary";
   }
   return "unknown status code";
 }

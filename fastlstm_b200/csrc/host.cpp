@@ -3,103 +3,11 @@
 // of fastlstm/lstm.py:31-146, :236-334 and :494-501 as they are seen from Python live in lstm.py; what they cost per
 // call in Python (ctypes, tensor checks, allocations, a status copy with its event: 130 us a layer) is what this file is
 // for.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <cuda_runtime_api.h>
-#include <torch/extension.h>
-
-#include <array>
-#include <atomic>
-#include <mutex>
-#include <optional>
-#include <string>
-#include <vector>
-
-#include "../../include/fastlstm_b200.h"
+#include "host.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-struct DeviceError {
-  int code;
-  std::string where;
-};
-
-int g_flags = 0;              // BLSTM_FLAG_FORCE_GENERIC or 0
-int g_wait_limit_us = 0;
-bool g_sync_check = false;
-PyObject* g_error_class = nullptr;
-
-// One mailbox per device, kept for the life of the process.  [1] code, [2..3] detail.
-constexpr int kMaxDevices = 64;
-std::array<std::atomic<int32_t*>, kMaxDevices> g_mail{};
-std::mutex g_mail_mutex;
-
-void cuda_ok(cudaError_t e, const char* what) {
-  TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
-}
-
-int32_t* mailbox(int dev) {
-  TORCH_CHECK(dev >= 0 && dev < kMaxDevices, "device index out of range");
-  int32_t* m = g_mail[dev].load(std::memory_order_acquire);
-  if (m) return m;
-  std::lock_guard<std::mutex> lock(g_mail_mutex);
-  m = g_mail[dev].load(std::memory_order_acquire);
-  if (!m) {
-    void* p = nullptr;
-    cuda_ok(cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable), "cudaHostAlloc");
-    m = static_cast<int32_t*>(p);
-    for (int i = 0; i < 16; ++i) m[i] = 0;
-    g_mail[dev].store(m, std::memory_order_release);
-  }
-  return m;
-}
-
-// Throws when a finished launch of this device has left an error.
-void poll(int dev) {
-  volatile int32_t* m = mailbox(dev);
-  if (__builtin_expect(m[1] == 0, 1)) return;
-  const int code = m[1], d0 = m[2], d1 = m[3];
-  m[1] = 0;
-  throw DeviceError{code, "recurrence (step " + std::to_string(d0) + ", batch tile " + std::to_string(d1) + ")"};
-}
-
-void check(int rc, const char* where) {
-  if (rc != BLSTM_OK) throw DeviceError{rc, where};
-}
-
-int dtype_code(at::ScalarType t) {
-  if (t == at::kFloat) return BLSTM_F32;
-  if (t == at::kHalf) return BLSTM_F16;
-  if (t == at::kBFloat16) return BLSTM_BF16;
-  throw py::value_error(std::string("unsupported dtype ") + c10::toString(t) + "; expected float32, float16 or bfloat16");
-}
-
-std::string shape_str(at::IntArrayRef s) {
-  std::string r = "(";
-  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
-  return r + ")";
-}
-
-void require(const Tensor& t, const char* name) {
-  if (!t.is_cuda()) throw py::value_error(std::string(name) + " must be a CUDA tensor (there is no CPU path)");
-  if (!t.is_contiguous()) throw py::value_error(std::string(name) + " must be contiguous");
-}
-void require(const Tensor& t, const char* name, at::ScalarType dt, const at::Device& dev, at::IntArrayRef shape) {
-  require(t, name);
-  if (t.scalar_type() != dt)
-    throw py::value_error(std::string(name) + " has dtype " + c10::toString(t.scalar_type()) + ", expected " + c10::toString(dt));
-  if (t.device() != dev) throw py::value_error(std::string(name) + " is on " + t.device().str() + ", expected " + dev.str());
-  if (t.sizes() != shape) throw py::value_error(std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected " + shape_str(shape));
-}
-void require(const OptTensor& t, const char* name, at::ScalarType dt, const at::Device& dev, at::IntArrayRef shape) {
-  if (t) require(*t, name, dt, dev, shape);
-}
-
-const void* ptr(const Tensor& t) { return t.const_data_ptr(); }
-const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; }
+using namespace blstm_host;
 
 blstm_desc desc(at::ScalarType dt, int64_t T, int64_t B, int64_t I, int64_t H, int flags) {
   blstm_desc d{};
@@ -109,21 +17,6 @@ blstm_desc desc(at::ScalarType dt, int64_t T, int64_t B, int64_t I, int64_t H, i
   d.wait_limit_us = g_wait_limit_us;
   return d;
 }
-
-// What every call does around its launches.
-struct Call {
-  c10::cuda::CUDAGuard guard;
-  int dev;
-  void* stream;
-  explicit Call(const at::Device& d) : guard(d), dev(d.index()), stream(at::cuda::getCurrentCUDAStream(d.index()).stream()) {
-    poll(dev);
-    blstm_set_mailbox(mailbox(dev));
-  }
-  ~Call() { blstm_set_mailbox(nullptr); }
-  void done(const Tensor& ws, const char* where) {
-    if (g_sync_check && ws.defined()) check(blstm_read_status(ws.const_data_ptr(), nullptr, stream), where);
-  }
-};
 
 struct FwdOut {
   Tensor out, cell, ifgo;
@@ -525,4 +418,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("gather_rows", &gather_rows);
   m.def("packed_maps", &packed_maps);
   m.def("check_status", &check_status);
+  bind_language(m);
 }

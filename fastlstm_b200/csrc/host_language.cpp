@@ -1,0 +1,325 @@
+// Host side of the operators around a language model: argument checks, buffers, the calls of the C ABI and the autograd
+// nodes.  Tensors keep their strides as long as two strides describe their rows and the last dimension is dense; others
+// are copied first.
+#include <cmath>
+
+#include "host.h"
+
+namespace {
+
+using namespace blstm_host;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+py::value_error wrong(const std::string& what) { return py::value_error(what); }
+
+void on_gpu(const Tensor& t, const char* name) {
+  if (!t.is_cuda()) throw wrong(std::string(name) + " must be a CUDA tensor (there is no CPU path)");
+}
+void beside(const Tensor& t, const char* name, const Tensor& other) {
+  on_gpu(t, name);
+  if (t.device() != other.device()) throw wrong(std::string(name) + " is on " + t.device().str() + ", expected " + other.device().str());
+}
+int token_bits(const Tensor& tokens) {
+  if (tokens.scalar_type() == at::kLong) return 64;
+  if (tokens.scalar_type() == at::kInt) return 32;
+  throw wrong(std::string("tokens have dtype ") + c10::toString(tokens.scalar_type()) + ", expected int64 or int32");
+}
+
+// The leading dimensions of an operator's tensors as [n0, n1].
+struct Lead {
+  int64_t dims, n0, n1;
+  explicit Lead(at::IntArrayRef s) : dims((int64_t)s.size()), n0(1), n1(1) {
+    if (dims == 2) { n0 = s[0]; n1 = s[1]; }
+    else n1 = c10::multiply_integers(s);
+    if (n0 > 0 && n1 > INT32_MAX / n0) throw wrong("more than 2^31 - 1 rows");
+  }
+  // t with `dims` leading dimensions as one whose rows stride[0..1] reach
+  Tensor rows(const Tensor& t, int64_t stride[2]) const {
+    Tensor v = dims > 2 ? t.flatten(0, dims - 1) : t;
+    const int64_t lead = dims > 2 ? 1 : dims;
+    if (v.dim() > lead && v.size(-1) > 1 && v.stride(-1) != 1) v = v.contiguous();
+    stride[0] = lead == 2 ? v.stride(0) : 0;
+    stride[1] = lead == 0 ? 0 : v.stride(lead - 1);
+    return v;
+  }
+};
+
+bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+void only_once() { TORCH_CHECK(!at::GradMode::is_enabled(), "fastlstm_b200: gradients of gradients (create_graph) are not there for this operator"); }
+
+std::vector<int64_t> plus(at::IntArrayRef s, int64_t last) {
+  std::vector<int64_t> v = s.vec();
+  v.push_back(last);
+  return v;
+}
+
+// ---------------------------------------------------------------- embedding
+blstm_embed_desc embed_desc(at::ScalarType dt, const Tensor& tokens, const Lead& lead, int64_t V, int64_t D, double scale, int64_t padding) {
+  blstm_embed_desc d{};
+  d.dtype = dtype_code(dt);
+  d.token_bits = token_bits(tokens);
+  d.n0 = lead.n0; d.n1 = lead.n1;
+  d.vocab = V; d.width = D;
+  d.padding = padding;
+  d.scale = (float)scale;
+  return d;
+}
+
+Tensor embedding_impl(const Tensor& tokens_in, const Tensor& weight_in, double scale) {
+  const Lead lead(tokens_in.sizes());
+  const Tensor weight = weight_in.size(1) > 1 && weight_in.stride(1) != 1 ? weight_in.contiguous() : weight_in;
+  blstm_embed_desc d = embed_desc(weight.scalar_type(), tokens_in, lead, weight.size(0), weight.size(1), scale, -1);
+  const Tensor tokens = lead.rows(tokens_in, d.token_stride);
+  d.row_stride[0] = weight.stride(0);
+  Call call(weight.device());
+  const Tensor out = at::empty(plus(tokens_in.sizes(), weight.size(1)), weight.options().requires_grad(false));
+  check(blstm_embedding(&d, ptr(tokens), ptr(weight), out.data_ptr(), call.stream), "embedding");
+  return out;
+}
+
+struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{weight.size(0), weight.size(1), padding};
+    return embedding_impl(tokens, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_once();
+    const Tensor saved = ctx->get_saved_variables()[0];
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const Lead lead(saved.sizes());
+    blstm_embed_desc d = embed_desc(g[0].scalar_type(), saved, lead, sizes[0], sizes[1], ctx->saved_data["scale"].toDouble(), sizes[2]);
+    const Tensor tokens = lead.rows(saved, d.token_stride), dout = lead.rows(g[0], d.row_stride);
+    Call call(dout.device());
+    const auto opt = dout.options().requires_grad(false);
+    const Tensor dW = at::empty({sizes[0], sizes[1]}, opt);
+    const Tensor ws = at::empty({(int64_t)blstm_embedding_grad_workspace(&d)}, opt.dtype(at::kByte));
+    check(blstm_embedding_grad(&d, ptr(tokens), ptr(dout), dW.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), call.stream), "embedding gradient");
+    return {dW, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+  py::gil_scoped_release nogil;
+  on_gpu(weight, "weight");
+  dtype_code(weight.scalar_type());
+  if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0) throw wrong("expected weight as [vocabulary, width], got " + shape_str(weight.sizes()));
+  beside(tokens, "tokens", weight);
+  token_bits(tokens);
+  if (!std::isfinite(scale)) throw wrong("scale must be finite");
+  const int64_t V = weight.size(0);
+  int64_t padding = -1;
+  if (padding_idx) {
+    if (*padding_idx < -V || *padding_idx >= V) throw wrong("padding_idx " + std::to_string(*padding_idx) + " is outside of the vocabulary of " + std::to_string(V));
+    padding = *padding_idx < 0 ? *padding_idx + V : *padding_idx;
+  }
+  return wants_grad(weight) ? EmbeddingFn::apply(weight, tokens, scale, padding) : embedding_impl(tokens, weight, scale);
+}
+
+// ---------------------------------------------------------------- dropout
+struct Mask {
+  double p;
+  uint64_t seed, offset;
+  OptTensor seed_at;
+  int64_t shared;             // dimension, or -1
+};
+
+Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
+  const auto sizes = x_in.sizes();
+  const int64_t dims = x_in.dim();
+  blstm_dropout_desc d{};
+  d.dtype = dtype_code(x_in.scalar_type());
+  d.shared = -1;
+  d.p = k.p; d.seed = k.seed; d.offset = k.offset;
+  d.n0 = d.n1 = 1;
+  Tensor x = x_in;
+  const bool two = dims == 3 && !x.is_contiguous() && x.stride(2) == 1;
+  if (!two) x = x.contiguous();
+  if (two) {                              // rows with strides of their own
+    d.n0 = sizes[0]; d.n1 = sizes[1]; d.cols = sizes[2];
+    d.stride[0] = x.stride(0); d.stride[1] = x.stride(1);
+    d.shared = (int32_t)k.shared;
+  } else if (k.shared < 0) {              // one row
+    d.cols = x.numel();
+  } else {
+    for (int64_t i = 0; i < k.shared; ++i) d.n0 *= sizes[i];
+    d.n1 = sizes[k.shared];
+    d.cols = 1;
+    for (int64_t i = k.shared + 1; i < dims; ++i) d.cols *= sizes[i];
+    d.stride[0] = d.n1 * d.cols; d.stride[1] = d.cols;
+    d.shared = 1;
+  }
+  Call call(x.device());
+  const Tensor y = at::empty(sizes, x.options().requires_grad(false));
+  check(blstm_dropout(&d, ptr(x), k.seed_at ? static_cast<const int64_t*>(ptr(*k.seed_at)) : nullptr, y.data_ptr(), call.stream), "dropout");
+  return y;
+}
+
+struct DropoutFn : public torch::autograd::Function<DropoutFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Mask& k) {
+    if (k.seed_at) ctx->save_for_backward({*k.seed_at});
+    ctx->saved_data["p"] = k.p;
+    ctx->saved_data["mask"] = std::vector<int64_t>{(int64_t)k.seed, (int64_t)k.offset, k.shared};
+    return dropout_impl(x, k);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_once();
+    const auto saved = ctx->get_saved_variables();
+    const auto m = ctx->saved_data["mask"].toIntVector();
+    Mask k{ctx->saved_data["p"].toDouble(), (uint64_t)m[0], (uint64_t)m[1], std::nullopt, m[2]};
+    if (!saved.empty()) k.seed_at = saved[0];
+    return {dropout_impl(g[0], k), Tensor()};
+  }
+};
+
+Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& seed_at, uint64_t offset, std::optional<int64_t> shared_dim) {
+  py::gil_scoped_release nogil;
+  on_gpu(x, "x");
+  dtype_code(x.scalar_type());
+  if (!(p >= 0.0 && p <= 1.0)) throw wrong("p must be in the range [0, 1]");
+  Mask k{p, seed, offset, seed_at, -1};
+  if (shared_dim) {
+    const int64_t d = *shared_dim < 0 ? *shared_dim + x.dim() : *shared_dim;
+    if (d < 0 || d >= x.dim() - 1) throw wrong("shared_dim must be a dimension of x and not its last one");
+    k.shared = d;
+  }
+  if (seed_at) {
+    beside(*seed_at, "seed", x);
+    if (seed_at->scalar_type() != at::kLong || seed_at->numel() != 1) throw wrong("a seed on the GPU is one int64 element");
+  }
+  return wants_grad(x) ? DropoutFn::apply(x, k) : dropout_impl(x, k);
+}
+
+// ---------------------------------------------------------------- log probabilities
+struct Score {
+  int64_t top;
+  double temperature;
+  int64_t ignore;
+};
+
+blstm_score_desc score_desc(const Tensor& logits, const Tensor& tokens, const Lead& lead, const Score& c) {
+  blstm_score_desc d{};
+  d.dtype = dtype_code(logits.scalar_type());
+  d.token_bits = token_bits(tokens);
+  d.n0 = lead.n0; d.n1 = lead.n1;
+  d.vocab = logits.size(-1);
+  d.ignore = c.ignore;
+  d.top = (int32_t)c.top;
+  d.temperature = (float)c.temperature;
+  return d;
+}
+
+// {log_probs, entropy, top_log_probs, top_tokens, stats}
+std::array<Tensor, 5> score_impl(const Tensor& logits_in, const Tensor& tokens_in, const Score& c) {
+  const Lead lead(tokens_in.sizes());
+  blstm_score_desc d = score_desc(logits_in, tokens_in, lead, c);
+  const Tensor logits = lead.rows(logits_in, d.logits_stride), tokens = lead.rows(tokens_in, d.token_stride);
+  Call call(logits.device());
+  const auto f32 = logits.options().requires_grad(false).dtype(at::kFloat);
+  std::array<Tensor, 5> r{at::empty(tokens_in.sizes(), f32), at::empty(tokens_in.sizes(), f32), Tensor(), Tensor(), at::empty({3, lead.n0 * lead.n1}, f32)};
+  if (c.top) {
+    r[2] = at::empty(plus(tokens_in.sizes(), c.top), f32);
+    r[3] = at::empty(plus(tokens_in.sizes(), c.top), f32.dtype(at::kLong));
+  }
+  check(blstm_token_log_probs(&d, ptr(logits), ptr(tokens), (float*)r[0].data_ptr(), (float*)r[1].data_ptr(), c.top ? (float*)r[2].data_ptr() : nullptr,
+                              c.top ? (int64_t*)r[3].data_ptr() : nullptr, (float*)r[4].data_ptr(), call.stream),
+        "token_log_probs");
+  return r;
+}
+
+// Memory for the gradient of logits [n0, n1, V] with rows on the same address modulo 16: laid out as the logits are where
+// that wastes little, else with the shortest strides that are the same modulo 16 bytes.
+Tensor grad_like(const Tensor& logits, const Lead& lead, const int64_t stride[2], int64_t dstride[2]) {
+  const int64_t e = logits.element_size(), V = logits.size(-1), per = 16 / e;
+  const int64_t own = V + (lead.n0 - 1) * stride[0] + (lead.n1 - 1) * stride[1];
+  const bool inner0 = stride[0] < stride[1];          // the first dimension is the inner one in memory
+  const int64_t n_in = inner0 ? lead.n0 : lead.n1, s_in = stride[inner0 ? 0 : 1], n_out = inner0 ? lead.n1 : lead.n0, s_out = stride[inner0 ? 1 : 0];
+  const bool apart = (n_in == 1 || s_in >= V) && (n_out == 1 || s_out >= n_in * s_in);
+  const int64_t numel = lead.n0 * lead.n1 * V;
+  if (apart && own <= numel + numel / 8) {
+    dstride[0] = stride[0]; dstride[1] = stride[1];
+  } else {
+    auto at_least = [&](int64_t least, int64_t like) { return least + (((like - least) % per) + per) % per; };
+    dstride[1] = at_least(V, stride[1]);
+    dstride[0] = at_least(lead.n1 * dstride[1], stride[0]);
+  }
+  const int64_t shift = (reinterpret_cast<uintptr_t>(logits.const_data_ptr()) & 15) / e;
+  const int64_t extent = V + (lead.n0 - 1) * dstride[0] + (lead.n1 - 1) * dstride[1];
+  return at::empty({extent + shift}, logits.options().requires_grad(false)).as_strided({lead.n0, lead.n1, V}, {dstride[0], dstride[1], 1}, shift);
+}
+
+struct ScoreFn : public torch::autograd::Function<ScoreFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Score& c) {
+    const auto r = score_impl(logits, tokens, c);
+    ctx->saved_data["temperature"] = c.temperature;
+    ctx->saved_data["score"] = std::vector<int64_t>{c.top, c.ignore};
+    ctx->set_materialize_grads(false);
+    if (!c.top) {
+      ctx->save_for_backward({logits, tokens, r[4]});
+      return {r[0], r[1]};
+    }
+    ctx->save_for_backward({logits, tokens, r[4], r[3]});
+    ctx->mark_non_differentiable({r[3]});
+    return {r[0], r[1], r[2], r[3]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_once();
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["score"].toIntVector();
+    const Score c{n[0], ctx->saved_data["temperature"].toDouble(), n[1]};
+    const Lead lead(saved[1].sizes());
+    blstm_score_desc d = score_desc(saved[0], saved[1], lead, c);
+    const Tensor logits = lead.rows(saved[0], d.logits_stride), tokens = lead.rows(saved[1], d.token_stride);
+    if (lead.n0 * lead.n1 == 0) return {at::zeros_like(saved[0]), Tensor(), Tensor()};
+    Call call(logits.device());
+    int64_t ds[2], s0[2], s1[2];
+    const Tensor dl = grad_like(logits, lead, d.logits_stride, ds);
+    const Tensor g0 = g[0].defined() ? lead.rows(g[0], s0) : Tensor(), g1 = g[1].defined() ? lead.rows(g[1], s1) : Tensor();
+    const Tensor g2 = c.top && g[2].defined() ? g[2].contiguous() : Tensor();
+    check(blstm_token_log_probs_grad(&d, ptr(logits), ptr(tokens), (const float*)ptr(saved[2]), c.top ? (const int64_t*)ptr(saved[3]) : nullptr,
+                                     g0.defined() ? (const float*)ptr(g0) : nullptr, s0, g1.defined() ? (const float*)ptr(g1) : nullptr, s1,
+                                     g2.defined() ? (const float*)ptr(g2) : nullptr, dl.data_ptr(), ds, call.stream),
+          "token_log_probs gradient");
+    return {lead.dims == 2 ? dl : dl.reshape(saved[0].sizes()), Tensor(), Tensor()};
+  }
+};
+
+py::tuple token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t top, double temperature, int64_t ignore_index) {
+  variable_list r(4);
+  {
+    py::gil_scoped_release nogil;
+    on_gpu(logits, "logits");
+    dtype_code(logits.scalar_type());
+    if (logits.dim() < 1 || logits.size(-1) == 0) throw wrong("expected logits as [..., vocabulary], got " + shape_str(logits.sizes()));
+    beside(tokens, "tokens", logits);
+    token_bits(tokens);
+    if (tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+      throw wrong("tokens have shape " + shape_str(tokens.sizes()) + ", expected " + shape_str(logits.sizes().slice(0, logits.dim() - 1)));
+    if (top < 0 || top > BLSTM_MAX_TOP || top > logits.size(-1))
+      throw wrong("top must be between 0 and " + std::to_string(std::min<int64_t>(BLSTM_MAX_TOP, logits.size(-1))));
+    if (!(temperature >= 1e-30 && std::isfinite((float)temperature))) throw wrong("temperature must be positive (at least 1e-30) and finite");
+    const Score c{top, temperature, ignore_index};
+    if (wants_grad(logits)) {
+      const auto v = ScoreFn::apply(logits, tokens, c);
+      std::copy(v.begin(), v.end(), r.begin());
+    } else {
+      const auto v = score_impl(logits, tokens, c);
+      std::copy(v.begin(), v.begin() + 4, r.begin());
+    }
+  }
+  return py::make_tuple(r[0], r[1], top ? py::cast(r[2]) : py::none(), top ? py::cast(r[3]) : py::none());
+}
+
+}  // namespace
+
+namespace blstm_host {
+
+void bind_language(py::module_& m) {
+  m.def("embedding", &embedding);
+  m.def("dropout", &dropout);
+  m.def("token_log_probs", &token_log_probs);
+}
+
+}  // namespace blstm_host

@@ -1,0 +1,64 @@
+// What the operators around a language model share: rows of strided tensors, tokens and what is wrong with them, elements
+// moved several at a time.
+#pragma once
+
+#include "common.cuh"
+
+namespace blstm {
+
+// Row r of a tensor [n0, n1, ...]: r = i0 * n1 + i1, strides in elements.
+struct RowMap {
+  long long s0, s1;
+  unsigned n1;
+  __device__ __forceinline__ long long operator()(unsigned r) const {
+    const unsigned i0 = r / n1;
+    return i0 * s0 + (r - i0 * n1) * s1;
+  }
+};
+inline RowMap row_map(int64_t n1, const int64_t stride[2]) { return {(long long)stride[0], (long long)stride[1], (unsigned)n1}; }
+
+struct Tokens {
+  const void* p;
+  RowMap map;
+  bool wide;                 // 64-bit, else 32
+  __device__ __forceinline__ long long operator()(unsigned r) const {
+    const long long i = map(r);
+    return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+  }
+};
+
+// The mailbox that the calling thread has set (blstm_set_mailbox), or null.
+int* current_mailbox();
+
+// A token outside of the vocabulary: one report is kept, position and token in one store, the status word last.
+static __device__ __noinline__ void report_token(int* mailbox, unsigned position, long long token) {
+  if (!mailbox) return;
+  volatile int* m = mailbox;
+  const int shown = token > INT32_MAX ? INT32_MAX : token < INT32_MIN ? INT32_MIN : (int)token;
+  *reinterpret_cast<volatile unsigned long long*>(m + 2) = (unsigned long long)(unsigned)shown << 32 | position;
+  __threadfence_system();
+  m[1] = BLSTM_E_TOKEN;
+}
+
+// VEC elements of T on their natural boundary, as floats.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+inline bool valid_dtype(int dtype) { return dtype == BLSTM_F32 || dtype == BLSTM_F16 || dtype == BLSTM_BF16; }
+inline int dtype_bytes(int dtype) { return dtype == BLSTM_F32 ? 4 : 2; }
+inline bool valid_rows(int64_t n0, int64_t n1) { return n0 >= 0 && n1 >= 0 && (n0 == 0 || n1 <= INT32_MAX / n0); }
+
+// The widest piece, of 16, 4 and the element's own bytes, that addresses and lengths (in bytes) are multiples of.
+inline int piece_bytes(uintptr_t bits, int element) { return (bits & 15u) == 0 ? 16 : (bits & 3u) == 0 ? 4 : element; }
+
+// f(T{}) with the element type of a dtype code.
+template <typename F>
+int with_type(int dtype, F&& f) {
+  if (dtype == BLSTM_F32) return f(float{});
+  if (dtype == BLSTM_F16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+
+}  // namespace blstm

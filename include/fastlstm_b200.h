@@ -46,7 +46,8 @@ enum {
   BLSTM_E_NOT_CORESIDENT = 5,  /* persistent grid cannot be made co-resident on this GPU */
   BLSTM_E_WAIT_TIMEOUT = 6,    /* device: a bounded cross-CTA wait ran out               */
   BLSTM_E_ARCH = 7,            /* device is not sm_100                                    */
-  BLSTM_E_TOO_LARGE = 8        /* request exceeds a fixed capacity (no-allocation entry) */
+  BLSTM_E_TOO_LARGE = 8,       /* request exceeds a fixed capacity (no-allocation entry) or a grid */
+  BLSTM_E_TOKEN = 9            /* device: a token outside of the vocabulary                */
 };
 
 /* blstm_desc.flags */
@@ -244,6 +245,75 @@ int blstm_gather_rows(void* dst, const void* src, const int32_t* idx, int64_t n,
  * No reference counterpart (packed sequences are listed as missing, README.md:92-93). */
 int blstm_packed_maps(const int32_t* batch_sizes, const int32_t* offsets, const int64_t* rank, int T, int B,
                       int32_t* maps, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Operators around a language model of LSTM layers.  No reference counterpart: the reference has the
+ * layers alone.  Rows (a token, a prediction, a step of a sequence) are numbered [n0, n1] row-major; every
+ * strided tensor gives the strides of the two in elements, its last dimension is dense.  Addresses are
+ * multiples of the element's size; wider accesses are used where addresses and strides allow them.
+ * A token outside of the vocabulary is reported as BLSTM_E_TOKEN through the mailbox (blstm_set_mailbox:
+ * detail[0] its row, detail[1] its value), its row of the result is NaN and it takes part in no gradient.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct blstm_embed_desc {
+  int32_t dtype;             /* of weight, out, dout and dweight                                       */
+  int32_t token_bits;        /* 32 or 64                                                               */
+  int64_t n0, n1;            /* tokens [n0, n1], n0 * n1 < 2^31                                        */
+  int64_t token_stride[2];
+  int64_t vocab, width;      /* weight [vocab, width]                                                  */
+  int64_t row_stride[2];     /* lookup: [0] = between the weight's rows; gradient: dout's two strides  */
+  int64_t padding;           /* a token that gets no gradient, or -1                                   */
+  float scale;
+} blstm_embed_desc;
+
+/* out[n0*n1, width] (dense) = round(scale * weight[tokens]); one rounding. */
+int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* weight, void* out, void* stream);
+
+/* dweight[vocab, width] (dense, every row is written) = round(scale * sum of dout's rows of that token): added in
+ * 32 bits in an order that the tokens alone fix, rounded once.  The workspace is 256-byte aligned. */
+size_t blstm_embedding_grad_workspace(const blstm_embed_desc* d);
+int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const void* dout, void* dweight,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct blstm_dropout_desc {
+  int32_t dtype;
+  int32_t shared;            /* -1: every element has its own word; 0 / 1: the n0 / n1 rows of a column share them */
+  int64_t n0, n1, cols;      /* x [n0, n1, cols], n0 * n1 < 2^31                                       */
+  int64_t stride[2];         /* of x                                                                   */
+  double p;                  /* an element is dropped with probability p, to 2^-33                     */
+  uint64_t seed, offset;
+} blstm_dropout_desc;
+
+/* y[n0,n1,cols] (dense) = word < p 2^32 ? 0 : x / (1 - p), word m = Philox4x32-10(key seed, counter (m / 4, offset))[m % 4],
+ * m the element's row-major number (with `shared`, in [n1,cols] / [n0,cols]).  The same call on dy is the gradient.
+ * seed_at: the seed in device memory, read when the kernel runs (graphs), or NULL for d->seed. */
+int blstm_dropout(const blstm_dropout_desc* d, const void* x, const int64_t* seed_at, void* y, void* stream);
+
+#define BLSTM_MAX_TOP 32
+typedef struct blstm_score_desc {
+  int32_t dtype;             /* of logits and dlogits                                                  */
+  int32_t token_bits;        /* 32 or 64                                                               */
+  int64_t n0, n1;            /* predictions [n0, n1], n0 * n1 < 2^31                                   */
+  int64_t token_stride[2];
+  int64_t vocab;             /* logits [n0, n1, vocab]                                                 */
+  int64_t logits_stride[2];
+  int64_t ignore;            /* predictions of this token are left out (0, 0, -inf and -1; no gradient) */
+  int32_t top;               /* alternatives, at most BLSTM_MAX_TOP and vocab                          */
+  float temperature;         /* of at least 1e-30                                                      */
+} blstm_score_desc;
+
+/* With z = logits / temperature: log_probs[n0*n1] = log softmax(z)[token], entropy[n0*n1] of softmax(z), and of the `top`
+ * largest logits (equal ones by their number) top_log_probs and top_tokens [n0*n1, top] (NULL where top is 0).  A row
+ * whose logits are all -inf: -inf, 0, -inf and the first tokens, gradient 0.  stats [3, n0*n1]: what the gradient
+ * needs of the row. */
+int blstm_token_log_probs(const blstm_score_desc* d, const void* logits, const void* tokens, float* log_probs,
+                          float* entropy, float* top_log_probs, int64_t* top_tokens, float* stats, void* stream);
+
+/* dlogits [n0,n1,vocab] from the gradients of log_probs, entropy (strided, or NULL: zero) and top_log_probs (dense, or
+ * NULL).  Rows of dlogits lie on the same address modulo 16 as those of logits. */
+int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, const void* tokens, const float* stats,
+                               const int64_t* top_tokens, const float* g_log_probs, const int64_t g_log_probs_stride[2],
+                               const float* g_entropy, const int64_t g_entropy_stride[2], const float* g_top,
+                               void* dlogits, const int64_t dlogits_stride[2], void* stream);
 
 /* Host memory (mapped into the device, 16 bytes: -, status, detail[2]) that the CALLING THREAD's later
  * launches write a device-side error to as well, or NULL (default): a caller that looks there need not
