@@ -47,110 +47,541 @@ __device__ __forceinline__ unsigned value_key(float z) {
 }
 __device__ __forceinline__ unsigned long long order_key(float z, unsigned j) { return (unsigned long long)value_key(z) << 32 | (0xffffffffu - j); }
 
-// A part of a row: its maximum, sum of 2^(d) and of d 2^(d), d = distance from the maximum in powers of two.
+__device__ __forceinline__ float key_value(unsigned key) {      // the logit of a value key
+  return key == 0xffffffffu ? __int_as_float(0x7fffffff) : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// 2^x to 2^-22; subnormal results are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two 32-bit floats that one instruction works on.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ static Pair of(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+  }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+template <typename T> constexpr int kPer = 16 / (int)sizeof(T);        // elements of a 16-byte piece
+
+__device__ __forceinline__ void unpack(const uint4& v, float* z, float) {
+  z[0] = __uint_as_float(v.x); z[1] = __uint_as_float(v.y); z[2] = __uint_as_float(v.z); z[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(const uint4& v, float* z, __nv_bfloat16) {
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { z[2 * i] = __uint_as_float(w[i] << 16); z[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void unpack(const uint4& v, float* z, __half) {
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    z[2 * i] = f.x; z[2 * i + 1] = f.y;
+  }
+}
+
+// A part of a row: its largest logit, and the sums of 2^d and of d 2^d over it, d the distance from the reference
+// max(m, kLowest) in powers of two.
 struct Part {
   float m, s, t;
-  __device__ __forceinline__ void add(const Part& o, float to_log2) {
-    const float M = max_nan(m, o.m);
-    const float a = max_nan((m - M) * to_log2, kFar), b = max_nan((o.m - M) * to_log2, kFar);
-    const float fa = exp2f(a), fb = exp2f(b);
-    t = fa * (t + s * a) + fb * (o.t + o.s * b);
-    s = fa * s + fb * o.s;
+  __device__ __forceinline__ float ref() const { return max_nan(m, kLowest); }
+  __device__ __forceinline__ void rescale(float to, float to_log2) {      // to a reference of at least its own
+    const float a = max_nan((ref() - to) * to_log2, kFar), f = exp2_fast(a);
+    t = f * (t + s * a);
+    s *= f;
+  }
+  // The whole of the parts that the 2^n lanes of a group hold, in each of them.
+  __device__ __forceinline__ void join(int lanes, float to_log2) {
+    float M = m;
+    for (int o = lanes / 2; o; o >>= 1) M = max_nan(M, __shfl_xor_sync(~0u, M, o));
+    rescale(max_nan(M, kLowest), to_log2);
     m = M;
+    for (int o = lanes / 2; o; o >>= 1) {
+      s += __shfl_xor_sync(~0u, s, o);
+      t += __shfl_xor_sync(~0u, t, o);
+    }
   }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ ScoreParams p) {
-  __shared__ Part s_part[8];
-  __shared__ unsigned long long s_key[8];
-  const unsigned r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// N logits into a thread's part: one comparison with the maximum so far, a rescaling where it moves.
+template <int N>
+__device__ __forceinline__ void take(Part& a, const float (&z)[N], float to_log2) {
+  float m = z[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = max_nan(m, z[i]);
+  if (!(m <= a.m)) {
+    Part b = a;
+    a.m = max_nan(a.m, m);
+    b.rescale(a.ref(), to_log2);
+    a.s = b.s; a.t = b.t;
+  }
+  const float ref = a.ref();
+  const Pair down = Pair::of(-ref, -ref), c = Pair::of(to_log2, to_log2);
+  Pair s = Pair::of(a.s, 0.f), t = Pair::of(a.t, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    float x, y;
+    ((Pair::of(z[i], z[i + 1]) + down) * c).get(x, y);
+    x = max_nan(x, kFar);
+    y = max_nan(y, kFar);
+    const Pair e = Pair::of(exp2_fast(x), exp2_fast(y));
+    s = s + e;
+    t = fma2(e, Pair::of(x, y), t);
+  }
+  float s0, s1, t0, t1;
+  s.get(s0, s1);
+  t.get(t0, t1);
+  a.s = s0 + s1;
+  a.t = t0 + t1;
+}
+
+// What a row's statistics give.
+struct Row {
+  float m, log2s, entropy;
+  bool none;                   // every logit is -inf
+  __device__ __forceinline__ explicit Row(const Part& a) : m(a.ref()), log2s(log2f(a.s)), none(a.s == 0.f) {
+    entropy = none ? 0.f : (log2s - a.t / a.s) * kLn2;
+  }
+  __device__ __forceinline__ float log_prob(float z, float per_temperature) const {
+    return none ? -INFINITY : (z - m) * per_temperature - log2s * kLn2;
+  }
+};
+
+__device__ __forceinline__ void put_row(const ScoreParams& p, unsigned r, const Row& w, long long token, float at_token) {
+  const bool in = token >= 0 && token < p.vocab;
+  p.log_probs[r] = in ? w.log_prob(at_token, p.per_temperature) : __int_as_float(0x7fffffff);
+  p.entropy[r] = w.entropy;
+  p.stats[r] = w.m;
+  p.stats[(size_t)p.n + r] = w.log2s;
+  p.stats[2 * (size_t)p.n + r] = w.entropy;
+  if (!in) report_token(p.mailbox, r, token);
+}
+__device__ __forceinline__ void put_top(const ScoreParams& p, unsigned r, const Row& w, int k, unsigned long long key) {
+  p.top_log_probs[(size_t)r * p.top + k] = w.log_prob(key_value((unsigned)(key >> 32)), p.per_temperature);
+  p.top_tokens[(size_t)r * p.top + k] = 0xffffffffu - (unsigned)key;
+}
+// A row whose token is ignored, by the threads i = 0 .. top - 1 and one at least.
+__device__ __forceinline__ void put_ignored(const ScoreParams& p, unsigned r, unsigned i) {
+  if (i == 0) {
+    p.log_probs[r] = 0.f;
+    p.entropy[r] = 0.f;
+    for (int k = 0; k < 3; ++k) p.stats[(size_t)k * p.n + r] = 0.f;
+  }
+  if (i < (unsigned)p.top) {
+    p.top_log_probs[(size_t)r * p.top + i] = -INFINITY;
+    p.top_tokens[(size_t)r * p.top + i] = -1;
+  }
+}
+
+// ---------------------------------------------------------------- small vocabularies: a warp has a row in its registers
+constexpr int kWarpVocab = 1024, kWarpRows = 4, kWarpCand = 128;
+
+template <typename T, int VPL, bool TOP>
+__global__ void __launch_bounds__(32 * kWarpRows) score_warp_kernel(const __grid_constant__ ScoreParams p) {
+  __shared__ unsigned long long s_cand[TOP ? kWarpRows : 1][TOP ? kWarpCand : 1];
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * kWarpRows + warp;
+  if (r >= p.n) return;
+  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
   const long long token = p.tokens(r);
   if (token == p.ignore) {
-    if (tid == 0) {
-      p.log_probs[r] = 0.f;
-      p.entropy[r] = 0.f;
-      for (int i = 0; i < 3; ++i) p.stats[(size_t)i * p.n + r] = 0.f;
-    }
-    if (tid < (unsigned)p.top) {
-      p.top_log_probs[(size_t)r * p.top + tid] = -INFINITY;
-      p.top_tokens[(size_t)r * p.top + tid] = -1;
-    }
+    put_ignored(p, r, lane);
     return;
   }
-  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
-  Part a{kLowest, 0.f, 0.f};
-  for (unsigned j = tid; j < p.vocab; j += 256) {
-    const float z = ld_f(row + j);
-    if (!(z <= a.m)) a.add(Part{z, 1.f, 0.f}, p.to_log2);
-    else {
-      const float d = max_nan((z - a.m) * p.to_log2, kFar), e = exp2f(d);
-      a.s += e;
-      a.t += e * d;
-    }
-  }
+  float z[VPL];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) a.add(Part{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)}, p.to_log2);
-  if (lane == 0) s_part[warp] = a;
-  __syncthreads();
-  a = s_part[0];
-  for (int w = 1; w < 8; ++w) a.add(s_part[w], p.to_log2);
-  const bool none = a.s == 0.f;               // every logit is -inf
-  const float log2s = log2f(a.s);
-  auto lp = [&](float z) { return none ? -INFINITY : (z - a.m) * p.per_temperature - log2s * kLn2; };
-  if (tid == 0) {
-    const bool in = token >= 0 && token < p.vocab;
-    const float h = none ? 0.f : (log2s - a.t / a.s) * kLn2;
-    p.log_probs[r] = in ? lp(ld_f(row + token)) : __int_as_float(0x7fffffff);
-    p.entropy[r] = h;
-    p.stats[r] = a.m; p.stats[(size_t)p.n + r] = log2s; p.stats[2 * (size_t)p.n + r] = h;
-    if (!in) report_token(p.mailbox, r, token);
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    unsigned long long best = 0;
-    for (unsigned j = tid; j < p.vocab; j += 256) {
-      const unsigned long long q = order_key(ld_f(row + j), j);
-      if (q < last && q > best) best = q;
+  for (int i = 0; i < VPL; ++i) z[i] = i * 32 + lane < p.vocab ? ld_f(row + i * 32 + lane) : -INFINITY;
+  const float at_token = token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
+  Part a{-INFINITY, 0.f, 0.f};
+  take(a, z, p.to_log2);
+  const unsigned mine = value_key(a.m);        // (of a lane without logits: that of -inf)
+  a.join(32, p.to_log2);
+  const Row w(a);
+  if (lane == 0) put_row(p, r, w, token, at_token);
+  if constexpr (TOP) {
+    // The k-th largest of the lanes' maxima is a lower bound of the k-th largest logit: what is below it is out.
+    unsigned rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+      const unsigned o = __shfl_sync(~0u, mine, i);
+      rank += o > mine || (o == mine && i < lane);
     }
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-    __syncthreads();
-    if (lane == 0) s_key[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) best = max(best, s_key[w]);
-    last = best;
-    if (tid == 0) {
-      const unsigned j = 0xffffffffu - (unsigned)best;
-      p.top_log_probs[(size_t)r * p.top + k] = lp(ld_f(row + j));
-      p.top_tokens[(size_t)r * p.top + k] = j;
+    const unsigned bound = __shfl_sync(~0u, mine, __ffs(__ballot_sync(~0u, rank == (unsigned)p.top - 1)) - 1);
+    unsigned count = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const unsigned j = i * 32 + lane;
+      const unsigned long long key = order_key(z[i], j);
+      const bool in = j < p.vocab && (unsigned)(key >> 32) >= bound;
+      const unsigned who = __ballot_sync(~0u, in);
+      const unsigned at = count + __popc(who & ((1u << lane) - 1));
+      if (in && at < kWarpCand) s_cand[warp][at] = key;
+      count += __popc(who);
+    }
+    __syncwarp();
+    if (count <= kWarpCand) {
+      for (unsigned i = lane; i < count; i += 32) {
+        const unsigned long long key = s_cand[warp][i];
+        unsigned before = 0;
+        for (unsigned q = 0; q < count; ++q) before += s_cand[warp][q] > key;
+        if (before < (unsigned)p.top) put_top(p, r, w, (int)before, key);
+      }
+    } else {                                   // (many equal logits) one after the other
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < p.top; ++k) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const unsigned long long key = order_key(z[i], i * 32 + lane);
+          if (i * 32 + lane < p.vocab && key < last && key > best) best = key;
+        }
+        for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
+        if (lane == 0) put_top(p, r, w, k, best);
+        last = best;
+      }
     }
   }
 }
 
+// ---------------------------------------------------------------- large vocabularies: a block, or a cluster of them, has a row
+constexpr int kThreads = 256, kWarps = kThreads / 32, kUnroll = 4, kGroups = 64, kCand = 1024, kMaxCluster = 8;
+
+// What a block reads of a row: elements up to the first 16-byte boundary, pieces of 16 bytes, and the elements behind them.
 template <typename T>
-__global__ void __launch_bounds__(256) score_grad_kernel(const __grid_constant__ ScoreParams p) {
-  const unsigned r = blockIdx.x;
+struct Span {
+  const T* row;
+  unsigned head, pieces, tail;   // of the row
+  unsigned begin, end;           // this block's pieces
+  bool first;                    // this block has the head and the tail
+  __device__ __forceinline__ Span(const T* row, unsigned vocab, unsigned part, unsigned parts) : row(row), first(part == 0) {
+    head = min(vocab, (unsigned)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (unsigned)sizeof(T));
+    pieces = (vocab - head) / kPer<T>;
+    tail = vocab - head - pieces * kPer<T>;
+    const unsigned each = (pieces + parts - 1) / parts;
+    begin = min(pieces, part * each);
+    end = min(pieces, begin + each);
+  }
+  __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(row + head); }
+  __device__ __forceinline__ unsigned number(unsigned piece) const { return head + piece * kPer<T>; }
+  // elements of the head and the tail, in one numbering: 2 * kPer - 2 at most
+  __device__ __forceinline__ unsigned edges() const { return first ? head + tail : 0; }
+  __device__ __forceinline__ unsigned edge(unsigned i) const { return i < head ? i : head + pieces * kPer<T> + (i - head); }
+};
+
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned v;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(v));
+  return v;
+}
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned v;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v));
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// the same variable in the first block of the cluster
+template <typename V>
+__device__ __forceinline__ void store_first(V* p, unsigned long long v) {
+  static_assert(sizeof(V) == 8, "");
+  unsigned a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+
+struct ScoreShared {
+  Part part[kWarps];
+  uint2 peers[kMaxCluster][2];                          // maximum and sum, second sum, of every block of a cluster
+  unsigned group[kGroups];
+  unsigned owner[kThreads];
+  unsigned owners, count, bound;
+  unsigned long long bound_key;
+  unsigned long long cand[kCand];
+  unsigned long long best[kMaxCluster * BLSTM_MAX_TOP]; // of this block; in a cluster's first one, of all
+};
+
+// The `top` first of a block's logits in order, into s.best: thread's maxima bound them from below, the threads whose
+// maximum reaches that bound (few more than `top`) look at their logits again.
+template <typename T>
+__device__ __forceinline__ void block_top(ScoreShared& s, const Span<T>& span, float thread_max, unsigned top) {
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned mine = value_key(thread_max);
+  unsigned g = mine;
+#pragma unroll
+  for (int o = 1; o < kThreads / kGroups; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
+  if (tid % (kThreads / kGroups) == 0) s.group[tid / (kThreads / kGroups)] = g;
+  if (tid == 0) { s.owners = 0; s.count = 0; }
+  __syncthreads();
+  if (tid < kGroups) {
+    const unsigned v = s.group[tid];
+    unsigned rank = 0;
+#pragma unroll 16
+    for (unsigned i = 0; i < kGroups; ++i) rank += s.group[i] > v || (s.group[i] == v && i < tid);
+    if (rank == top - 1) s.bound = v;
+  }
+  __syncthreads();
+  const unsigned bound = s.bound;
+  if (mine >= bound) s.owner[atomicAdd(&s.owners, 1u)] = tid;
+  __syncthreads();
+  auto offer = [&](float z, unsigned j, unsigned long long least) {
+    const unsigned long long key = order_key(z, j);
+    if (key < least) return;
+    const unsigned at = atomicAdd(&s.count, 1u);
+    if (at < kCand) s.cand[at] = key;
+  };
+  auto look = [&](unsigned piece, unsigned long long least) {
+    float z[kPer<T>];
+    unpack(span.body()[piece], z, T{});
+#pragma unroll
+    for (int i = 0; i < kPer<T>; ++i) offer(z[i], span.number(piece) + i, least);
+  };
+  const unsigned owners = s.owners;
+  const unsigned long long least = (unsigned long long)bound << 32;
+  for (unsigned o = warp; o < owners; o += kWarps) {
+    const unsigned t = s.owner[o];
+    for (unsigned piece = span.begin + t + lane * kThreads; piece < span.end; piece += 32 * kThreads) look(piece, least);
+    if (lane == 0 && t < span.edges()) offer(ld_f(span.row + span.edge(t)), span.edge(t), least);
+  }
+  __syncthreads();
+  while (s.count > kCand) {                    // (many equal logits) a higher bound, from some of them, until they fit
+    unsigned before = 0;
+    const unsigned long long key = s.cand[tid];
+    for (unsigned i = 0; i < kThreads; ++i) before += s.cand[i] > key;
+    if (before == top - 1) s.bound_key = key;
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    const unsigned long long more = s.bound_key;
+    for (unsigned piece = span.begin + tid; piece < span.end; piece += kThreads) look(piece, more);
+    if (tid < span.edges()) offer(ld_f(span.row + span.edge(tid)), span.edge(tid), more);
+    __syncthreads();
+  }
+  const unsigned count = s.count;
+  if (tid < top) s.best[tid] = 0;              // (a block may have fewer)
+  __syncthreads();
+  for (unsigned i = tid; i < count; i += kThreads) {
+    const unsigned long long key = s.cand[i];
+    unsigned before = 0;
+    for (unsigned q = 0; q < count; ++q) before += s.cand[q] > key;
+    if (before < top) s.best[before] = key;
+  }
+  __syncthreads();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__ ScoreParams p) {
+  __shared__ ScoreShared s;
+  const unsigned parts = cluster_size(), part = cluster_rank(), r = blockIdx.x / parts;
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long token = p.tokens(r);
-  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
-  T* out = static_cast<T*>(p.dlogits) + p.drows(r);
-  const float m = p.stats[r], log2s = p.stats[(size_t)p.n + r], h = p.stats[2 * (size_t)p.n + r];
-  if (token == p.ignore || log2s == -INFINITY) {
-    for (unsigned j = threadIdx.x; j < p.vocab; j += 256) out[j] = Elem<T>::from_f(0.f);
+  if (token == p.ignore) {                     // (the same for a whole cluster)
+    if (part == 0) put_ignored(p, r, tid);
     return;
   }
-  const float g_lp = p.g_lp && token >= 0 && token < p.vocab ? p.g_lp[p.g_lp_map(r)] : 0.f, g_h = p.g_h ? p.g_h[p.g_h_map(r)] : 0.f;
-  float g = g_lp;
-  if (p.g_top)
-    for (int k = 0; k < p.top; ++k) g += p.g_top[(size_t)r * p.top + k];
-  const float a = g + g_h * h, b = g_h * kLn2;
-  for (unsigned j = threadIdx.x; j < p.vocab; j += 256) {
-    const float d = max_nan((ld_f(row + j) - m) * p.to_log2, kFar) - log2s;
-    float v = -exp2f(d) * (a + b * d);
-    if (j == token) v += g_lp;
+  if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
+  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
+  const float at_token = tid == 0 && part == 0 && token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
+  const Span<T> span(row, p.vocab, part, parts);
+  const uint4* body = span.body();
+  Part a{-INFINITY, 0.f, 0.f};
+  if (tid < span.edges()) {
+    const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
+    take(a, z, p.to_log2);
+  }
+  unsigned i = span.begin + tid;
+  for (; i + (kUnroll - 1) * kThreads < span.end; i += kUnroll * kThreads) {
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = load_once(body + i + u * kThreads);
+    float z[kUnroll * kPer<T>];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) unpack(v[u], z + u * kPer<T>, T{});
+    take(a, z, p.to_log2);
+  }
+  if (i < span.end) {
+    uint4 v[kUnroll - 1];
+#pragma unroll
+    for (int u = 0; u < kUnroll - 1; ++u) if (i + u * kThreads < span.end) v[u] = load_once(body + i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kUnroll - 1; ++u)
+      if (i + u * kThreads < span.end) {
+        float z[kPer<T>];
+        unpack(v[u], z, T{});
+        take(a, z, p.to_log2);
+      }
+  }
+  const float thread_max = a.m;
+  a.join(32, p.to_log2);
+  if (lane == 0) s.part[warp] = a;
+  if constexpr (TOP) block_top(s, span, thread_max, (unsigned)p.top);
+  else __syncthreads();
+  a = s.part[lane % kWarps];
+  a.join(kWarps, p.to_log2);
+  if (parts > 1) {
+    cluster_wait();
+    if (tid == 0) {
+      store_first(&s.peers[part][0], (unsigned long long)__float_as_uint(a.s) << 32 | __float_as_uint(a.m));
+      store_first(&s.peers[part][1], __float_as_uint(a.t));
+    }
+    if (TOP && part > 0 && tid < (unsigned)p.top) store_first(&s.best[part * p.top + tid], s.best[tid]);
+    cluster_arrive();
+    cluster_wait();
+    if (part > 0) return;
+    const unsigned q = lane % kMaxCluster;
+    a = q < parts ? Part{__uint_as_float(s.peers[q][0].x), __uint_as_float(s.peers[q][0].y), __uint_as_float(s.peers[q][1].x)} : Part{-INFINITY, 0.f, 0.f};
+    a.join(kMaxCluster, p.to_log2);
+  }
+  const Row w(a);
+  if (tid == 0) put_row(p, r, w, token, at_token);
+  if constexpr (TOP) {
+    if (parts == 1) {
+      if (tid < (unsigned)p.top) put_top(p, r, w, tid, s.best[tid]);
+    } else if (tid < parts * p.top) {
+      const unsigned long long key = s.best[tid];
+      unsigned before = 0;
+      for (unsigned q = 0; q < parts * p.top; ++q) before += s.best[q] > key;
+      if (before < (unsigned)p.top && key) put_top(p, r, w, before, key);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient
+struct RowGrad {
+  float m, log2s, g_lp, a, b;  // dz_j = 2^d (a + b d) and what given and top tokens add, d = log2 p_j
+  long long token;
+  bool zero;
+  __device__ __forceinline__ RowGrad(const ScoreParams& p, unsigned r) : token(p.tokens(r)) {
+    m = p.stats[r];
+    log2s = p.stats[(size_t)p.n + r];
+    const float h = p.stats[2 * (size_t)p.n + r];
+    zero = token == p.ignore || log2s == -INFINITY;
+    g_lp = p.g_lp && token >= 0 && token < p.vocab ? p.g_lp[p.g_lp_map(r)] : 0.f;
+    const float g_h = p.g_h ? p.g_h[p.g_h_map(r)] : 0.f;
+    float g = g_lp;
+    if (p.g_top && !zero)
+      for (int k = 0; k < p.top; ++k) g += p.g_top[(size_t)r * p.top + k];
+    a = -(g + g_h * h) * p.per_temperature;
+    b = -g_h * kLn2 * p.per_temperature;
+  }
+  __device__ __forceinline__ float operator()(float z, float to_log2) const {
+    const float d = max_nan(fmaf(z - m, to_log2, -log2s), kFar);
+    return exp2_fast(d) * fmaf(b, d, a);
+  }
+  // The i-th of the token (0) and the top tokens (1 .. top): its number where nobody before it has the same, else -1.
+  __device__ __forceinline__ long long special(const ScoreParams& p, unsigned r, unsigned i) const {
+    const long long* tops = p.top_tokens + (size_t)r * p.top;
+    const long long j = i == 0 ? token : tops[i - 1];
+    if (i > 0 && (p.g_top == nullptr || j == token)) return -1;
+    return j >= 0 && j < p.vocab ? j : -1;
+  }
+  // The gradient of logit j, which is the token or a top token.
+  __device__ __forceinline__ float at(const ScoreParams& p, unsigned r, float z, long long j) const {
+    float extra = j == token ? g_lp : 0.f;
     if (p.g_top)
       for (int k = 0; k < p.top; ++k)
-        if (p.top_tokens[(size_t)r * p.top + k] == j) v += p.g_top[(size_t)r * p.top + k];
-    out[j] = Elem<T>::from_f(v * p.per_temperature);
+        if (p.top_tokens[(size_t)r * p.top + k] == j) extra += p.g_top[(size_t)r * p.top + k];
+    return fmaf(extra, p.per_temperature, (*this)(z, p.to_log2));
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const __grid_constant__ ScoreParams p) {
+  const unsigned lane = threadIdx.x & 31, r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+  if (r >= p.n) return;
+  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
+  T* out = static_cast<T*>(p.dlogits) + p.drows(r);
+  const RowGrad g(p, r);
+  if (g.zero) {
+    for (unsigned j = lane; j < p.vocab; j += 32) out[j] = Elem<T>::from_f(0.f);
+    return;
+  }
+#pragma unroll 8
+  for (unsigned j = lane; j < p.vocab; j += 32) out[j] = Elem<T>::from_f(g(ld_f(row + j), p.to_log2));
+  __syncwarp();
+  for (unsigned i = lane; i <= (p.g_top ? (unsigned)p.top : 0u); i += 32) {
+    const long long j = g.special(p, r, i);
+    if (j >= 0) out[j] = Elem<T>::from_f(g.at(p, r, ld_f(row + j), j));
+  }
+}
+
+__device__ __forceinline__ uint4 pack(const float* z, float) { return make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3])); }
+__device__ __forceinline__ unsigned two(float a, float b, __nv_bfloat16) { const __nv_bfloat162 v = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const unsigned*>(&v); }
+__device__ __forceinline__ unsigned two(float a, float b, __half) { const __half2 v = __floats2half2_rn(a, b); return *reinterpret_cast<const unsigned*>(&v); }
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float* z, T t) { return make_uint4(two(z[0], z[1], t), two(z[2], z[3], t), two(z[4], z[5], t), two(z[6], z[7], t)); }
+
+// A block has a row, or one of gridDim.y parts of it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
+  const unsigned r = blockIdx.x, tid = threadIdx.x;
+  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
+  T* out = static_cast<T*>(p.dlogits) + p.drows(r);
+  const RowGrad g(p, r);
+  const Span<T> span(row, p.vocab, blockIdx.y, gridDim.y);
+  const uint4* body = span.body();
+  uint4* out_body = reinterpret_cast<uint4*>(out + span.head);        // (the same address modulo 16 as the logits')
+  if (g.zero) {
+    for (unsigned i = span.begin + tid; i < span.end; i += kThreads) out_body[i] = make_uint4(0, 0, 0, 0);
+    if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(0.f);
+    return;
+  }
+  if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(g(ld_f(row + span.edge(tid)), p.to_log2));
+  const Pair down = Pair::of(-g.m, -g.m), c = Pair::of(p.to_log2, p.to_log2), minus = Pair::of(-g.log2s, -g.log2s);
+  const Pair a = Pair::of(g.a, g.a), b = Pair::of(g.b, g.b);
+  for (unsigned i = span.begin + tid; i < span.end; i += kUnroll * kThreads) {
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) if (i + u * kThreads < span.end) v[u] = load_once(body + i + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (i + u * kThreads < span.end) {
+        float z[kPer<T>];
+        unpack(v[u], z, T{});
+#pragma unroll
+        for (int k = 0; k < kPer<T>; k += 2) {
+          float x, y;
+          fma2(Pair::of(z[k], z[k + 1]) + down, c, minus).get(x, y);
+          x = max_nan(x, kFar);
+          y = max_nan(y, kFar);
+          (Pair::of(exp2_fast(x), exp2_fast(y)) * fma2(b, Pair::of(x, y), a)).get(z[k], z[k + 1]);
+        }
+        out_body[i + u * kThreads] = pack(z, T{});
+      }
+  }
+  __syncthreads();                             // the few logits that get more are written again, behind the others
+  if (tid <= (p.g_top ? (unsigned)p.top : 0u)) {
+    const long long j = g.special(p, r, tid);
+    const bool edge = j >= 0 && (j < span.head || j >= span.head + span.pieces * kPer<T>);
+    const unsigned piece = (unsigned)(j - span.head) / kPer<T>;
+    if (j >= 0 && (edge ? span.first : piece >= span.begin && piece < span.end)) out[j] = Elem<T>::from_f(g.at(p, r, ld_f(row + j), j));
   }
 }
 
@@ -174,6 +605,42 @@ static ScoreParams score_params(const blstm_score_desc& d, const void* logits, c
   return p;
 }
 
+// How many blocks share a row: as many (a power of two) as give four blocks to an SM, with a full turn of the unrolled loop
+// for each of them.
+static unsigned score_parts(const ScoreParams& p, size_t element, unsigned most) {
+  const unsigned long long pieces = (unsigned long long)p.vocab * element / 16;
+  unsigned parts = 1;
+  while (parts < most && (unsigned long long)p.n * parts * 2 <= 4ull * plan_sm_count() && pieces / (parts * 2) >= kThreads) parts *= 2;
+  return parts;
+}
+
+template <typename T, bool TOP>
+static int launch_score(const ScoreParams& p, cudaStream_t st) {
+  if (p.vocab <= kWarpVocab) {
+    const unsigned grid = (p.n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows;
+    if (p.vocab <= 128) score_warp_kernel<T, 4, TOP><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= 256) score_warp_kernel<T, 8, TOP><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= 512) score_warp_kernel<T, 16, TOP><<<grid, block, 0, st>>>(p);
+    else score_warp_kernel<T, 32, TOP><<<grid, block, 0, st>>>(p);
+    BLSTM_CUDA_OK(cudaGetLastError());
+  } else {
+    const unsigned parts = score_parts(p, sizeof(T), kMaxCluster);
+    if ((unsigned long long)p.n * parts > INT32_MAX) return BLSTM_E_TOO_LARGE;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {parts, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = p.n * parts;
+    cfg.blockDim = kThreads;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, score_kernel<T, TOP>, p));
+  }
+  count_launch();
+  return BLSTM_OK;
+}
+
 }  // namespace blstm
 
 using namespace blstm;
@@ -190,10 +657,8 @@ int blstm_token_log_probs(const blstm_score_desc* d, const void* logits, const v
   p.top_log_probs = top_log_probs; p.top_tokens = reinterpret_cast<long long*>(top_tokens);
   p.mailbox = current_mailbox();
   return with_type(d->dtype, [&](auto t) -> int {
-    score_kernel<decltype(t)><<<p.n, 256, 0, (cudaStream_t)stream>>>(p);
-    BLSTM_CUDA_OK(cudaGetLastError());
-    count_launch();
-    return BLSTM_OK;
+    using T = decltype(t);
+    return d->top ? launch_score<T, true>(p, (cudaStream_t)stream) : launch_score<T, false>(p, (cudaStream_t)stream);
   });
 }
 
@@ -217,7 +682,10 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
   if (g_log_probs) p.g_lp_map = row_map(d->n1, g_log_probs_stride);
   if (g_entropy) p.g_h_map = row_map(d->n1, g_entropy_stride);
   return with_type(d->dtype, [&](auto t) -> int {
-    score_grad_kernel<decltype(t)><<<p.n, 256, 0, (cudaStream_t)stream>>>(p);
+    using T = decltype(t);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (p.vocab <= kWarpVocab) score_grad_warp_kernel<T><<<(p.n + kWarpRows - 1) / kWarpRows, 32 * kWarpRows, 0, st>>>(p);
+    else score_grad_kernel<T><<<dim3(p.n, score_parts(p, sizeof(T), 1 << 16)), kThreads, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
