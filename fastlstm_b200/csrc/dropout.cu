@@ -4,6 +4,8 @@
 //
 // Philox is Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3" (2011).  m counts the elements in
 // row-major order whatever the strides and the type, and only those of one step where the steps share a mask.
+#include <algorithm>
+
 #include "language.cuh"
 
 namespace blstm {
@@ -16,7 +18,7 @@ struct DropoutParams {
   long long count;               // masked elements (of one step where steps share the mask)
   long long cols;
   RowMap in, out;                // rows of `cols` elements
-  unsigned steps;                // that share a mask
+  unsigned steps, each;          // that share a mask, and how many of them a block walks
   long long in_step, out_step;
   unsigned threshold;
   float scale;
@@ -38,23 +40,113 @@ __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned long 
   return make_uint4(c0, c1, c2, c3);
 }
 
-// A thread draws one block of four words and walks the steps that share it.
-template <typename T>
+// The mask's words for N elements from element m0, a multiple of 4, as bits: set where an element stays.
+template <int N>
+__device__ __forceinline__ unsigned kept_bits(const DropoutParams& p, long long m0, unsigned long long seed) {
+  unsigned bits = 0;
+#pragma unroll
+  for (int k = 0; k < N; k += 4) {
+    const uint4 w = philox((m0 + k) / 4, p.offset, seed);
+    bits |= (w.x >= p.threshold ? 1u : 0u) << k | (w.y >= p.threshold ? 2u : 0u) << k | (w.z >= p.threshold ? 4u : 0u) << k |
+            (w.w >= p.threshold ? 8u : 0u) << k;
+  }
+  return bits;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> masked(const Pack<T, N>& x, unsigned bits, float scale) {
+  Pack<T, N> y;
+#pragma unroll
+  for (int k = 0; k < N; ++k) y.v[k] = Elem<T>::from_f(bits >> k & 1 ? Elem<T>::to_f(x.v[k]) * scale : 0.f);
+  return y;
+}
+
+__device__ __forceinline__ unsigned long long seed_of(const DropoutParams& p) { return p.seed_at ? *p.seed_at : p.seed; }
+
+// Every element its own word, 16-byte pieces, kPieces a thread.  ROWS: rows of x have strides of their own.
+constexpr int kPieces = 2;
+
+template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  const long long block = (long long)blockIdx.x * blockDim.x + threadIdx.x, m0 = block * 4;
+  constexpr int N = 16 / sizeof(T);
+  using V = Pack<T, N>;
+  const unsigned long long seed = seed_of(p);
+  const long long pieces = (p.count + N - 1) / N, first = (long long)blockIdx.x * (256 * kPieces) + threadIdx.x;
+  const T* x = static_cast<const T*>(p.x);
+  T* y = static_cast<T*>(p.y);
+  V v[kPieces];
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    const long long q = first + u * 256, m = q * N;
+    if (m + N > p.count) continue;
+    long long at = m;
+    if constexpr (ROWS) {
+      const unsigned per_row = (unsigned)(p.cols / N);
+      const unsigned r = pieces <= 0xffffffffll ? (unsigned)q / per_row : (unsigned)(q / per_row);
+      at = p.in(r) + (q - (long long)r * per_row) * N;
+    }
+    v[u] = *reinterpret_cast<const V*>(x + at);
+  }
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    const long long m = (first + u * 256) * N;
+    if (m >= p.count) continue;
+    const unsigned bits = kept_bits<N>(p, m, seed);
+    if (m + N <= p.count) *reinterpret_cast<V*>(y + m) = masked<T, N>(v[u], bits, p.scale);
+    else                                       // (not with ROWS, whose rows are whole pieces)
+      for (int k = 0; m + k < p.count; ++k) y[m + k] = Elem<T>::from_f(bits >> k & 1 ? Elem<T>::to_f(x[m + k]) * p.scale : 0.f);
+  }
+}
+
+// Steps that share a mask: a thread draws the words of one piece and walks a part of the steps (blockIdx.y).
+constexpr int kSteps = 4;            // on their way at a time
+
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_shared_kernel(const __grid_constant__ DropoutParams p) {
+  constexpr int N = 16 / sizeof(T);
+  using V = Pack<T, N>;
+  const long long q = (long long)blockIdx.x * 256 + threadIdx.x, m = q * N;
+  if (m >= p.count) return;
+  const unsigned bits = kept_bits<N>(p, m, seed_of(p));
+  const unsigned r = (unsigned)(m / p.cols);
+  const long long c = m - r * p.cols;
+  const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
+  const T* x = static_cast<const T*>(p.x) + p.in(r) + c + begin * p.in_step;
+  T* y = static_cast<T*>(p.y) + p.out(r) + c + begin * p.out_step;
+  unsigned s = begin;
+  for (; s + kSteps <= end; s += kSteps) {
+    V v[kSteps];
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) v[u] = *reinterpret_cast<const V*>(x + u * p.in_step);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) *reinterpret_cast<V*>(y + u * p.out_step) = masked<T, N>(v[u], bits, p.scale);
+    x += kSteps * p.in_step;
+    y += kSteps * p.out_step;
+  }
+  for (; s < end; ++s) {
+    *reinterpret_cast<V*>(y) = masked<T, N>(*reinterpret_cast<const V*>(x), bits, p.scale);
+    x += p.in_step;
+    y += p.out_step;
+  }
+}
+
+// Rows that are no whole pieces, or not on 16-byte boundaries: four elements a thread, one by one.
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_elements_kernel(const __grid_constant__ DropoutParams p) {
+  const long long m0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   if (m0 >= p.count) return;
-  const uint4 w = philox(block, p.offset, p.seed_at ? *p.seed_at : p.seed);
-  const unsigned word[4] = {w.x, w.y, w.z, w.w};
+  const unsigned bits = kept_bits<4>(p, m0, seed_of(p));
   unsigned r = (unsigned)(m0 / p.cols);
   long long c = m0 - r * p.cols;
+  const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (m0 + j >= p.count) break;
     const T* x = static_cast<const T*>(p.x) + p.in(r) + c;
     T* y = static_cast<T*>(p.y) + p.out(r) + c;
-    const bool keep = word[j] >= p.threshold;
-    for (unsigned s = 0; s < p.steps; ++s)
-      y[s * p.out_step] = Elem<T>::from_f(keep ? Elem<T>::to_f(x[s * p.in_step]) * p.scale : 0.f);
+    const bool keep = bits >> j & 1;
+#pragma unroll 4
+    for (unsigned s = begin; s < end; ++s) y[s * p.out_step] = Elem<T>::from_f(keep ? Elem<T>::to_f(x[s * p.in_step]) * p.scale : 0.f);
     if (++c == p.cols) { c = 0; ++r; }
   }
 }
@@ -101,10 +193,24 @@ extern "C" int blstm_dropout(const blstm_dropout_desc* d, const void* x, const i
     p.out = {n1 * C, 0, 1};
     p.steps = (unsigned)n1; p.in_step = d->stride[1]; p.out_step = C;
   }
-  const long long grid = (p.count + 1023) / 1024;
-  if (grid > INT32_MAX) return BLSTM_E_TOO_LARGE;
+  // 16-byte pieces need rows that are whole pieces on 16-byte boundaries; a tensor without gaps is one row, whose end may be ragged
+  const bool dense = d->shared < 0 && (n1 == 1 || d->stride[1] == C) && (d->n0 == 1 || d->stride[0] == n1 * C);
+  const uintptr_t strides = (d->n0 > 1 ? (uintptr_t)d->stride[0] : 0) | (d->n1 > 1 ? (uintptr_t)d->stride[1] : 0) | (uintptr_t)C;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | (dense ? 0 : strides * e);
+  const bool pieces = (bits & 15u) == 0;
+  const int per_thread = !pieces ? 4 : 16 / e * (d->shared < 0 ? kPieces : 1);
+  const long long blocks = (p.count + 256ll * per_thread - 1) / (256ll * per_thread);
+  if (blocks > INT32_MAX) return BLSTM_E_TOO_LARGE;
+  // the steps in as many parts as give eight blocks to an SM, eight steps each at least: the words are drawn for each part
+  const long long parts = std::max(1ll, std::min<long long>({8ll * plan_sm_count() / blocks, p.steps / 8, 65535}));
+  p.each = (unsigned)((p.steps + parts - 1) / parts);
+  const dim3 grid((unsigned)blocks, (p.steps + p.each - 1) / p.each);
   return with_type(d->dtype, [&](auto t) -> int {
-    dropout_kernel<decltype(t)><<<(unsigned)grid, 256, 0, st>>>(p);
+    using T = decltype(t);
+    if (!pieces) dropout_elements_kernel<T><<<grid, 256, 0, st>>>(p);
+    else if (d->shared >= 0) dropout_shared_kernel<T><<<grid, 256, 0, st>>>(p);
+    else if (dense) dropout_kernel<T, false><<<grid, 256, 0, st>>>(p);
+    else dropout_kernel<T, true><<<grid, 256, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
