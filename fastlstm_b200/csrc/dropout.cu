@@ -24,40 +24,41 @@ struct DropoutParams {
   float scale;
 };
 
-__device__ __forceinline__ uint4 philox(unsigned long long block, unsigned long long offset, unsigned long long seed) {
-  unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = (unsigned)offset, c3 = (unsigned)(offset >> 32);
+// The words of N elements from element m0, a multiple of 4.  Blocks go through the rounds side by side, with one schedule of
+// keys; `high`, the upper half of the block's number, is the same for all.
+template <int N>
+__device__ __forceinline__ void draw(unsigned (&w)[N], unsigned block, unsigned high, unsigned long long offset, unsigned long long seed) {
   unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
 #pragma unroll
+  for (int b = 0; b < N; b += 4) {
+    w[b] = block + b / 4;
+    w[b + 1] = high;
+    w[b + 2] = (unsigned)offset;
+    w[b + 3] = (unsigned)(offset >> 32);
+  }
+#pragma unroll
   for (int r = 0; r < 10; ++r) {
-    const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
-    c1 = (unsigned)b;
-    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
-    c3 = (unsigned)a;
+#pragma unroll
+    for (int b = 0; b < N; b += 4) {
+      const unsigned long long x = (unsigned long long)w[b] * 0xD2511F53u, y = (unsigned long long)w[b + 2] * 0xCD9E8D57u;
+      w[b] = (unsigned)(y >> 32) ^ w[b + 1] ^ k0;
+      w[b + 1] = (unsigned)y;
+      w[b + 2] = (unsigned)(x >> 32) ^ w[b + 3] ^ k1;
+      w[b + 3] = (unsigned)x;
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return make_uint4(c0, c1, c2, c3);
-}
-
-// The mask's words for N elements from element m0, a multiple of 4, as bits: set where an element stays.
-template <int N>
-__device__ __forceinline__ unsigned kept_bits(const DropoutParams& p, long long m0, unsigned long long seed) {
-  unsigned bits = 0;
-#pragma unroll
-  for (int k = 0; k < N; k += 4) {
-    const uint4 w = philox((m0 + k) / 4, p.offset, seed);
-    bits |= (w.x >= p.threshold ? 1u : 0u) << k | (w.y >= p.threshold ? 2u : 0u) << k | (w.z >= p.threshold ? 4u : 0u) << k |
-            (w.w >= p.threshold ? 8u : 0u) << k;
-  }
-  return bits;
 }
 
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> masked(const Pack<T, N>& x, unsigned bits, float scale) {
+__device__ __forceinline__ Pack<T, N> masked(const Pack<T, N>& x, const unsigned (&w)[N], unsigned threshold, float scale) {
   Pack<T, N> y;
 #pragma unroll
-  for (int k = 0; k < N; ++k) y.v[k] = Elem<T>::from_f(bits >> k & 1 ? Elem<T>::to_f(x.v[k]) * scale : 0.f);
+  for (int k = 0; k < N; ++k) {
+    const float v = Elem<T>::to_f(x.v[k]) * scale;
+    y.v[k] = Elem<T>::from_f(w[k] >= threshold ? v : 0.f);
+  }
   return y;
 }
 
@@ -71,13 +72,14 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
   constexpr int N = 16 / sizeof(T);
   using V = Pack<T, N>;
   const unsigned long long seed = seed_of(p);
-  const long long pieces = (p.count + N - 1) / N, first = (long long)blockIdx.x * (256 * kPieces) + threadIdx.x;
+  const long long pieces = (p.count + N - 1) / N, begin = (long long)blockIdx.x * (256 * kPieces);
+  const unsigned long long blocks = (unsigned long long)begin * (N / 4);     // (a whole number of tiles: no carry inside of one)
   const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
   V v[kPieces];
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
-    const long long q = first + u * 256, m = q * N;
+    const long long q = begin + u * 256 + threadIdx.x, m = q * N;
     if (m + N > p.count) continue;
     long long at = m;
     if constexpr (ROWS) {
@@ -89,12 +91,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
   }
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
-    const long long m = (first + u * 256) * N;
+    const long long m = (begin + u * 256 + threadIdx.x) * N;
     if (m >= p.count) continue;
-    const unsigned bits = kept_bits<N>(p, m, seed);
-    if (m + N <= p.count) *reinterpret_cast<V*>(y + m) = masked<T, N>(v[u], bits, p.scale);
+    unsigned w[N];
+    draw<N>(w, (unsigned)blocks + (u * 256 + threadIdx.x) * (N / 4), (unsigned)(blocks >> 32), p.offset, seed);
+    if (m + N <= p.count) *reinterpret_cast<V*>(y + m) = masked<T, N>(v[u], w, p.threshold, p.scale);
     else                                       // (not with ROWS, whose rows are whole pieces)
-      for (int k = 0; m + k < p.count; ++k) y[m + k] = Elem<T>::from_f(bits >> k & 1 ? Elem<T>::to_f(x[m + k]) * p.scale : 0.f);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (m + k < p.count) y[m + k] = Elem<T>::from_f(w[k] >= p.threshold ? Elem<T>::to_f(x[m + k]) * p.scale : 0.f);
   }
 }
 
@@ -107,7 +112,8 @@ __global__ void __launch_bounds__(256) dropout_shared_kernel(const __grid_consta
   using V = Pack<T, N>;
   const long long q = (long long)blockIdx.x * 256 + threadIdx.x, m = q * N;
   if (m >= p.count) return;
-  const unsigned bits = kept_bits<N>(p, m, seed_of(p));
+  unsigned w[N];
+  draw<N>(w, (unsigned)(m / 4), (unsigned)((unsigned long long)m >> 34), p.offset, seed_of(p));
   const unsigned r = (unsigned)(m / p.cols);
   const long long c = m - r * p.cols;
   const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
@@ -119,12 +125,12 @@ __global__ void __launch_bounds__(256) dropout_shared_kernel(const __grid_consta
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) v[u] = *reinterpret_cast<const V*>(x + u * p.in_step);
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) *reinterpret_cast<V*>(y + u * p.out_step) = masked<T, N>(v[u], bits, p.scale);
+    for (int u = 0; u < kSteps; ++u) *reinterpret_cast<V*>(y + u * p.out_step) = masked<T, N>(v[u], w, p.threshold, p.scale);
     x += kSteps * p.in_step;
     y += kSteps * p.out_step;
   }
   for (; s < end; ++s) {
-    *reinterpret_cast<V*>(y) = masked<T, N>(*reinterpret_cast<const V*>(x), bits, p.scale);
+    *reinterpret_cast<V*>(y) = masked<T, N>(*reinterpret_cast<const V*>(x), w, p.threshold, p.scale);
     x += p.in_step;
     y += p.out_step;
   }
@@ -135,7 +141,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) dropout_elements_kernel(const __grid_constant__ DropoutParams p) {
   const long long m0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   if (m0 >= p.count) return;
-  const unsigned bits = kept_bits<4>(p, m0, seed_of(p));
+  unsigned w[4];
+  draw<4>(w, (unsigned)(m0 / 4), (unsigned)((unsigned long long)m0 >> 34), p.offset, seed_of(p));
   unsigned r = (unsigned)(m0 / p.cols);
   long long c = m0 - r * p.cols;
   const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
@@ -144,7 +151,7 @@ __global__ void __launch_bounds__(256) dropout_elements_kernel(const __grid_cons
     if (m0 + j >= p.count) break;
     const T* x = static_cast<const T*>(p.x) + p.in(r) + c;
     T* y = static_cast<T*>(p.y) + p.out(r) + c;
-    const bool keep = bits >> j & 1;
+    const bool keep = w[j] >= p.threshold;
 #pragma unroll 4
     for (unsigned s = begin; s < end; ++s) y[s * p.out_step] = Elem<T>::from_f(keep ? Elem<T>::to_f(x[s * p.in_step]) * p.scale : 0.f);
     if (++c == p.cols) { c = 0; ++r; }
