@@ -5,6 +5,7 @@
 // Philox is Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3" (2011).  m counts the elements in
 // row-major order whatever the strides and the type, and only those of one step where the steps share a mask.
 #include <algorithm>
+#include <type_traits>
 
 #include "language.cuh"
 
@@ -13,8 +14,9 @@ namespace blstm {
 struct DropoutParams {
   const void* x;
   void* y;
-  const long long* seed_at;      // the seed in device memory, or null: `seed`
-  unsigned long long seed, offset;
+  const long long* seed_at;      // the seed in device memory, or null
+  unsigned long long offset;
+  unsigned keys[20];             // of the rounds, where the seed is not in device memory
   long long count;               // masked elements (of one step where steps share the mask)
   long long cols;
   RowMap in, out;                // rows of `cols` elements
@@ -24,125 +26,170 @@ struct DropoutParams {
   float scale;
 };
 
-// The words of N elements from element m0, a multiple of 4.  Blocks go through the rounds side by side, with one schedule of
-// keys; `high`, the upper half of the block's number, is the same for all.
-template <int N>
-__device__ __forceinline__ void draw(unsigned (&w)[N], unsigned block, unsigned high, unsigned long long offset, unsigned long long seed) {
-  unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+// The keys of the ten rounds: from the host, where they come with the parameters and cost nothing, or from a seed in device
+// memory.
+template <bool SEED_AT>
+struct Keys {
+  unsigned k[SEED_AT ? 20 : 1];
+  __device__ __forceinline__ explicit Keys(const DropoutParams& p) {
+    if constexpr (SEED_AT) {
+      const unsigned long long seed = *p.seed_at;
+#pragma unroll
+      for (int r = 0; r < 10; ++r) {
+        k[2 * r] = (unsigned)seed + r * 0x9E3779B9u;
+        k[2 * r + 1] = (unsigned)(seed >> 32) + r * 0xBB67AE85u;
+      }
+    }
+  }
+  __device__ __forceinline__ unsigned operator()(const DropoutParams& p, int i) const { return SEED_AT ? k[SEED_AT ? i : 0] : p.keys[i]; }
+};
+
+// The words of N elements from element 4 block; `high`, the upper half of the block's number, is the same for all of them.
+template <int N, bool SEED_AT>
+__device__ __forceinline__ void draw(unsigned (&w)[N], const DropoutParams& p, const Keys<SEED_AT>& keys, unsigned block, unsigned high) {
 #pragma unroll
   for (int b = 0; b < N; b += 4) {
     w[b] = block + b / 4;
     w[b + 1] = high;
-    w[b + 2] = (unsigned)offset;
-    w[b + 3] = (unsigned)(offset >> 32);
+    w[b + 2] = (unsigned)p.offset;
+    w[b + 3] = (unsigned)(p.offset >> 32);
   }
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
 #pragma unroll
     for (int b = 0; b < N; b += 4) {
       const unsigned long long x = (unsigned long long)w[b] * 0xD2511F53u, y = (unsigned long long)w[b + 2] * 0xCD9E8D57u;
-      w[b] = (unsigned)(y >> 32) ^ w[b + 1] ^ k0;
+      w[b] = (unsigned)(y >> 32) ^ w[b + 1] ^ keys(p, 2 * r);
       w[b + 1] = (unsigned)y;
-      w[b + 2] = (unsigned)(x >> 32) ^ w[b + 3] ^ k1;
+      w[b + 2] = (unsigned)(x >> 32) ^ w[b + 3] ^ keys(p, 2 * r + 1);
       w[b + 3] = (unsigned)x;
     }
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> masked(const Pack<T, N>& x, const unsigned (&w)[N], unsigned threshold, float scale) {
-  Pack<T, N> y;
+// A piece with the elements dropped whose words are below the threshold, whatever they hold.
+template <typename T>
+__device__ __forceinline__ uint4 masked(const uint4& v, const unsigned (&w)[kPer<T>], const DropoutParams& p) {
+  float z[kPer<T>];
+  unpack(v, z, T{});
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const float v = Elem<T>::to_f(x.v[k]) * scale;
-    y.v[k] = Elem<T>::from_f(w[k] >= threshold ? v : 0.f);
+  for (int k = 0; k < kPer<T>; ++k) {
+    const float y = z[k] * p.scale;
+    z[k] = w[k] >= p.threshold ? y : 0.f;
   }
-  return y;
+  return pack(z, T{});
 }
 
-__device__ __forceinline__ unsigned long long seed_of(const DropoutParams& p) { return p.seed_at ? *p.seed_at : p.seed; }
+// The same in two steps, for words that serve many pieces: bits that stay, and a piece with them.
+template <typename T>
+__device__ __forceinline__ uint4 stays(const unsigned (&w)[kPer<T>], unsigned threshold) {
+  unsigned b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) b[i] = w[i] >= threshold ? ~0u : 0u;
+    else b[i] = (w[2 * i] >= threshold ? 0xffffu : 0u) | (w[2 * i + 1] >= threshold ? 0xffff0000u : 0u);
+  }
+  return make_uint4(b[0], b[1], b[2], b[3]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 masked(const uint4& v, const uint4& bits, float scale) {
+  float z[kPer<T>];
+  unpack(v, z, T{});
+#pragma unroll
+  for (int k = 0; k < kPer<T>; ++k) z[k] *= scale;
+  const uint4 y = pack(z, T{});
+  return make_uint4(y.x & bits.x, y.y & bits.y, y.z & bits.z, y.w & bits.w);
+}
 
 // Every element its own word, 16-byte pieces, kPieces a thread.  ROWS: rows of x have strides of their own.
 constexpr int kPieces = 2;
 
-template <typename T, bool ROWS>
+template <typename T, bool SEED_AT, bool ROWS>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  constexpr int N = 16 / sizeof(T);
-  using V = Pack<T, N>;
-  const unsigned long long seed = seed_of(p);
-  const long long pieces = (p.count + N - 1) / N, begin = (long long)blockIdx.x * (256 * kPieces);
-  const unsigned long long blocks = (unsigned long long)begin * (N / 4);     // (a whole number of tiles: no carry inside of one)
+  constexpr int N = kPer<T>, kTile = 256 * kPieces;
+  const Keys<SEED_AT> keys(p);
+  const unsigned long long begin = (unsigned long long)blockIdx.x * kTile, whole = p.count / N;      // pieces
+  const unsigned long long number = begin * (N / 4);        // Philox blocks: a whole number of tiles, no carry inside of one
   const T* x = static_cast<const T*>(p.x);
-  T* y = static_cast<T*>(p.y);
-  V v[kPieces];
+  uint4* y = static_cast<uint4*>(p.y) + begin;
+  const uint4* from[kPieces];
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
-    const long long q = begin + u * 256 + threadIdx.x, m = q * N;
-    if (m + N > p.count) continue;
-    long long at = m;
+    const unsigned i = u * 256 + threadIdx.x;
     if constexpr (ROWS) {
       const unsigned per_row = (unsigned)(p.cols / N);
-      const unsigned r = pieces <= 0xffffffffll ? (unsigned)q / per_row : (unsigned)(q / per_row);
-      at = p.in(r) + (q - (long long)r * per_row) * N;
+      const unsigned long long q = begin + i;
+      const unsigned r = q <= 0xffffffffu ? (unsigned)q / per_row : (unsigned)(q / per_row);
+      from[u] = reinterpret_cast<const uint4*>(x + p.in(r) + (long long)(q - (unsigned long long)r * per_row) * N);
+    } else {
+      from[u] = reinterpret_cast<const uint4*>(x) + begin + i;
     }
-    v[u] = *reinterpret_cast<const V*>(x + at);
   }
+  auto words = [&](unsigned (&w)[N], unsigned i) { draw(w, p, keys, (unsigned)number + i * (N / 4), (unsigned)(number >> 32)); };
+  if (begin + kTile <= whole) {
+    uint4 v[kPieces];
 #pragma unroll
+    for (int u = 0; u < kPieces; ++u) v[u] = *from[u];
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u) {
+      unsigned w[N];
+      words(w, u * 256 + threadIdx.x);
+      y[u * 256 + threadIdx.x] = masked<T>(v[u], w, p);
+    }
+    return;
+  }
   for (int u = 0; u < kPieces; ++u) {
-    const long long m = (begin + u * 256 + threadIdx.x) * N;
-    if (m >= p.count) continue;
+    const unsigned i = u * 256 + threadIdx.x;
+    if (begin + i > whole) continue;
     unsigned w[N];
-    draw<N>(w, (unsigned)blocks + (u * 256 + threadIdx.x) * (N / 4), (unsigned)(blocks >> 32), p.offset, seed);
-    if (m + N <= p.count) *reinterpret_cast<V*>(y + m) = masked<T, N>(v[u], w, p.threshold, p.scale);
-    else                                       // (not with ROWS, whose rows are whole pieces)
+    words(w, i);
+    if (begin + i < whole) y[i] = masked<T>(*from[u], w, p);
+    else                                       // the elements behind the last piece (not with ROWS, whose rows are whole pieces)
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (m + k < p.count) y[m + k] = Elem<T>::from_f(w[k] >= p.threshold ? Elem<T>::to_f(x[m + k]) * p.scale : 0.f);
+      for (int k = 0; k < N; ++k) {
+        const unsigned long long m = whole * N + k;
+        if ((long long)m < p.count) static_cast<T*>(p.y)[m] = Elem<T>::from_f(w[k] >= p.threshold ? Elem<T>::to_f(x[m]) * p.scale : 0.f);
+      }
   }
 }
 
-// Steps that share a mask: a thread draws the words of one piece and walks a part of the steps (blockIdx.y).
-constexpr int kSteps = 4;            // on their way at a time
+// Steps that share a mask: a thread draws the words of one piece and walks a part of the steps (blockIdx.y), all of which are
+// on their way together.  Short parts keep the blocks that run at a time in neighbouring memory (512 x 256 x 1024 fp16:
+// 8 steps 82.7 us, 16 84.5, 32 86.7, parts of 52 steps 92), and drawing the words again for every eighth step is hidden.
+constexpr int kSteps = 8;
 
-template <typename T>
+template <typename T, bool SEED_AT>
 __global__ void __launch_bounds__(256) dropout_shared_kernel(const __grid_constant__ DropoutParams p) {
-  constexpr int N = 16 / sizeof(T);
-  using V = Pack<T, N>;
+  constexpr int N = kPer<T>;
   const long long q = (long long)blockIdx.x * 256 + threadIdx.x, m = q * N;
   if (m >= p.count) return;
   unsigned w[N];
-  draw<N>(w, (unsigned)(m / 4), (unsigned)((unsigned long long)m >> 34), p.offset, seed_of(p));
+  draw(w, p, Keys<SEED_AT>(p), (unsigned)(m / 4), (unsigned)((unsigned long long)m >> 34));
+  const uint4 bits = stays<T>(w, p.threshold);
   const unsigned r = (unsigned)(m / p.cols);
   const long long c = m - r * p.cols;
   const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
-  const T* x = static_cast<const T*>(p.x) + p.in(r) + c + begin * p.in_step;
-  T* y = static_cast<T*>(p.y) + p.out(r) + c + begin * p.out_step;
-  unsigned s = begin;
-  for (; s + kSteps <= end; s += kSteps) {
-    V v[kSteps];
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + p.in(r) + c + begin * p.in_step);
+  uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(p.y) + p.out(r) + c + begin * p.out_step);
+  const long long in_step = p.in_step / N, out_step = p.out_step / N;
+  for (unsigned s = begin; s < end; s += kSteps) {
+    uint4 v[kSteps];
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) v[u] = *reinterpret_cast<const V*>(x + u * p.in_step);
+    for (int u = 0; u < kSteps; ++u) if (s + u < end) v[u] = x[u * in_step];
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) *reinterpret_cast<V*>(y + u * p.out_step) = masked<T, N>(v[u], w, p.threshold, p.scale);
-    x += kSteps * p.in_step;
-    y += kSteps * p.out_step;
-  }
-  for (; s < end; ++s) {
-    *reinterpret_cast<V*>(y) = masked<T, N>(*reinterpret_cast<const V*>(x), w, p.threshold, p.scale);
-    x += p.in_step;
-    y += p.out_step;
+    for (int u = 0; u < kSteps; ++u) if (s + u < end) y[u * out_step] = masked<T>(v[u], bits, p.scale);
+    x += kSteps * in_step;
+    y += kSteps * out_step;
   }
 }
 
 // Rows that are no whole pieces, or not on 16-byte boundaries: four elements a thread, one by one.
-template <typename T>
+template <typename T, bool SEED_AT>
 __global__ void __launch_bounds__(256) dropout_elements_kernel(const __grid_constant__ DropoutParams p) {
   const long long m0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   if (m0 >= p.count) return;
   unsigned w[4];
-  draw<4>(w, (unsigned)(m0 / 4), (unsigned)((unsigned long long)m0 >> 34), p.offset, seed_of(p));
+  draw(w, p, Keys<SEED_AT>(p), (unsigned)(m0 / 4), (unsigned)((unsigned long long)m0 >> 34));
   unsigned r = (unsigned)(m0 / p.cols);
   long long c = m0 - r * p.cols;
   const unsigned begin = blockIdx.y * p.each, end = min(p.steps, begin + p.each);
@@ -179,7 +226,11 @@ extern "C" int blstm_dropout(const blstm_dropout_desc* d, const void* x, const i
   DropoutParams p{};
   p.x = x; p.y = y;
   p.seed_at = reinterpret_cast<const long long*>(seed);
-  p.seed = d->seed; p.offset = d->offset;
+  p.offset = d->offset;
+  for (unsigned r = 0; r < 10; ++r) {
+    p.keys[2 * r] = (unsigned)d->seed + r * 0x9E3779B9u;
+    p.keys[2 * r + 1] = (unsigned)(d->seed >> 32) + r * 0xBB67AE85u;
+  }
   p.cols = d->cols;
   p.threshold = (unsigned)bound;
   p.scale = (float)(1.0 / (1.0 - d->p));
@@ -208,16 +259,19 @@ extern "C" int blstm_dropout(const blstm_dropout_desc* d, const void* x, const i
   const int per_thread = !pieces ? 4 : 16 / e * (d->shared < 0 ? kPieces : 1);
   const long long blocks = (p.count + 256ll * per_thread - 1) / (256ll * per_thread);
   if (blocks > INT32_MAX) return BLSTM_E_TOO_LARGE;
-  // the steps in as many parts as give eight blocks to an SM, eight steps each at least: the words are drawn for each part
-  const long long parts = std::max(1ll, std::min<long long>({8ll * plan_sm_count() / blocks, p.steps / 8, 65535}));
-  p.each = (unsigned)((p.steps + parts - 1) / parts);
+  p.each = std::max((unsigned)kSteps, (p.steps + 65534) / 65535);        // (a grid has 65535 parts at most)
   const dim3 grid((unsigned)blocks, (p.steps + p.each - 1) / p.each);
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (!pieces) dropout_elements_kernel<T><<<grid, 256, 0, st>>>(p);
-    else if (d->shared >= 0) dropout_shared_kernel<T><<<grid, 256, 0, st>>>(p);
-    else if (dense) dropout_kernel<T, false><<<grid, 256, 0, st>>>(p);
-    else dropout_kernel<T, true><<<grid, 256, 0, st>>>(p);
+    auto launch = [&](auto at) {
+      constexpr bool A = decltype(at)::value;
+      if (!pieces) dropout_elements_kernel<T, A><<<grid, 256, 0, st>>>(p);
+      else if (d->shared >= 0) dropout_shared_kernel<T, A><<<grid, 256, 0, st>>>(p);
+      else if (dense) dropout_kernel<T, A, false><<<grid, 256, 0, st>>>(p);
+      else dropout_kernel<T, A, true><<<grid, 256, 0, st>>>(p);
+    };
+    if (seed) launch(std::true_type{});
+    else launch(std::false_type{});
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;

@@ -84,25 +84,6 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return r;
 }
 
-template <typename T> constexpr int kPer = 16 / (int)sizeof(T);        // elements of a 16-byte piece
-
-__device__ __forceinline__ void unpack(const uint4& v, float* z, float) {
-  z[0] = __uint_as_float(v.x); z[1] = __uint_as_float(v.y); z[2] = __uint_as_float(v.z); z[3] = __uint_as_float(v.w);
-}
-__device__ __forceinline__ void unpack(const uint4& v, float* z, __nv_bfloat16) {
-  const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { z[2 * i] = __uint_as_float(w[i] << 16); z[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void unpack(const uint4& v, float* z, __half) {
-  const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    z[2 * i] = f.x; z[2 * i + 1] = f.y;
-  }
-}
-
 // A part of a row: its largest logit, and the sums of 2^d and of d 2^d over it, d the distance from the reference
 // max(m, kLowest) in powers of two.
 struct Part {
@@ -531,12 +512,6 @@ __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const _
     if (j >= 0) out[j] = Elem<T>::from_f(g.at(p, r, ld_f(row + j), j));
   }
 }
-
-__device__ __forceinline__ uint4 pack(const float* z, float) { return make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3])); }
-__device__ __forceinline__ unsigned two(float a, float b, __nv_bfloat16) { const __nv_bfloat162 v = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const unsigned*>(&v); }
-__device__ __forceinline__ unsigned two(float a, float b, __half) { const __half2 v = __floats2half2_rn(a, b); return *reinterpret_cast<const unsigned*>(&v); }
-template <typename T>
-__device__ __forceinline__ uint4 pack(const float* z, T t) { return make_uint4(two(z[0], z[1], t), two(z[2], z[3], t), two(z[4], z[5], t), two(z[6], z[7], t)); }
 
 // A block has a row, or one of gridDim.y parts of it.
 template <typename T>
