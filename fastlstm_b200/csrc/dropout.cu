@@ -238,7 +238,7 @@ extern "C" int blstm_dropout(const blstm_dropout_desc* d, const void* x, const i
   const long long n1 = d->n1, C = d->cols;
   if (d->shared < 0) {
     p.count = (long long)d->n0 * n1 * C;
-    p.in = row_map(n1, d->stride);
+    p.in = row_map(d->n0, n1, d->stride);
     p.out = {n1 * C, C, (unsigned)n1};
   } else if (d->shared == 0) {                    // the mask of [n1, cols], n0 times
     p.count = n1 * C;

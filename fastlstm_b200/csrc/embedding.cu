@@ -2,10 +2,11 @@
 //
 //   out[n,:] = round(scale W[t_n,:])            dW[v,:] = round(scale sum over n with t_n = v, v != padding, of dout[n,:])
 //
-// The gradient sorts the tokens' positions by token (stable, digits of at most nine bits from the lowest), adds equal
+// The gradient of many tokens sorts the tokens' positions by token (stable, digits of at most nine bits from the lowest), adds equal
 // tokens' rows in 32 bits and writes every row of dW once.  The order of the additions depends on the tokens alone:
 // results repeat bit by bit.  Bound by memory: what is met of the table and `out` once; dout and dW once.
 #include <algorithm>
+#include <type_traits>
 
 #include "language.cuh"
 
@@ -17,30 +18,58 @@ struct LookupParams {
   void* out;
   Tokens tokens;
   long long vocab, weight_stride;
-  unsigned pieces;                  // of a row
-  unsigned long long total;         // pieces of all rows
+  unsigned n, pieces, group;        // tokens; pieces of a row; threads side by side in a row, a power of two up to 32
   float scale;
   int* mailbox;
 };
 
-template <typename T, int VEC>
+// A thread has four pieces on their way, COLS of them in a row: no divisions, which at 16 bytes a piece would take longer than
+// the memory.
+constexpr int kLookups = 4;
+
+template <typename T, int VEC, int COLS>
 __global__ void __launch_bounds__(256) lookup_kernel(const __grid_constant__ LookupParams p) {
   using V = Pack<T, VEC>;
-  const unsigned long long i = (unsigned long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= p.total) return;
-  const unsigned row = (unsigned)(i / p.pieces), c = (unsigned)(i - (unsigned long long)row * p.pieces);
-  const long long t = p.tokens(row);
-  V v;
-  if (t >= 0 && t < p.vocab) {
-    v = *reinterpret_cast<const V*>(static_cast<const T*>(p.weight) + t * p.weight_stride + (long long)c * VEC);
+  constexpr int R = kLookups / COLS;
+  const unsigned row0 = (blockIdx.x * 256 + threadIdx.x) / p.group * R, c0 = blockIdx.y * (p.group * COLS) + threadIdx.x % p.group;
+  long long t[R];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v.v[k] = Elem<T>::from_f(Elem<T>::to_f(v.v[k]) * p.scale);
-  } else {
+  for (int r = 0; r < R; ++r) t[r] = row0 + r < p.n ? p.tokens(row0 + r) : -1;
+  V v[R][COLS];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v.v[k] = Elem<T>::from_f(__int_as_float(0x7fffffff));
-    if (c == 0) report_token(p.mailbox, row, t);
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < COLS; ++j)
+      if (t[r] >= 0 && t[r] < p.vocab && c0 + j * p.group < p.pieces)
+        v[r][j] = reinterpret_cast<const V*>(static_cast<const T*>(p.weight) + t[r] * p.weight_stride)[c0 + j * p.group];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (row0 + r >= p.n) return;
+    const bool in = t[r] >= 0 && t[r] < p.vocab;
+    V* out = static_cast<V*>(p.out) + (size_t)(row0 + r) * p.pieces;
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) {
+      const unsigned c = c0 + j * p.group;
+      if (c >= p.pieces) break;
+      if (!in) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[r][j].v[k] = Elem<T>::from_f(__int_as_float(0x7fffffff));
+      } else if (p.scale != 1.f) {
+        if constexpr (VEC == kPer<T>) {
+          float z[VEC];
+          unpack(*reinterpret_cast<const uint4*>(&v[r][j]), z, T{});
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) z[k] *= p.scale;
+          *reinterpret_cast<uint4*>(&v[r][j]) = pack(z, T{});
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v[r][j].v[k] = Elem<T>::from_f(Elem<T>::to_f(v[r][j].v[k]) * p.scale);
+        }
+      }
+      out[c] = v[r][j];
+    }
+    if (!in && c0 == 0) report_token(p.mailbox, row0 + r, t[r]);
   }
-  static_cast<V*>(p.out)[i] = v;
 }
 
 // ---------------------------------------------------------------- sorting positions by token
@@ -54,7 +83,25 @@ struct SortParams {
   const unsigned *keys_in, *pos_in; // pos_in null: the position itself
   unsigned *keys, *pos;
   unsigned* counts;                 // [passes][tiles][bins]
+  char* zero;                       // what the blocks behind the tiles clear in this launch, and how much of it each
+  unsigned long long zero_bytes, zero_each;
+  int element;
 };
+
+// The sort is a chain of short kernels that keep few SMs busy; the others clear dW meanwhile, a part of it in each launch.
+// (Looking up which rows no token names, to clear those alone, took 10 us at 16384 tokens and came after the sort.)
+__device__ __forceinline__ void clear(const SortParams& p) {
+  const unsigned long long begin = (blockIdx.x - p.tiles) * p.zero_each, end = min(p.zero_bytes, begin + p.zero_each);
+  if ((reinterpret_cast<uintptr_t>(p.zero) & 15) == 0) {
+    const unsigned long long whole = end & ~15ull;
+    for (unsigned long long i = begin + threadIdx.x * 16; i < whole; i += kSortThreads * 16) *reinterpret_cast<uint4*>(p.zero + i) = make_uint4(0, 0, 0, 0);
+    for (unsigned long long i = max(begin, whole) + threadIdx.x; i < end; i += kSortThreads) p.zero[i] = 0;
+  } else if (p.element == 4) {
+    for (unsigned long long i = begin + threadIdx.x * 4; i < end; i += kSortThreads * 4) *reinterpret_cast<unsigned*>(p.zero + i) = 0;
+  } else {
+    for (unsigned long long i = begin + threadIdx.x * 2; i < end; i += kSortThreads * 2) *reinterpret_cast<unsigned short*>(p.zero + i) = 0;
+  }
+}
 
 // A token's sort key: itself, or the vocabulary's size (behind all of them) where it gets no gradient.
 __device__ __forceinline__ unsigned sort_key(const SortParams& p, unsigned i) {
@@ -67,6 +114,7 @@ template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_constant__ SortParams p) {
   __shared__ unsigned hist[kMaxBins];
   const unsigned bins = 1u << p.bits, tile = blockIdx.x;
+  if (tile >= p.tiles) return clear(p);
   for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
 #pragma unroll
@@ -90,11 +138,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_c
 // the tiles they have come to.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid_constant__ SortParams p) {
-  __shared__ unsigned hist[kSortWarps][kMaxBins];
+  __shared__ unsigned short hist[kSortWarps][kMaxBins];    // of a tile, whose numbers 16 bits hold
+  __shared__ unsigned base[kMaxBins];
   __shared__ unsigned sums[kSortWarps];
   const unsigned bins = 1u << p.bits, tile = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = p.pass * p.bits;
-  for (unsigned b = tid; b < kSortWarps * kMaxBins; b += kSortThreads) (&hist[0][0])[b] = 0;
+  if (tile >= p.tiles) return clear(p);
+  for (unsigned b = tid; b < kSortWarps * kMaxBins / 2; b += kSortThreads) reinterpret_cast<unsigned*>(hist)[b] = 0;
   __syncthreads();
 
   unsigned key[ITEMS], rank[ITEMS];
@@ -109,21 +159,32 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
     const unsigned below = __popc(peers & ((1u << lane) - 1));
     rank[j] = in ? hist[warp][d] + below : 0;
     __syncwarp();
-    if (in && below == 0) hist[warp][d] += __popc(peers);
+    if (in && below == 0) hist[warp][d] += (unsigned short)__popc(peers);
     __syncwarp();
   }
 
-  // counts of this digit before this tile, and in all of them
-  unsigned before = 0, total = 0;
-  if (tid < bins) {
-    const unsigned* c = p.counts + (size_t)p.pass * p.tiles * bins + tid;
+  // counts of this digit before this tile, and in all of them: a thread takes four digits of every fourth to sixty-fourth tile
+  __shared__ uint4 sum_before[kSortThreads], sum_total[kSortThreads];
+  {
+    const unsigned quads = bins / 4, lanes = kSortThreads / quads, q = tid % quads;
+    const uint4* c = reinterpret_cast<const uint4*>(p.counts + (size_t)p.pass * p.tiles * bins) + q;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
 #pragma unroll 8
-    for (unsigned t = 0; t < p.tiles; ++t) {
-      const unsigned v = c[(size_t)t * bins];
-      total += v;
-      before += t < tile ? v : 0;
+    for (unsigned t = tid / quads; t < p.tiles; t += lanes) {
+      const uint4 v = c[(size_t)t * quads];
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+      if (t < tile) { b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w; }
     }
+    sum_total[tid] = a;
+    sum_before[tid] = b;
   }
+  __syncthreads();
+  unsigned before = 0, total = 0;
+  if (tid < bins)
+    for (unsigned l = 0; l < kSortThreads * 4 / bins; ++l) {
+      total += reinterpret_cast<const unsigned*>(sum_total)[l * bins + tid];
+      before += reinterpret_cast<const unsigned*>(sum_before)[l * bins + tid];
+    }
   unsigned scan = total;                       // inclusive over the digits
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -135,10 +196,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
   if (tid < bins) {
     unsigned at = scan - total + before;
     for (unsigned w = 0; w < warp; ++w) at += sums[w];
+    base[tid] = at;
+    unsigned short in_tile = 0;
+#pragma unroll
     for (int w = 0; w < kSortWarps; ++w) {     // where every warp's elements of this digit begin
-      const unsigned v = hist[w][tid];
-      hist[w][tid] = at;
-      at += v;
+      const unsigned short v = hist[w][tid];
+      hist[w][tid] = in_tile;
+      in_tile += v;
     }
   }
   __syncthreads();
@@ -148,7 +212,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
   for (int j = 0; j < ITEMS; ++j) {
     const unsigned i = first + j * 32;
     if (i >= p.n) continue;
-    const unsigned to = hist[warp][(key[j] >> shift) & (bins - 1)] + rank[j];
+    const unsigned d = (key[j] >> shift) & (bins - 1), to = base[d] + hist[warp][d] + rank[j];
     p.keys[to] = key[j];
     p.pos[to] = p.pos_in ? p.pos_in[i] : i;
     if (more) atomicAdd(&next[(size_t)(to / (ITEMS * kSortThreads)) * bins + ((key[j] >> (shift + p.bits)) & (bins - 1))], 1u);
@@ -156,15 +220,19 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
 }
 
 // ---------------------------------------------------------------- sums of equal tokens' rows
-constexpr int kRun = 32;             // sorted positions that one group of threads adds up
+constexpr int kRunStep = 8;          // rows on their way at a time
+constexpr int kMaxRun = 32;          // sorted positions that one group of threads adds up
+constexpr int kZeroRows = 64;        // rows of dW that one block looks after
 
 struct SumParams {
   const void* dout;
   void* dweight;
   RowMap rows;
+  Tokens tokens;                     // (of the kernel for few tokens)
+  long long padding;
   const unsigned *keys, *pos;
   float* part;                       // [runs][2][width]: of a token that began in an earlier run, of one that goes on in the next
-  unsigned n, vocab, runs, sum_blocks;
+  unsigned n, vocab, run, runs;
   unsigned width, pieces, group;     // group: threads of a run, a power of two
   float scale;
 };
@@ -178,30 +246,34 @@ __device__ __forceinline__ unsigned lower_bound(const unsigned* keys, unsigned n
   return lo;
 }
 
-constexpr int kZeroRows = 64;        // rows of dW that one block looks after
+// Zeros into those of the rows v0 .. v0 + rows - 1 of dW that are not `met`.
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_rows(const SumParams& p, unsigned v0, unsigned rows, const unsigned* met) {
+  using V = Pack<T, VEC>;
+  V z;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) z.v[k] = Elem<T>::from_f(0.f);
+  for (unsigned v = threadIdx.x / 32; v < rows; v += 8) {
+    if (met[v]) continue;
+    V* d = static_cast<V*>(p.dweight) + (size_t)(v0 + v) * p.pieces;
+    for (unsigned i = threadIdx.x % 32; i < p.pieces; i += 32) d[i] = z;
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void put_sum(const SumParams& p, unsigned t, unsigned c, const float (&acc)[VEC]) {
+  Pack<T, VEC> r;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) r.v[k] = Elem<T>::from_f(acc[k] * p.scale);
+  static_cast<Pack<T, VEC>*>(p.dweight)[(size_t)t * p.pieces + c] = r;
+}
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumParams p) {
   using V = Pack<T, VEC>;
-  __shared__ unsigned s_key[256 / 4 * kRun], s_pos[256 / 4 * kRun];
-  if (blockIdx.x >= p.sum_blocks) {            // rows that no token names
-    if (blockIdx.y) return;
-    const unsigned v0 = (blockIdx.x - p.sum_blocks) * kZeroRows, rows = min((unsigned)kZeroRows, p.vocab - v0);
-    if (threadIdx.x < rows) {
-      const unsigned at = lower_bound(p.keys, p.n, v0 + threadIdx.x);
-      s_key[threadIdx.x] = at < p.n && p.keys[at] == v0 + threadIdx.x;
-    }
-    __syncthreads();
-    V z;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) z.v[k] = Elem<T>::from_f(0.f);
-    V* d = static_cast<V*>(p.dweight) + (size_t)v0 * p.pieces;
-    for (unsigned i = threadIdx.x; i < rows * p.pieces; i += 256)
-      if (!s_key[i / p.pieces]) d[i] = z;
-    return;
-  }
-  const unsigned runs_here = 256 / p.group, first = blockIdx.x * runs_here * kRun;
-  for (unsigned i = threadIdx.x; i < runs_here * kRun; i += 256) {
+  __shared__ unsigned s_key[256 / 4 * kMaxRun], s_pos[256 / 4 * kMaxRun];
+  const unsigned runs_here = 256 / p.group, first = blockIdx.x * runs_here * p.run;
+  for (unsigned i = threadIdx.x; i < runs_here * p.run; i += 256) {
     s_key[i] = first + i < p.n ? p.keys[first + i] : p.vocab;
     s_pos[i] = first + i < p.n ? p.pos[first + i] : 0;
   }
@@ -209,69 +281,201 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumPar
   const unsigned mine = threadIdx.x / p.group, run = blockIdx.x * runs_here + mine;
   const unsigned c = blockIdx.y * 256 + threadIdx.x % p.group;
   if (c >= p.pieces || run >= p.runs) return;
-  const unsigned* key = s_key + mine * kRun;
-  const unsigned* pos = s_pos + mine * kRun;
-  const unsigned i0 = run * kRun;
-  const unsigned before = i0 ? p.keys[i0 - 1] : p.vocab, after = i0 + kRun < p.n ? p.keys[i0 + kRun] : p.vocab;
+  const unsigned* key = s_key + mine * p.run;
+  const unsigned* pos = s_pos + mine * p.run;
+  const unsigned i0 = run * p.run;
+  const unsigned before = i0 ? p.keys[i0 - 1] : p.vocab, after = i0 + p.run < p.n ? p.keys[i0 + p.run] : p.vocab;
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-  for (int j = 0; j < kRun; ++j) {
-    const unsigned t = key[j];
-    if (t == p.vocab) break;
-    const V v = *reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(pos[j]) + (size_t)c * VEC);
+  for (unsigned j0 = 0; j0 < p.run && key[j0] != p.vocab; j0 += kRunStep) {
+    V v[kRunStep];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += Elem<T>::to_f(v.v[k]);
-    const unsigned then = j + 1 < kRun ? key[j + 1] : after;
-    if (then == t && j + 1 < kRun) continue;
-    const bool began_before = t == before;
-    if (began_before || then == t) {           // a part of a token's sum
-      float* q = p.part + ((size_t)run * 2 + (began_before ? 0 : 1)) * p.width + (size_t)c * VEC;
+    for (int u = 0; u < kRunStep; ++u)
+      if (key[j0 + u] != p.vocab) v[u] = *reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(pos[j0 + u]) + (size_t)c * VEC);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) q[k] = acc[k];
-    } else {
-      V r;
+    for (int u = 0; u < kRunStep; ++u) {
+      const unsigned j = j0 + u, t = key[j];
+      if (t == p.vocab) break;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) r.v[k] = Elem<T>::from_f(acc[k] * p.scale);
-      static_cast<V*>(p.dweight)[(size_t)t * p.pieces + c] = r;
+      for (int k = 0; k < VEC; ++k) acc[k] += Elem<T>::to_f(v[u].v[k]);
+      const unsigned then = j + 1 < p.run ? key[j + 1] : after;
+      if (then == t && j + 1 < p.run) continue;
+      const bool began_before = t == before;
+      if (began_before || then == t) {         // a part of a token's sum
+        Pack<float, VEC % 4 ? VEC : 4>* q = reinterpret_cast<Pack<float, VEC % 4 ? VEC : 4>*>(p.part + ((size_t)run * 2 + (began_before ? 0 : 1)) * p.width + (size_t)c * VEC);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) q[k / 4].v[k % 4] = acc[k];
+      } else {
+        put_sum<T, VEC>(p, t, c, acc);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
     }
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   }
 }
 
-// Tokens whose positions reach over several runs: the parts in order.
+// Tokens whose positions reach over several runs.  A block looks after 32 runs and 128 columns: of the tokens that begin in
+// these runs and go on a warp adds up the parts of one; where there are many parts all warps do, each every eighth of them.
+constexpr unsigned kLong = 64;
+
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumParams p) {
-  const unsigned run = blockIdx.x, i0 = run * kRun, i1 = i0 + kRun;
-  if (i1 >= p.n) return;
-  const unsigned t = p.keys[i1 - 1];
-  if (t == p.vocab || p.keys[i1] != t || (i0 && p.keys[i0 - 1] == t)) return;
-  const unsigned last = (lower_bound(p.keys, p.n, t + 1) - 1) / kRun;
-  for (unsigned c = blockIdx.y * 256 + threadIdx.x; c < p.width; c += gridDim.y * 256) {
-    float acc = p.part[((size_t)run * 2 + 1) * p.width + c];
-    for (unsigned r = run + 1; r <= last; ++r) acc += p.part[(size_t)r * 2 * p.width + c];
-    static_cast<T*>(p.dweight)[(size_t)t * p.width + c] = Elem<T>::from_f(acc * p.scale);
+  __shared__ float s_sum[8][128];
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned mine = blockIdx.x * 32 + lane, end = (mine + 1) * p.run;         // (every warp looks at all 32)
+  unsigned t = p.vocab, parts = 0;
+  if (end < p.n) {
+    t = p.keys[end - 1];
+    if (t != p.vocab && p.keys[end] == t && !(mine && p.keys[end - p.run - 1] == t)) parts = (lower_bound(p.keys, p.n, t + 1) - 1) / p.run - mine + 1;
+  }
+  const unsigned c0 = blockIdx.y * 128 + lane;
+  auto add = [&](unsigned run, unsigned from, unsigned parts, unsigned step, float (&acc)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = 0.f;
+#pragma unroll 4
+    for (unsigned r = from; r < parts; r += step) {
+      const float* q = p.part + ((size_t)(run + r) * 2 + (r == 0)) * p.width + c0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (c0 + k * 32 < p.width) acc[k] += q[k * 32];
+    }
+  };
+  auto put = [&](unsigned t, const float (&acc)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + k * 32 < p.width) static_cast<T*>(p.dweight)[(size_t)t * p.width + c0 + k * 32] = Elem<T>::from_f(acc[k] * p.scale);
+  };
+  const unsigned some = __ballot_sync(~0u, parts > 0), many = __ballot_sync(~0u, parts > kLong);
+  float acc[4];
+  unsigned turn = 0;
+  for (unsigned left = some & ~many; left; left &= left - 1, ++turn) {
+    const unsigned l = __ffs(left) - 1, of = __shfl_sync(~0u, parts, l), token = __shfl_sync(~0u, t, l);
+    if (turn % 8 != warp) continue;
+    add(blockIdx.x * 32 + l, 0, of, 1, acc);
+    put(token, acc);
+  }
+  for (unsigned left = many; left; left &= left - 1) {
+    const unsigned l = __ffs(left) - 1, of = __shfl_sync(~0u, parts, l), token = __shfl_sync(~0u, t, l);
+    add(blockIdx.x * 32 + l, warp, of, 8, acc);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s_sum[warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < 8; ++w)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += s_sum[w][k * 32 + lane];
+      put(token, acc);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- few tokens: one launch, nothing sorted
+// A block has a position: it looks for its token among all of them and, where it is the first that names it, adds the rows
+// up, several groups of threads in turn and then the groups in order.  Other blocks write the rows that no token names.
+constexpr int kFew = 2048;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) few_kernel(const __grid_constant__ SumParams p) {
+  using V = Pack<T, VEC>;
+  __shared__ unsigned s_met[kZeroRows];
+  __shared__ unsigned s_bits[kFew / 32];
+  __shared__ unsigned short s_list[kFew];
+  __shared__ float s_sum[256 * VEC];
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (blockIdx.x >= p.n) {
+    const unsigned v0 = (blockIdx.x - p.n) * kZeroRows, rows = min((unsigned)kZeroRows, p.vocab - v0);
+    if (tid < kZeroRows) s_met[tid] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (unsigned i = tid; i < p.n; i += 256) {
+      const long long t = p.tokens(i);
+      if (t >= v0 && t < v0 + rows && t != p.padding) s_met[t - v0] = 1;
+    }
+    __syncthreads();
+    zero_rows<T, VEC>(p, v0, rows, s_met);
+    return;
+  }
+  const long long t = p.tokens(blockIdx.x);
+  if (t < 0 || t >= p.vocab || t == p.padding) return;
+  bool earlier = false;
+  const unsigned words = (p.n + 31) / 32;
+#pragma unroll 8
+  for (unsigned w = warp; w < words; w += 8) {
+    const unsigned i = w * 32 + lane;
+    const bool same = i < p.n && p.tokens(i) == t;
+    earlier |= same && i < blockIdx.x;
+    const unsigned bits = __ballot_sync(~0u, same);
+    if (lane == 0) s_bits[w] = bits;
+  }
+  if (__syncthreads_or(earlier)) return;
+  // the positions in order: a word's begin behind those of the words before it
+  for (unsigned w = warp; w < words; w += 8) {
+    const unsigned bits = s_bits[w];
+    if (bits == 0) continue;
+    unsigned at = 0;
+    for (unsigned q = lane; q < w; q += 32) at += __popc(s_bits[q]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) at += __shfl_xor_sync(~0u, at, o);
+    if (bits >> lane & 1) s_list[at + __popc(bits & ((1u << lane) - 1))] = (unsigned short)(w * 32 + lane);
+  }
+  unsigned count = 0;
+  for (unsigned w = lane; w < words; w += 32) count += __popc(s_bits[w]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(~0u, count, o);
+  __syncthreads();
+  const unsigned groups = count == 1 ? 1 : 256 / p.group, width = 256 / groups;    // threads of a group
+  const unsigned g = tid / width, x = tid % width;
+  for (unsigned c0 = 0; c0 < p.pieces; c0 += width) {
+    const unsigned c = c0 + x;
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    if (c < p.pieces) {
+#pragma unroll 4
+      for (unsigned j = g; j < count; j += groups) {
+        const V v = *reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(s_list[j]) + (size_t)c * VEC);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += Elem<T>::to_f(v.v[k]);
+      }
+    }
+    if (groups > 1) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s_sum[k * 256 + tid] = acc[k];
+      __syncthreads();
+      if (g == 0)
+        for (unsigned q = 1; q < groups; ++q)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += s_sum[k * 256 + q * width + x];
+      __syncthreads();
+    }
+    if (g == 0 && c < p.pieces) put_sum<T, VEC>(p, (unsigned)t, c, acc);
   }
 }
 
 // ---------------------------------------------------------------- workspace
 struct GradPlan {
   int items, passes, bits;
-  unsigned tiles, runs;
+  unsigned tiles, run, runs;
   size_t keys[2], pos[2], counts, part, total;
 };
 
 static GradPlan grad_plan(int64_t n, int64_t vocab, int64_t width) {
-  GradPlan g;
+  GradPlan g{};
+  if (n <= kFew) {
+    g.total = 0;
+    return g;
+  }
   // tiles of 2048 keep many SMs busy; larger ones where the counts of all tiles, which every block adds up, would get long
-  g.items = n <= 65536 ? 4 : 16;
+  g.items = n <= 262144 ? 4 : 16;
   g.tiles = (unsigned)((n + g.items * kSortThreads - 1) / (g.items * kSortThreads));
   int bits = 1;
   while (bits < 32 && (vocab >> bits) != 0) ++bits;       // keys go up to `vocab` itself
   g.passes = (bits + 8) / 9;
-  g.bits = (bits + g.passes - 1) / g.passes;
-  g.runs = (unsigned)((n + kRun - 1) / kRun);
+  g.bits = std::max(2, (bits + g.passes - 1) / g.passes);
+  // runs of eight positions where there are few, so that many are on their way; long ones leave fewer parts to join
+  g.run = n <= 32768 ? kRunStep : kMaxRun;
+  g.runs = (unsigned)((n + g.run - 1) / g.run);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t o = at; at = round_up(at + bytes, 256); return o; };
   for (int k = 0; k < 2; ++k) { g.keys[k] = take(4 * n); g.pos[k] = take(4 * n); }
@@ -288,7 +492,7 @@ static int check_embed(const blstm_embed_desc* d) {
   return BLSTM_OK;
 }
 
-static Tokens make_tokens(const blstm_embed_desc& d, const void* tokens) { return {tokens, row_map(d.n1, d.token_stride), d.token_bits == 64}; }
+static Tokens make_tokens(const blstm_embed_desc& d, const void* tokens) { return {tokens, row_map(d.n0, d.n1, d.token_stride), d.token_bits == 64}; }
 
 }  // namespace blstm
 
@@ -305,15 +509,23 @@ int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* w
   const uintptr_t bits = reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out) | (uintptr_t)(d->width * e) | (uintptr_t)(d->row_stride[0] * e);
   if (bits % e) return BLSTM_E_INVALID_ARG;
   const int piece = piece_bytes(bits, e);
-  LookupParams p{weight, out, make_tokens(*d, tokens), d->vocab, d->row_stride[0], (unsigned)(d->width * e / piece), 0, d->scale, current_mailbox()};
-  p.total = (unsigned long long)n * p.pieces;
-  const unsigned long long grid = (p.total + 255) / 256;
-  if (grid > INT32_MAX) return BLSTM_E_TOO_LARGE;
+  LookupParams p{weight, out, make_tokens(*d, tokens), d->vocab, d->row_stride[0], (unsigned)n, (unsigned)(d->width * e / piece), 1, d->scale,
+                 current_mailbox()};
+  while (p.group < 32 && p.group < p.pieces) p.group *= 2;
+  const int cols = p.pieces > 64 ? 4 : p.pieces > 32 ? 2 : 1, rows = 256 / (int)p.group * (kLookups / cols);   // of a block
+  const dim3 grid((unsigned)((n + rows - 1) / rows), (p.pieces + p.group * cols - 1) / (p.group * cols));
+  if (grid.y > 65535) return BLSTM_E_TOO_LARGE;
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (piece == 16) lookup_kernel<T, 16 / sizeof(T)><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(p);
-    else if (piece == 4) lookup_kernel<T, 4 / sizeof(T)><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(p);
-    else lookup_kernel<T, 1><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(p);
+    auto launch = [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      if (cols == 4) lookup_kernel<T, V, 4><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+      else if (cols == 2) lookup_kernel<T, V, 2><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+      else lookup_kernel<T, V, 1><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+    };
+    if (piece == 16) launch(std::integral_constant<int, 16 / sizeof(T)>{});
+    else if (piece == 4) launch(std::integral_constant<int, 4 / sizeof(T)>{});
+    else launch(std::integral_constant<int, 1>{});
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
@@ -322,7 +534,7 @@ int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* w
 
 size_t blstm_embedding_grad_workspace(const blstm_embed_desc* d) {
   if (check_embed(d)) return 0;
-  return round_up(grad_plan(d->n0 * d->n1, d->vocab, d->width).total + 256, 256);
+  return grad_plan(d->n0 * d->n1, d->vocab, d->width).total;
 }
 
 int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const void* dout, void* dweight, void* workspace,
@@ -337,53 +549,80 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
     return BLSTM_OK;
   }
   if (!tokens || !dout) return BLSTM_E_INVALID_ARG;
-  const GradPlan g = grad_plan(n, d->vocab, d->width);
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < g.total) return BLSTM_E_WORKSPACE;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dweight) | (uintptr_t)(d->width * e) |
                          (uintptr_t)(d->row_stride[0] * e) | (uintptr_t)(d->row_stride[1] * e);
   if (bits % e) return BLSTM_E_INVALID_ARG;
+  const GradPlan g = grad_plan(n, d->vocab, d->width);
+  if (g.total && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < g.total)) return BLSTM_E_WORKSPACE;
+  const int piece = piece_bytes(bits, e);
+  SumParams p{};
+  p.dout = dout; p.dweight = dweight;
+  p.rows = row_map(d->n0, d->n1, d->row_stride);
+  p.tokens = make_tokens(*d, tokens); p.padding = d->padding;
+  p.n = (unsigned)n; p.vocab = (unsigned)d->vocab;
+  p.width = (unsigned)d->width; p.pieces = (unsigned)(d->width * e / piece);
+  p.group = 4;
+  while (p.group < 256 && p.group < p.pieces) p.group *= 2;
+  p.scale = d->scale;
+  const unsigned zero_blocks = (p.vocab + kZeroRows - 1) / kZeroRows;
+  if (n <= kFew) {
+    p.group = std::min(p.group, 64u);                    // four groups at least, for tokens that come often
+    return with_type(d->dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      if (piece == 16) few_kernel<T, 16 / sizeof(T)><<<p.n + zero_blocks, 256, 0, st>>>(p);
+      else if (piece == 4) few_kernel<T, 4 / sizeof(T)><<<p.n + zero_blocks, 256, 0, st>>>(p);
+      else few_kernel<T, 1><<<p.n + zero_blocks, 256, 0, st>>>(p);
+      BLSTM_CUDA_OK(cudaGetLastError());
+      count_launch();
+      return BLSTM_OK;
+    });
+  }
+
   char* ws = static_cast<char*>(workspace);
   auto at = [&](size_t o) { return reinterpret_cast<unsigned*>(ws + o); };
-
   SortParams s{};
-  s.tokens = make_tokens(*d, tokens);
+  s.tokens = p.tokens;
   s.vocab = d->vocab; s.padding = d->padding;
   s.n = (unsigned)n; s.tiles = g.tiles;
   s.passes = g.passes; s.bits = g.bits;
   s.keys = at(g.keys[0]); s.counts = at(g.counts);
-  if (g.items == 4) sort_count_kernel<4><<<g.tiles, kSortThreads, 0, st>>>(s);
-  else sort_count_kernel<16><<<g.tiles, kSortThreads, 0, st>>>(s);
+  // a third or so of dW in each launch, 64 KB a block
+  const unsigned long long all = (unsigned long long)d->vocab * d->width * e;
+  const unsigned long long part = ((all + g.passes) / (g.passes + 1) + 15) & ~15ull;
+  s.zero_each = 65536;
+  s.element = e;
+  auto blocks = [&](int launch) {
+    const unsigned long long begin = std::min(all, part * launch), end = std::min(all, begin + part);
+    s.zero = static_cast<char*>(dweight) + begin;
+    s.zero_bytes = end - begin;
+    return (unsigned)(g.tiles + (s.zero_bytes + s.zero_each - 1) / s.zero_each);
+  };
+  unsigned grid = blocks(0);
+  if (g.items == 4) sort_count_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
+  else sort_count_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
   BLSTM_CUDA_OK(cudaGetLastError());
   for (s.pass = 0; s.pass < g.passes; ++s.pass) {
     const int from = s.pass & 1;
     s.keys_in = at(g.keys[from]); s.pos_in = s.pass ? at(g.pos[from]) : nullptr;
     s.keys = at(g.keys[1 - from]); s.pos = at(g.pos[1 - from]);
-    if (g.items == 4) sort_scatter_kernel<4><<<g.tiles, kSortThreads, 0, st>>>(s);
-    else sort_scatter_kernel<16><<<g.tiles, kSortThreads, 0, st>>>(s);
+    grid = blocks(1 + s.pass);
+    if (g.items == 4) sort_scatter_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
+    else sort_scatter_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
     BLSTM_CUDA_OK(cudaGetLastError());
   }
 
-  const int piece = piece_bytes(bits, e);
-  SumParams p{};
-  p.dout = dout; p.dweight = dweight;
-  p.rows = row_map(d->n1, d->row_stride);
   p.keys = s.keys; p.pos = s.pos;
   p.part = reinterpret_cast<float*>(ws + g.part);
-  p.n = (unsigned)n; p.vocab = (unsigned)d->vocab; p.runs = g.runs;
-  p.width = (unsigned)d->width; p.pieces = (unsigned)(d->width * e / piece);
-  p.group = 4;
-  while (p.group < 256 && p.group < p.pieces) p.group *= 2;
-  p.scale = d->scale;
-  p.sum_blocks = (g.runs + 256 / p.group - 1) / (256 / p.group);
-  const dim3 grid(p.sum_blocks + (p.vocab + kZeroRows - 1) / kZeroRows, (p.pieces + 255) / 256);
-  if (grid.y > 65535) return BLSTM_E_TOO_LARGE;
+  p.run = g.run; p.runs = g.runs;
+  const dim3 sums((g.runs + 256 / p.group - 1) / (256 / p.group), (p.pieces + 255) / 256), joins((g.runs + 31) / 32, (p.width + 127) / 128);
+  if (sums.y > 65535 || joins.y > 65535) return BLSTM_E_TOO_LARGE;
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (piece == 16) sum_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(p);
-    else if (piece == 4) sum_kernel<T, 4 / sizeof(T)><<<grid, 256, 0, st>>>(p);
-    else sum_kernel<T, 1><<<grid, 256, 0, st>>>(p);
+    if (piece == 16) sum_kernel<T, 16 / sizeof(T)><<<sums, 256, 0, st>>>(p);
+    else if (piece == 4) sum_kernel<T, 4 / sizeof(T)><<<sums, 256, 0, st>>>(p);
+    else sum_kernel<T, 1><<<sums, 256, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
-    join_kernel<T><<<dim3(g.runs, std::min((p.width + 255) / 256, 64u)), 256, 0, st>>>(p);
+    join_kernel<T><<<joins, 256, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch(3 + g.passes);
     return BLSTM_OK;

@@ -95,8 +95,10 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
     Call call(dout.device());
     const auto opt = dout.options().requires_grad(false);
     const Tensor dW = at::empty({sizes[0], sizes[1]}, opt);
-    const Tensor ws = at::empty({(int64_t)blstm_embedding_grad_workspace(&d)}, opt.dtype(at::kByte));
-    check(blstm_embedding_grad(&d, ptr(tokens), ptr(dout), dW.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), call.stream), "embedding gradient");
+    const size_t bytes = blstm_embedding_grad_workspace(&d);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, opt.dtype(at::kByte));
+    check(blstm_embedding_grad(&d, ptr(tokens), ptr(dout), dW.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, call.stream), "embedding gradient");
     return {dW, Tensor(), Tensor(), Tensor()};
   }
 };

@@ -11,11 +11,16 @@ struct RowMap {
   long long s0, s1;
   unsigned n1;
   __device__ __forceinline__ long long operator()(unsigned r) const {
+    if (r < n1) return r * s1;
     const unsigned i0 = r / n1;
     return i0 * s0 + (r - i0 * n1) * s1;
   }
 };
-inline RowMap row_map(int64_t n1, const int64_t stride[2]) { return {(long long)stride[0], (long long)stride[1], (unsigned)n1}; }
+// (rows that one stride describes are one dimension, without a division)
+inline RowMap row_map(int64_t n0, int64_t n1, const int64_t stride[2]) {
+  if (stride[0] == n1 * stride[1]) n1 *= n0;
+  return {(long long)stride[0], (long long)stride[1], (unsigned)n1};
+}
 
 struct Tokens {
   const void* p;

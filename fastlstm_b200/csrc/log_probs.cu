@@ -571,8 +571,8 @@ static int check_score(const blstm_score_desc* d, const void* logits, const void
 static ScoreParams score_params(const blstm_score_desc& d, const void* logits, const void* tokens) {
   ScoreParams p{};
   p.logits = logits;
-  p.rows = row_map(d.n1, d.logits_stride);
-  p.tokens = {tokens, row_map(d.n1, d.token_stride), d.token_bits == 64};
+  p.rows = row_map(d.n0, d.n1, d.logits_stride);
+  p.tokens = {tokens, row_map(d.n0, d.n1, d.token_stride), d.token_bits == 64};
   p.ignore = d.ignore;
   p.n = (unsigned)(d.n0 * d.n1); p.vocab = (unsigned)d.vocab; p.top = d.top;
   p.per_temperature = (float)(1.0 / d.temperature);
@@ -650,12 +650,12 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
     return BLSTM_E_INVALID_ARG;
   ScoreParams p = score_params(*d, logits, tokens);
   p.dlogits = dlogits;
-  p.drows = row_map(d->n1, dlogits_stride);
+  p.drows = row_map(d->n0, d->n1, dlogits_stride);
   p.stats = const_cast<float*>(stats);
   p.top_tokens = reinterpret_cast<long long*>(const_cast<int64_t*>(top_tokens));
   p.g_lp = g_log_probs; p.g_h = g_entropy; p.g_top = g_top;
-  if (g_log_probs) p.g_lp_map = row_map(d->n1, g_log_probs_stride);
-  if (g_entropy) p.g_h_map = row_map(d->n1, g_entropy_stride);
+  if (g_log_probs) p.g_lp_map = row_map(d->n0, d->n1, g_log_probs_stride);
+  if (g_entropy) p.g_h_map = row_map(d->n0, d->n1, g_entropy_stride);
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;

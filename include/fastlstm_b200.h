@@ -269,7 +269,8 @@ typedef struct blstm_embed_desc {
 int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* weight, void* out, void* stream);
 
 /* dweight[vocab, width] (dense, every row is written) = round(scale * sum of dout's rows of that token): added in
- * 32 bits in an order that the tokens alone fix, rounded once.  The workspace is 256-byte aligned. */
+ * 32 bits in an order that the tokens alone fix, rounded once.  The workspace is 256-byte aligned; few tokens need none
+ * (0 bytes, NULL). */
 size_t blstm_embedding_grad_workspace(const blstm_embed_desc* d);
 int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const void* dout, void* dweight,
                          void* workspace, size_t workspace_bytes, void* stream);

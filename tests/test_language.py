@@ -87,6 +87,8 @@ def test_embedding_pointers_refused():
     d = _desc(_lib.EmbedDesc, **EMBED)
     for a in ((None, PTR, PTR), (PTR, None, PTR), (PTR, PTR, None), (PTR, PTR + 1, PTR), (PTR, PTR, PTR + 1)):
         assert lib.blstm_embedding(d, *a, None) == 1
+    assert lib.blstm_embedding_grad_workspace(d) == 0            # (few tokens)
+    d.n1 = 100000
     need = lib.blstm_embedding_grad_workspace(d)
     assert need > 0 and need % 256 == 0
     for a in ((None, PTR, PTR), (PTR, None, PTR), (PTR, PTR, None), (PTR, PTR + 1, PTR)):
