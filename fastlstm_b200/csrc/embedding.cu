@@ -237,15 +237,6 @@ struct SumParams {
   float scale;
 };
 
-__device__ __forceinline__ unsigned lower_bound(const unsigned* keys, unsigned n, unsigned v) {
-  unsigned lo = 0, hi = n;
-  while (lo < hi) {
-    const unsigned mid = (lo + hi) >> 1;
-    if (keys[mid] < v) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 // Zeros into those of the rows v0 .. v0 + rows - 1 of dW that are not `met`.
 template <typename T, int VEC>
 __device__ __forceinline__ void zero_rows(const SumParams& p, unsigned v0, unsigned rows, const unsigned* met) {
@@ -315,25 +306,39 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumPar
   }
 }
 
-// Tokens whose positions reach over several runs.  A block looks after 32 runs and 128 columns: of the tokens that begin in
-// these runs and go on a warp adds up the parts of one; where there are many parts all warps do, each every eighth of them.
-constexpr unsigned kLong = 64;
+// Tokens whose positions reach over several runs.  A warp looks after a run, and 128 columns: where a token begins in it and
+// goes on, it adds the parts up; where there are more than a few the eight warps of the block do, each every eighth of them.
+constexpr unsigned kLong = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumParams p) {
   __shared__ float s_sum[8][128];
+  __shared__ unsigned s_parts[8], s_token[8];
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned mine = blockIdx.x * 32 + lane, end = (mine + 1) * p.run;         // (every warp looks at all 32)
+  const unsigned mine = blockIdx.x * 8 + warp, end = (mine + 1) * p.run;
   unsigned t = p.vocab, parts = 0;
   if (end < p.n) {
     t = p.keys[end - 1];
-    if (t != p.vocab && p.keys[end] == t && !(mine && p.keys[end - p.run - 1] == t)) parts = (lower_bound(p.keys, p.n, t + 1) - 1) / p.run - mine + 1;
+    if (t != p.vocab && p.keys[end] == t && !(mine && p.keys[end - p.run - 1] == t)) {
+      // the runs that it is in, 32 tried at a time, in larger steps as long as all of them are
+      unsigned last = 1, step = 1;
+      for (;;) {
+        const unsigned k = mine + last + (lane + 1) * step;
+        const unsigned hits = __popc(__ballot_sync(~0u, k < p.runs && p.keys[k * p.run] == t));
+        last += hits * step;
+        if (hits == 32 && step < 1024) step *= 32;
+        else if (hits < 32 && step == 1) break;
+        else if (hits < 32) step /= 32;
+      }
+      parts = last + 1;
+    }
   }
+  if (lane == 0) { s_parts[warp] = parts; s_token[warp] = t; }
   const unsigned c0 = blockIdx.y * 128 + lane;
   auto add = [&](unsigned run, unsigned from, unsigned parts, unsigned step, float (&acc)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (unsigned r = from; r < parts; r += step) {
       const float* q = p.part + ((size_t)(run + r) * 2 + (r == 0)) * p.width + c0;
 #pragma unroll
@@ -345,26 +350,23 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumPa
     for (int k = 0; k < 4; ++k)
       if (c0 + k * 32 < p.width) static_cast<T*>(p.dweight)[(size_t)t * p.width + c0 + k * 32] = Elem<T>::from_f(acc[k] * p.scale);
   };
-  const unsigned some = __ballot_sync(~0u, parts > 0), many = __ballot_sync(~0u, parts > kLong);
   float acc[4];
-  unsigned turn = 0;
-  for (unsigned left = some & ~many; left; left &= left - 1, ++turn) {
-    const unsigned l = __ffs(left) - 1, of = __shfl_sync(~0u, parts, l), token = __shfl_sync(~0u, t, l);
-    if (turn % 8 != warp) continue;
-    add(blockIdx.x * 32 + l, 0, of, 1, acc);
-    put(token, acc);
+  if (parts > 0 && parts <= kLong) {
+    add(mine, 0, parts, 1, acc);
+    put(t, acc);
   }
-  for (unsigned left = many; left; left &= left - 1) {
-    const unsigned l = __ffs(left) - 1, of = __shfl_sync(~0u, parts, l), token = __shfl_sync(~0u, t, l);
-    add(blockIdx.x * 32 + l, warp, of, 8, acc);
+  __syncthreads();
+  for (unsigned w = 0; w < 8; ++w) {
+    if (s_parts[w] <= kLong) continue;
+    add(blockIdx.x * 8 + w, warp, s_parts[w], 8, acc);
 #pragma unroll
     for (int k = 0; k < 4; ++k) s_sum[warp][k * 32 + lane] = acc[k];
     __syncthreads();
     if (warp == 0) {
-      for (int w = 1; w < 8; ++w)
+      for (int q = 1; q < 8; ++q)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += s_sum[w][k * 32 + lane];
-      put(token, acc);
+        for (int k = 0; k < 4; ++k) acc[k] += s_sum[q][k * 32 + lane];
+      put(s_token[w], acc);
     }
     __syncthreads();
   }
@@ -614,7 +616,7 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
   p.keys = s.keys; p.pos = s.pos;
   p.part = reinterpret_cast<float*>(ws + g.part);
   p.run = g.run; p.runs = g.runs;
-  const dim3 sums((g.runs + 256 / p.group - 1) / (256 / p.group), (p.pieces + 255) / 256), joins((g.runs + 31) / 32, (p.width + 127) / 128);
+  const dim3 sums((g.runs + 256 / p.group - 1) / (256 / p.group), (p.pieces + 255) / 256), joins((g.runs + 7) / 8, (p.width + 127) / 128);
   if (sums.y > 65535 || joins.y > 65535) return BLSTM_E_TOO_LARGE;
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
