@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
 // ---------------------------------------------------------------- sums of equal tokens' rows
 constexpr int kRunStep = 8;          // rows on their way at a time
 constexpr int kMaxRun = 32;          // sorted positions that one group of threads adds up
-constexpr int kZeroRows = 64;        // rows of dW that one block looks after
+constexpr int kZeroRows = 16;        // rows of dW that one block of few_kernel clears
 
 struct SumParams {
   const void* dout;
@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumPa
 }
 
 // ---------------------------------------------------------------- few tokens: one launch, nothing sorted
-// A block has a position: it looks for its token among all of them and, where it is the first that names it, adds the rows
-// up, several groups of threads in turn and then the groups in order.  Other blocks write the rows that no token names.
+// A block has a position (and a part of the columns): it looks for its token among all of them and, where it is the first
+// that names it, adds the rows up, each warp some of them and then the warps in order.  Other blocks write the rows that no token names.
 constexpr int kFew = 2048;
 
 template <typename T, int VEC>
@@ -383,9 +383,10 @@ __global__ void __launch_bounds__(256) few_kernel(const __grid_constant__ SumPar
   __shared__ unsigned s_met[kZeroRows];
   __shared__ unsigned s_bits[kFew / 32];
   __shared__ unsigned short s_list[kFew];
-  __shared__ float s_sum[256 * VEC];
+  __shared__ float s_sum[7][32][32];
   const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (blockIdx.x >= p.n) {
+    if (blockIdx.y) return;
     const unsigned v0 = (blockIdx.x - p.n) * kZeroRows, rows = min((unsigned)kZeroRows, p.vocab - v0);
     if (tid < kZeroRows) s_met[tid] = 0;
     __syncthreads();
@@ -426,33 +427,43 @@ __global__ void __launch_bounds__(256) few_kernel(const __grid_constant__ SumPar
 #pragma unroll
   for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(~0u, count, o);
   __syncthreads();
-  const unsigned groups = count == 1 ? 1 : 256 / p.group, width = 256 / groups;    // threads of a group
-  const unsigned g = tid / width, x = tid % width;
-  for (unsigned c0 = 0; c0 < p.pieces; c0 += width) {
-    const unsigned c = c0 + x;
-    float acc[VEC];
+  // a warp has every eighth of the positions and K pieces of a row in each lane
+  constexpr int K = VEC == 8 ? 4 : 8;
+  const unsigned c0 = blockIdx.y * (32 * K) + lane;
+  float acc[K][VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-    if (c < p.pieces) {
-#pragma unroll 4
-      for (unsigned j = g; j < count; j += groups) {
-        const V v = *reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(s_list[j]) + (size_t)c * VEC);
+  for (int q = 0; q < K; ++q)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += Elem<T>::to_f(v.v[k]);
-      }
-    }
-    if (groups > 1) {
+    for (int k = 0; k < VEC; ++k) acc[q][k] = 0.f;
+#pragma unroll 2
+  for (unsigned j = warp; j < count; j += 8) {
+    const V* row = reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(s_list[j]));
+    V v[K];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s_sum[k * 256 + tid] = acc[k];
-      __syncthreads();
-      if (g == 0)
-        for (unsigned q = 1; q < groups; ++q)
+    for (int q = 0; q < K; ++q) if (c0 + q * 32 < p.pieces) v[q] = row[c0 + q * 32];
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] += s_sum[k * 256 + q * width + x];
-      __syncthreads();
-    }
-    if (g == 0 && c < p.pieces) put_sum<T, VEC>(p, (unsigned)t, c, acc);
+    for (int q = 0; q < K; ++q)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[q][k] += c0 + q * 32 < p.pieces ? Elem<T>::to_f(v[q].v[k]) : 0.f;
   }
+  if (count > 1) {
+    if (warp > 0 && warp < count)
+#pragma unroll
+      for (int q = 0; q < K; ++q)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s_sum[warp - 1][q * VEC + k][lane] = acc[q][k];
+    __syncthreads();
+    if (warp == 0)
+      for (unsigned w = 1; w < min(count, 8u); ++w)
+#pragma unroll
+        for (int q = 0; q < K; ++q)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[q][k] += s_sum[w - 1][q * VEC + k][lane];
+  }
+  if (warp == 0)
+#pragma unroll
+    for (int q = 0; q < K; ++q)
+      if (c0 + q * 32 < p.pieces) put_sum<T, VEC>(p, (unsigned)t, c0 + q * 32, acc[q]);
 }
 
 // ---------------------------------------------------------------- workspace
@@ -568,12 +579,14 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
   p.scale = d->scale;
   const unsigned zero_blocks = (p.vocab + kZeroRows - 1) / kZeroRows;
   if (n <= kFew) {
-    p.group = std::min(p.group, 64u);                    // four groups at least, for tokens that come often
+    const unsigned lane_pieces = piece == 16 && e == 2 ? 4 : 8;          // (K of the kernel)
+    const dim3 grid(p.n + zero_blocks, (p.pieces + 32 * lane_pieces - 1) / (32 * lane_pieces));
+    if (grid.y > 65535) return BLSTM_E_TOO_LARGE;
     return with_type(d->dtype, [&](auto t) -> int {
       using T = decltype(t);
-      if (piece == 16) few_kernel<T, 16 / sizeof(T)><<<p.n + zero_blocks, 256, 0, st>>>(p);
-      else if (piece == 4) few_kernel<T, 4 / sizeof(T)><<<p.n + zero_blocks, 256, 0, st>>>(p);
-      else few_kernel<T, 1><<<p.n + zero_blocks, 256, 0, st>>>(p);
+      if (piece == 16) few_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(p);
+      else if (piece == 4) few_kernel<T, 4 / sizeof(T)><<<grid, 256, 0, st>>>(p);
+      else few_kernel<T, 1><<<grid, 256, 0, st>>>(p);
       BLSTM_CUDA_OK(cudaGetLastError());
       count_launch();
       return BLSTM_OK;

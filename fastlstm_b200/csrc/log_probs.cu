@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) score_warp_kernel(const __grid
 }
 
 // ---------------------------------------------------------------- large vocabularies: a block, or a cluster of them, has a row
-constexpr int kThreads = 256, kWarps = kThreads / 32, kUnroll = 4, kGroups = 64, kCand = 1024, kMaxCluster = 8;
+constexpr int kUnroll = 2, kGradThreads = 256, kGradUnroll = 4, kGroups = 64, kCand = 1024, kMaxCluster = 8;
 
 // What a block reads of a row: elements up to the first 16-byte boundary, pieces of 16 bytes, and the elements behind them.
 template <typename T>
@@ -277,6 +277,10 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
   return v;
 }
 
+__device__ __forceinline__ uint4 minus_infinity(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+__device__ __forceinline__ uint4 minus_infinity(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+__device__ __forceinline__ uint4 minus_infinity(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
 __device__ __forceinline__ unsigned cluster_size() {
   unsigned v;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(v));
@@ -298,38 +302,39 @@ __device__ __forceinline__ void store_first(V* p, unsigned long long v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
+template <int NT>
 struct ScoreShared {
-  Part part[kWarps];
+  Part part[NT / 32];
   uint2 peers[kMaxCluster][2];                          // maximum and sum, second sum, of every block of a cluster
   unsigned group[kGroups];
-  unsigned owner[kThreads];
-  unsigned owners, count, bound;
-  unsigned long long bound_key;
+  unsigned owner[NT];
+  unsigned owners, count;
+  unsigned long long bound;
   unsigned long long cand[kCand];
   unsigned long long best[kMaxCluster * BLSTM_MAX_TOP]; // of this block; in a cluster's first one, of all
 };
 
-// The `top` first of a block's logits in order, into s.best: thread's maxima bound them from below, the threads whose
-// maximum reaches that bound (few more than `top`) look at their logits again.
-template <typename T>
-__device__ __forceinline__ void block_top(ScoreShared& s, const Span<T>& span, float thread_max, unsigned top) {
-  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// The `top` first of a block's logits in order, into s.best: threads' maxima bound them from below, the threads whose
+// maximum reaches that bound (few more than `top`) have their logits looked at again.
+template <typename T, int NT>
+__device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& span, float thread_max, unsigned top) {
+  const unsigned tid = threadIdx.x, lane = tid & 31;
   const unsigned mine = value_key(thread_max);
   unsigned g = mine;
 #pragma unroll
-  for (int o = 1; o < kThreads / kGroups; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
-  if (tid % (kThreads / kGroups) == 0) s.group[tid / (kThreads / kGroups)] = g;
+  for (int o = 1; o < NT / kGroups; o <<= 1) g = max(g, __shfl_xor_sync(~0u, g, o));
+  if (tid % (NT / kGroups) == 0) s.group[tid / (NT / kGroups)] = g;
   if (tid == 0) { s.owners = 0; s.count = 0; }
+  if (tid < top) s.best[tid] = 0;              // (a block may have fewer)
   __syncthreads();
-  if (tid < kGroups) {
-    const unsigned v = s.group[tid];
-    unsigned rank = 0;
-#pragma unroll 16
-    for (unsigned i = 0; i < kGroups; ++i) rank += s.group[i] > v || (s.group[i] == v && i < tid);
-    if (rank == top - 1) s.bound = v;
-  }
-  __syncthreads();
-  const unsigned bound = s.bound;
+  // the `top`-th largest of the groups' maxima, in every warp: the largest, those that are left without it, and so on
+  unsigned a = s.group[lane], b = s.group[lane + 32], bound, found = 0;
+  do {
+    bound = __reduce_max_sync(~0u, max(a, b));
+    found += __popc(__ballot_sync(~0u, a == bound)) + __popc(__ballot_sync(~0u, b == bound));
+    if (a == bound) a = 0;                     // (no key is 0)
+    if (b == bound) b = 0;
+  } while (found < top);
   if (mine >= bound) s.owner[atomicAdd(&s.owners, 1u)] = tid;
   __syncthreads();
   auto offer = [&](float z, unsigned j, unsigned long long least) {
@@ -338,48 +343,63 @@ __device__ __forceinline__ void block_top(ScoreShared& s, const Span<T>& span, f
     const unsigned at = atomicAdd(&s.count, 1u);
     if (at < kCand) s.cand[at] = key;
   };
-  auto look = [&](unsigned piece, unsigned long long least) {
-    float z[kPer<T>];
-    unpack(span.body()[piece], z, T{});
+  auto look = [&](const uint4& v, unsigned piece, unsigned long long least) {
+    float z[kPer<T>], m;
+    unpack(v, z, T{});
+    m = z[0];
+#pragma unroll
+    for (int i = 1; i < kPer<T>; ++i) m = max_nan(m, z[i]);
+    if (value_key(m) < (unsigned)(least >> 32)) return;
 #pragma unroll
     for (int i = 0; i < kPer<T>; ++i) offer(z[i], span.number(piece) + i, least);
   };
-  const unsigned owners = s.owners;
+  // the owners' pieces, all threads side by side
+  const unsigned owners = s.owners, each = (span.end - span.begin + NT - 1) / NT;
   const unsigned long long least = (unsigned long long)bound << 32;
-  for (unsigned o = warp; o < owners; o += kWarps) {
-    const unsigned t = s.owner[o];
-    for (unsigned piece = span.begin + t + lane * kThreads; piece < span.end; piece += 32 * kThreads) look(piece, least);
-    if (lane == 0 && t < span.edges()) offer(ld_f(span.row + span.edge(t)), span.edge(t), least);
+  constexpr int kLook = 4;
+  for (unsigned i0 = tid; i0 < owners * each; i0 += kLook * NT) {
+    uint4 v[kLook];
+    unsigned piece[kLook];
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) {
+      const unsigned i = i0 + u * NT;
+      piece[u] = i < owners * each ? span.begin + s.owner[i / each] + i % each * NT : span.end;
+      if (piece[u] < span.end) v[u] = span.body()[piece[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kLook; ++u)
+      if (piece[u] < span.end) look(v[u], piece[u], least);
   }
+  for (unsigned i = tid; i < owners; i += NT)
+    if (s.owner[i] < span.edges()) offer(ld_f(span.row + span.edge(s.owner[i])), span.edge(s.owner[i]), least);
   __syncthreads();
   while (s.count > kCand) {                    // (many equal logits) a higher bound, from some of them, until they fit
     unsigned before = 0;
     const unsigned long long key = s.cand[tid];
-    for (unsigned i = 0; i < kThreads; ++i) before += s.cand[i] > key;
-    if (before == top - 1) s.bound_key = key;
+    for (unsigned i = 0; i < NT; ++i) before += s.cand[i] > key;
+    if (before == top - 1) s.bound = key;
     __syncthreads();
     if (tid == 0) s.count = 0;
     __syncthreads();
-    const unsigned long long more = s.bound_key;
-    for (unsigned piece = span.begin + tid; piece < span.end; piece += kThreads) look(piece, more);
+    const unsigned long long more = s.bound;
+    for (unsigned piece = span.begin + tid; piece < span.end; piece += NT) look(span.body()[piece], piece, more);
     if (tid < span.edges()) offer(ld_f(span.row + span.edge(tid)), span.edge(tid), more);
     __syncthreads();
   }
   const unsigned count = s.count;
-  if (tid < top) s.best[tid] = 0;              // (a block may have fewer)
-  __syncthreads();
-  for (unsigned i = tid; i < count; i += kThreads) {
+  for (unsigned i = tid; i < count; i += NT) {
     const unsigned long long key = s.cand[i];
     unsigned before = 0;
+#pragma unroll 16
     for (unsigned q = 0; q < count; ++q) before += s.cand[q] > key;
     if (before < top) s.best[before] = key;
   }
   __syncthreads();
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__ ScoreParams p) {
-  __shared__ ScoreShared s;
+template <typename T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_constant__ ScoreParams p) {
+  __shared__ ScoreShared<NT> s;
   const unsigned parts = cluster_size(), part = cluster_rank(), r = blockIdx.x / parts;
   const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long token = p.tokens(r);
@@ -397,35 +417,27 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__
     const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
     take(a, z, p.to_log2);
   }
-  unsigned i = span.begin + tid;
-  for (; i + (kUnroll - 1) * kThreads < span.end; i += kUnroll * kThreads) {
-    uint4 v[kUnroll];
+  // kUnroll pieces are on their way while those before them are added up
+  auto fetch = [&](unsigned i, uint4 (&v)[kUnroll]) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) v[u] = load_once(body + i + u * kThreads);
+    for (int u = 0; u < kUnroll; ++u) v[u] = i + u * NT < span.end ? load_once(body + i + u * NT) : minus_infinity(T{});
+  };
+  uint4 next[kUnroll];
+  fetch(span.begin + tid, next);
+  for (unsigned i = span.begin + tid; i < span.end; i += kUnroll * NT) {
     float z[kUnroll * kPer<T>];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) unpack(v[u], z + u * kPer<T>, T{});
+    for (int u = 0; u < kUnroll; ++u) unpack(next[u], z + u * kPer<T>, T{});
+    fetch(i + kUnroll * NT, next);
     take(a, z, p.to_log2);
-  }
-  if (i < span.end) {
-    uint4 v[kUnroll - 1];
-#pragma unroll
-    for (int u = 0; u < kUnroll - 1; ++u) if (i + u * kThreads < span.end) v[u] = load_once(body + i + u * kThreads);
-#pragma unroll
-    for (int u = 0; u < kUnroll - 1; ++u)
-      if (i + u * kThreads < span.end) {
-        float z[kPer<T>];
-        unpack(v[u], z, T{});
-        take(a, z, p.to_log2);
-      }
   }
   const float thread_max = a.m;
   a.join(32, p.to_log2);
   if (lane == 0) s.part[warp] = a;
   if constexpr (TOP) block_top(s, span, thread_max, (unsigned)p.top);
   else __syncthreads();
-  a = s.part[lane % kWarps];
-  a.join(kWarps, p.to_log2);
+  a = s.part[lane % (NT / 32)];
+  a.join((NT / 32), p.to_log2);
   if (parts > 1) {
     cluster_wait();
     if (tid == 0) {
@@ -448,6 +460,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__
     } else if (tid < parts * p.top) {
       const unsigned long long key = s.best[tid];
       unsigned before = 0;
+#pragma unroll 16
       for (unsigned q = 0; q < parts * p.top; ++q) before += s.best[q] > key;
       if (before < (unsigned)p.top && key) put_top(p, r, w, before, key);
     }
@@ -458,12 +471,13 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const __grid_constant__
 struct RowGrad {
   float m, log2s, g_lp, a, b;  // dz_j = 2^d (a + b d) and what given and top tokens add, d = log2 p_j
   long long token;
-  bool zero;
+  bool ignored, zero;
   __device__ __forceinline__ RowGrad(const ScoreParams& p, unsigned r) : token(p.tokens(r)) {
     m = p.stats[r];
     log2s = p.stats[(size_t)p.n + r];
     const float h = p.stats[2 * (size_t)p.n + r];
-    zero = token == p.ignore || log2s == -INFINITY;
+    ignored = token == p.ignore;
+    zero = ignored || log2s == -INFINITY;
     g_lp = p.g_lp && token >= 0 && token < p.vocab ? p.g_lp[p.g_lp_map(r)] : 0.f;
     const float g_h = p.g_h ? p.g_h[p.g_h_map(r)] : 0.f;
     float g = g_lp;
@@ -493,21 +507,24 @@ struct RowGrad {
   }
 };
 
-template <typename T>
+template <typename T, int VPL>
 __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const __grid_constant__ ScoreParams p) {
   const unsigned lane = threadIdx.x & 31, r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
   if (r >= p.n) return;
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
   T* out = static_cast<T*>(p.dlogits) + p.drows(r);
+  float z[VPL];
   const RowGrad g(p, r);
-  if (g.zero) {
-    for (unsigned j = lane; j < p.vocab; j += 32) out[j] = Elem<T>::from_f(0.f);
-    return;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) z[i] = i * 32 + lane < p.vocab && !g.ignored ? ld_f(row + i * 32 + lane) : 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const unsigned j = i * 32 + lane;
+    if (j < p.vocab) out[j] = Elem<T>::from_f(g.zero ? 0.f : j == g.token ? fmaf(g.g_lp, p.per_temperature, g(z[i], p.to_log2)) : g(z[i], p.to_log2));
   }
-#pragma unroll 8
-  for (unsigned j = lane; j < p.vocab; j += 32) out[j] = Elem<T>::from_f(g(ld_f(row + j), p.to_log2));
-  __syncwarp();
-  for (unsigned i = lane; i <= (p.g_top ? (unsigned)p.top : 0u); i += 32) {
+  if (p.g_top == nullptr || g.zero) return;
+  __syncwarp();                                // top tokens are written again, behind the others
+  for (unsigned i = lane; i <= (unsigned)p.top; i += 32) {
     const long long j = g.special(p, r, i);
     if (j >= 0) out[j] = Elem<T>::from_f(g.at(p, r, ld_f(row + j), j));
   }
@@ -515,7 +532,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const _
 
 // A block has a row, or one of gridDim.y parts of it.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
+__global__ void __launch_bounds__(kGradThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
   const unsigned r = blockIdx.x, tid = threadIdx.x;
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
   T* out = static_cast<T*>(p.dlogits) + p.drows(r);
@@ -524,20 +541,20 @@ __global__ void __launch_bounds__(kThreads) score_grad_kernel(const __grid_const
   const uint4* body = span.body();
   uint4* out_body = reinterpret_cast<uint4*>(out + span.head);        // (the same address modulo 16 as the logits')
   if (g.zero) {
-    for (unsigned i = span.begin + tid; i < span.end; i += kThreads) out_body[i] = make_uint4(0, 0, 0, 0);
+    for (unsigned i = span.begin + tid; i < span.end; i += kGradThreads) out_body[i] = make_uint4(0, 0, 0, 0);
     if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(0.f);
     return;
   }
   if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(g(ld_f(row + span.edge(tid)), p.to_log2));
   const Pair down = Pair::of(-g.m, -g.m), c = Pair::of(p.to_log2, p.to_log2), minus = Pair::of(-g.log2s, -g.log2s);
   const Pair a = Pair::of(g.a, g.a), b = Pair::of(g.b, g.b);
-  for (unsigned i = span.begin + tid; i < span.end; i += kUnroll * kThreads) {
-    uint4 v[kUnroll];
+  for (unsigned i = span.begin + tid; i < span.end; i += kGradUnroll * kGradThreads) {
+    uint4 v[kGradUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) if (i + u * kThreads < span.end) v[u] = load_once(body + i + u * kThreads);
+    for (int u = 0; u < kGradUnroll; ++u) if (i + u * kGradThreads < span.end) v[u] = load_once(body + i + u * kGradThreads);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (i + u * kThreads < span.end) {
+    for (int u = 0; u < kGradUnroll; ++u)
+      if (i + u * kGradThreads < span.end) {
         float z[kPer<T>];
         unpack(v[u], z, T{});
 #pragma unroll
@@ -548,7 +565,7 @@ __global__ void __launch_bounds__(kThreads) score_grad_kernel(const __grid_const
           y = max_nan(y, kFar);
           (Pair::of(exp2_fast(x), exp2_fast(y)) * fma2(b, Pair::of(x, y), a)).get(z[k], z[k + 1]);
         }
-        out_body[i + u * kThreads] = pack(z, T{});
+        out_body[i + u * kGradThreads] = pack(z, T{});
       }
   }
   __syncthreads();                             // the few logits that get more are written again, behind the others
@@ -580,12 +597,23 @@ static ScoreParams score_params(const blstm_score_desc& d, const void* logits, c
   return p;
 }
 
-// How many blocks share a row: as many (a power of two) as give four blocks to an SM, with a full turn of the unrolled loop
-// for each of them.
+// Threads of a block.  Rows end with a few hundred clocks in which nothing is read, and the more rows an SM has the less
+// that shows (8192 x 50000 bf16 with 64 / 128 / 256 threads: 129 / 132 / 139 us; 32768 x 10007: 121 / 144 / 234).  Looking for
+// alternatives takes more threads a row: each of theirs that has one reads its share of the row again (with 5: 198 / 166 / 177,
+// with 20: 292 / 248 / 220, 131072 logits 371 / 291 / 253; 4096 logits 323 / 400 / 701).  Few rows take more threads each.
+static unsigned score_threads(const ScoreParams& p, size_t element) {
+  const unsigned long long pieces = (unsigned long long)p.vocab * element / 16;
+  unsigned threads = p.top == 0 || pieces < 1024 ? 64 : pieces < 6000 ? 128 : 256;
+  while (threads < 256 && (unsigned long long)p.n * threads < 1024ull * plan_sm_count() && pieces >= threads * 2) threads *= 2;
+  return threads;
+}
+
+// How many blocks of 256 threads share a row: as many (a power of two) as give four blocks to an SM, with a piece at least for
+// each of their threads.
 static unsigned score_parts(const ScoreParams& p, size_t element, unsigned most) {
   const unsigned long long pieces = (unsigned long long)p.vocab * element / 16;
   unsigned parts = 1;
-  while (parts < most && (unsigned long long)p.n * parts * 2 <= 4ull * plan_sm_count() && pieces / (parts * 2) >= kThreads) parts *= 2;
+  while (parts < most && (unsigned long long)p.n * parts * 2 <= 4ull * plan_sm_count() && pieces / (parts * 2) >= 256) parts *= 2;
   return parts;
 }
 
@@ -599,18 +627,21 @@ static int launch_score(const ScoreParams& p, cudaStream_t st) {
     else score_warp_kernel<T, 32, TOP><<<grid, block, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
   } else {
-    const unsigned parts = score_parts(p, sizeof(T), kMaxCluster);
+    const unsigned threads = score_threads(p, sizeof(T));
+    const unsigned parts = threads == 256 ? score_parts(p, sizeof(T), kMaxCluster) : 1;
     if ((unsigned long long)p.n * parts > INT32_MAX) return BLSTM_E_TOO_LARGE;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {parts, 1, 1};
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = p.n * parts;
-    cfg.blockDim = kThreads;
+    cfg.blockDim = threads;
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, score_kernel<T, TOP>, p));
+    if (threads == 64) BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, score_kernel<T, TOP, 64>, p));
+    else if (threads == 128) BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, score_kernel<T, TOP, 128>, p));
+    else BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, score_kernel<T, TOP, 256>, p));
   }
   count_launch();
   return BLSTM_OK;
@@ -659,8 +690,12 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    if (p.vocab <= kWarpVocab) score_grad_warp_kernel<T><<<(p.n + kWarpRows - 1) / kWarpRows, 32 * kWarpRows, 0, st>>>(p);
-    else score_grad_kernel<T><<<dim3(p.n, score_parts(p, sizeof(T), 1 << 16)), kThreads, 0, st>>>(p);
+    const unsigned grid = (p.n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows;
+    if (p.vocab <= 128) score_grad_warp_kernel<T, 4><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= 256) score_grad_warp_kernel<T, 8><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= 512) score_grad_warp_kernel<T, 16><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= kWarpVocab) score_grad_warp_kernel<T, 32><<<grid, block, 0, st>>>(p);
+    else score_grad_kernel<T><<<dim3(p.n, score_parts(p, sizeof(T), 1 << 16)), kGradThreads, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
