@@ -8,6 +8,8 @@
 // Forward reads the logits once, backward once more and writes their gradient: bound by memory.  The softmax's statistics
 // are kept in 32 bits, and a logit enters as its distance from the row's maximum, so that large common offsets cost no
 // digits; distances are cut at 2^-10000, whose term is 0, so that masked logits (-inf or the type's lowest value) are finite.
+#include <algorithm>
+
 #include "language.cuh"
 
 namespace blstm {
@@ -21,7 +23,7 @@ struct ScoreParams {
   RowMap rows, drows;
   Tokens tokens;
   long long ignore;
-  unsigned n, vocab;
+  unsigned n, vocab, parts;    // parts of a row (gradient)
   int top;
   float to_log2;               // log2(e) / temperature
   float per_temperature;       // 1 / temperature
@@ -82,6 +84,14 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   Pair r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
+}
+
+// How many of n keys in shared memory come before `key`.
+__device__ __forceinline__ unsigned rank_of(const unsigned long long* keys, unsigned n, unsigned long long key) {
+  unsigned before = 0;
+#pragma unroll 16
+  for (unsigned q = 0; q < n; ++q) before += keys[q] > key;
+  return before;
 }
 
 // A part of a row: its largest logit, and the sums of 2^d and of d 2^d over it, d the distance from the reference
@@ -177,78 +187,7 @@ __device__ __forceinline__ void put_ignored(const ScoreParams& p, unsigned r, un
   }
 }
 
-// ---------------------------------------------------------------- small vocabularies: a warp has a row in its registers
-constexpr int kWarpVocab = 1024, kWarpRows = 4, kWarpCand = 128;
-
-template <typename T, int VPL, bool TOP>
-__global__ void __launch_bounds__(32 * kWarpRows) score_warp_kernel(const __grid_constant__ ScoreParams p) {
-  __shared__ unsigned long long s_cand[TOP ? kWarpRows : 1][TOP ? kWarpCand : 1];
-  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * kWarpRows + warp;
-  if (r >= p.n) return;
-  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
-  const long long token = p.tokens(r);
-  if (token == p.ignore) {
-    put_ignored(p, r, lane);
-    return;
-  }
-  float z[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) z[i] = i * 32 + lane < p.vocab ? ld_f(row + i * 32 + lane) : -INFINITY;
-  const float at_token = token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
-  Part a{-INFINITY, 0.f, 0.f};
-  take(a, z, p.to_log2);
-  const unsigned mine = value_key(a.m);        // (of a lane without logits: that of -inf)
-  a.join(32, p.to_log2);
-  const Row w(a);
-  if (lane == 0) put_row(p, r, w, token, at_token);
-  if constexpr (TOP) {
-    // The k-th largest of the lanes' maxima is a lower bound of the k-th largest logit: what is below it is out.
-    unsigned rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      const unsigned o = __shfl_sync(~0u, mine, i);
-      rank += o > mine || (o == mine && i < lane);
-    }
-    const unsigned bound = __shfl_sync(~0u, mine, __ffs(__ballot_sync(~0u, rank == (unsigned)p.top - 1)) - 1);
-    unsigned count = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const unsigned j = i * 32 + lane;
-      const unsigned long long key = order_key(z[i], j);
-      const bool in = j < p.vocab && (unsigned)(key >> 32) >= bound;
-      const unsigned who = __ballot_sync(~0u, in);
-      const unsigned at = count + __popc(who & ((1u << lane) - 1));
-      if (in && at < kWarpCand) s_cand[warp][at] = key;
-      count += __popc(who);
-    }
-    __syncwarp();
-    if (count <= kWarpCand) {
-      for (unsigned i = lane; i < count; i += 32) {
-        const unsigned long long key = s_cand[warp][i];
-        unsigned before = 0;
-        for (unsigned q = 0; q < count; ++q) before += s_cand[warp][q] > key;
-        if (before < (unsigned)p.top) put_top(p, r, w, (int)before, key);
-      }
-    } else {                                   // (many equal logits) one after the other
-      unsigned long long last = ~0ull;
-      for (int k = 0; k < p.top; ++k) {
-        unsigned long long best = 0;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const unsigned long long key = order_key(z[i], i * 32 + lane);
-          if (i * 32 + lane < p.vocab && key < last && key > best) best = key;
-        }
-        for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-        if (lane == 0) put_top(p, r, w, k, best);
-        last = best;
-      }
-    }
-  }
-}
-
-// ---------------------------------------------------------------- large vocabularies: a block, or a cluster of them, has a row
-constexpr int kUnroll = 2, kGradThreads = 256, kGradUnroll = 4, kGroups = 64, kCand = 1024, kMaxCluster = 8;
-
+// ---------------------------------------------------------------- a row in 16-byte pieces
 // What a block reads of a row: elements up to the first 16-byte boundary, pieces of 16 bytes, and the elements behind them.
 template <typename T>
 struct Span {
@@ -280,6 +219,99 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 __device__ __forceinline__ uint4 minus_infinity(float) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 __device__ __forceinline__ uint4 minus_infinity(__nv_bfloat16) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 __device__ __forceinline__ uint4 minus_infinity(__half) { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
+// ---------------------------------------------------------------- small vocabularies: a warp has a row in its registers
+// (16384 rows of 1000 fp32 logits: forward 13 us, with blocks 21, backward 22; of 1500 to 2000 bf16 forward 20, with blocks 24, but
+// with 5 alternatives 77 and with blocks 47, and backward 41 where blocks take 27: so half as long for those.)
+constexpr int kWarpPieces = 256, kWarpRows = 8, kWarpCand = 128;
+
+// PPL pieces and an element of the edges in each lane.
+template <typename T, int PPL>
+struct WarpRow {
+  Span<T> span;
+  unsigned lane;
+  float z[PPL * kPer<T>], edge;
+  __device__ __forceinline__ WarpRow(const T* row, unsigned vocab) : span(row, vocab, 0, 1), lane(threadIdx.x & 31) {
+    uint4 v[PPL];
+#pragma unroll
+    for (int u = 0; u < PPL; ++u) v[u] = u * 32 + lane < span.pieces ? load_once(span.body() + u * 32 + lane) : minus_infinity(T{});
+    edge = lane < span.edges() ? ld_f(row + span.edge(lane)) : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < PPL; ++u) unpack(v[u], z + u * kPer<T>, T{});
+  }
+  // f(logit, number) for every logit that this lane has; the lanes stay together (f may use the warp), `in` says whose are real
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int i = 0; i < PPL * kPer<T>; ++i) {
+      const unsigned piece = i / kPer<T> * 32 + lane;
+      f(z[i], span.number(piece) + i % kPer<T>, piece < span.pieces);
+    }
+    f(edge, span.edge(lane), lane < span.edges());
+  }
+};
+
+template <typename T, int PPL, bool TOP>
+__global__ void __launch_bounds__(32 * kWarpRows) score_warp_kernel(const __grid_constant__ ScoreParams p) {
+  __shared__ unsigned long long s_cand[TOP ? kWarpRows : 1][TOP ? kWarpCand : 1];
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * kWarpRows + warp;
+  if (r >= p.n) return;
+  const T* row = static_cast<const T*>(p.logits) + p.rows(r);
+  const long long token = p.tokens(r);
+  const WarpRow<T, PPL> w(row, p.vocab);       // (before the token is there; a row that is ignored is small)
+  if (token == p.ignore) {
+    put_ignored(p, r, lane);
+    return;
+  }
+  const float at_token = token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
+  Part a{-INFINITY, 0.f, 0.f};
+  take(a, w.z, p.to_log2);
+  const float edge[2] = {w.edge, -INFINITY};
+  take(a, edge, p.to_log2);
+  const unsigned mine = value_key(a.m);        // (of a lane without logits: that of -inf)
+  a.join(32, p.to_log2);
+  const Row stats(a);
+  if (lane == 0) put_row(p, r, stats, token, at_token);
+  if constexpr (TOP) {
+    // The k-th largest of the lanes' maxima is a lower bound of the k-th largest logit: what is below it is out.
+    unsigned left = mine, bound, found = 0;
+    do {
+      bound = __reduce_max_sync(~0u, left);
+      found += __popc(__ballot_sync(~0u, left == bound));
+      if (left == bound) left = 0;             // (no key is 0)
+    } while (found < (unsigned)p.top);
+    unsigned count = 0;
+    w.each([&](float z, unsigned j, bool in) {
+      const unsigned key = value_key(z), who = __ballot_sync(~0u, in && key >= bound);
+      const unsigned at = count + __popc(who & ((1u << lane) - 1));
+      if (in && key >= bound && at < kWarpCand) s_cand[warp][at] = order_key(z, j);
+      count += __popc(who);
+    });
+    __syncwarp();
+    if (count <= kWarpCand) {
+      for (unsigned i = lane; i < count; i += 32) {
+        const unsigned long long key = s_cand[warp][i];
+        const unsigned before = rank_of(s_cand[warp], count, key);
+        if (before < (unsigned)p.top) put_top(p, r, stats, (int)before, key);
+      }
+    } else {                                   // (many equal logits) one after the other
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < p.top; ++k) {
+        unsigned long long best = 0;
+        w.each([&](float z, unsigned j, bool in) {
+          const unsigned long long key = order_key(z, j);
+          if (in && key < last && key > best) best = key;
+        });
+        for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
+        if (lane == 0) put_top(p, r, stats, k, best);
+        last = best;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- large vocabularies: a block, or a cluster of them, has a row
+constexpr int kUnroll = 2, kGroups = 64, kCand = 1024, kMaxCluster = 8;
 
 __device__ __forceinline__ unsigned cluster_size() {
   unsigned v;
@@ -374,10 +406,8 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
     if (s.owner[i] < span.edges()) offer(ld_f(span.row + span.edge(s.owner[i])), span.edge(s.owner[i]), least);
   __syncthreads();
   while (s.count > kCand) {                    // (many equal logits) a higher bound, from some of them, until they fit
-    unsigned before = 0;
     const unsigned long long key = s.cand[tid];
-    for (unsigned i = 0; i < NT; ++i) before += s.cand[i] > key;
-    if (before == top - 1) s.bound = key;
+    if (rank_of(s.cand, NT, key) == top - 1) s.bound = key;
     __syncthreads();
     if (tid == 0) s.count = 0;
     __syncthreads();
@@ -389,9 +419,7 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
   const unsigned count = s.count;
   for (unsigned i = tid; i < count; i += NT) {
     const unsigned long long key = s.cand[i];
-    unsigned before = 0;
-#pragma unroll 16
-    for (unsigned q = 0; q < count; ++q) before += s.cand[q] > key;
+    const unsigned before = rank_of(s.cand, count, key);
     if (before < top) s.best[before] = key;
   }
   __syncthreads();
@@ -402,28 +430,29 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
   __shared__ ScoreShared<NT> s;
   const unsigned parts = cluster_size(), part = cluster_rank(), r = blockIdx.x / parts;
   const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long token = p.tokens(r);
-  if (token == p.ignore) {                     // (the same for a whole cluster)
-    if (part == 0) put_ignored(p, r, tid);
-    return;
-  }
-  if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
-  const float at_token = tid == 0 && part == 0 && token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
   const Span<T> span(row, p.vocab, part, parts);
   const uint4* body = span.body();
-  Part a{-INFINITY, 0.f, 0.f};
-  if (tid < span.edges()) {
-    const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
-    take(a, z, p.to_log2);
-  }
   // kUnroll pieces are on their way while those before them are added up
   auto fetch = [&](unsigned i, uint4 (&v)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) v[u] = i + u * NT < span.end ? load_once(body + i + u * NT) : minus_infinity(T{});
   };
   uint4 next[kUnroll];
-  fetch(span.begin + tid, next);
+  if (parts > 1) fetch(span.begin + tid, next);      // (few rows: not behind the token)
+  const long long token = p.tokens(r);
+  if (token == p.ignore) {                     // (the same for a whole cluster)
+    if (part == 0) put_ignored(p, r, tid);
+    return;
+  }
+  if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
+  else fetch(span.begin + tid, next);
+  const float at_token = tid == 0 && part == 0 && token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
+  Part a{-INFINITY, 0.f, 0.f};
+  if (tid < span.edges()) {
+    const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
+    take(a, z, p.to_log2);
+  }
   for (unsigned i = span.begin + tid; i < span.end; i += kUnroll * NT) {
     float z[kUnroll * kPer<T>];
 #pragma unroll
@@ -459,9 +488,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
       if (tid < (unsigned)p.top) put_top(p, r, w, tid, s.best[tid]);
     } else if (tid < parts * p.top) {
       const unsigned long long key = s.best[tid];
-      unsigned before = 0;
-#pragma unroll 16
-      for (unsigned q = 0; q < parts * p.top; ++q) before += s.best[q] > key;
+      const unsigned before = rank_of(s.best, parts * p.top, key);
       if (before < (unsigned)p.top && key) put_top(p, r, w, before, key);
     }
   }
@@ -471,13 +498,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
 struct RowGrad {
   float m, log2s, g_lp, a, b;  // dz_j = 2^d (a + b d) and what given and top tokens add, d = log2 p_j
   long long token;
-  bool ignored, zero;
+  bool zero;
   __device__ __forceinline__ RowGrad(const ScoreParams& p, unsigned r) : token(p.tokens(r)) {
     m = p.stats[r];
     log2s = p.stats[(size_t)p.n + r];
     const float h = p.stats[2 * (size_t)p.n + r];
-    ignored = token == p.ignore;
-    zero = ignored || log2s == -INFINITY;
+    zero = token == p.ignore || log2s == -INFINITY;
     g_lp = p.g_lp && token >= 0 && token < p.vocab ? p.g_lp[p.g_lp_map(r)] : 0.f;
     const float g_h = p.g_h ? p.g_h[p.g_h_map(r)] : 0.f;
     float g = g_lp;
@@ -507,21 +533,24 @@ struct RowGrad {
   }
 };
 
-template <typename T, int VPL>
+template <typename T, int PPL>
 __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const __grid_constant__ ScoreParams p) {
   const unsigned lane = threadIdx.x & 31, r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
   if (r >= p.n) return;
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
   T* out = static_cast<T*>(p.dlogits) + p.drows(r);
-  float z[VPL];
+  WarpRow<T, PPL> w(row, p.vocab);
   const RowGrad g(p, r);
+  auto grad = [&](float z, unsigned j) { return g.zero ? 0.f : j == g.token ? fmaf(g.g_lp, p.per_temperature, g(z, p.to_log2)) : g(z, p.to_log2); };
+  uint4* body = reinterpret_cast<uint4*>(out + w.span.head);          // (the same address modulo 16 as the logits')
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) z[i] = i * 32 + lane < p.vocab && !g.ignored ? ld_f(row + i * 32 + lane) : 0.f;
+  for (int u = 0; u < PPL; ++u) {
+    const unsigned piece = u * 32 + lane;
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const unsigned j = i * 32 + lane;
-    if (j < p.vocab) out[j] = Elem<T>::from_f(g.zero ? 0.f : j == g.token ? fmaf(g.g_lp, p.per_temperature, g(z[i], p.to_log2)) : g(z[i], p.to_log2));
+    for (int i = 0; i < kPer<T>; ++i) w.z[u * kPer<T> + i] = grad(w.z[u * kPer<T> + i], w.span.number(piece) + i);
+    if (piece < w.span.pieces) body[piece] = pack(w.z + u * kPer<T>, T{});
   }
+  if (lane < w.span.edges()) out[w.span.edge(lane)] = Elem<T>::from_f(grad(w.edge, w.span.edge(lane)));
   if (p.g_top == nullptr || g.zero) return;
   __syncwarp();                                // top tokens are written again, behind the others
   for (unsigned i = lane; i <= (unsigned)p.top; i += 32) {
@@ -530,44 +559,48 @@ __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const _
   }
 }
 
-// A block has a row, or one of gridDim.y parts of it.
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) score_grad_kernel(const __grid_constant__ ScoreParams p) {
-  const unsigned r = blockIdx.x, tid = threadIdx.x;
+// A block has a part of a row, kGradPieces pieces a thread at most: blocks that run at a time write neighbouring memory (4096 x
+// 50000 fp32 and 8192 x 50000 bf16 with whole rows 290 and 267 us, with 4 pieces a thread 254 and 276, with 6 248 and 265, with 8
+// 248 and 269).
+constexpr int kGradPieces = 6;
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) score_grad_kernel(const __grid_constant__ ScoreParams p) {
+  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, tid = threadIdx.x;
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
   T* out = static_cast<T*>(p.dlogits) + p.drows(r);
-  const RowGrad g(p, r);
-  const Span<T> span(row, p.vocab, blockIdx.y, gridDim.y);
-  const uint4* body = span.body();
+  const Span<T> span(row, p.vocab, part, p.parts);
+  const unsigned first = span.begin + tid;
   uint4* out_body = reinterpret_cast<uint4*>(out + span.head);        // (the same address modulo 16 as the logits')
+  uint4 v[kGradPieces];
+  if (p.tokens(r) != p.ignore)
+#pragma unroll
+    for (int u = 0; u < kGradPieces; ++u) if (first + u * NT < span.end) v[u] = load_once(span.body() + first + u * NT);
+  const RowGrad g(p, r);
   if (g.zero) {
-    for (unsigned i = span.begin + tid; i < span.end; i += kGradThreads) out_body[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < kGradPieces; ++u) if (first + u * NT < span.end) out_body[first + u * NT] = make_uint4(0, 0, 0, 0);
     if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(0.f);
     return;
   }
   if (tid < span.edges()) out[span.edge(tid)] = Elem<T>::from_f(g(ld_f(row + span.edge(tid)), p.to_log2));
   const Pair down = Pair::of(-g.m, -g.m), c = Pair::of(p.to_log2, p.to_log2), minus = Pair::of(-g.log2s, -g.log2s);
   const Pair a = Pair::of(g.a, g.a), b = Pair::of(g.b, g.b);
-  for (unsigned i = span.begin + tid; i < span.end; i += kGradUnroll * kGradThreads) {
-    uint4 v[kGradUnroll];
 #pragma unroll
-    for (int u = 0; u < kGradUnroll; ++u) if (i + u * kGradThreads < span.end) v[u] = load_once(body + i + u * kGradThreads);
+  for (int u = 0; u < kGradPieces; ++u)
+    if (first + u * NT < span.end) {
+      float z[kPer<T>];
+      unpack(v[u], z, T{});
 #pragma unroll
-    for (int u = 0; u < kGradUnroll; ++u)
-      if (i + u * kGradThreads < span.end) {
-        float z[kPer<T>];
-        unpack(v[u], z, T{});
-#pragma unroll
-        for (int k = 0; k < kPer<T>; k += 2) {
-          float x, y;
-          fma2(Pair::of(z[k], z[k + 1]) + down, c, minus).get(x, y);
-          x = max_nan(x, kFar);
-          y = max_nan(y, kFar);
-          (Pair::of(exp2_fast(x), exp2_fast(y)) * fma2(b, Pair::of(x, y), a)).get(z[k], z[k + 1]);
-        }
-        out_body[i + u * kGradThreads] = pack(z, T{});
+      for (int k = 0; k < kPer<T>; k += 2) {
+        float x, y;
+        fma2(Pair::of(z[k], z[k + 1]) + down, c, minus).get(x, y);
+        x = max_nan(x, kFar);
+        y = max_nan(y, kFar);
+        (Pair::of(exp2_fast(x), exp2_fast(y)) * fma2(b, Pair::of(x, y), a)).get(z[k], z[k + 1]);
       }
-  }
+      out_body[first + u * NT] = pack(z, T{});
+    }
   __syncthreads();                             // the few logits that get more are written again, behind the others
   if (tid <= (p.g_top ? (unsigned)p.top : 0u)) {
     const long long j = g.special(p, r, tid);
@@ -597,12 +630,15 @@ static ScoreParams score_params(const blstm_score_desc& d, const void* logits, c
   return p;
 }
 
+// 16-byte pieces of a row: what they are at least, and at most where it does not begin on a boundary (fewer elements are left).
+static unsigned row_pieces(const ScoreParams& p, size_t element) { return (unsigned)((unsigned long long)p.vocab * element / 16); }
+
 // Threads of a block.  Rows end with a few hundred clocks in which nothing is read, and the more rows an SM has the less
 // that shows (8192 x 50000 bf16 with 64 / 128 / 256 threads: 129 / 132 / 139 us; 32768 x 10007: 121 / 144 / 234).  Looking for
 // alternatives takes more threads a row: each of theirs that has one reads its share of the row again (with 5: 198 / 166 / 177,
 // with 20: 292 / 248 / 220, 131072 logits 371 / 291 / 253; 4096 logits 323 / 400 / 701).  Few rows take more threads each.
 static unsigned score_threads(const ScoreParams& p, size_t element) {
-  const unsigned long long pieces = (unsigned long long)p.vocab * element / 16;
+  const unsigned pieces = row_pieces(p, element);
   unsigned threads = p.top == 0 || pieces < 1024 ? 64 : pieces < 6000 ? 128 : 256;
   while (threads < 256 && (unsigned long long)p.n * threads < 1024ull * plan_sm_count() && pieces >= threads * 2) threads *= 2;
   return threads;
@@ -611,7 +647,7 @@ static unsigned score_threads(const ScoreParams& p, size_t element) {
 // How many blocks of 256 threads share a row: as many (a power of two) as give four blocks to an SM, with a piece at least for
 // each of their threads.
 static unsigned score_parts(const ScoreParams& p, size_t element, unsigned most) {
-  const unsigned long long pieces = (unsigned long long)p.vocab * element / 16;
+  const unsigned pieces = row_pieces(p, element);
   unsigned parts = 1;
   while (parts < most && (unsigned long long)p.n * parts * 2 <= 4ull * plan_sm_count() && pieces / (parts * 2) >= 256) parts *= 2;
   return parts;
@@ -619,12 +655,14 @@ static unsigned score_parts(const ScoreParams& p, size_t element, unsigned most)
 
 template <typename T, bool TOP>
 static int launch_score(const ScoreParams& p, cudaStream_t st) {
-  if (p.vocab <= kWarpVocab) {
+  const unsigned pieces = row_pieces(p, sizeof(T));
+  constexpr int kMost = TOP && sizeof(T) == 2 ? kWarpPieces / 2 : kWarpPieces;
+  if (pieces <= kMost) {
     const unsigned grid = (p.n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows;
-    if (p.vocab <= 128) score_warp_kernel<T, 4, TOP><<<grid, block, 0, st>>>(p);
-    else if (p.vocab <= 256) score_warp_kernel<T, 8, TOP><<<grid, block, 0, st>>>(p);
-    else if (p.vocab <= 512) score_warp_kernel<T, 16, TOP><<<grid, block, 0, st>>>(p);
-    else score_warp_kernel<T, 32, TOP><<<grid, block, 0, st>>>(p);
+    if (pieces <= 32) score_warp_kernel<T, 1, TOP><<<grid, block, 0, st>>>(p);
+    else if (pieces <= 64) score_warp_kernel<T, 2, TOP><<<grid, block, 0, st>>>(p);
+    else if (pieces <= 128) score_warp_kernel<T, 4, TOP><<<grid, block, 0, st>>>(p);
+    else if constexpr (kMost > 128) score_warp_kernel<T, 8, TOP><<<grid, block, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
   } else {
     const unsigned threads = score_threads(p, sizeof(T));
@@ -690,12 +728,20 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
     cudaStream_t st = (cudaStream_t)stream;
-    const unsigned grid = (p.n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows;
-    if (p.vocab <= 128) score_grad_warp_kernel<T, 4><<<grid, block, 0, st>>>(p);
-    else if (p.vocab <= 256) score_grad_warp_kernel<T, 8><<<grid, block, 0, st>>>(p);
-    else if (p.vocab <= 512) score_grad_warp_kernel<T, 16><<<grid, block, 0, st>>>(p);
-    else if (p.vocab <= kWarpVocab) score_grad_warp_kernel<T, 32><<<grid, block, 0, st>>>(p);
-    else score_grad_kernel<T><<<dim3(p.n, score_parts(p, sizeof(T), 1 << 16)), kGradThreads, 0, st>>>(p);
+    const unsigned grid = (p.n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows, pieces = row_pieces(p, sizeof(T));
+    if (pieces <= 32) score_grad_warp_kernel<T, 1><<<grid, block, 0, st>>>(p);
+    else if (pieces <= 64) score_grad_warp_kernel<T, 2><<<grid, block, 0, st>>>(p);
+    else if (pieces <= 128) score_grad_warp_kernel<T, 4><<<grid, block, 0, st>>>(p);
+    else if (sizeof(T) == 4 && pieces <= kWarpPieces) score_grad_warp_kernel<float, 8><<<grid, block, 0, st>>>(p);
+    else {
+      // small blocks for short rows, so that every thread has a few pieces
+      const unsigned threads = pieces <= 64 * kGradPieces ? 64 : pieces <= 128 * kGradPieces ? 128 : 256;
+      p.parts = std::max(score_parts(p, sizeof(T), 1 << 16), (pieces + threads * kGradPieces - 1) / (threads * kGradPieces));
+      if ((unsigned long long)p.n * p.parts > INT32_MAX) return BLSTM_E_TOO_LARGE;
+      if (threads == 64) score_grad_kernel<T, 64><<<p.n * p.parts, threads, 0, st>>>(p);
+      else if (threads == 128) score_grad_kernel<T, 128><<<p.n * p.parts, threads, 0, st>>>(p);
+      else score_grad_kernel<T, 256><<<p.n * p.parts, threads, 0, st>>>(p);
+    }
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
