@@ -1,6 +1,11 @@
 // Host side of the operators around a language model: argument checks, buffers, the calls of the C ABI and the autograd
 // nodes.  Tensors keep their strides as long as two strides describe their rows and the last dimension is dense; others
 // are copied first.
+#include <ATen/cuda/EmptyTensor.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
 #include <cmath>
 
 #include "host.h"
@@ -8,7 +13,8 @@
 namespace {
 
 using namespace blstm_host;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 py::value_error wrong(const std::string& what) { return py::value_error(what); }
@@ -45,6 +51,17 @@ struct Lead {
   }
 };
 
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& like) { return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt); }
+
+// A node of the graph that an operator's gradient is, with what it needs as members (a torch::autograd::Function keeps that in a
+// dictionary: 4 us a call).  Backward goes through it once.
+template <typename N>
+std::shared_ptr<N> make_node(const Tensor& input) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(input));
+  return node;
+}
+
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 void only_once() { TORCH_CHECK(!at::GradMode::is_enabled(), "fastlstm_b200: gradients of gradients (create_graph) are not there for this operator"); }
 
@@ -73,33 +90,31 @@ Tensor embedding_impl(const Tensor& tokens_in, const Tensor& weight_in, double s
   const Tensor tokens = lead.rows(tokens_in, d.token_stride);
   d.row_stride[0] = weight.stride(0);
   Call call(weight.device());
-  const Tensor out = at::empty(plus(tokens_in.sizes(), weight.size(1)), weight.options().requires_grad(false));
+  const Tensor out = fresh(plus(tokens_in.sizes(), weight.size(1)), weight.scalar_type(), weight);
   check(blstm_embedding(&d, ptr(tokens), ptr(weight), out.data_ptr(), call.stream), "embedding");
   return out;
 }
 
-struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, double scale, int64_t padding) {
-    ctx->save_for_backward({tokens});
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["sizes"] = std::vector<int64_t>{weight.size(0), weight.size(1), padding};
-    return embedding_impl(tokens, weight, scale);
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+struct EmbeddingGrad : public Node {
+  SavedVariable tokens;
+  at::ScalarType dtype;
+  int64_t vocab, width, padding;
+  double scale;
+  void release_variables() override { tokens.reset_data(); }
+  variable_list apply(variable_list&& g) override {
     only_once();
-    const Tensor saved = ctx->get_saved_variables()[0];
-    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    if (!g[0].defined()) return {Tensor()};
+    const Tensor saved = tokens.unpack();
     const Lead lead(saved.sizes());
-    blstm_embed_desc d = embed_desc(g[0].scalar_type(), saved, lead, sizes[0], sizes[1], ctx->saved_data["scale"].toDouble(), sizes[2]);
+    blstm_embed_desc d = embed_desc(dtype, saved, lead, vocab, width, scale, padding);
     const Tensor tokens = lead.rows(saved, d.token_stride), dout = lead.rows(g[0], d.row_stride);
     Call call(dout.device());
-    const auto opt = dout.options().requires_grad(false);
-    const Tensor dW = at::empty({sizes[0], sizes[1]}, opt);
+    const Tensor dW = fresh({vocab, width}, dtype, dout);
     const size_t bytes = blstm_embedding_grad_workspace(&d);
     Tensor ws;
-    if (bytes) ws = at::empty({(int64_t)bytes}, opt.dtype(at::kByte));
+    if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, dout);
     check(blstm_embedding_grad(&d, ptr(tokens), ptr(dout), dW.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, call.stream), "embedding gradient");
-    return {dW, Tensor(), Tensor(), Tensor()};
+    return {dW};
   }
 };
 
@@ -117,15 +132,28 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::
     if (*padding_idx < -V || *padding_idx >= V) throw wrong("padding_idx " + std::to_string(*padding_idx) + " is outside of the vocabulary of " + std::to_string(V));
     padding = *padding_idx < 0 ? *padding_idx + V : *padding_idx;
   }
-  return wants_grad(weight) ? EmbeddingFn::apply(weight, tokens, scale, padding) : embedding_impl(tokens, weight, scale);
+  if (!wants_grad(weight)) return embedding_impl(tokens, weight, scale);
+  const auto node = make_node<EmbeddingGrad>(weight);
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out = embedding_impl(tokens, weight, scale);
+  }
+  node->tokens = SavedVariable(tokens, false);
+  node->dtype = weight.scalar_type();
+  node->vocab = V; node->width = weight.size(1); node->padding = padding;
+  node->scale = scale;
+  torch::autograd::set_history(out, node);
+  return out;
 }
 
 // ---------------------------------------------------------------- dropout
 struct Mask {
-  double p;
-  uint64_t seed, offset;
-  OptTensor seed_at;
-  int64_t shared;             // dimension, or -1
+  double p = 0;
+  uint64_t seed = 0, offset = 0;
+  int64_t shared = -1;        // dimension, or -1
+  bool on_gpu = false;        // the seed
+  Tensor seed_at;
 };
 
 Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
@@ -154,25 +182,21 @@ Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
     d.shared = 1;
   }
   Call call(x.device());
-  const Tensor y = at::empty(sizes, x.options().requires_grad(false));
-  check(blstm_dropout(&d, ptr(x), k.seed_at ? static_cast<const int64_t*>(ptr(*k.seed_at)) : nullptr, y.data_ptr(), call.stream), "dropout");
+  const Tensor y = fresh(sizes, x.scalar_type(), x);
+  check(blstm_dropout(&d, ptr(x), k.on_gpu ? static_cast<const int64_t*>(ptr(k.seed_at)) : nullptr, y.data_ptr(), call.stream), "dropout");
   return y;
 }
 
-struct DropoutFn : public torch::autograd::Function<DropoutFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Mask& k) {
-    if (k.seed_at) ctx->save_for_backward({*k.seed_at});
-    ctx->saved_data["p"] = k.p;
-    ctx->saved_data["mask"] = std::vector<int64_t>{(int64_t)k.seed, (int64_t)k.offset, k.shared};
-    return dropout_impl(x, k);
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+struct DropoutGrad : public Node {
+  Mask mask;
+  SavedVariable seed_at;
+  void release_variables() override { seed_at.reset_data(); }
+  variable_list apply(variable_list&& g) override {
     only_once();
-    const auto saved = ctx->get_saved_variables();
-    const auto m = ctx->saved_data["mask"].toIntVector();
-    Mask k{ctx->saved_data["p"].toDouble(), (uint64_t)m[0], (uint64_t)m[1], std::nullopt, m[2]};
-    if (!saved.empty()) k.seed_at = saved[0];
-    return {dropout_impl(g[0], k), Tensor()};
+    if (!g[0].defined()) return {Tensor()};
+    Mask k = mask;
+    if (k.on_gpu) k.seed_at = seed_at.unpack();
+    return {dropout_impl(g[0], k)};
   }
 };
 
@@ -181,7 +205,8 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& seed_a
   on_gpu(x, "x");
   dtype_code(x.scalar_type());
   if (!(p >= 0.0 && p <= 1.0)) throw wrong("p must be in the range [0, 1]");
-  Mask k{p, seed, offset, seed_at, -1};
+  Mask k;
+  k.p = p; k.seed = seed; k.offset = offset;
   if (shared_dim) {
     const int64_t d = *shared_dim < 0 ? *shared_dim + x.dim() : *shared_dim;
     if (d < 0 || d >= x.dim() - 1) throw wrong("shared_dim must be a dimension of x and not its last one");
@@ -190,15 +215,28 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& seed_a
   if (seed_at) {
     beside(*seed_at, "seed", x);
     if (seed_at->scalar_type() != at::kLong || seed_at->numel() != 1) throw wrong("a seed on the GPU is one int64 element");
+    k.on_gpu = true;
+    k.seed_at = *seed_at;
   }
-  return wants_grad(x) ? DropoutFn::apply(x, k) : dropout_impl(x, k);
+  if (!wants_grad(x)) return dropout_impl(x, k);
+  const auto node = make_node<DropoutGrad>(x);
+  Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    y = dropout_impl(x, k);
+  }
+  if (k.on_gpu) node->seed_at = SavedVariable(k.seed_at, false);
+  k.seed_at.reset();
+  node->mask = std::move(k);
+  torch::autograd::set_history(y, node);
+  return y;
 }
 
 // ---------------------------------------------------------------- log probabilities
 struct Score {
-  int64_t top;
-  double temperature;
-  int64_t ignore;
+  int64_t top = 0;
+  double temperature = 1;
+  int64_t ignore = -100;
 };
 
 blstm_score_desc score_desc(const Tensor& logits, const Tensor& tokens, const Lead& lead, const Score& c) {
@@ -213,20 +251,20 @@ blstm_score_desc score_desc(const Tensor& logits, const Tensor& tokens, const Le
   return d;
 }
 
-// {log_probs, entropy, top_log_probs, top_tokens, stats}
-std::array<Tensor, 5> score_impl(const Tensor& logits_in, const Tensor& tokens_in, const Score& c) {
+// {log_probs, entropy, top_log_probs, top_tokens, stats}; the last one for a gradient alone
+std::array<Tensor, 5> score_impl(const Tensor& logits_in, const Tensor& tokens_in, const Score& c, bool grad) {
   const Lead lead(tokens_in.sizes());
   blstm_score_desc d = score_desc(logits_in, tokens_in, lead, c);
   const Tensor logits = lead.rows(logits_in, d.logits_stride), tokens = lead.rows(tokens_in, d.token_stride);
   Call call(logits.device());
-  const auto f32 = logits.options().requires_grad(false).dtype(at::kFloat);
-  std::array<Tensor, 5> r{at::empty(tokens_in.sizes(), f32), at::empty(tokens_in.sizes(), f32), Tensor(), Tensor(), at::empty({3, lead.n0 * lead.n1}, f32)};
+  std::array<Tensor, 5> r{fresh(tokens_in.sizes(), at::kFloat, logits), fresh(tokens_in.sizes(), at::kFloat, logits)};
   if (c.top) {
-    r[2] = at::empty(plus(tokens_in.sizes(), c.top), f32);
-    r[3] = at::empty(plus(tokens_in.sizes(), c.top), f32.dtype(at::kLong));
+    r[2] = fresh(plus(tokens_in.sizes(), c.top), at::kFloat, logits);
+    r[3] = fresh(plus(tokens_in.sizes(), c.top), at::kLong, logits);
   }
+  if (grad) r[4] = fresh({3, lead.n0 * lead.n1}, at::kFloat, logits);
   check(blstm_token_log_probs(&d, ptr(logits), ptr(tokens), (float*)r[0].data_ptr(), (float*)r[1].data_ptr(), c.top ? (float*)r[2].data_ptr() : nullptr,
-                              c.top ? (int64_t*)r[3].data_ptr() : nullptr, (float*)r[4].data_ptr(), call.stream),
+                              c.top ? (int64_t*)r[3].data_ptr() : nullptr, grad ? (float*)r[4].data_ptr() : nullptr, call.stream),
         "token_log_probs");
   return r;
 }
@@ -249,42 +287,36 @@ Tensor grad_like(const Tensor& logits, const Lead& lead, const int64_t stride[2]
   }
   const int64_t shift = (reinterpret_cast<uintptr_t>(logits.const_data_ptr()) & 15) / e;
   const int64_t extent = V + (lead.n0 - 1) * dstride[0] + (lead.n1 - 1) * dstride[1];
-  return at::empty({extent + shift}, logits.options().requires_grad(false)).as_strided({lead.n0, lead.n1, V}, {dstride[0], dstride[1], 1}, shift);
+  return fresh({extent + shift}, logits.scalar_type(), logits).as_strided({lead.n0, lead.n1, V}, {dstride[0], dstride[1], 1}, shift);
 }
 
-struct ScoreFn : public torch::autograd::Function<ScoreFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Score& c) {
-    const auto r = score_impl(logits, tokens, c);
-    ctx->saved_data["temperature"] = c.temperature;
-    ctx->saved_data["score"] = std::vector<int64_t>{c.top, c.ignore};
-    ctx->set_materialize_grads(false);
-    if (!c.top) {
-      ctx->save_for_backward({logits, tokens, r[4]});
-      return {r[0], r[1]};
-    }
-    ctx->save_for_backward({logits, tokens, r[4], r[3]});
-    ctx->mark_non_differentiable({r[3]});
-    return {r[0], r[1], r[2], r[3]};
+struct ScoreGrad : public Node {
+  SavedVariable logits, tokens, stats, tops;
+  Score c;
+  void release_variables() override {
+    for (SavedVariable* v : {&logits, &tokens, &stats, &tops}) v->reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+  variable_list apply(variable_list&& g) override {
     only_once();
-    const auto saved = ctx->get_saved_variables();
-    const auto n = ctx->saved_data["score"].toIntVector();
-    const Score c{n[0], ctx->saved_data["temperature"].toDouble(), n[1]};
-    const Lead lead(saved[1].sizes());
-    blstm_score_desc d = score_desc(saved[0], saved[1], lead, c);
-    const Tensor logits = lead.rows(saved[0], d.logits_stride), tokens = lead.rows(saved[1], d.token_stride);
-    if (lead.n0 * lead.n1 == 0) return {at::zeros_like(saved[0]), Tensor(), Tensor()};
-    Call call(logits.device());
+    const Tensor z = logits.unpack(), at_tokens = tokens.unpack(), saved = stats.unpack();
+    const Lead lead(at_tokens.sizes());
+    blstm_score_desc d = score_desc(z, at_tokens, lead, c);
+    const Tensor rows = lead.rows(z, d.logits_stride), given = lead.rows(at_tokens, d.token_stride);
+    if (lead.n0 * lead.n1 == 0) return {at::zeros_like(z)};
+    Call call(z.device());
     int64_t ds[2], s0[2], s1[2];
-    const Tensor dl = grad_like(logits, lead, d.logits_stride, ds);
+    const Tensor dl = grad_like(rows, lead, d.logits_stride, ds);
     const Tensor g0 = g[0].defined() ? lead.rows(g[0], s0) : Tensor(), g1 = g[1].defined() ? lead.rows(g[1], s1) : Tensor();
-    const Tensor g2 = c.top && g[2].defined() ? g[2].contiguous() : Tensor();
-    check(blstm_token_log_probs_grad(&d, ptr(logits), ptr(tokens), (const float*)ptr(saved[2]), c.top ? (const int64_t*)ptr(saved[3]) : nullptr,
-                                     g0.defined() ? (const float*)ptr(g0) : nullptr, s0, g1.defined() ? (const float*)ptr(g1) : nullptr, s1,
-                                     g2.defined() ? (const float*)ptr(g2) : nullptr, dl.data_ptr(), ds, call.stream),
+    Tensor g2, best;
+    if (c.top) {
+      best = tops.unpack();
+      if (g[2].defined()) g2 = g[2].contiguous();
+    }
+    auto f32 = [](const Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; };
+    check(blstm_token_log_probs_grad(&d, ptr(rows), ptr(given), f32(saved), c.top ? static_cast<const int64_t*>(ptr(best)) : nullptr, f32(g0), s0,
+                                     f32(g1), s1, f32(g2), dl.data_ptr(), ds, call.stream),
           "token_log_probs gradient");
-    return {lead.dims == 2 ? dl : dl.reshape(saved[0].sizes()), Tensor(), Tensor()};
+    return {lead.dims == 2 ? dl : dl.reshape(z.sizes())};
   }
 };
 
@@ -303,12 +335,22 @@ py::tuple token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t to
       throw wrong("top must be between 0 and " + std::to_string(std::min<int64_t>(BLSTM_MAX_TOP, logits.size(-1))));
     if (!(temperature >= 1e-30 && std::isfinite((float)temperature))) throw wrong("temperature must be positive (at least 1e-30) and finite");
     const Score c{top, temperature, ignore_index};
-    if (wants_grad(logits)) {
-      const auto v = ScoreFn::apply(logits, tokens, c);
-      std::copy(v.begin(), v.end(), r.begin());
-    } else {
-      const auto v = score_impl(logits, tokens, c);
-      std::copy(v.begin(), v.begin() + 4, r.begin());
+    const bool grad = wants_grad(logits);
+    const auto node = grad ? make_node<ScoreGrad>(logits) : nullptr;
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const auto v = score_impl(logits, tokens, c, grad);
+    std::copy(v.begin(), v.begin() + 4, r.begin());
+    if (grad) {
+      node->logits = SavedVariable(logits, false);
+      node->tokens = SavedVariable(tokens, false);
+      node->stats = SavedVariable(v[4], false);
+      node->c = c;
+      torch::autograd::set_history(r[0], node);
+      torch::autograd::set_history(r[1], node);
+      if (top) {
+        torch::autograd::set_history(r[2], node);
+        node->tops = SavedVariable(r[3], false);
+      }
     }
   }
   return py::make_tuple(r[0], r[1], top ? py::cast(r[2]) : py::none(), top ? py::cast(r[3]) : py::none());

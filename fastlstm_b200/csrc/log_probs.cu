@@ -165,9 +165,11 @@ __device__ __forceinline__ void put_row(const ScoreParams& p, unsigned r, const 
   const bool in = token >= 0 && token < p.vocab;
   p.log_probs[r] = in ? w.log_prob(at_token, p.per_temperature) : __int_as_float(0x7fffffff);
   p.entropy[r] = w.entropy;
-  p.stats[r] = w.m;
-  p.stats[(size_t)p.n + r] = w.log2s;
-  p.stats[2 * (size_t)p.n + r] = w.entropy;
+  if (p.stats) {
+    p.stats[r] = w.m;
+    p.stats[(size_t)p.n + r] = w.log2s;
+    p.stats[2 * (size_t)p.n + r] = w.entropy;
+  }
   if (!in) report_token(p.mailbox, r, token);
 }
 __device__ __forceinline__ void put_top(const ScoreParams& p, unsigned r, const Row& w, int k, unsigned long long key) {
@@ -179,7 +181,8 @@ __device__ __forceinline__ void put_ignored(const ScoreParams& p, unsigned r, un
   if (i == 0) {
     p.log_probs[r] = 0.f;
     p.entropy[r] = 0.f;
-    for (int k = 0; k < 3; ++k) p.stats[(size_t)k * p.n + r] = 0.f;
+    if (p.stats)
+      for (int k = 0; k < 3; ++k) p.stats[(size_t)k * p.n + r] = 0.f;
   }
   if (i < (unsigned)p.top) {
     p.top_log_probs[(size_t)r * p.top + i] = -INFINITY;
@@ -695,7 +698,7 @@ int blstm_token_log_probs(const blstm_score_desc* d, const void* logits, const v
                           float* top_log_probs, int64_t* top_tokens, float* stats, void* stream) {
   if (int rc = check_score(d, logits, tokens)) return rc;
   if (d->n0 == 0 || d->n1 == 0) return BLSTM_OK;
-  if (!log_probs || !entropy || !stats || (d->top && (!top_log_probs || !top_tokens))) return BLSTM_E_INVALID_ARG;
+  if (!log_probs || !entropy || (d->top && (!top_log_probs || !top_tokens))) return BLSTM_E_INVALID_ARG;
   ScoreParams p = score_params(*d, logits, tokens);
   p.log_probs = log_probs; p.entropy = entropy; p.stats = stats;
   p.top_log_probs = top_log_probs; p.top_tokens = reinterpret_cast<long long*>(top_tokens);

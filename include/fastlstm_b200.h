@@ -305,7 +305,7 @@ typedef struct blstm_score_desc {
 /* With z = logits / temperature: log_probs[n0*n1] = log softmax(z)[token], entropy[n0*n1] of softmax(z), and of the `top`
  * largest logits (equal ones by their number) top_log_probs and top_tokens [n0*n1, top] (NULL where top is 0).  A row
  * whose logits are all -inf: -inf, 0, -inf and the first tokens, gradient 0.  stats [3, n0*n1]: what the gradient
- * needs of the row. */
+ * needs of the row, or NULL. */
 int blstm_token_log_probs(const blstm_score_desc* d, const void* logits, const void* tokens, float* log_probs,
                           float* entropy, float* top_log_probs, int64_t* top_tokens, float* stats, void* stream);
 

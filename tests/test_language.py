@@ -125,7 +125,7 @@ def test_score_descriptors_refused(change):
 
 def test_score_pointers_refused():
     lib, d = _lib.load(), _desc(_lib.ScoreDesc, **SCORE)
-    for i in range(7):                    # logits, tokens, log_probs, entropy, top_log_probs, top_tokens, stats
+    for i in range(6):                    # logits, tokens, log_probs, entropy, top_log_probs, top_tokens
         a = [PTR] * 7
         a[i] = None
         assert lib.blstm_token_log_probs(d, *a, None) == 1
