@@ -88,18 +88,19 @@ struct SortParams {
   int element;
 };
 
-// The sort is a chain of short kernels that keep few SMs busy; the others clear dW meanwhile, a part of it in each launch.
-// (Looking up which rows no token names, to clear those alone, took 10 us at 16384 tokens and came after the sort.)
+// The sort is a chain of short kernels that keep few SMs busy; the others clear dW meanwhile, as much of it as that hides in
+// each launch.  What is left sum_kernel clears where no token names a row.
+template <int NT>
 __device__ __forceinline__ void clear(const SortParams& p) {
   const unsigned long long begin = (blockIdx.x - p.tiles) * p.zero_each, end = min(p.zero_bytes, begin + p.zero_each);
   if ((reinterpret_cast<uintptr_t>(p.zero) & 15) == 0) {
     const unsigned long long whole = end & ~15ull;
-    for (unsigned long long i = begin + threadIdx.x * 16; i < whole; i += kSortThreads * 16) *reinterpret_cast<uint4*>(p.zero + i) = make_uint4(0, 0, 0, 0);
-    for (unsigned long long i = max(begin, whole) + threadIdx.x; i < end; i += kSortThreads) p.zero[i] = 0;
+    for (unsigned long long i = begin + threadIdx.x * 16; i < whole; i += NT * 16) *reinterpret_cast<uint4*>(p.zero + i) = make_uint4(0, 0, 0, 0);
+    for (unsigned long long i = max(begin, whole) + threadIdx.x; i < end; i += NT) p.zero[i] = 0;
   } else if (p.element == 4) {
-    for (unsigned long long i = begin + threadIdx.x * 4; i < end; i += kSortThreads * 4) *reinterpret_cast<unsigned*>(p.zero + i) = 0;
+    for (unsigned long long i = begin + threadIdx.x * 4; i < end; i += NT * 4) *reinterpret_cast<unsigned*>(p.zero + i) = 0;
   } else {
-    for (unsigned long long i = begin + threadIdx.x * 2; i < end; i += kSortThreads * 2) *reinterpret_cast<unsigned short*>(p.zero + i) = 0;
+    for (unsigned long long i = begin + threadIdx.x * 2; i < end; i += NT * 2) *reinterpret_cast<unsigned short*>(p.zero + i) = 0;
   }
 }
 
@@ -114,7 +115,7 @@ template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_constant__ SortParams p) {
   __shared__ unsigned hist[kMaxBins];
   const unsigned bins = 1u << p.bits, tile = blockIdx.x;
-  if (tile >= p.tiles) return clear(p);
+  if (tile >= p.tiles) return clear<kSortThreads>(p);
   for (unsigned b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
 #pragma unroll
@@ -143,14 +144,34 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
   __shared__ unsigned sums[kSortWarps];
   const unsigned bins = 1u << p.bits, tile = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = p.pass * p.bits;
-  if (tile >= p.tiles) return clear(p);
+  if (tile >= p.tiles) return clear<kSortThreads>(p);
   for (unsigned b = tid; b < kSortWarps * kMaxBins / 2; b += kSortThreads) reinterpret_cast<unsigned*>(hist)[b] = 0;
   __syncthreads();
 
-  unsigned key[ITEMS], rank[ITEMS];
+  unsigned key[ITEMS], pos[ITEMS], rank[ITEMS];
   const unsigned first = tile * (ITEMS * kSortThreads) + warp * (ITEMS * 32) + lane;
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) key[j] = first + j * 32 < p.n ? p.keys_in[first + j * 32] : 0;
+  for (int j = 0; j < ITEMS; ++j) {
+    const unsigned i = first + j * 32;
+    key[j] = i < p.n ? p.keys_in[i] : 0;
+    pos[j] = i < p.n && p.pos_in ? p.pos_in[i] : i;
+  }
+
+  // counts of this digit before this tile, and in all of them: a thread takes four digits of every fourth to sixty-fourth tile
+  __shared__ uint4 sum_before[kSortThreads], sum_total[kSortThreads];
+  {
+    const unsigned quads = bins / 4, lanes = kSortThreads / quads, q = tid % quads;
+    const uint4* c = reinterpret_cast<const uint4*>(p.counts + (size_t)p.pass * p.tiles * bins) + q;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+#pragma unroll 16
+    for (unsigned t = tid / quads; t < p.tiles; t += lanes) {
+      const uint4 v = c[(size_t)t * quads];
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+      if (t < tile) { b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w; }
+    }
+    sum_total[tid] = a;
+    sum_before[tid] = b;
+  }
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) {
     const bool in = first + j * 32 < p.n;
@@ -161,22 +182,6 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
     __syncwarp();
     if (in && below == 0) hist[warp][d] += (unsigned short)__popc(peers);
     __syncwarp();
-  }
-
-  // counts of this digit before this tile, and in all of them: a thread takes four digits of every fourth to sixty-fourth tile
-  __shared__ uint4 sum_before[kSortThreads], sum_total[kSortThreads];
-  {
-    const unsigned quads = bins / 4, lanes = kSortThreads / quads, q = tid % quads;
-    const uint4* c = reinterpret_cast<const uint4*>(p.counts + (size_t)p.pass * p.tiles * bins) + q;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-#pragma unroll 8
-    for (unsigned t = tid / quads; t < p.tiles; t += lanes) {
-      const uint4 v = c[(size_t)t * quads];
-      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-      if (t < tile) { b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w; }
-    }
-    sum_total[tid] = a;
-    sum_before[tid] = b;
   }
   __syncthreads();
   unsigned before = 0, total = 0;
@@ -214,15 +219,111 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid
     if (i >= p.n) continue;
     const unsigned d = (key[j] >> shift) & (bins - 1), to = base[d] + hist[warp][d] + rank[j];
     p.keys[to] = key[j];
-    p.pos[to] = p.pos_in ? p.pos_in[i] : i;
+    p.pos[to] = pos[j];
     if (more) atomicAdd(&next[(size_t)(to / (ITEMS * kSortThreads)) * bins + ((key[j] >> (shift + p.bits)) & (bins - 1))], 1u);
   }
 }
 
+// The same sort of up to 32768 positions in one launch, by a cluster of eight blocks whose tiles are all there is: the counts of
+// a digit are read from the other blocks' shared memory, and the elements change places through global memory.
+constexpr int kClusterBlocks = 8, kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterSort = kClusterBlocks * kClusterThreads * 4;
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __grid_constant__ SortParams p, unsigned* keys2, unsigned* pos2) {
+  __shared__ unsigned short hist[kClusterWarps][kMaxBins];
+  __shared__ unsigned base[kMaxBins], count[kMaxBins];
+  __shared__ unsigned sums[kClusterWarps];
+  const unsigned bins = 1u << p.bits, tile = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tile >= kClusterBlocks) return clear<kClusterThreads>(p);       // (a cluster of its own)
+  const unsigned first = tile * (ITEMS * kClusterThreads) + warp * (ITEMS * 32) + lane;
+  unsigned key[ITEMS], pos[ITEMS], rank[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    pos[j] = first + j * 32;
+    key[j] = pos[j] < p.n ? sort_key(p, pos[j]) : 0;
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    unsigned* keys = (p.passes - pass) & 1 ? p.keys : keys2;          // (the last pass ends in p.keys)
+    unsigned* to_pos = (p.passes - pass) & 1 ? p.pos : pos2;
+    for (unsigned b = tid; b < kClusterWarps * kMaxBins / 2; b += kClusterThreads) reinterpret_cast<unsigned*>(hist)[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const bool in = first + j * 32 < p.n;
+      const unsigned d = in ? (key[j] >> shift) & (bins - 1) : bins;
+      const unsigned peers = __match_any_sync(0xffffffffu, d);
+      const unsigned below = __popc(peers & ((1u << lane) - 1));
+      rank[j] = in ? hist[warp][d] + below : 0;
+      __syncwarp();
+      if (in && below == 0) hist[warp][d] += (unsigned short)__popc(peers);
+      __syncwarp();
+    }
+    __syncthreads();
+    if (tid < bins) {
+      unsigned short in_tile = 0;
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const unsigned short v = hist[w][tid];
+        hist[w][tid] = in_tile;
+        in_tile += v;
+      }
+      count[tid] = in_tile;
+    }
+    cluster_sync();
+    unsigned before = 0, total = 0;
+    if (tid < bins) {
+      const unsigned at = (unsigned)__cvta_generic_to_shared(&count[tid]);
+#pragma unroll
+      for (unsigned r = 0; r < kClusterBlocks; ++r) {
+        unsigned remote, v;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(r));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+        total += v;
+        before += r < tile ? v : 0;
+      }
+    }
+    unsigned scan = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= (unsigned)o) scan += v;
+    }
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    if (tid < bins) {
+      unsigned at = scan - total + before;
+      for (unsigned w = 0; w < warp; ++w) at += sums[w];
+      base[tid] = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      if (first + j * 32 >= p.n) continue;
+      const unsigned d = (key[j] >> shift) & (bins - 1), to = base[d] + hist[warp][d] + rank[j];
+      keys[to] = key[j];
+      to_pos[to] = pos[j];
+    }
+    cluster_sync();                            // (also: nobody reads this block's counts any more)
+    if (pass + 1 < p.passes)
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j)
+        if (first + j * 32 < p.n) {
+          key[j] = __ldcg(keys + first + j * 32);
+          pos[j] = __ldcg(to_pos + first + j * 32);
+        }
+  }
+}
+
 // ---------------------------------------------------------------- sums of equal tokens' rows
-constexpr int kRunStep = 8;          // rows on their way at a time
-constexpr int kMaxRun = 32;          // sorted positions that one group of threads adds up
-constexpr int kZeroRows = 16;        // rows of dW that one block of few_kernel clears
+constexpr int kRunStep = 4;          // rows on their way at a time
+constexpr int kMinRun = 8, kMaxRun = 64;     // sorted positions that one group of threads adds up
+constexpr int kZeroRows = 16, kClearRows = 64;   // rows of dW that one block of few_kernel, of sum_kernel looks after
 
 struct SumParams {
   const void* dout;
@@ -232,7 +333,8 @@ struct SumParams {
   long long padding;
   const unsigned *keys, *pos;
   float* part;                       // [runs][2][width]: of a token that began in an earlier run, of one that goes on in the next
-  unsigned n, vocab, run, runs;
+  unsigned n, vocab, run, runs, sum_blocks;
+  unsigned cleared;                  // rows of dW that the sort has cleared
   unsigned width, pieces, group;     // group: threads of a run, a power of two
   float scale;
 };
@@ -259,14 +361,42 @@ __device__ __forceinline__ void put_sum(const SumParams& p, unsigned t, unsigned
   static_cast<Pack<T, VEC>*>(p.dweight)[(size_t)t * p.pieces + c] = r;
 }
 
+// What follows a position of a run: the same token, the token's last one, or its last one here of a token that goes on, or that
+// began before.
+enum : unsigned { kGoesOn = 0, kWhole = 1, kLastPart = 2, kFirstPart = 3 };
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumParams p) {
   using V = Pack<T, VEC>;
   __shared__ unsigned s_key[256 / 4 * kMaxRun], s_pos[256 / 4 * kMaxRun];
+  __shared__ unsigned char s_then[256 / 4 * kMaxRun];
+  if (blockIdx.x >= p.sum_blocks) {            // rows that no token names
+    if (blockIdx.y) return;
+    const unsigned v0 = p.cleared + (blockIdx.x - p.sum_blocks) * kClearRows, rows = min((unsigned)kClearRows, p.vocab - v0);
+    if (threadIdx.x < rows) {
+      unsigned lo = 0, hi = p.n;
+      while (lo < hi) {
+        const unsigned mid = (lo + hi) >> 1;
+        if (p.keys[mid] < v0 + threadIdx.x) lo = mid + 1; else hi = mid;
+      }
+      s_key[threadIdx.x] = lo < p.n && p.keys[lo] == v0 + threadIdx.x;
+    }
+    __syncthreads();
+    zero_rows<T, VEC>(p, v0, rows, s_key);
+    return;
+  }
   const unsigned runs_here = 256 / p.group, first = blockIdx.x * runs_here * p.run;
   for (unsigned i = threadIdx.x; i < runs_here * p.run; i += 256) {
-    s_key[i] = first + i < p.n ? p.keys[first + i] : p.vocab;
-    s_pos[i] = first + i < p.n ? p.pos[first + i] : 0;
+    const unsigned at = first + i, j = i % p.run;
+    const unsigned t = at < p.n ? p.keys[at] : p.vocab, after = at + 1 < p.n ? p.keys[at + 1] : p.vocab;
+    s_key[i] = t;
+    s_pos[i] = at < p.n ? p.pos[at] : 0;
+    unsigned then = kGoesOn;
+    if (t != p.vocab && (after != t || j + 1 == p.run)) {
+      const bool began_before = at > j && p.keys[at - j - 1] == t;
+      then = began_before ? kLastPart : after == t ? kFirstPart : kWhole;
+    }
+    s_then[i] = (unsigned char)then;
   }
   __syncthreads();
   const unsigned mine = threadIdx.x / p.group, run = blockIdx.x * runs_here + mine;
@@ -274,8 +404,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumPar
   if (c >= p.pieces || run >= p.runs) return;
   const unsigned* key = s_key + mine * p.run;
   const unsigned* pos = s_pos + mine * p.run;
-  const unsigned i0 = run * p.run;
-  const unsigned before = i0 ? p.keys[i0 - 1] : p.vocab, after = i0 + p.run < p.n ? p.keys[i0 + p.run] : p.vocab;
+  const unsigned char* then = s_then + mine * p.run;
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
@@ -283,22 +412,21 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumPar
     V v[kRunStep];
 #pragma unroll
     for (int u = 0; u < kRunStep; ++u)
-      if (key[j0 + u] != p.vocab) v[u] = *reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(pos[j0 + u]) + (size_t)c * VEC);
+      if (key[j0 + u] != p.vocab) v[u] = reinterpret_cast<const V*>(static_cast<const T*>(p.dout) + p.rows(pos[j0 + u]))[c];
 #pragma unroll
     for (int u = 0; u < kRunStep; ++u) {
-      const unsigned j = j0 + u, t = key[j];
-      if (t == p.vocab) break;
+      if (key[j0 + u] == p.vocab) break;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] += Elem<T>::to_f(v[u].v[k]);
-      const unsigned then = j + 1 < p.run ? key[j + 1] : after;
-      if (then == t && j + 1 < p.run) continue;
-      const bool began_before = t == before;
-      if (began_before || then == t) {         // a part of a token's sum
-        Pack<float, VEC % 4 ? VEC : 4>* q = reinterpret_cast<Pack<float, VEC % 4 ? VEC : 4>*>(p.part + ((size_t)run * 2 + (began_before ? 0 : 1)) * p.width + (size_t)c * VEC);
+      const unsigned what = then[j0 + u];
+      if (what == kGoesOn) continue;
+      if (what == kWhole) {
+        put_sum<T, VEC>(p, key[j0 + u], c, acc);
+      } else {
+        using Q = Pack<float, VEC % 4 ? VEC : 4>;
+        Q* q = reinterpret_cast<Q*>(p.part + ((size_t)run * 2 + (what == kFirstPart)) * p.width + (size_t)c * VEC);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) q[k / 4].v[k % 4] = acc[k];
-      } else {
-        put_sum<T, VEC>(p, t, c, acc);
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
@@ -306,16 +434,19 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumPar
   }
 }
 
-// Tokens whose positions reach over several runs.  A warp looks after a run, and 128 columns: where a token begins in it and
-// goes on, it adds the parts up; where there are more than a few the eight warps of the block do, each every eighth of them.
-constexpr unsigned kLong = 8;
+// Tokens whose positions reach over several runs.  A warp looks after a run, and 256 columns: where a token begins in it and
+// goes on, it adds the parts up; where there are more than a few all warps of the block do, in turn.
+constexpr unsigned kLong = 8, kJoinWarps = 16, kJoinCols = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumParams p) {
-  __shared__ float s_sum[8][128];
-  __shared__ unsigned s_parts[8], s_token[8];
+// A: 4 where rows of parts begin on 16 bytes, else 1.
+template <typename T, int A>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ SumParams p) {
+  using Q = Pack<float, A>;
+  constexpr int K = kJoinCols / 32 / A;                    // of 32 lanes' Qs
+  __shared__ float s_sum[kJoinWarps - 1][kJoinCols];
+  __shared__ unsigned s_parts[kJoinWarps], s_token[kJoinWarps];
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned mine = blockIdx.x * 8 + warp, end = (mine + 1) * p.run;
+  const unsigned mine = blockIdx.x * kJoinWarps + warp, end = (mine + 1) * p.run;
   unsigned t = p.vocab, parts = 0;
   if (end < p.n) {
     t = p.keys[end - 1];
@@ -334,38 +465,46 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumPa
     }
   }
   if (lane == 0) { s_parts[warp] = parts; s_token[warp] = t; }
-  const unsigned c0 = blockIdx.y * 128 + lane;
-  auto add = [&](unsigned run, unsigned from, unsigned parts, unsigned step, float (&acc)[4]) {
+  const unsigned q0 = blockIdx.y * (kJoinCols / A) + lane, quads = p.width / A;
+  auto add = [&](unsigned run, unsigned from, unsigned parts, unsigned step, float (&acc)[K * A]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = 0.f;
-#pragma unroll 8
+    for (int k = 0; k < K * A; ++k) acc[k] = 0.f;
+#pragma unroll 4
     for (unsigned r = from; r < parts; r += step) {
-      const float* q = p.part + ((size_t)(run + r) * 2 + (r == 0)) * p.width + c0;
+      const Q* q = reinterpret_cast<const Q*>(p.part + ((size_t)(run + r) * 2 + (r == 0)) * p.width) + q0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) if (c0 + k * 32 < p.width) acc[k] += q[k * 32];
+      for (int k = 0; k < K; ++k)
+        if (q0 + k * 32 < quads) {
+          const Q v = q[k * 32];
+#pragma unroll
+          for (int i = 0; i < A; ++i) acc[k * A + i] += v.v[i];
+        }
     }
   };
-  auto put = [&](unsigned t, const float (&acc)[4]) {
+  auto put = [&](unsigned t, const float (&acc)[K * A]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c0 + k * 32 < p.width) static_cast<T*>(p.dweight)[(size_t)t * p.width + c0 + k * 32] = Elem<T>::from_f(acc[k] * p.scale);
+    for (int k = 0; k < K; ++k)
+      if (q0 + k * 32 < quads)
+#pragma unroll
+        for (int i = 0; i < A; ++i) static_cast<T*>(p.dweight)[(size_t)t * p.width + (q0 + k * 32) * A + i] = Elem<T>::from_f(acc[k * A + i] * p.scale);
   };
-  float acc[4];
+  float acc[K * A];
   if (parts > 0 && parts <= kLong) {
     add(mine, 0, parts, 1, acc);
     put(t, acc);
   }
   __syncthreads();
-  for (unsigned w = 0; w < 8; ++w) {
+  for (unsigned w = 0; w < kJoinWarps; ++w) {
     if (s_parts[w] <= kLong) continue;
-    add(blockIdx.x * 8 + w, warp, s_parts[w], 8, acc);
+    add(blockIdx.x * kJoinWarps + w, warp, s_parts[w], kJoinWarps, acc);
+    if (warp)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s_sum[warp][k * 32 + lane] = acc[k];
+      for (int k = 0; k < K * A; ++k) s_sum[warp - 1][k * 32 + lane] = acc[k];
     __syncthreads();
     if (warp == 0) {
-      for (int q = 1; q < 8; ++q)
+      for (unsigned q = 0; q < min(s_parts[w], kJoinWarps) - 1; ++q)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += s_sum[q][k * 32 + lane];
+        for (int k = 0; k < K * A; ++k) acc[k] += s_sum[q][k * 32 + lane];
       put(s_token[w], acc);
     }
     __syncthreads();
@@ -486,8 +625,9 @@ static GradPlan grad_plan(int64_t n, int64_t vocab, int64_t width) {
   while (bits < 32 && (vocab >> bits) != 0) ++bits;       // keys go up to `vocab` itself
   g.passes = (bits + 8) / 9;
   g.bits = std::max(2, (bits + g.passes - 1) / g.passes);
-  // runs of eight positions where there are few, so that many are on their way; long ones leave fewer parts to join
-  g.run = n <= 32768 ? kRunStep : kMaxRun;
+  // about 2048 runs: enough to keep all SMs busy, and no more parts to join than that takes
+  g.run = kMinRun;
+  while (g.run < kMaxRun && n > 2048ll * g.run) g.run *= 2;
   g.runs = (unsigned)((n + g.run - 1) / g.run);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t o = at; at = round_up(at + bytes, 256); return o; };
@@ -577,8 +717,8 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
   p.group = 4;
   while (p.group < 256 && p.group < p.pieces) p.group *= 2;
   p.scale = d->scale;
-  const unsigned zero_blocks = (p.vocab + kZeroRows - 1) / kZeroRows;
   if (n <= kFew) {
+    const unsigned zero_blocks = (p.vocab + kZeroRows - 1) / kZeroRows;
     const unsigned lane_pieces = piece == 16 && e == 2 ? 4 : 8;          // (K of the kernel)
     const dim3 grid(p.n + zero_blocks, (p.pieces + 32 * lane_pieces - 1) / (32 * lane_pieces));
     if (grid.y > 65535) return BLSTM_E_TOO_LARGE;
@@ -601,35 +741,56 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
   s.n = (unsigned)n; s.tiles = g.tiles;
   s.passes = g.passes; s.bits = g.bits;
   s.keys = at(g.keys[0]); s.counts = at(g.counts);
-  // a third or so of dW in each launch, 64 KB a block
-  const unsigned long long all = (unsigned long long)d->vocab * d->width * e;
-  const unsigned long long part = ((all + g.passes) / (g.passes + 1) + 15) & ~15ull;
+  // dW, as much of it in each launch as the sort hides (32 MB take 5 us), 64 KB a block
+  const bool cluster = n <= kClusterSort;
+  const int launches = cluster ? 1 : g.passes + 1;
+  const size_t row_bytes = (size_t)d->width * e;
+  p.cleared = (unsigned)std::min<unsigned long long>(p.vocab, (unsigned long long)launches * (cluster ? 64u << 20 : 32u << 20) / row_bytes);
+  if (bits & 15) p.cleared = p.vocab;                     // (rows in pieces of 16 bytes alone)
+  const unsigned long long all = (unsigned long long)p.cleared * row_bytes, part = ((all + launches - 1) / launches + 15) & ~15ull;
   s.zero_each = 65536;
   s.element = e;
   auto blocks = [&](int launch) {
     const unsigned long long begin = std::min(all, part * launch), end = std::min(all, begin + part);
     s.zero = static_cast<char*>(dweight) + begin;
     s.zero_bytes = end - begin;
-    return (unsigned)(g.tiles + (s.zero_bytes + s.zero_each - 1) / s.zero_each);
+    return (unsigned)((s.zero_bytes + s.zero_each - 1) / s.zero_each);
   };
-  unsigned grid = blocks(0);
-  if (g.items == 4) sort_count_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
-  else sort_count_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
-  BLSTM_CUDA_OK(cudaGetLastError());
-  for (s.pass = 0; s.pass < g.passes; ++s.pass) {
-    const int from = s.pass & 1;
-    s.keys_in = at(g.keys[from]); s.pos_in = s.pass ? at(g.pos[from]) : nullptr;
-    s.keys = at(g.keys[1 - from]); s.pos = at(g.pos[1 - from]);
-    grid = blocks(1 + s.pass);
-    if (g.items == 4) sort_scatter_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
-    else sort_scatter_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
+  if (cluster) {
+    s.tiles = kClusterBlocks;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {kClusterBlocks, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = kClusterBlocks + (blocks(0) + kClusterBlocks - 1) / kClusterBlocks * kClusterBlocks;
+    cfg.blockDim = kClusterThreads;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    s.pos = at(g.pos[0]);
+    if (n <= kClusterSort / 2) BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<2>, s, at(g.keys[1]), at(g.pos[1])));
+    else BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<4>, s, at(g.keys[1]), at(g.pos[1])));
+  } else {
+    unsigned grid = g.tiles + blocks(0);
+    if (g.items == 4) sort_count_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
+    else sort_count_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
     BLSTM_CUDA_OK(cudaGetLastError());
+    for (s.pass = 0; s.pass < g.passes; ++s.pass) {
+      const int from = s.pass & 1;
+      s.keys_in = at(g.keys[from]); s.pos_in = s.pass ? at(g.pos[from]) : nullptr;
+      s.keys = at(g.keys[1 - from]); s.pos = at(g.pos[1 - from]);
+      grid = g.tiles + blocks(1 + s.pass);
+      if (g.items == 4) sort_scatter_kernel<4><<<grid, kSortThreads, 0, st>>>(s);
+      else sort_scatter_kernel<16><<<grid, kSortThreads, 0, st>>>(s);
+      BLSTM_CUDA_OK(cudaGetLastError());
+    }
   }
 
   p.keys = s.keys; p.pos = s.pos;
   p.part = reinterpret_cast<float*>(ws + g.part);
   p.run = g.run; p.runs = g.runs;
-  const dim3 sums((g.runs + 256 / p.group - 1) / (256 / p.group), (p.pieces + 255) / 256), joins((g.runs + 7) / 8, (p.width + 127) / 128);
+  p.sum_blocks = (g.runs + 256 / p.group - 1) / (256 / p.group);
+  const dim3 sums(p.sum_blocks + (p.vocab - p.cleared + kClearRows - 1) / kClearRows, (p.pieces + 255) / 256), joins((g.runs + kJoinWarps - 1) / kJoinWarps, (p.width + kJoinCols - 1) / kJoinCols);
   if (sums.y > 65535 || joins.y > 65535) return BLSTM_E_TOO_LARGE;
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
@@ -637,9 +798,10 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
     else if (piece == 4) sum_kernel<T, 4 / sizeof(T)><<<sums, 256, 0, st>>>(p);
     else sum_kernel<T, 1><<<sums, 256, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
-    join_kernel<T><<<joins, 256, 0, st>>>(p);
+    if (p.width % 4 == 0) join_kernel<T, 4><<<joins, 32 * kJoinWarps, 0, st>>>(p);
+    else join_kernel<T, 1><<<joins, 32 * kJoinWarps, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
-    count_launch(3 + g.passes);
+    count_launch(launches + 2);
     return BLSTM_OK;
   });
 }
