@@ -114,6 +114,39 @@ def test_embedding_layouts(T, B, width):
         check_embedding(tokens, cut, "bf16")
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [2048, 2049, 16384, 16385, 32768, 32769, 65536, 262144, 262145])
+def test_embedding_at_the_lines_between_sorts(n, dtype):
+    g = gen(n)
+    tokens = (700 ** torch.rand(n, generator=g, device="cuda")).long()
+    check_embedding(tokens, torch.randn(700, 12, generator=g, device="cuda").to(DT[dtype]), dtype, padding=0)
+
+
+@pytest.mark.parametrize("n,vocab,width,dtype", [(700, 60000, 640, "fp16"), (3000, 150000, 512, "bf16"), (3000, 40001, 700, "fp32"),
+                                                 (40000, 120000, 512, "fp16"), (33000, 60000, 800, "fp32"), (33000, 70001, 301, "fp32")])
+def test_embedding_rows_that_no_token_names(n, vocab, width, dtype):
+    """Tables larger than what is cleared beside the sort; the memory that the gradient gets held NaN before."""
+    g = gen(n + width)
+    tokens = torch.cat([torch.randint(0, vocab, (n - 3,), generator=g, device="cuda"), torch.tensor([vocab - 1, 0, vocab - 1], device="cuda")])
+    W = torch.zeros(vocab, width, device="cuda", dtype=DT[dtype]).requires_grad_()
+    out = F.embedding(tokens, W, padding_idx=5)
+    dout = torch.randn(n, width, generator=g, device="cuda").to(W.dtype)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    poison = torch.full_like(W, float("nan"))
+    del poison
+    (dW,) = torch.autograd.grad(out, W, dout)
+    met = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    met[tokens] = True
+    met[5] = False
+    assert not dW[~met].any()
+    want = torch.zeros(vocab, width, device="cuda", dtype=torch.float64).index_add_(0, tokens, dout.double())
+    size = torch.zeros(vocab, width, device="cuda", dtype=torch.float64).index_add_(0, tokens, dout.double().abs())
+    terms = torch.bincount(tokens, minlength=vocab).double()[:, None]
+    bound = (terms + 2) * U * size + EPS[dtype] * want.abs() + TINY[dtype]
+    assert ((dW.double() - want).abs() <= bound)[met].all()
+
+
 def test_embedding_without_tokens():
     W = torch.randn(5, 3, device="cuda", requires_grad=True)
     out = F.embedding(torch.zeros(0, 4, dtype=torch.long, device="cuda"), W)
@@ -540,3 +573,56 @@ def test_another_stream_and_no_gradients():
     for a, b, c in zip(want, got, free):
         assert torch.equal(a, b) and torch.equal(a, c)
     assert torch.equal(grads[0], again[0])
+
+
+# ---------------------------------------------------------------- together
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "language_model.py")
+    spec = importlib.util.spec_from_file_location("language_model", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_language_model_gradients_match_torch():
+    """One step of the example's model without dropout against torch's own layers in 64 bits: each of the four operators that the
+    gradients pass through is within 1e-5 of its tensor's norm in fp32."""
+    m = _example()
+    torch.manual_seed(3)
+    model = m.LanguageModel(70, 48, layers=2, dropout=0.0, dtype=torch.float32)
+    tokens, targets = m.batch(70, 12, 5, gen(1))
+    loss = model.loss(tokens, targets, entropy_weight=0.1)
+    grads = torch.autograd.grad(loss, list(model.parameters()))
+    table = model.table.detach().double().requires_grad_()
+    layers = [torch.nn.LSTM(48, 48, dtype=torch.float64, device="cuda") for _ in range(2)]
+    for a, b in zip(layers, model.layers):
+        a.load_state_dict({k: v.double() for k, v in b.state_dict().items()})
+    x = torch.nn.functional.embedding(tokens, table, padding_idx=m.PADDING) * 48 ** 0.5
+    for layer in layers:
+        x, _ = layer(x)
+    lp = torch.log_softmax(x @ table.t(), -1)
+    live = targets != m.PADDING
+    want = -((lp.gather(2, targets[..., None])[..., 0] - 0.1 * (lp.exp() * lp).sum(-1)) * live).sum() / live.sum()
+    ref = torch.autograd.grad(want, [table] + [p for layer in layers for p in layer.parameters()])
+    assert abs(float(loss.detach()) - float(want.detach())) <= 4e-5 * abs(float(want.detach()))
+    for (name, _), a, b in zip(model.named_parameters(), grads, ref):
+        assert float((a.double() - b).norm()) <= 4e-5 * float(b.norm()), name
+
+
+def test_language_model_learns_and_repeats():
+    m = _example()
+
+    def once():
+        torch.manual_seed(5)
+        model = m.LanguageModel(60, 64, layers=2, dropout=0.1, dtype=torch.float32)
+        return model, m.train(model, 60, T=24, B=32)
+    model, losses = once()
+    assert losses == once()[1]
+    assert sum(losses[-5:]) < 0.5 * sum(losses[:5])
+    model.eval()
+    start = 1 + torch.arange(8, device="cuda")[:, None] * torch.tensor([1, 2], device="cuda")
+    tokens, lp, top_tokens, top_lp = model.go_on(start, 4, top=3)
+    assert tokens.shape == lp.shape == (4, 2) and top_tokens.shape == top_lp.shape == (4, 2, 3)
+    assert torch.equal(tokens, top_tokens[..., 0]) and (top_lp[..., :-1] >= top_lp[..., 1:]).all()
