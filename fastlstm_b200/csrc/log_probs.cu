@@ -341,7 +341,7 @@ template <int NT>
 struct ScoreShared {
   Part part[NT / 32];
   uint2 peers[kMaxCluster][2];                          // maximum and sum, second sum, of every block of a cluster
-  unsigned group[kGroups];
+  alignas(16) unsigned group[kGroups];
   unsigned owner[NT];
   unsigned owners, count;
   unsigned long long bound;
@@ -362,14 +362,28 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
   if (tid == 0) { s.owners = 0; s.count = 0; }
   if (tid < top) s.best[tid] = 0;              // (a block may have fewer)
   __syncthreads();
-  // the `top`-th largest of the groups' maxima, in every warp: the largest, those that are left without it, and so on
-  unsigned a = s.group[lane], b = s.group[lane + 32], bound, found = 0;
-  do {
-    bound = __reduce_max_sync(~0u, max(a, b));
-    found += __popc(__ballot_sync(~0u, a == bound)) + __popc(__ballot_sync(~0u, b == bound));
-    if (a == bound) a = 0;                     // (no key is 0)
-    if (b == bound) b = 0;
-  } while (found < top);
+  // The `top`-th largest of the groups' maxima, in every warp.  A few: the largest, those that are left without it, and so on.
+  // Many: every lane counts how many of the 64 are above its two.
+  unsigned a = s.group[lane], b = s.group[lane + 32], bound;
+  if (top <= 8) {
+    unsigned found = 0;
+    do {
+      bound = __reduce_max_sync(~0u, max(a, b));
+      found += __popc(__ballot_sync(~0u, a == bound)) + __popc(__ballot_sync(~0u, b == bound));
+      if (a == bound) a = 0;                   // (no key is 0)
+      if (b == bound) b = 0;
+    } while (found < top);
+  } else {
+    unsigned above_a = 0, above_b = 0;
+#pragma unroll 4
+    for (unsigned i = 0; i < kGroups; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(s.group + i);
+      above_a += (v.x > a) + (v.y > a) + (v.z > a) + (v.w > a);
+      above_b += (v.x > b) + (v.y > b) + (v.z > b) + (v.w > b);
+    }
+    // (equal ones count alike: the smallest that fewer than `top` are above)
+    bound = __reduce_min_sync(~0u, min(above_a < top ? a : ~0u, above_b < top ? b : ~0u));
+  }
   if (mine >= bound) s.owner[atomicAdd(&s.owners, 1u)] = tid;
   __syncthreads();
   auto offer = [&](float z, unsigned j, unsigned long long least) {
@@ -385,13 +399,19 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
 #pragma unroll
     for (int i = 1; i < kPer<T>; ++i) m = max_nan(m, z[i]);
     if (value_key(m) < (unsigned)(least >> 32)) return;
+    unsigned some = 0;
 #pragma unroll
-    for (int i = 0; i < kPer<T>; ++i) offer(z[i], span.number(piece) + i, least);
+    for (int i = 0; i < kPer<T>; ++i) some |= (value_key(z[i]) >= (unsigned)(least >> 32) ? 1u : 0u) << i;
+#pragma unroll 1
+    for (; some; some &= some - 1) {           // (few, so in little code: it runs once a block)
+      const unsigned j = span.number(piece) + __ffs(some) - 1;
+      offer(ld_f(span.row + j), j, least);
+    }
   };
   // the owners' pieces, all threads side by side
   const unsigned owners = s.owners, each = (span.end - span.begin + NT - 1) / NT;
   const unsigned long long least = (unsigned long long)bound << 32;
-  constexpr int kLook = 4;
+  constexpr int kLook = 2;
   for (unsigned i0 = tid; i0 < owners * each; i0 += kLook * NT) {
     uint4 v[kLook];
     unsigned piece[kLook];
@@ -489,10 +509,22 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
   if constexpr (TOP) {
     if (parts == 1) {
       if (tid < (unsigned)p.top) put_top(p, r, w, tid, s.best[tid]);
-    } else if (tid < parts * p.top) {
-      const unsigned long long key = s.best[tid];
-      const unsigned before = rank_of(s.best, parts * p.top, key);
-      if (before < (unsigned)p.top && key) put_top(p, r, w, before, key);
+    } else {
+      // The blocks' lists, each in order, as one: eight lanes a key, each of which finds how many of one list come before it.
+      const unsigned q = tid % kMaxCluster;
+#pragma unroll 1
+      for (unsigned i0 = 0; i0 < parts * p.top; i0 += NT / kMaxCluster) {
+        const unsigned i = i0 + tid / kMaxCluster;
+        const unsigned long long key = i < parts * p.top ? s.best[i] : 0;
+        unsigned before = 0;
+        if (q < parts)
+#pragma unroll
+          for (unsigned step = BLSTM_MAX_TOP; step; step >>= 1)
+            if (before + step <= (unsigned)p.top && s.best[q * p.top + before + step - 1] > key) before += step;
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) before += __shfl_xor_sync(~0u, before, o);
+        if (q == 0 && key && before < (unsigned)p.top) put_top(p, r, w, before, key);
+      }
     }
   }
 }
