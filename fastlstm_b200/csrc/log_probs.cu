@@ -668,13 +668,14 @@ static ScoreParams score_params(const blstm_score_desc& d, const void* logits, c
 // 16-byte pieces of a row: what they are at least, and at most where it does not begin on a boundary (fewer elements are left).
 static unsigned row_pieces(const ScoreParams& p, size_t element) { return (unsigned)((unsigned long long)p.vocab * element / 16); }
 
-// Threads of a block.  Rows end with a few hundred clocks in which nothing is read, and the more rows an SM has the less
-// that shows (8192 x 50000 bf16 with 64 / 128 / 256 threads: 129 / 132 / 139 us; 32768 x 10007: 121 / 144 / 234).  Looking for
-// alternatives takes more threads a row: each of theirs that has one reads its share of the row again (with 5: 198 / 166 / 177,
-// with 20: 292 / 248 / 220, 131072 logits 371 / 291 / 253; 4096 logits 323 / 400 / 701).  Few rows take more threads each.
+// Threads of a block.  A row ends with some hundred clocks in which nothing is read, and the more rows an SM has at a time the
+// less that shows; long rows have it seldom and take the threads.  bf16, us with 64 / 128 / 256 threads: 32768 x 10007 118 / 136 /
+// 221, 8192 x 50000 130 / 133 / 139, 4096 x 131072 176 / 169 / 169.  Alternatives cost more at every row's end, but each thread
+// that has one has its share of the row read again, which is shorter the more there are: with 5 at 65536 x 4096 187 / 287 / 492, at
+// 16384 x 20000 155 / 151 / 198, at 8192 x 50000 193 / 164 / 171, at 4096 x 131072 257 / 209 / 194.  Few rows take more threads each.
 static unsigned score_threads(const ScoreParams& p, size_t element) {
   const unsigned pieces = row_pieces(p, element);
-  unsigned threads = p.top == 0 || pieces < 1024 ? 64 : pieces < 6000 ? 128 : 256;
+  unsigned threads = p.top == 0 ? (pieces < 8192 ? 64 : 128) : pieces < 1024 ? 64 : pieces < 8192 ? 128 : 256;
   while (threads < 256 && (unsigned long long)p.n * threads < 1024ull * plan_sm_count() && pieces >= threads * 2) threads *= 2;
   return threads;
 }
