@@ -102,6 +102,9 @@ __device__ __forceinline__ uint4 masked(const uint4& v, const uint4& bits, float
 }
 
 // Every element its own word, 16-byte pieces, kPieces a thread.  ROWS: rows of x have strides of their own.
+// A block of four words takes 20 products of 32 x 32 bits to 64, which an SM makes 32 lanes of a clock: 1.77e12 words/s.  256 x 512 x
+// 512: fp32 81 us (6.6 TB/s: the copy bandwidth), bf16 55.6 us (4.8 TB/s), where the words alone take 38 us and the copy alone 41; with one
+// piece a thread 61.6, with four 55.8, in a persistent grid with its loads ahead 57.5.
 constexpr int kPieces = 2;
 
 template <typename T, bool SEED_AT, bool ROWS>
@@ -183,7 +186,7 @@ __global__ void __launch_bounds__(256) dropout_shared_kernel(const __grid_consta
   }
 }
 
-// Rows that are no whole pieces, or not on 16-byte boundaries: four elements a thread, one by one.
+// Rows that are no whole pieces, or not on 16-byte boundaries: a block of words a thread, its four elements one by one.
 template <typename T, bool SEED_AT>
 __global__ void __launch_bounds__(256) dropout_elements_kernel(const __grid_constant__ DropoutParams p) {
   const long long m0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;

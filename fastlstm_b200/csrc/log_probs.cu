@@ -448,6 +448,8 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
   __syncthreads();
 }
 
+// 8192 x 50000 bf16 130 us (6.3 TB/s; the exponentials, one a logit, at 73 % of their unit), fp32 at the copy bandwidth.  Few rows are a
+// chain of latencies: 1 x 131072 4.2 us, with 20 alternatives 8.3.
 template <typename T, bool TOP, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_constant__ ScoreParams p) {
   __shared__ ScoreShared<NT> s;
@@ -568,6 +570,7 @@ struct RowGrad {
   }
 };
 
+// 16384 x 205 fp32 8.2 us, x 1000 22 us (91 % of the copy bandwidth).
 template <typename T, int PPL>
 __global__ void __launch_bounds__(32 * kWarpRows) score_grad_warp_kernel(const __grid_constant__ ScoreParams p) {
   const unsigned lane = threadIdx.x & 31, r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);

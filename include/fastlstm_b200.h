@@ -250,7 +250,8 @@ int blstm_packed_maps(const int32_t* batch_sizes, const int32_t* offsets, const 
  * Operators around a language model of LSTM layers.  No reference counterpart: the reference has the
  * layers alone.  Rows (a token, a prediction, a step of a sequence) are numbered [n0, n1] row-major; every
  * strided tensor gives the strides of the two in elements, its last dimension is dense.  Addresses are
- * multiples of the element's size; wider accesses are used where addresses and strides allow them.
+ * multiples of the element's size; wider accesses are used where addresses and strides allow them.  Outputs
+ * overlap no inputs.
  * A token outside of the vocabulary is reported as BLSTM_E_TOKEN through the mailbox (blstm_set_mailbox:
  * detail[0] its row, detail[1] its value), its row of the result is NaN and it takes part in no gradient.
  * ------------------------------------------------------------------------------------------------ */
