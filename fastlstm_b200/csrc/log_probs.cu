@@ -328,12 +328,12 @@ __device__ __forceinline__ unsigned cluster_rank() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// the same variable in the first block of the cluster
+// the same variable in another block of the cluster
 template <typename V>
-__device__ __forceinline__ void store_first(V* p, unsigned long long v) {
+__device__ __forceinline__ void store_to(unsigned block, V* p, unsigned long long v) {
   static_assert(sizeof(V) == 8, "");
   unsigned a;
-  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(block));
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
@@ -343,10 +343,12 @@ struct ScoreShared {
   uint2 peers[kMaxCluster][2];                          // maximum and sum, second sum, of every block of a cluster
   alignas(16) unsigned group[kGroups];
   unsigned owner[NT];
+  unsigned least[kGroups / 32];
   unsigned owners, count;
   unsigned long long bound;
   unsigned long long cand[kCand];
-  unsigned long long best[kMaxCluster * BLSTM_MAX_TOP]; // of this block; in a cluster's first one, of all
+  unsigned long long best[BLSTM_MAX_TOP];               // of this block
+  unsigned long long all[kMaxCluster * BLSTM_MAX_TOP];  // of every block of a cluster
 };
 
 // The `top` first of a block's logits in order, into s.best: threads' maxima bound them from below, the threads whose
@@ -362,28 +364,20 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
   if (tid == 0) { s.owners = 0; s.count = 0; }
   if (tid < top) s.best[tid] = 0;              // (a block may have fewer)
   __syncthreads();
-  // The `top`-th largest of the groups' maxima, in every warp.  A few: the largest, those that are left without it, and so on.
-  // Many: every lane counts how many of the 64 are above its two.
-  unsigned a = s.group[lane], b = s.group[lane + 32], bound;
-  if (top <= 8) {
-    unsigned found = 0;
-    do {
-      bound = __reduce_max_sync(~0u, max(a, b));
-      found += __popc(__ballot_sync(~0u, a == bound)) + __popc(__ballot_sync(~0u, b == bound));
-      if (a == bound) a = 0;                   // (no key is 0)
-      if (b == bound) b = 0;
-    } while (found < top);
-  } else {
-    unsigned above_a = 0, above_b = 0;
+  // the `top`-th largest of the groups' maxima: the smallest that fewer than `top` are above (equal ones count alike)
+  if (tid < kGroups) {
+    const unsigned g = s.group[tid];
+    unsigned above = 0;
 #pragma unroll 4
     for (unsigned i = 0; i < kGroups; i += 4) {
       const uint4 v = *reinterpret_cast<const uint4*>(s.group + i);
-      above_a += (v.x > a) + (v.y > a) + (v.z > a) + (v.w > a);
-      above_b += (v.x > b) + (v.y > b) + (v.z > b) + (v.w > b);
+      above += (v.x > g) + (v.y > g) + (v.z > g) + (v.w > g);
     }
-    // (equal ones count alike: the smallest that fewer than `top` are above)
-    bound = __reduce_min_sync(~0u, min(above_a < top ? a : ~0u, above_b < top ? b : ~0u));
+    const unsigned least = __reduce_min_sync(~0u, above < top ? g : ~0u);
+    if (lane == 0) s.least[tid / 32] = least;
   }
+  __syncthreads();
+  const unsigned bound = min(s.least[0], s.least[1]);
   if (mine >= bound) s.owner[atomicAdd(&s.owners, 1u)] = tid;
   __syncthreads();
   auto offer = [&](float z, unsigned j, unsigned long long least) {
@@ -493,40 +487,38 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
   a = s.part[lane % (NT / 32)];
   a.join((NT / 32), p.to_log2);
   if (parts > 1) {
+    // every block tells all what its part has come to
     cluster_wait();
-    if (tid == 0) {
-      store_first(&s.peers[part][0], (unsigned long long)__float_as_uint(a.s) << 32 | __float_as_uint(a.m));
-      store_first(&s.peers[part][1], __float_as_uint(a.t));
+    if (tid < parts) {
+      store_to(tid, &s.peers[part][0], (unsigned long long)__float_as_uint(a.s) << 32 | __float_as_uint(a.m));
+      store_to(tid, &s.peers[part][1], __float_as_uint(a.t));
     }
-    if (TOP && part > 0 && tid < (unsigned)p.top) store_first(&s.best[part * p.top + tid], s.best[tid]);
+    if (TOP && tid < parts * p.top) store_to(tid / p.top, &s.all[part * p.top + tid % p.top], s.best[tid % p.top]);
     cluster_arrive();
     cluster_wait();
-    if (part > 0) return;
     const unsigned q = lane % kMaxCluster;
     a = q < parts ? Part{__uint_as_float(s.peers[q][0].x), __uint_as_float(s.peers[q][0].y), __uint_as_float(s.peers[q][1].x)} : Part{-INFINITY, 0.f, 0.f};
     a.join(kMaxCluster, p.to_log2);
   }
   const Row w(a);
-  if (tid == 0) put_row(p, r, w, token, at_token);
+  if (tid == 0 && part == 0) put_row(p, r, w, token, at_token);
   if constexpr (TOP) {
     if (parts == 1) {
       if (tid < (unsigned)p.top) put_top(p, r, w, tid, s.best[tid]);
-    } else {
-      // The blocks' lists, each in order, as one: eight lanes a key, each of which finds how many of one list come before it.
+    } else if (tid / kMaxCluster < (unsigned)p.top) {
+      // The blocks' lists, each in order, as one: a block has the places of its own keys, eight lanes a key, each of which finds
+      // how many of one list come before it.
+      static_assert(NT < 256 || NT == kMaxCluster * BLSTM_MAX_TOP, "clusters have blocks of 256 threads");
       const unsigned q = tid % kMaxCluster;
-#pragma unroll 1
-      for (unsigned i0 = 0; i0 < parts * p.top; i0 += NT / kMaxCluster) {
-        const unsigned i = i0 + tid / kMaxCluster;
-        const unsigned long long key = i < parts * p.top ? s.best[i] : 0;
-        unsigned before = 0;
-        if (q < parts)
+      const unsigned long long key = s.best[tid / kMaxCluster];
+      unsigned before = 0;
+      if (q < parts)
 #pragma unroll
-          for (unsigned step = BLSTM_MAX_TOP; step; step >>= 1)
-            if (before + step <= (unsigned)p.top && s.best[q * p.top + before + step - 1] > key) before += step;
+        for (unsigned step = BLSTM_MAX_TOP; step; step >>= 1)
+          if (before + step <= (unsigned)p.top && s.all[q * p.top + before + step - 1] > key) before += step;
 #pragma unroll
-        for (int o = 1; o < kMaxCluster; o <<= 1) before += __shfl_xor_sync(~0u, before, o);
-        if (q == 0 && key && before < (unsigned)p.top) put_top(p, r, w, before, key);
-      }
+      for (int o = 1; o < kMaxCluster; o <<= 1) before += __shfl_xor_sync(0xffu << (lane & ~7u), before, o);
+      if (q == 0 && key && before < (unsigned)p.top) put_top(p, r, w, before, key);
     }
   }
 }
