@@ -62,7 +62,10 @@ std::shared_ptr<N> make_node(const Tensor& input) {
   return node;
 }
 
-bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+bool wants_grad(const Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "fastlstm_b200: forward-mode gradients are not there for this operator");
+  return at::GradMode::is_enabled() && t.requires_grad();
+}
 void only_once() { TORCH_CHECK(!at::GradMode::is_enabled(), "fastlstm_b200: gradients of gradients (create_graph) are not there for this operator"); }
 
 std::vector<int64_t> plus(at::IntArrayRef s, int64_t last) {

@@ -443,7 +443,7 @@ __device__ __forceinline__ void block_top(ScoreShared<NT>& s, const Span<T>& spa
 }
 
 // 8192 x 50000 bf16 130 us (6.3 TB/s; the exponentials, one a logit, at 73 % of their unit), fp32 at the copy bandwidth.  Few rows are a
-// chain of latencies: 1 x 131072 4.2 us, with 20 alternatives 8.3.
+// chain of latencies: 1 x 131072 4.2 us, with 20 alternatives 6.6.
 template <typename T, bool TOP, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_constant__ ScoreParams p) {
   __shared__ ScoreShared<NT> s;
@@ -664,10 +664,10 @@ static ScoreParams score_params(const blstm_score_desc& d, const void* logits, c
 static unsigned row_pieces(const ScoreParams& p, size_t element) { return (unsigned)((unsigned long long)p.vocab * element / 16); }
 
 // Threads of a block.  A row ends with some hundred clocks in which nothing is read, and the more rows an SM has at a time the
-// less that shows; long rows have it seldom and take the threads.  bf16, us with 64 / 128 / 256 threads: 32768 x 10007 118 / 136 /
-// 221, 8192 x 50000 130 / 133 / 139, 4096 x 131072 176 / 169 / 169.  Alternatives cost more at every row's end, but each thread
-// that has one has its share of the row read again, which is shorter the more there are: with 5 at 65536 x 4096 187 / 287 / 492, at
-// 16384 x 20000 155 / 151 / 198, at 8192 x 50000 193 / 164 / 171, at 4096 x 131072 257 / 209 / 194.  Few rows take more threads each.
+// less that shows; long rows have it seldom and take the threads.  bf16, us with 64 / 128 / 256 threads: 32768 x 10007 118 / 142 /
+// 225, 8192 x 50000 130 / 132 / 139, 4096 x 131072 175 / 168 / 168.  Alternatives cost more at every row's end, but each thread
+// that has one has its share of the row read again, which is shorter the more there are: with 5 at 65536 x 4096 201 / 300 / 503, at
+// 16384 x 20000 157 / 154 / 203, at 8192 x 50000 194 / 168 / 177, at 4096 x 131072 258 / 210 / 194.  Few rows take more threads each.
 static unsigned score_threads(const ScoreParams& p, size_t element) {
   const unsigned pieces = row_pieces(p, element);
   unsigned threads = p.top == 0 ? (pieces < 8192 ? 64 : 128) : pieces < 1024 ? 64 : pieces < 8192 ? 128 : 256;

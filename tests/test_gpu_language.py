@@ -550,6 +550,16 @@ def test_gradients_of_gradients_are_refused():
             torch.autograd.grad(out.sum(), x, create_graph=True)
 
 
+def test_forward_mode_gradients_are_refused():
+    from torch.autograd import forward_ad
+    x, t = torch.randn(3, 4, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: F.embedding(t, dual), lambda: F.dropout(dual, 0.5, 0), lambda: F.token_log_probs(dual, t)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
 def test_another_stream_and_no_gradients():
     """Calls on a side stream are ordered with it, and what they return without gradients is the same."""
     g = gen(24)
