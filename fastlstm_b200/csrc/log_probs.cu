@@ -458,15 +458,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
     for (int u = 0; u < kUnroll; ++u) v[u] = i + u * NT < span.end ? load_once(body + i + u * NT) : minus_infinity(T{});
   };
   uint4 next[kUnroll];
-  if (parts > 1) fetch(span.begin + tid, next);      // (few rows: not behind the token)
   const long long token = p.tokens(r);
-  if (token == p.ignore) {                     // (the same for a whole cluster)
-    if (part == 0) put_ignored(p, r, tid);
-    return;
+  if (parts > 1) {                             // few rows: nothing waits for the token, not even where it is to be ignored
+    fetch(span.begin + tid, next);
+    cluster_arrive();                          // this block has begun: the others may write to it
+  } else {
+    if (token == p.ignore) {
+      put_ignored(p, r, tid);
+      return;
+    }
+    fetch(span.begin + tid, next);
   }
-  if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
-  else fetch(span.begin + tid, next);
-  const float at_token = tid == 0 && part == 0 && token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
   Part a{-INFINITY, 0.f, 0.f};
   if (tid < span.edges()) {
     const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
@@ -479,6 +481,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
     fetch(i + kUnroll * NT, next);
     take(a, z, p.to_log2);
   }
+  const float at_token = tid == 0 && part == 0 && token >= 0 && token < p.vocab ? ld_f(row + token) : 0.f;
   const float thread_max = a.m;
   a.join(32, p.to_log2);
   if (lane == 0) s.part[warp] = a;
@@ -499,6 +502,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) score_kernel(const __grid_const
     const unsigned q = lane % kMaxCluster;
     a = q < parts ? Part{__uint_as_float(s.peers[q][0].x), __uint_as_float(s.peers[q][0].y), __uint_as_float(s.peers[q][1].x)} : Part{-INFINITY, 0.f, 0.f};
     a.join(kMaxCluster, p.to_log2);
+    if (token == p.ignore) {                   // (the same for the whole cluster)
+      if (part == 0) put_ignored(p, r, tid);
+      return;
+    }
   }
   const Row w(a);
   if (tid == 0 && part == 0) put_row(p, r, w, token, at_token);
