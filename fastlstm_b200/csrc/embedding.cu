@@ -12,6 +12,8 @@
 
 namespace blstm {
 
+static_assert(sizeof(blstm_embed_desc) == 88 && sizeof(blstm_dropout_desc) == 72 && sizeof(blstm_score_desc) == 80, "as bindings lay them out");
+
 // ---------------------------------------------------------------- lookup
 struct LookupParams {
   const void* weight;

@@ -59,6 +59,11 @@ def test_cpu_tensors_are_refused():
             F.dropout(x, 0.5, **bad)
 
 
+def test_descriptor_layouts_match_the_library():
+    # (the library asserts the same sizes when it is compiled)
+    assert [ctypes.sizeof(c) for c in (_lib.EmbedDesc, _lib.DropoutDesc, _lib.ScoreDesc)] == [88, 72, 80]
+
+
 def _desc(cls, **given):
     d = cls()
     for k, v in given.items():
