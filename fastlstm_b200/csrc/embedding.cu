@@ -6,7 +6,6 @@
 // tokens' rows in 32 bits and writes every row of dW once.  The order of the additions depends on the tokens alone:
 // results repeat bit by bit.  Bound by memory: what is met of the table and `out` once; dout and dW once.
 #include <algorithm>
-#include <type_traits>
 
 #include "language.cuh"
 
@@ -20,58 +19,108 @@ struct LookupParams {
   void* out;
   Tokens tokens;
   long long vocab, weight_stride;
-  unsigned n, pieces, group;        // tokens; pieces of a row; threads side by side in a row, a power of two up to 32
+  unsigned n, width, pieces, group; // tokens; elements and 16-byte pieces of a row; threads side by side in a row, a power of two up to 32
   float scale;
   int* mailbox;
 };
 
 // A thread has four pieces on their way, COLS of them in a row: no divisions, which at 16 bytes a piece would take longer than
-// the memory (131072 x 1024 fp16 of 131072: 85 us with them, 55 without, 95 % of the copy bandwidth).  Pieces of 4 bytes or of one
-// element, where widths and addresses allow no more, are bound by instructions (65536 x 301 fp32: 35 us, 43 %).
+// the memory (131072 x 1024 fp16 of 131072: 85 us with them, 55 without, 95 % of the copy bandwidth).
 constexpr int kLookups = 4;
 
-template <typename T, int VEC, int COLS>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(256) lookup_kernel(const __grid_constant__ LookupParams p) {
-  using V = Pack<T, VEC>;
-  constexpr int R = kLookups / COLS;
+  constexpr int N = kPer<T>, R = kLookups / COLS;
   const unsigned row0 = blockIdx.x * (256 / p.group * R) + threadIdx.x / p.group * R, c0 = blockIdx.y * (p.group * COLS) + threadIdx.x % p.group;
   long long t[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) t[r] = row0 + r < p.n ? p.tokens(row0 + r) : -1;
-  V v[R][COLS];
+  uint4 v[R][COLS];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int j = 0; j < COLS; ++j)
       if (t[r] >= 0 && t[r] < p.vocab && c0 + j * p.group < p.pieces)
-        v[r][j] = reinterpret_cast<const V*>(static_cast<const T*>(p.weight) + t[r] * p.weight_stride)[c0 + j * p.group];
+        v[r][j] = reinterpret_cast<const uint4*>(static_cast<const T*>(p.weight) + t[r] * p.weight_stride)[c0 + j * p.group];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (row0 + r >= p.n) return;
     const bool in = t[r] >= 0 && t[r] < p.vocab;
-    V* out = static_cast<V*>(p.out) + (size_t)(row0 + r) * p.pieces;
+    uint4* out = static_cast<uint4*>(p.out) + (size_t)(row0 + r) * p.pieces;
 #pragma unroll
     for (int j = 0; j < COLS; ++j) {
       const unsigned c = c0 + j * p.group;
       if (c >= p.pieces) break;
-      if (!in) {
+      if (!in || p.scale != 1.f) {
+        float z[N];
+        unpack(v[r][j], z, T{});
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[r][j].v[k] = Elem<T>::from_f(__int_as_float(0x7fffffff));
-      } else if (p.scale != 1.f) {
-        if constexpr (VEC == kPer<T>) {
-          float z[VEC];
-          unpack(*reinterpret_cast<const uint4*>(&v[r][j]), z, T{});
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) z[k] *= p.scale;
-          *reinterpret_cast<uint4*>(&v[r][j]) = pack(z, T{});
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) v[r][j].v[k] = Elem<T>::from_f(Elem<T>::to_f(v[r][j].v[k]) * p.scale);
-        }
+        for (int e = 0; e < N; ++e) z[e] = in ? z[e] * p.scale : __int_as_float(0x7fffffff);
+        v[r][j] = pack(z, T{});
       }
       out[c] = v[r][j];
     }
     if (!in && c0 == 0) report_token(p.mailbox, row0 + r, t[r]);
+  }
+}
+
+// Rows that are no whole 16-byte pieces: a thread makes two pieces of `out`, which has no gaps, out of loads of L elements.  Bound by
+// those loads (131072 x 643: fp32 95 us, bf16 80, with stores as narrow as the loads 154 and 127; 65536 x 302 bf16 27, so 24).
+template <typename T, int L>
+__global__ void __launch_bounds__(256) lookup_gather_kernel(const __grid_constant__ LookupParams p) {
+  constexpr int N = kPer<T>, kTwo = 2;
+  using V = Pack<T, L>;
+  const unsigned long long total = (unsigned long long)p.n * p.width, begin = (unsigned long long)blockIdx.x * (256 * kTwo);
+  alignas(16) T v[kTwo][N];
+#pragma unroll
+  for (int u = 0; u < kTwo; ++u) {
+    const unsigned long long m = (begin + u * 256 + threadIdx.x) * N;
+    if (m >= total) break;
+    unsigned r = m <= 0xffffffffull ? (unsigned)m / p.width : (unsigned)(m / p.width), c = (unsigned)(m - (unsigned long long)r * p.width);
+    auto known = [&](long long t) { return t >= 0 && t < p.vocab; };
+    auto row = [&](long long t) { return static_cast<const T*>(p.weight) + t * p.weight_stride; };
+    const T none = Elem<T>::from_f(__int_as_float(0x7fffffff));
+    const long long t = p.tokens(r);
+    if (!known(t) && c == 0) report_token(p.mailbox, r, t);
+    if (c + N <= p.width) {
+#pragma unroll
+      for (int k = 0; k < N; k += L)
+        if (known(t)) *reinterpret_cast<V*>(v[u] + k) = *reinterpret_cast<const V*>(row(t) + c + k);
+        else
+          for (int e = 0; e < L; ++e) v[u][k + e] = none;
+    } else if (p.width >= N) {                 // the end of a row and the begin of the next one, or the end of all
+      const bool more = r + 1 < p.n;
+      const long long t2 = more ? p.tokens(r + 1) : t;
+      if (more && !known(t2)) report_token(p.mailbox, r + 1, t2);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const bool here = c + k < p.width;
+        v[u][k] = known(here ? t : t2) && m + k < total ? (here ? row(t) + c : row(t2) - (p.width - c))[k] : none;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k, ++c) {
+        if (m + k >= total) break;
+        if (c == p.width) { c = 0; ++r; }
+        const long long q = p.tokens(r);
+        v[u][k] = known(q) ? row(q)[c] : none;
+        if (!known(q) && c == 0 && k > 0) report_token(p.mailbox, r, q);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kTwo; ++u) {
+    const unsigned long long m = (begin + u * 256 + threadIdx.x) * N;
+    if (m >= total) break;
+    T* out = static_cast<T*>(p.out) + m;
+    Pack<T, N> o;
+#pragma unroll
+    for (int k = 0; k < N; ++k) o.v[k] = p.scale != 1.f ? Elem<T>::from_f(Elem<T>::to_f(v[u][k]) * p.scale) : v[u][k];
+    if (m + N <= total && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0) *reinterpret_cast<Pack<T, N>*>(out) = o;
+    else
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (m + k < total) out[k] = o.v[k];
   }
 }
 
@@ -326,7 +375,6 @@ __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(const __g
 }
 
 // ---------------------------------------------------------------- sums of equal tokens' rows
-constexpr int kRunStep = 4;          // rows on their way at a time
 constexpr int kMinRun = 8, kMaxRun = 64;     // sorted positions that one group of threads adds up
 constexpr int kZeroRows = 16, kClearRows = 64;   // rows of dW that one block of few_kernel, of sum_kernel looks after
 
@@ -370,11 +418,12 @@ __device__ __forceinline__ void put_sum(const SumParams& p, unsigned t, unsigned
 // began before.
 enum : unsigned { kGoesOn = 0, kWhole = 1, kLastPart = 2, kFirstPart = 3 };
 
-// A group of threads adds a run's rows up, four of them on their way.  Bound by memory where there are many: 131072 x 1024 fp16 and
+// A group of threads adds a run's rows up, four or eight of them on their way.  Bound by memory where there are many: 131072 x 1024 fp16 and
 // 172 MB of zeros 88 us (5.9 TB/s); 16384 x 512 bf16 9 us, which are a run's latency.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumParams p) {
   using V = Pack<T, VEC>;
+  constexpr int kRunStep = VEC * sizeof(T) == 16 ? 4 : 8;            // rows on their way at a time
   __shared__ unsigned s_key[256 / 4 * kMaxRun], s_pos[256 / 4 * kMaxRun];
   __shared__ unsigned char s_then[256 / 4 * kMaxRun];
   if (blockIdx.x >= p.sum_blocks) {            // rows that no token names
@@ -671,24 +720,30 @@ int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* w
   const int e = dtype_bytes(d->dtype);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out) | (uintptr_t)(d->width * e) | (uintptr_t)(d->row_stride[0] * e);
   if (bits % e) return BLSTM_E_INVALID_ARG;
-  const int piece = piece_bytes(bits, e);
-  LookupParams p{weight, out, make_tokens(*d, tokens), d->vocab, d->row_stride[0], (unsigned)n, (unsigned)(d->width * e / piece), 1, d->scale,
-                 current_mailbox()};
+  LookupParams p{weight, out, make_tokens(*d, tokens), d->vocab, d->row_stride[0], (unsigned)n, (unsigned)d->width, (unsigned)(d->width * e / 16), 1,
+                 d->scale, current_mailbox()};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (bits & 15u) {
+    const unsigned long long blocks = ((unsigned long long)n * d->width * e + 8191) / 8192;      // of 512 pieces
+    if (blocks > INT32_MAX) return BLSTM_E_TOO_LARGE;
+    return with_type(d->dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      if ((bits & 3u) == 0) lookup_gather_kernel<T, 4 / sizeof(T)><<<(unsigned)blocks, 256, 0, st>>>(p);
+      else lookup_gather_kernel<T, 1><<<(unsigned)blocks, 256, 0, st>>>(p);
+      BLSTM_CUDA_OK(cudaGetLastError());
+      count_launch();
+      return BLSTM_OK;
+    });
+  }
   while (p.group < 32 && p.group < p.pieces) p.group *= 2;
   const int cols = p.pieces > 64 ? 4 : p.pieces > 32 ? 2 : 1, rows = 256 / (int)p.group * (kLookups / cols);   // of a block
   const dim3 grid((unsigned)((n + rows - 1) / rows), (p.pieces + p.group * cols - 1) / (p.group * cols));
   if (grid.y > 65535) return BLSTM_E_TOO_LARGE;
   return with_type(d->dtype, [&](auto t) -> int {
     using T = decltype(t);
-    auto launch = [&](auto vec) {
-      constexpr int V = decltype(vec)::value;
-      if (cols == 4) lookup_kernel<T, V, 4><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-      else if (cols == 2) lookup_kernel<T, V, 2><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-      else lookup_kernel<T, V, 1><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    };
-    if (piece == 16) launch(std::integral_constant<int, 16 / sizeof(T)>{});
-    else if (piece == 4) launch(std::integral_constant<int, 4 / sizeof(T)>{});
-    else launch(std::integral_constant<int, 1>{});
+    if (cols == 4) lookup_kernel<T, 4><<<grid, 256, 0, st>>>(p);
+    else if (cols == 2) lookup_kernel<T, 2><<<grid, 256, 0, st>>>(p);
+    else lookup_kernel<T, 1><<<grid, 256, 0, st>>>(p);
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     return BLSTM_OK;
