@@ -279,7 +279,7 @@ Tensor grad_like(const Tensor& logits, const Lead& lead, const int64_t stride[2]
   const int64_t own = V + (lead.n0 - 1) * stride[0] + (lead.n1 - 1) * stride[1];
   const bool inner0 = stride[0] < stride[1];          // the first dimension is the inner one in memory
   const int64_t n_in = inner0 ? lead.n0 : lead.n1, s_in = stride[inner0 ? 0 : 1], n_out = inner0 ? lead.n1 : lead.n0, s_out = stride[inner0 ? 1 : 0];
-  const bool apart = (n_in == 1 || s_in >= V) && (n_out == 1 || s_out >= n_in * s_in);
+  const bool apart = (n_in == 1 || s_in >= V) && (n_out == 1 || s_out >= V + (n_in - 1) * s_in);   // no two rows share an element (windows do)
   const int64_t numel = lead.n0 * lead.n1 * V;
   if (apart && own <= numel + numel / 8) {
     dstride[0] = stride[0]; dstride[1] = stride[1];
