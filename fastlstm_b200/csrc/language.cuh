@@ -35,12 +35,18 @@ struct Tokens {
 // The mailbox that the calling thread has set (blstm_set_mailbox), or null.
 int* current_mailbox();
 
-// A token outside of the vocabulary: one report is kept, position and token in one store, the status word last.
+// A token outside of the vocabulary: one report is kept, position and token in one store, the status word last.  (A mailbox of
+// ints need not lie on 8 bytes: there, position and token of two reports at a time may mix.)
 static __device__ __noinline__ void report_token(int* mailbox, unsigned position, long long token) {
   if (!mailbox) return;
   volatile int* m = mailbox;
   const int shown = token > INT32_MAX ? INT32_MAX : token < INT32_MIN ? INT32_MIN : (int)token;
-  *reinterpret_cast<volatile unsigned long long*>(m + 2) = (unsigned long long)(unsigned)shown << 32 | position;
+  if ((reinterpret_cast<uintptr_t>(mailbox) & 7) == 0) {
+    *reinterpret_cast<volatile unsigned long long*>(m + 2) = (unsigned long long)(unsigned)shown << 32 | position;
+  } else {
+    m[2] = (int)position;
+    m[3] = shown;
+  }
   __threadfence_system();
   m[1] = BLSTM_E_TOKEN;
 }

@@ -317,10 +317,10 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
                                const float* g_entropy, const int64_t g_entropy_stride[2], const float* g_top,
                                void* dlogits, const int64_t dlogits_stride[2], void* stream);
 
-/* Host memory (mapped into the device, 16 bytes: -, status, detail[2]) that the CALLING THREAD's later
- * launches write a device-side error to as well, or NULL (default): a caller that looks there need not
- * read control blocks back.  The status word is written last; the caller clears it.  No reference
- * counterpart. */
+/* Host memory (mapped into the device, four int32: -, status, detail[2]; on an 8-byte boundary both details
+ * are always of one report) that the CALLING THREAD's later launches write a device-side error to as well, or
+ * NULL (default): a caller that looks there need not read control blocks back.  The status word is written
+ * last; the caller clears it.  No reference counterpart. */
 void blstm_set_mailbox(int32_t* mapped);
 
 /* Number of kernels this library has launched in this process so far (HOST

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import fastlstm_b200 as F
+from fastlstm_b200 import _lib
 from test_gpu_language import U, check_scores, gen, make_logits
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +34,29 @@ def test_scores_gradient_of_windows_adds_up_in_the_tensor():
     (want,) = torch.autograd.grad(lp.gather(1, tokens[:, None]).sum(), ref)
     # 20 windows, each gradient at most 1 and with distances of up to D = 35 powers of two off by (6 D + 16) u of it
     assert float((d.double() - want).abs().max()) <= 20 * (6 * 35 + 16) * U
+
+
+# ---------------------------------------------------------------- C ABI
+def descriptor(cls, **given):
+    d = cls()
+    for k, v in given.items():
+        setattr(d, k, type(getattr(d, k))(*v) if isinstance(v, tuple) else v)
+    return d
+
+
+@pytest.mark.parametrize("at", [0, 1, 2, 3])
+@pytest.mark.parametrize("width", [16, 7])
+def test_reports_reach_a_mailbox_on_any_int(width, at):
+    lib = _lib.load()
+    tokens, W, out = torch.tensor([3, 1, 9, 0], device="cuda"), torch.ones(5, width, device="cuda"), torch.zeros(4, width, device="cuda")
+    mail = torch.zeros(16, dtype=torch.int32).pin_memory()
+    d = descriptor(_lib.EmbedDesc, dtype=_lib.F32, token_bits=64, n0=1, n1=4, token_stride=(0, 1), vocab=5, width=width, row_stride=(width, 0), padding=-1, scale=1.0)
+    stream = torch.cuda.current_stream().cuda_stream
+    lib.blstm_set_mailbox(mail.data_ptr() + 4 * at)
+    try:
+        assert lib.blstm_embedding(d, tokens.data_ptr(), W.data_ptr(), out.data_ptr(), stream) == 0
+    finally:
+        lib.blstm_set_mailbox(None)
+    torch.cuda.synchronize()
+    assert mail.tolist() == [0] * at + [0, _lib.E_TOKEN, 2, 9] + [0] * (12 - at)
+    assert out[2].isnan().all() and torch.equal(out[[0, 1, 3]], W[:3])
