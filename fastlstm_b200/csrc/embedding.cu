@@ -716,7 +716,7 @@ int blstm_embedding(const blstm_embed_desc* d, const void* tokens, const void* w
   if (int rc = check_embed(d)) return rc;
   const int64_t n = d->n0 * d->n1;
   if (n == 0) return BLSTM_OK;
-  if (!tokens || !weight || !out) return BLSTM_E_INVALID_ARG;
+  if (!tokens || !weight || !out || !aligned(d->token_bits / 8, tokens)) return BLSTM_E_INVALID_ARG;
   const int e = dtype_bytes(d->dtype);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(out) | (uintptr_t)(d->width * e) | (uintptr_t)(d->row_stride[0] * e);
   if (bits % e) return BLSTM_E_INVALID_ARG;
@@ -766,7 +766,7 @@ int blstm_embedding_grad(const blstm_embed_desc* d, const void* tokens, const vo
     BLSTM_CUDA_OK(cudaMemsetAsync(dweight, 0, (size_t)d->vocab * d->width * e, st));
     return BLSTM_OK;
   }
-  if (!tokens || !dout) return BLSTM_E_INVALID_ARG;
+  if (!tokens || !dout || !aligned(d->token_bits / 8, tokens)) return BLSTM_E_INVALID_ARG;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dweight) | (uintptr_t)(d->width * e) |
                          (uintptr_t)(d->row_stride[0] * e) | (uintptr_t)(d->row_stride[1] * e);
   if (bits % e) return BLSTM_E_INVALID_ARG;

@@ -82,6 +82,10 @@ __device__ __forceinline__ unsigned two(float a, float b, __half) { const __half
 template <typename T>
 __device__ __forceinline__ uint4 pack(const float* z, T t) { return make_uint4(two(z[0], z[1], t), two(z[2], z[3], t), two(z[4], z[5], t), two(z[6], z[7], t)); }
 
+// Whether all addresses are multiples of `bytes`, a power of two.
+template <typename... P>
+bool aligned(size_t bytes, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0; }
+
 inline bool valid_dtype(int dtype) { return dtype == BLSTM_F32 || dtype == BLSTM_F16 || dtype == BLSTM_BF16; }
 inline int dtype_bytes(int dtype) { return dtype == BLSTM_F32 ? 4 : 2; }
 inline bool valid_rows(int64_t n0, int64_t n1) { return n0 >= 0 && n1 >= 0 && (n0 == 0 || n1 <= INT32_MAX / n0); }

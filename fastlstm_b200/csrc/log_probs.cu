@@ -651,7 +651,7 @@ static int check_score(const blstm_score_desc* d, const void* logits, const void
   if (!d || !valid_dtype(d->dtype) || (d->token_bits != 32 && d->token_bits != 64) || !valid_rows(d->n0, d->n1) || d->vocab <= 0 ||
       d->vocab >= INT32_MAX || d->top < 0 || d->top > BLSTM_MAX_TOP || d->top > d->vocab || !(d->temperature >= 1e-30f && d->temperature < INFINITY))
     return BLSTM_E_INVALID_ARG;
-  if (d->n0 && d->n1 && (!logits || !tokens || reinterpret_cast<uintptr_t>(logits) % dtype_bytes(d->dtype))) return BLSTM_E_INVALID_ARG;
+  if (d->n0 && d->n1 && (!logits || !tokens || !aligned(dtype_bytes(d->dtype), logits) || !aligned(d->token_bits / 8, tokens))) return BLSTM_E_INVALID_ARG;
   return BLSTM_OK;
 }
 
@@ -733,7 +733,8 @@ int blstm_token_log_probs(const blstm_score_desc* d, const void* logits, const v
                           float* top_log_probs, int64_t* top_tokens, float* stats, void* stream) {
   if (int rc = check_score(d, logits, tokens)) return rc;
   if (d->n0 == 0 || d->n1 == 0) return BLSTM_OK;
-  if (!log_probs || !entropy || (d->top && (!top_log_probs || !top_tokens))) return BLSTM_E_INVALID_ARG;
+  if (!log_probs || !entropy || (d->top && (!top_log_probs || !top_tokens)) || !aligned(4, log_probs, entropy, top_log_probs, stats) || !aligned(8, top_tokens))
+    return BLSTM_E_INVALID_ARG;
   ScoreParams p = score_params(*d, logits, tokens);
   p.log_probs = log_probs; p.entropy = entropy; p.stats = stats;
   p.top_log_probs = top_log_probs; p.top_tokens = reinterpret_cast<long long*>(top_tokens);
@@ -750,7 +751,7 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
                                void* stream) {
   if (int rc = check_score(d, logits, tokens)) return rc;
   if (d->n0 == 0 || d->n1 == 0) return BLSTM_OK;
-  if (!stats || !dlogits || !dlogits_stride || (g_log_probs && !g_log_probs_stride) || (g_entropy && !g_entropy_stride) || (g_top && (!top_tokens || d->top == 0)) ||
+  if (!aligned(4, stats, g_log_probs, g_entropy, g_top) || !aligned(8, top_tokens) || !stats || !dlogits || !dlogits_stride || (g_log_probs && !g_log_probs_stride) || (g_entropy && !g_entropy_stride) || (g_top && (!top_tokens || d->top == 0)) ||
       ((reinterpret_cast<uintptr_t>(dlogits) - reinterpret_cast<uintptr_t>(logits)) & 15u) ||
       (d->n0 > 1 && ((dlogits_stride[0] - d->logits_stride[0]) * dtype_bytes(d->dtype) & 15)) ||
       (d->n1 > 1 && ((dlogits_stride[1] - d->logits_stride[1]) * dtype_bytes(d->dtype) & 15)))
