@@ -41,16 +41,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// The order of top alternatives: larger logits first (NaN before all), then lower numbers.  Never 0.
+// The order of top alternatives: larger logits first (NaN before all), then lower numbers.  Never 0, and an order key never ~0:
+// both stand for none.
 __device__ __forceinline__ unsigned value_key(float z) {
-  if (z != z) return 0xffffffffu;
+  if (z != z) return 0xfffffffeu;
   const unsigned b = __float_as_uint(z + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ unsigned long long order_key(float z, unsigned j) { return (unsigned long long)value_key(z) << 32 | (0xffffffffu - j); }
 
-__device__ __forceinline__ float key_value(unsigned key) {      // the logit of a value key
-  return key == 0xffffffffu ? __int_as_float(0x7fffffff) : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+__device__ __forceinline__ float key_value(unsigned key) {      // the logit of a value key (0x7ffffffe is a NaN)
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 // 2^x to 2^-22; subnormal results are 0.

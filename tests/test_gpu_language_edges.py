@@ -5,7 +5,7 @@ import torch
 
 import fastlstm_b200 as F
 from fastlstm_b200 import _lib
-from test_gpu_language import U, check_scores, gen, make_logits
+from test_gpu_language import DT, U, check_scores, gen, make_logits
 
 pytestmark = pytest.mark.gpu
 
@@ -34,6 +34,21 @@ def test_scores_gradient_of_windows_adds_up_in_the_tensor():
     (want,) = torch.autograd.grad(lp.gather(1, tokens[:, None]).sum(), ref)
     # 20 windows, each gradient at most 1 and with distances of up to D = 35 powers of two off by (6 D + 16) u of it
     assert float((d.double() - want).abs().max()) <= 20 * (6 * 35 + 16) * U
+
+
+@pytest.mark.parametrize("vocab", [40, 100, 129, 300, 700, 1000, 1500, 9000, 40000])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_scores_alternatives_of_rows_with_nan(vocab, dtype):
+    """NaN comes before all logits, and equal ones by their number: all NaN; one at number 0 or 1 or the last before equal logits."""
+    nan, top = float("nan"), min(32, vocab)
+    z = torch.full((4, vocab), 1.5, device="cuda").to(DT[dtype])
+    z[0] = nan
+    for row, j in ((1, 0), (2, 1), (3, vocab - 1)):
+        z[row, j] = nan
+    r = F.token_log_probs(z, torch.zeros(4, dtype=torch.long, device="cuda"), top=top)
+    want = [list(range(top))] + [([j] + [k for k in range(top + 1) if k != j])[:top] for j in (0, 1, vocab - 1)]
+    assert r.top_tokens.tolist() == want
+    assert r.log_probs.isnan().all() and r.entropy.isnan().all() and r.top_log_probs.isnan().all()
 
 
 # ---------------------------------------------------------------- C ABI
