@@ -540,8 +540,9 @@ struct RowGrad {
     m = p.stats[r];
     log2s = p.stats[(size_t)p.n + r];
     const float h = p.stats[2 * (size_t)p.n + r];
-    zero = token == p.ignore || log2s == -INFINITY;
-    g_lp = p.g_lp && token >= 0 && token < p.vocab ? p.g_lp[p.g_lp_map(r)] : 0.f;
+    const bool in = token >= 0 && token < p.vocab;
+    zero = token == p.ignore || !in || log2s == -INFINITY;
+    g_lp = p.g_lp && in ? p.g_lp[p.g_lp_map(r)] : 0.f;
     const float g_h = p.g_h ? p.g_h[p.g_h_map(r)] : 0.f;
     float g = g_lp;
     if (p.g_top && !zero)

@@ -2,8 +2,9 @@
 
 Each is a call on CUDA tensors (float32, float16 or bfloat16) that runs on the current stream, allocates through torch and
 is differentiable once.  Invalid arguments raise ValueError.  A token outside of the vocabulary is found on the device: its
-row of the result is NaN, it gets no gradient, and `check_status()` or a later call raises BlstmError.  What a call does
-on the host is csrc/host_language.cpp; the kernels are csrc/embedding.cu, csrc/dropout.cu and csrc/log_probs.cu."""
+embedding or log probability is NaN, its row gives no gradient, and `check_status()` or a later call raises BlstmError.
+What a call does on the host is csrc/host_language.cpp; the kernels are csrc/embedding.cu, csrc/dropout.cu and
+csrc/log_probs.cu."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
@@ -55,5 +56,6 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     top_log_probs are differentiable.  Logits may be strided as long as the vocabulary is dense (a padded one, cut, is).
     Logits of -inf are impossible tokens.  A row of nothing else: log_probs and top_log_probs -inf, entropy 0, the first
     tokens, no gradient.  NaN or +inf in a row makes its results NaN.  Rows whose token is ignore_index are not read:
-    log_probs 0, entropy 0, top_log_probs -inf, top_tokens -1, no gradient."""
+    log_probs 0, entropy 0, top_log_probs -inf, top_tokens -1, no gradient.  Entropy and alternatives of a row whose token
+    is outside of the vocabulary are its own, without a gradient."""
     return TokenLogProbs(*_lib.host().token_log_probs(logits, tokens, int(top), float(temperature), int(ignore_index)))

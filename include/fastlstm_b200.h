@@ -253,7 +253,8 @@ int blstm_packed_maps(const int32_t* batch_sizes, const int32_t* offsets, const 
  * multiples of the element's size; wider accesses are used where addresses and strides allow them.  Outputs
  * overlap no inputs.
  * A token outside of the vocabulary is reported as BLSTM_E_TOKEN through the mailbox (blstm_set_mailbox:
- * detail[0] its row, detail[1] its value), its row of the result is NaN and it takes part in no gradient.
+ * detail[0] its row, detail[1] its value), its embedding or log probability is NaN and its row takes part in no
+ * gradient.  (Entropy and alternatives do not depend on the token and are the row's own.)
  * ------------------------------------------------------------------------------------------------ */
 typedef struct blstm_embed_desc {
   int32_t dtype;             /* of weight, out, dout and dweight                                       */

@@ -51,6 +51,31 @@ def test_scores_alternatives_of_rows_with_nan(vocab, dtype):
     assert r.log_probs.isnan().all() and r.entropy.isnan().all() and r.top_log_probs.isnan().all()
 
 
+@pytest.mark.parametrize("vocab,top", [(60, 2), (700, 0), (1500, 3), (5000, 3), (40000, 5)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_scores_of_tokens_outside_of_the_vocabulary_give_no_gradient(vocab, top, dtype):
+    """Neither through the entropy nor through the alternatives, which have the row's own values."""
+    z = make_logits(gen(32), 5, vocab, dtype=dtype).requires_grad_()
+    good = torch.tensor([0, 1, 5, 2, 3], device="cuda")
+    want = F.token_log_probs(z, good, top=top)
+    n = 3 if top else 2
+    ups = [torch.randn(t.shape, generator=gen(33), device="cuda") for t in want[:n]]
+    (ref,) = torch.autograd.grad(want[:n], z, ups)
+    for bad in (vocab, -1, 2 ** 40):
+        tokens = good.clone()
+        tokens[2] = bad
+        r = F.token_log_probs(z, tokens, top=top)
+        with pytest.raises(_lib.BlstmError, match="at position 2"):
+            F.check_status()
+        assert r.log_probs[2].isnan()
+        for a, b in list(zip(r, want))[1:2 + 2 * (top > 0)]:
+            assert torch.equal(a, b)
+        (d,) = torch.autograd.grad(r[:n], z, ups)
+        F.check_status()
+        rows = torch.arange(5, device="cuda") != 2
+        assert not d[2].any() and torch.equal(d[rows], ref[rows])
+
+
 # ---------------------------------------------------------------- C ABI
 def descriptor(cls, **given):
     d = cls()
