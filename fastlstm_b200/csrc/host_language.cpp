@@ -128,7 +128,7 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale, std::
   if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0) throw wrong("expected weight as [vocabulary, width], got " + shape_str(weight.sizes()));
   beside(tokens, "tokens", weight);
   token_bits(tokens);
-  if (!std::isfinite(scale)) throw wrong("scale must be finite");
+  if (!std::isfinite((float)scale)) throw wrong("scale must be finite in 32 bits");
   const int64_t V = weight.size(0);
   int64_t padding = -1;
   if (padding_idx) {

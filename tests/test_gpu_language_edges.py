@@ -76,6 +76,14 @@ def test_scores_of_tokens_outside_of_the_vocabulary_give_no_gradient(vocab, top,
         assert not d[2].any() and torch.equal(d[rows], ref[rows])
 
 
+# ---------------------------------------------------------------- arguments
+def test_scales_beyond_32_bits_are_refused():
+    x, t = torch.randn(3, 4, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
+    for scale in (1e39, -1e300, float("inf")):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            F.embedding(t, x, scale=scale)
+
+
 # ---------------------------------------------------------------- C ABI
 def descriptor(cls, **given):
     d = cls()
