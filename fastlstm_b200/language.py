@@ -14,12 +14,24 @@ import torch
 from . import _lib
 
 
+def _whole(v, name: str, low: int = -2 ** 63, high: int = 2 ** 63 - 1) -> int:
+    try:
+        n = int(v)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != v:
+        raise ValueError(f"{name} must be a whole number, got {v!r}")
+    if not low <= n <= high:
+        raise ValueError(f"{name} must be a whole number in the range [{low}, {high}], got {n}")
+    return n
+
+
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """scale * weight[tokens]: tokens [...] (int64 or int32, any strides), weight [vocabulary, width] -> [..., width].
 
     The gradient of the table is dense and in the table's type; equal tokens' rows are added in 32 bits in an order that the
     tokens alone fix (results repeat bit by bit) and rounded once.  padding_idx names a token that gets no gradient."""
-    return _lib.host().embedding(tokens, weight, float(scale), padding_idx)
+    return _lib.host().embedding(tokens, weight, float(scale), None if padding_idx is None else _whole(padding_idx, "padding_idx"))
 
 
 def dropout(x: torch.Tensor, p: float, seed, *, offset: int = 0, shared_dim: Optional[int] = None, training: bool = True) -> torch.Tensor:
@@ -34,10 +46,8 @@ def dropout(x: torch.Tensor, p: float, seed, *, offset: int = 0, shared_dim: Opt
     if not training:
         return x
     at = seed if isinstance(seed, torch.Tensor) else None
-    number = 0 if at is not None else int(seed)
-    if not 0 <= number < 2 ** 64 or not 0 <= offset < 2 ** 64:
-        raise ValueError("seed and offset must be in the range [0, 2^64)")
-    return _lib.host().dropout(x, float(p), number, at, int(offset), shared_dim)
+    return _lib.host().dropout(x, float(p), 0 if at is not None else _whole(seed, "seed", 0, 2 ** 64 - 1), at,
+                               _whole(offset, "offset", 0, 2 ** 64 - 1), None if shared_dim is None else _whole(shared_dim, "shared_dim"))
 
 
 class TokenLogProbs(NamedTuple):
@@ -58,4 +68,5 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     tokens, no gradient.  NaN or +inf in a row makes its results NaN.  Rows whose token is ignore_index are not read:
     log_probs 0, entropy 0, top_log_probs -inf, top_tokens -1, no gradient.  Entropy and alternatives of a row whose token
     is outside of the vocabulary are its own, without a gradient."""
-    return TokenLogProbs(*_lib.host().token_log_probs(logits, tokens, int(top), float(temperature), int(ignore_index)))
+    return TokenLogProbs(*_lib.host().token_log_probs(logits, tokens, _whole(top, "top"), float(temperature),
+                                                       _whole(ignore_index, "ignore_index")))

@@ -1,5 +1,6 @@
 """The operators around a language model where their promises end: overlapping rows, addresses, tokens and numbers that are none,
 masks held to bounds of their own.  Tolerances as in test_gpu_language.py unless a test derives its own."""
+import numpy as np
 import pytest
 import torch
 
@@ -82,6 +83,19 @@ def test_scales_beyond_32_bits_are_refused():
     for scale in (1e39, -1e300, float("inf")):
         with pytest.raises(ValueError, match="scale must be finite"):
             F.embedding(t, x, scale=scale)
+
+
+def test_numbers_that_are_none_are_refused():
+    x, t = torch.randn(3, 4, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
+    for call in (lambda v: F.dropout(x, 0.5, v), lambda v: F.dropout(x, 0.5, 1, offset=v), lambda v: F.token_log_probs(x, t, top=v),
+                 lambda v: F.token_log_probs(x, t, ignore_index=v), lambda v: F.embedding(t, x, padding_idx=v), lambda v: F.dropout(x, 0.5, 1, shared_dim=v)):
+        for v in (0.5, "1", float("nan"), float("inf")):
+            with pytest.raises(ValueError, match="whole number"):
+                call(v)
+    # whole numbers of other types are none the worse
+    assert torch.equal(F.dropout(x, 0.5, np.int64(7), offset=2.0, shared_dim=np.int32(0)), F.dropout(x, 0.5, 7, offset=2, shared_dim=0))
+    assert torch.equal(F.embedding(t, x, padding_idx=np.int64(1)), F.embedding(t, x))
+    assert F.token_log_probs(x, t, top=np.int64(2), ignore_index=np.int64(-5)).top_tokens.shape == (3, 2)
 
 
 # ---------------------------------------------------------------- C ABI

@@ -3,7 +3,9 @@ that are none."""
 import ctypes
 
 import pytest
+import torch
 
+import fastlstm_b200 as F
 from fastlstm_b200 import _lib
 
 from test_language import EMBED, PTR, SCORE, _desc
@@ -30,3 +32,16 @@ def test_misaligned_results_and_statistics_are_refused():
         a = [PTR, PTR, PTR, PTR, PTR, st, PTR, st, PTR, PTR, st]
         a[i] += shift
         assert lib.blstm_token_log_probs_grad(d, *a, None) == 1
+
+
+def test_numbers_outside_of_64_bits_are_refused():
+    x, t = torch.zeros(3, 4), torch.zeros(3, dtype=torch.long)
+    for call in (lambda v: F.embedding(t, x, padding_idx=v), lambda v: F.dropout(x, 0.5, 1, shared_dim=v), lambda v: F.token_log_probs(x, t, top=v),
+                 lambda v: F.token_log_probs(x, t, ignore_index=v), lambda v: F.dropout(x, 0.5, v), lambda v: F.dropout(x, 0.5, 1, offset=v)):
+        for v in (2 ** 64, -2 ** 64):
+            with pytest.raises(ValueError, match="range"):
+                call(v)
+        with pytest.raises(ValueError, match="whole number"):
+            call(1.5)
+    with pytest.raises(ValueError, match="CUDA"):
+        F.dropout(x, 0.5, 2 ** 64 - 1, offset=2 ** 64 - 1)
