@@ -168,12 +168,15 @@ Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
   d.p = k.p; d.seed = k.seed; d.offset = k.offset;
   d.n0 = d.n1 = 1;
   Tensor x = x_in;
-  const bool two = dims == 3 && !x.is_contiguous() && x.stride(2) == 1;
+  if (k.shared < 0 && dims > 3 && !x.is_contiguous()) x = x.flatten(0, dims - 2);     // (a copy where one stride does not do)
+  const bool two = (x.dim() == 2 || x.dim() == 3) && !x.is_contiguous() && x.stride(-1) == 1 && x.numel() / x.size(-1) <= INT32_MAX;
   if (!two) x = x.contiguous();
   if (two) {                              // rows with strides of their own
-    d.n0 = sizes[0]; d.n1 = sizes[1]; d.cols = sizes[2];
-    d.stride[0] = x.stride(0); d.stride[1] = x.stride(1);
-    d.shared = (int32_t)k.shared;
+    const bool three = x.dim() == 3;
+    if (three) { d.n0 = x.size(0); d.stride[0] = x.stride(0); }
+    d.n1 = x.size(-2); d.stride[1] = x.stride(-2);
+    d.cols = x.size(-1);
+    d.shared = k.shared < 0 ? -1 : three ? (int32_t)k.shared : 1;
   } else if (k.shared < 0) {              // one row
     d.cols = x.numel();
   } else {
@@ -183,6 +186,7 @@ Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
     for (int64_t i = k.shared + 1; i < dims; ++i) d.cols *= sizes[i];
     d.stride[0] = d.n1 * d.cols; d.stride[1] = d.cols;
     d.shared = 1;
+    if (d.n0 > 0 && d.n1 > INT32_MAX / d.n0) throw wrong("more than 2^31 - 1 rows that share masks");
   }
   Call call(x.device());
   const Tensor y = fresh(sizes, x.scalar_type(), x);

@@ -41,7 +41,8 @@ def dropout(x: torch.Tensor, p: float, seed, *, offset: int = 0, shared_dim: Opt
     backward, which draws it again instead of reading it.  Calls that should differ get different offsets (a layer's number,
     say) or seeds; both are whole numbers in [0, 2^64).  seed may also be a CUDA tensor of one int64, read when the kernel
     runs: a captured graph that changes it between replays draws new masks.
-    shared_dim: all positions along that dimension share one mask (one mask for all steps of a sequence).
+    shared_dim: all positions along that dimension share one mask (one mask for all steps of a sequence); the
+    product of the dimensions up to it is below 2^31.
     Elements that are dropped are 0 whatever they held."""
     if not training:
         return x

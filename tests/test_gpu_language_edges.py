@@ -6,7 +6,9 @@ import torch
 
 import fastlstm_b200 as F
 from fastlstm_b200 import _lib
-from test_gpu_language import DT, U, check_scores, gen, make_logits
+from oracle import language_oracle as O
+
+from test_gpu_language import DT, U, check_dropout, check_scores, gen, make_logits
 
 pytestmark = pytest.mark.gpu
 
@@ -96,6 +98,50 @@ def test_numbers_that_are_none_are_refused():
     assert torch.equal(F.dropout(x, 0.5, np.int64(7), offset=2.0, shared_dim=np.int32(0)), F.dropout(x, 0.5, 7, offset=2, shared_dim=0))
     assert torch.equal(F.embedding(t, x, padding_idx=np.int64(1)), F.embedding(t, x))
     assert F.token_log_probs(x, t, top=np.int64(2), ignore_index=np.int64(-5)).top_tokens.shape == (3, 2)
+
+
+# ---------------------------------------------------------------- dropout
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("rows,width,cut", [(700, 64, 8), (700, 64, 5), (513, 33, 1), (1, 96, 32), (4099, 3, 2)])
+def test_dropout_of_rows_apart(rows, width, cut, dtype):
+    """[rows, width] with gaps between its rows is read in place, forward and backward."""
+    wide = torch.randn(rows, width + cut, generator=gen(34), device="cuda").to(DT[dtype])
+    for x in (wide[:, :width], wide[:, cut:], wide[::2, :width], wide[:1, :width].expand(rows, width)):
+        for d in (None, 0):
+            check_dropout(x, 0.3, 11, 4, d, grad=wide[: x.shape[0], :width])
+    check_dropout(torch.randn(width, rows, generator=gen(35), device="cuda").to(DT[dtype]).t(), 0.3, 11, 4, 0)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_dropout_of_more_dimensions_apart(dtype):
+    x = torch.randn(3, 4, 5, 6, 40, generator=gen(36), device="cuda").to(DT[dtype])
+    for v in (x[..., :32], x[..., 3:], x[:, :, :, ::2], x.transpose(1, 2), x.transpose(0, 3)[..., :8], x[:, :1].expand_as(x), x.permute(4, 0, 1, 2, 3)):
+        for d in (None, 0, 2, 3):
+            check_dropout(v, 0.3, 13, 4, d)
+
+
+@pytest.mark.parametrize("shape,shared_dim", [((4096,), None), ((4096,), 0), ((16, 256), None), ((16, 256), 1), ((4, 4, 256), None)])
+def test_dropout_of_rows_apart_copies_nothing(shape, shared_dim):
+    x = torch.randn(*shape, 1024 + 8, device="cuda")[..., :1024]
+    F.dropout(x, 0.5, 1)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = F.dropout(x, 0.5, 1, shared_dim=shared_dim)
+    assert torch.cuda.max_memory_allocated() - before == y.numel() * 4
+
+
+def test_dropout_of_more_than_2_to_31_rows():
+    n0, n1 = 2 ** 16, 2 ** 15 + 3
+    x = torch.ones(n0, n1, 2, device="cuda", dtype=torch.bfloat16)[:, :, :1]
+    y = F.dropout(x, 0.25, 9, offset=2).view(-1)
+    for first in (0, 2 ** 31 - 2048, n0 * n1 // 4 * 4 - 4096):
+        assert torch.equal(y[first:first + 4096] != 0, torch.from_numpy(O.kept(4096, 0.25, 9, 2, first)).cuda())
+    del y
+    y = F.dropout(x, 0.25, 9, offset=2, shared_dim=0)
+    mask = torch.from_numpy(O.kept(n1, 0.25, 9, 2)).cuda()
+    assert (y.view(n0, n1)[::4093] != 0).eq(mask).all()
+    with pytest.raises(ValueError, match="more than 2\\^31 - 1 rows"):
+        F.dropout(x, 0.25, 9, shared_dim=1)
 
 
 # ---------------------------------------------------------------- C ABI
