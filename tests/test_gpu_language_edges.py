@@ -8,7 +8,7 @@ import fastlstm_b200 as F
 from fastlstm_b200 import _lib
 from oracle import language_oracle as O
 
-from test_gpu_language import DT, U, check_dropout, check_scores, gen, make_logits
+from test_gpu_language import DT, EPS, TINY, U, check_dropout, check_scores, gen, make_logits, np64
 
 pytestmark = pytest.mark.gpu
 
@@ -77,6 +77,95 @@ def test_scores_of_tokens_outside_of_the_vocabulary_give_no_gradient(vocab, top,
         F.check_status()
         rows = torch.arange(5, device="cuda") != 2
         assert not d[2].any() and torch.equal(d[rows], ref[rows])
+
+
+def masked_rows(vocab, dtype):
+    z = make_logits(gen(38), 9, vocab, dtype=dtype)
+    low = torch.finfo(DT[dtype]).min
+    z[1, ::2] = -float("inf")
+    z[2, 1:] = -float("inf")                    # one token possible
+    z[3] = -float("inf")                        # none
+    z[4, : vocab - 3] = low
+    z[5] = low                                  # all equal
+    z[6, 5:] = -float("inf")
+    z[7, torch.rand(vocab, generator=gen(39), device="cuda") < 0.7] = low
+    return z
+
+
+@pytest.mark.parametrize("temperature", [1.0, 1.5])
+@pytest.mark.parametrize("top", [0, 4])
+@pytest.mark.parametrize("vocab", [40, 600, 3000, 40000])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_scores_of_masked_rows_to_bounds_of_their_own(dtype, vocab, top, temperature):
+    """Every row and every logit has its own bound, over what counts in that row.
+
+    With D the largest distance in powers of two of a logit whose probability is not 0 in 32 bits (e^-104), a power of two is
+    relatively off by (3 D + 4) u, the sum over a row by V / 64 u more.  A log probability lp adds roundings of its own size: (8 |lp| +
+    3 D + 8 + V / 64) u.  The entropy H, a mean of distances (at most H) over that sum: (H + 1) (6 D + 20 + V / 32) u.  A gradient,
+    p (g + g_H (lp + H)) / T, whose p is relatively off by (6 D + 12 + V / 64) u and which rounds sums of at most 5 terms and the entropy:
+    (6 D + 88 + V / 64) u of its terms' size, p |g_H| times the entropy's bound, 40 u of itself, and what 2^-126 cuts off; then the type's rounding.
+    """
+    z = masked_rows(vocab, dtype).requires_grad_()
+    raw, V = np64(z), vocab
+    for token in (0, vocab - 1):
+        tokens = torch.full((9,), token, device="cuda")
+        r = F.token_log_probs(z, tokens, top=top, temperature=temperature)
+        want = O.token_log_probs(raw, tokens.cpu().numpy(), top, temperature)
+        lp = want["lp"]
+        D = np.where(lp > -104, np.abs(lp), 0).max(1) / np.log(2) + 1
+
+        def check(got, ref, bound, small, what):
+            fine = np.isfinite(ref)
+            assert np.array_equal(got[~fine], ref[~fine]), what
+            assert (bound[fine] <= small[fine]).all(), what + ": the bound would hold anything"
+            err = np.abs(got[fine] - ref[fine])
+            assert (err <= bound[fine]).all(), (what, err.max())
+
+        def of_log_probs(ref, D):
+            with np.errstate(invalid="ignore"):
+                return (8 * np.abs(ref) + 3 * D + 8 + V / 64) * U, 1e-4 * (1 + np.abs(ref))
+        check(np64(r.log_probs), want["log_probs"], *of_log_probs(want["log_probs"], D), "log_probs")
+        H = want["entropy"]
+        of_H = (H + 1) * (6 * D + 20 + V / 32) * U
+        check(np64(r.entropy), H, of_H, 2e-4 * (1 + H), "entropy")
+        if top:
+            assert np.array_equal(r.top_tokens.cpu().numpy(), want["top_tokens"])
+            check(np64(r.top_log_probs), want["top_log_probs"], *of_log_probs(want["top_log_probs"], D[:, None]), "top_log_probs")
+        outs = [r.log_probs, r.entropy] + ([r.top_log_probs] if top else [])
+        ups = [torch.randn(t.shape, generator=gen(40), device="cuda") for t in outs]
+        (d,) = torch.autograd.grad(outs, z, ups)
+        g = [np64(u) for u in ups]
+        ref, size = O.token_log_probs_grad(raw, tokens.cpu().numpy(), g[0], g[1], g[2] if top else None, temperature)
+        g_all = np.abs(g[0]) + (np.abs(g[2]).sum(1) if top else 0) + np.abs(g[1]) * (200 + H)
+        p = np.exp(lp)
+        inner = ((6 * D + 88 + V / 64)[:, None] * U * size + p * (np.abs(g[1]) * of_H / temperature)[:, None] + 40 * U * np.abs(ref)
+                 + 2.0 ** -126 * g_all[:, None] / temperature)
+        check(np64(d), ref, inner + EPS[dtype] * np.abs(ref) + TINY[dtype],
+              1e-3 * (p * g_all[:, None] / temperature + np.abs(ref)) + EPS[dtype] * np.abs(ref) + TINY[dtype] + 1e-34, "dlogits")
+
+
+# ---------------------------------------------------------------- embedding
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [1, 2, 3, 7, 33, 302])
+@pytest.mark.parametrize("bad", [[0], [22], [5, 6], [3, 11, 12, 13], list(range(23))])
+def test_lookups_of_tokens_outside_of_the_vocabulary_in_odd_widths(width, bad, dtype):
+    """Rows that begin and end inside of 16-byte pieces: a row of NaN ends where it should, and is reported."""
+    W = torch.randn(7, width, generator=gen(37), device="cuda").to(DT[dtype]).requires_grad_()
+    good = torch.arange(23, device="cuda") % 7
+    rows = torch.ones(23, dtype=torch.bool, device="cuda")
+    rows[bad] = False
+    for wrong, scale, kind in ((7, 1.0, torch.int64), (-1, 3.0, torch.int64), (2 ** 40 + 3, 1.0, torch.int64), (-2 ** 31, 1.0, torch.int32)):
+        tokens = torch.where(rows, good, wrong).to(kind)
+        out = F.embedding(tokens, W, scale=scale)
+        with pytest.raises(_lib.BlstmError, match="token %d at position" % min(wrong, 2 ** 31 - 1)) as e:
+            F.check_status()
+        assert e.value.code == _lib.E_TOKEN and int(str(e.value).split("position ")[1].split(":")[0]) in bad
+        F.check_status()
+        want = (W.detach().float() * scale).to(W.dtype)[good]
+        assert out[~rows].isnan().all() and torch.equal(out[rows], want[rows])
+        (dW,) = torch.autograd.grad(out, W, torch.ones_like(out))
+        count = torch.bincount(good[rows], minlength=7).float()[:, None] * scale
+        assert torch.equal(dW.float(), count.expand(7, width))
 
 
 # ---------------------------------------------------------------- arguments
