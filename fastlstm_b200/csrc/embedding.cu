@@ -163,7 +163,7 @@ __device__ __forceinline__ unsigned sort_key(const SortParams& p, unsigned i) {
 }
 
 // Keys, and every tile's counts of the first digit; clears the counts of the others.  Bound by latency, as the passes are: 4 us at
-// 16384 tokens, 9 at 131072 with 32 MB cleared beside it.
+// 16384 tokens, 8 at 131072 with 32 MB cleared beside it.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_constant__ SortParams p) {
   __shared__ unsigned hist[kMaxBins];
@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_c
 
 // One stable pass over a digit.  A block owns a tile: it adds up what the digit's counts say of the other tiles, ranks its
 // own elements (warp by warp, each a run of consecutive ones) and puts them in their places; it counts the next digit in
-// the tiles they have come to.  14 us at 131072 tokens with 32 MB cleared beside it.
+// the tiles they have come to.  15 to 18 us at 131072 tokens with 32 MB cleared beside it.  That every block reads the counts of all
+// tiles grows with their square: a pass takes 25 to 45 us at 2^20 tokens and 0.9 to 1.1 ms at 2^24, where the sums of 64 bf16 columns take 0.75.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const __grid_constant__ SortParams p) {
   __shared__ unsigned short hist[kSortWarps][kMaxBins];    // of a tile, whose numbers 16 bits hold
@@ -419,7 +420,7 @@ __device__ __forceinline__ void put_sum(const SumParams& p, unsigned t, unsigned
 enum : unsigned { kGoesOn = 0, kWhole = 1, kLastPart = 2, kFirstPart = 3 };
 
 // A group of threads adds a run's rows up, four or eight of them on their way.  Bound by memory where there are many: 131072 x 1024 fp16 and
-// 172 MB of zeros 88 us (5.9 TB/s); 16384 x 512 bf16 9 us, which are a run's latency.
+// 172 MB of zeros 80 to 83 us (6.2 TB/s); 16384 x 512 bf16 9 us, which are a run's latency.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumParams p) {
   using V = Pack<T, VEC>;

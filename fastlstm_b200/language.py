@@ -66,8 +66,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     With them the distribution's entropy and, for top > 0 (at most 32), the likeliest tokens; log_probs, entropy and
     top_log_probs are differentiable.  Logits may be strided as long as the vocabulary is dense (a padded one, cut, is).
     Logits of -inf are impossible tokens.  A row of nothing else: log_probs and top_log_probs -inf, entropy 0, the first
-    tokens, no gradient.  NaN or +inf in a row makes its results NaN.  Rows whose token is ignore_index are not read:
-    log_probs 0, entropy 0, top_log_probs -inf, top_tokens -1, no gradient.  Entropy and alternatives of a row whose token
+    tokens, no gradient.  NaN or +inf in a row makes its results NaN.  Rows whose token is ignore_index count for
+    nothing, whatever they hold: log_probs 0, entropy 0, top_log_probs -inf, top_tokens -1, no gradient.  Entropy and alternatives of a row whose token
     is outside of the vocabulary are its own, without a gradient."""
     return TokenLogProbs(*_lib.host().token_log_probs(logits, tokens, _whole(top, "top"), float(temperature),
                                                        _whole(ignore_index, "ignore_index")))
