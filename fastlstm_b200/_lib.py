@@ -51,6 +51,11 @@ class ScoreDesc(Structure):
                 ("vocab", c_int64), ("logits_stride", c_int64 * 2), ("ignore", c_int64), ("top", c_int32), ("temperature", c_float)]
 
 
+class NormDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("eps", c_float), ("n0", c_int64), ("n1", c_int64), ("width", c_int64),
+                ("x_stride", c_int64 * 2), ("residual_stride", c_int64 * 2), ("dy_stride", c_int64 * 2)]
+
+
 # name -> (restype, argtypes); every symbol include/fastlstm_b200.h declares
 P = c_void_p
 DP = POINTER(Desc)
@@ -88,6 +93,10 @@ SIGNATURES = {
     "blstm_dropout": (c_int, [POINTER(DropoutDesc), P, P, P, P]),
     "blstm_token_log_probs": (c_int, [POINTER(ScoreDesc)] + [P] * 8),
     "blstm_token_log_probs_grad": (c_int, [POINTER(ScoreDesc)] + [P] * 12),
+    "blstm_rms_norm": (c_int, [POINTER(NormDesc)] + [P] * 7),
+    "blstm_rms_norm_e4m3": (c_int, [POINTER(NormDesc)] + [P] * 7),
+    "blstm_rms_norm_grad_workspace": (c_size_t, [POINTER(NormDesc)]),
+    "blstm_rms_norm_grad": (c_int, [POINTER(NormDesc)] + [P] * 8 + [c_size_t, P]),
 }
 
 _lib = None

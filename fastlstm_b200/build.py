@@ -17,7 +17,7 @@ import sysconfig
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libfastlstm_b200.so")
-HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_language.cpp")]
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_language.cpp", "host_norm.cpp")]
 HOST_PATH = os.path.join(PKG_DIR, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 HEADERS = glob.glob(os.path.join(PKG_DIR, "..", "include", "*.h"))
 
@@ -72,7 +72,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(LIB_PATH, lib_deps):
         _run([_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB_PATH] + sources() + ["-lcuda"],
              "libfastlstm_b200.so", verbose)()
-    if force or _stale(HOST_PATH, HOST_SRCS + [os.path.join(CSRC, "host.h")] + HEADERS):
+    if force or _stale(HOST_PATH, HOST_SRCS + [os.path.join(CSRC, f) for f in ("host.h", "host_language.h")] + HEADERS):
         _run(_host_cmd(), "_host", verbose)()
     return LIB_PATH
 

@@ -419,4 +419,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("packed_maps", &packed_maps);
   m.def("check_status", &check_status);
   bind_language(m);
+  bind_norm(m);
 }

@@ -124,5 +124,6 @@ struct Call {
 };
 
 void bind_language(py::module_& m);   // host_language.cpp
+void bind_norm(py::module_& m);       // host_norm.cpp
 
 }  // namespace blstm_host

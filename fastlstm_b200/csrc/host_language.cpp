@@ -1,78 +1,11 @@
 // Host side of the operators around a language model: argument checks, buffers, the calls of the C ABI and the autograd
 // nodes.  Tensors keep their strides as long as two strides describe their rows and the last dimension is dense; others
 // are copied first.
-#include <ATen/cuda/EmptyTensor.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
-
-#include <cmath>
-
-#include "host.h"
+#include "host_language.h"
 
 namespace {
 
 using namespace blstm_host;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-py::value_error wrong(const std::string& what) { return py::value_error(what); }
-
-void on_gpu(const Tensor& t, const char* name) {
-  if (!t.is_cuda()) throw wrong(std::string(name) + " must be a CUDA tensor (there is no CPU path)");
-}
-void beside(const Tensor& t, const char* name, const Tensor& other) {
-  on_gpu(t, name);
-  if (t.device() != other.device()) throw wrong(std::string(name) + " is on " + t.device().str() + ", expected " + other.device().str());
-}
-int token_bits(const Tensor& tokens) {
-  if (tokens.scalar_type() == at::kLong) return 64;
-  if (tokens.scalar_type() == at::kInt) return 32;
-  throw wrong(std::string("tokens have dtype ") + c10::toString(tokens.scalar_type()) + ", expected int64 or int32");
-}
-
-// The leading dimensions of an operator's tensors as [n0, n1].
-struct Lead {
-  int64_t dims, n0, n1;
-  explicit Lead(at::IntArrayRef s) : dims((int64_t)s.size()), n0(1), n1(1) {
-    if (dims == 2) { n0 = s[0]; n1 = s[1]; }
-    else n1 = c10::multiply_integers(s);
-    if (n0 > 0 && n1 > INT32_MAX / n0) throw wrong("more than 2^31 - 1 rows");
-  }
-  // t with `dims` leading dimensions as one whose rows stride[0..1] reach
-  Tensor rows(const Tensor& t, int64_t stride[2]) const {
-    Tensor v = dims > 2 ? t.flatten(0, dims - 1) : t;
-    const int64_t lead = dims > 2 ? 1 : dims;
-    if (v.dim() > lead && v.size(-1) > 1 && v.stride(-1) != 1) v = v.contiguous();
-    stride[0] = lead == 2 ? v.stride(0) : 0;
-    stride[1] = lead == 0 ? 0 : v.stride(lead - 1);
-    return v;
-  }
-};
-
-Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& like) { return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt); }
-
-// A node of the graph that an operator's gradient is, with what it needs as members (a torch::autograd::Function keeps that in a
-// dictionary: 4 us a call).  Backward goes through it once.
-template <typename N>
-std::shared_ptr<N> make_node(const Tensor& input) {
-  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
-  node->set_next_edges(torch::autograd::collect_next_edges(input));
-  return node;
-}
-
-bool wants_grad(const Tensor& t) {
-  TORCH_CHECK(!t._fw_grad(0).defined(), "fastlstm_b200: forward-mode gradients are not there for this operator");
-  return at::GradMode::is_enabled() && t.requires_grad();
-}
-void only_once() { TORCH_CHECK(!at::GradMode::is_enabled(), "fastlstm_b200: gradients of gradients (create_graph) are not there for this operator"); }
-
-std::vector<int64_t> plus(at::IntArrayRef s, int64_t last) {
-  std::vector<int64_t> v = s.vec();
-  v.push_back(last);
-  return v;
-}
 
 // ---------------------------------------------------------------- embedding
 blstm_embed_desc embed_desc(at::ScalarType dt, const Tensor& tokens, const Lead& lead, int64_t V, int64_t D, double scale, int64_t padding) {

@@ -71,3 +71,26 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,
     is outside of the vocabulary are its own, without a gradient."""
     return TokenLogProbs(*_lib.host().token_log_probs(logits, tokens, _whole(top, "top"), float(temperature),
                                                        _whole(ignore_index, "ignore_index")))
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x; with a residual [of x's shape] h = x + residual, and
+    the result is (y, h): what goes into the next layer, and the next one's residual.
+
+    h is rounded to the tensors' type before the norm is taken of it.  y and h are dense; all of x, residual and weight are
+    differentiable, the weight's gradient is added up in 32 bits in an order that the sizes and strides fix."""
+    return _lib.host().rms_norm(x, weight, residual, float(eps))
+
+
+class EightBitRows(NamedTuple):
+    """What rms_norm_e4m3 returns: values * scales[..., None] is the norm; sum is None where there was no residual."""
+    values: torch.Tensor                     # [..., width] float8_e4m3fn
+    scales: torch.Tensor                     # [...]        float32: the row's largest magnitude / 448
+    sum: Optional[torch.Tensor]              # [..., width] x + residual
+
+
+def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> EightBitRows:
+    """rms_norm with its output in 8 bits and a scale for every row, for products of 8-bit operands; without gradients.
+
+    Values are rounded once, from 32 bits.  A row of zeros has scale 0 and values 0."""
+    return EightBitRows(*_lib.host().rms_norm_e4m3(x, weight, residual, float(eps)))

@@ -318,6 +318,29 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
                                const float* g_entropy, const int64_t g_entropy_stride[2], const float* g_top,
                                void* dlogits, const int64_t dlogits_stride[2], void* stream);
 
+/* Root-mean-square norm of a sum.  Strides of x (of h in the gradient), residual (dsum) and dy; y, values, sum and dx are dense. */
+typedef struct blstm_norm_desc {
+  int32_t dtype;             /* of every tensor but scales, rstd and values                            */
+  float eps;                 /* of at least 0                                                          */
+  int64_t n0, n1, width;     /* x [n0, n1, width], n0 * n1 < 2^31, width < 2^30                        */
+  int64_t x_stride[2], residual_stride[2], dy_stride[2];
+} blstm_norm_desc;
+
+/* h = round(x + residual), y = round(h i weight), i = 1 / sqrt(mean h^2 + eps).  residual and sum (h) are both given or both NULL
+ * (h = x).  rstd [n0*n1]: i, which the gradient needs, or NULL. */
+int blstm_rms_norm(const blstm_norm_desc* d, const void* x, const void* residual, const void* weight, void* y, void* sum,
+                   float* rstd, void* stream);
+
+/* The same in 8 bits: values [n0,n1,width] = e4m3(h i weight / scale), scales [n0*n1] = the row's largest magnitude / 448. */
+int blstm_rms_norm_e4m3(const blstm_norm_desc* d, const void* x, const void* residual, const void* weight, void* values,
+                        float* scales, void* sum, void* stream);
+
+/* dx = the gradient of x and of residual alike, from dy and dsum (the gradient of h, or NULL), and dweight [width] (or NULL): added up
+ * in 32 bits in an order that the sizes and strides fix, rounded once.  The workspace is 256-byte aligned and not needed without dweight. */
+size_t blstm_rms_norm_grad_workspace(const blstm_norm_desc* d);
+int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* dsum, const void* h, const void* weight,
+                        const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Host memory (mapped into the device, four int32: -, status, detail[2]; on an 8-byte boundary both details
  * are always of one report) that the CALLING THREAD's later launches write a device-side error to as well, or
  * NULL (default): a caller that looks there need not read control blocks back.  The status word is written

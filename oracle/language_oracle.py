@@ -87,3 +87,32 @@ def token_log_probs_grad(logits, tokens, g_lp=None, g_h=None, g_top=None, temper
     for k in range(top):
         np.add.at(d, (rows[live], r["top_tokens"][live, k]), g_top[live, k].astype(np.float64))
     return np.where(live[:, None], d / temperature, 0.0), np.where(live[:, None], size / temperature, 0.0)
+
+
+# ---------------------------------------------------------------- root-mean-square norm
+def rms_norm(h, weight, eps=1e-6):
+    """Rows of h (already a sum, as it is stored): (y, i) with i [..., 1] the inverse of the root."""
+    h, weight = h.astype(np.float64), weight.astype(np.float64)
+    i = 1 / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+    return h * i * weight, i
+
+
+def rms_norm_grad(h, weight, dy, dh=None, eps=1e-6):
+    """(dh of the sum, dweight) and the sums of the terms' magnitudes that bound what rounding may do to each."""
+    h, weight, dy = (t.astype(np.float64) for t in (h, weight, dy))
+    _, i = rms_norm(h, weight, eps)
+    n, D = dy * weight, h.shape[-1]
+    by = i * i * (n * h).sum(-1, keepdims=True) / D
+    size = i * (np.abs(n) + np.abs(h) * i * i * np.abs(n * h).sum(-1, keepdims=True) / D)
+    dx = i * (n - h * by)
+    if dh is not None:
+        dx, size = dx + dh, size + np.abs(dh)
+    lead = tuple(range(h.ndim - 1))
+    return dx, (dy * h * i).sum(lead), size, np.abs(dy * h * i).sum(lead)
+
+
+def e4m3(x):
+    """The nearest e4m3 number (even ones where two are as near), for magnitudes up to 448."""
+    a = np.abs(x).astype(np.float64)
+    step = 2.0 ** (np.floor(np.log2(np.maximum(a, 2.0 ** -6))) - 3)
+    return np.sign(x) * np.rint(a / step) * step
