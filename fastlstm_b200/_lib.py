@@ -56,6 +56,27 @@ class NormDesc(Structure):
                 ("x_stride", c_int64 * 2), ("residual_stride", c_int64 * 2), ("dy_stride", c_int64 * 2)]
 
 
+class AdamWItem(Structure):
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p), ("exp_avg_scale", c_void_p),
+                ("exp_avg_sq_scale", c_void_p), ("master", c_void_p), ("step", c_void_p), ("n", c_int64), ("number", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class AdamWDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("bits", c_int32), ("items", c_int32), ("reserved", c_int32), ("item", POINTER(AdamWItem)), ("lr", c_double),
+                ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double), ("seed", c_uint64), ("lr_at", c_void_p),
+                ("factor", c_void_p), ("ticket", c_void_p)]
+
+
+class GradItem(Structure):
+    _fields_ = [("grad", c_void_p), ("n", c_int64), ("dtype", c_int32), ("reserved", c_int32)]
+
+
+class GradNormDesc(Structure):
+    _fields_ = [("item", POINTER(GradItem)), ("items", c_int32), ("max_norm", c_float), ("out", c_void_p), ("ticket", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/fastlstm_b200.h declares
 P = c_void_p
 DP = POINTER(Desc)
@@ -93,6 +114,9 @@ SIGNATURES = {
     "blstm_dropout": (c_int, [POINTER(DropoutDesc), P, P, P, P]),
     "blstm_token_log_probs": (c_int, [POINTER(ScoreDesc)] + [P] * 8),
     "blstm_token_log_probs_grad": (c_int, [POINTER(ScoreDesc)] + [P] * 12),
+    "blstm_adamw": (c_int, [POINTER(AdamWDesc), P]),
+    "blstm_grad_norm_workspace": (c_size_t, [c_int]),
+    "blstm_grad_norm": (c_int, [POINTER(GradNormDesc), P]),
     "blstm_rms_norm": (c_int, [POINTER(NormDesc)] + [P] * 7),
     "blstm_rms_norm_e4m3": (c_int, [POINTER(NormDesc)] + [P] * 7),
     "blstm_rms_norm_grad_workspace": (c_size_t, [POINTER(NormDesc)]),

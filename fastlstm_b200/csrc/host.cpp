@@ -420,4 +420,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("check_status", &check_status);
   bind_language(m);
   bind_norm(m);
+  bind_adamw(m);
 }

@@ -125,5 +125,6 @@ struct Call {
 
 void bind_language(py::module_& m);   // host_language.cpp
 void bind_norm(py::module_& m);       // host_norm.cpp
+void bind_adamw(py::module_& m);      // host_adamw.cpp
 
 }  // namespace blstm_host

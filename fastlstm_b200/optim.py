@@ -1,0 +1,164 @@
+"""AdamW over all of a model's tensors in one launch a data type, its states in 32 or 8 bits (csrc/adamw.cu; what a call does on the
+host is csrc/host_adamw.cpp)."""
+from __future__ import annotations
+
+import math
+from itertools import chain
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .language import _whole
+
+BLOCK = 256                  # elements of a tensor, in row-major order, that share a scale in 8-bit states
+
+
+class AdamW(torch.optim.Optimizer):
+    """Adam with decoupled weight decay, on contiguous CUDA parameters in float32, float16 or bfloat16:
+
+        m = beta1 m + (1 - beta1) g     v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+
+    state_bits=32 keeps m and v as `exp_avg` and `exp_avg_sq` in float32; state dicts of torch.optim.AdamW can be loaded.
+    state_bits=8 keeps m and sqrt(v) as `exp_avg` and `exp_avg_sq_root` in float8_e4m3fn, times `exp_avg_scale` and
+    `exp_avg_sq_root_scale`, one for every 256 elements (their largest magnitude / 448).  Numbers between two of e4m3 go up with the
+    probability of what would be cut off, a function of `seed`, step, tensor and element: means are kept, and a run repeats
+    bit by bit.  A gradient that is not finite spoils the 256 elements that it shares scales with (see max_norm).
+    master_weights: 16-bit parameters have their weight in float32 in the state (`master`) and are it, rounded.  Without, steps that
+    are less than half the distance of two 16-bit numbers are lost.
+    max_norm: gradients are multiplied by min(1, max_norm / (norm + 1e-6)), the norm taken over all parameters (on one device) and
+    found in `grad_norm`.  Where it is not finite the step does nothing and does not count.
+    lr may be a CUDA tensor of one float32, read when the step runs: a captured step can be replayed with another rate.  (Take a
+    step, or load a state, before a capture; step counts lie in device memory and go on in replays.)"""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 master_weights: bool = True, max_norm: Optional[float] = None, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
+        if max_norm is not None and not (max_norm > 0 and math.isfinite(max_norm)):
+            raise ValueError(f"max_norm must be positive and finite, got {max_norm!r}")
+        self.state_bits, self.master_weights = int(state_bits), bool(master_weights)
+        self.max_norm = None if max_norm is None else float(max_norm)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, seed=_whole(seed, "seed", 0, 2 ** 64 - 1)))
+
+    def add_param_group(self, param_group):
+        group = {**self.defaults, **param_group}
+        lr, betas = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or not lr.is_floating_point():
+                raise ValueError("lr as a tensor must be one floating-point element")
+        elif not (lr >= 0 and math.isfinite(lr)):
+            raise ValueError(f"lr must be at least 0 and finite, got {lr!r}")
+        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"betas must be two numbers in [0, 1), got {betas!r}")
+        for name in ("eps", "weight_decay"):
+            if not (group[name] >= 0 and math.isfinite(group[name])):
+                raise ValueError(f"{name} must be at least 0 and finite, got {group[name]!r}")
+        super().add_param_group(param_group)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "master_weights": self.master_weights, "max_norm": self.max_norm}
+
+    # ------------------------------------------------------------------ state
+    def _format(self, p):
+        """The state's tensors as {name: (shape, dtype)}, in the order that the extension takes them."""
+        moment = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+        f = {"exp_avg": (p.shape, moment), "exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root": (p.shape, moment), "step": ((), torch.int64)}
+        if self.state_bits == 8:
+            blocks = ((p.numel() + BLOCK - 1) // BLOCK,)
+            f["exp_avg_scale"] = f["exp_avg_sq_root_scale"] = (blocks, torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            f["master"] = (p.shape, torch.float32)
+        return f
+
+    def _start(self, p):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: take a step or load a state before a capture, which would begin with new states at every replay")
+        self.state[p] = {name: p.detach().float() if name == "master" else torch.zeros(shape, dtype=dtype, device=p.device)
+                         for name, (shape, dtype) in self._format(p).items()}
+        return self.state[p]
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Takes copies in the types that this optimizer keeps.  Masters that the state does not have are the parameters."""
+        ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = dict(zip(ids, chain.from_iterable(g["params"] for g in self.param_groups)))
+        loaded = {}
+        for k, saved in state_dict["state"].items():
+            if k not in params:
+                raise ValueError("loaded state dict has a state of a parameter that is in none of its groups")
+            p, loaded[k] = params[k], {}
+            for name, (shape, dtype) in self._format(p).items():
+                if name == "master" and name not in saved:
+                    loaded[k][name] = p.detach().float()
+                    continue
+                if name not in saved:
+                    raise ValueError(f"loaded state has no {name}: it is of an optimizer with other state_bits")
+                t = torch.as_tensor(saved[name])
+                if tuple(t.shape) != tuple(shape):
+                    raise ValueError(f"{name} of the loaded state has shape {tuple(t.shape)}, expected {tuple(shape)}")
+                if (t.dtype == torch.float8_e4m3fn) != (dtype == torch.float8_e4m3fn):
+                    raise ValueError(f"{name} of the loaded state has dtype {t.dtype}, expected {dtype}: it is of an optimizer with other state_bits")
+                loaded[k][name] = torch.empty(shape, dtype=dtype, device=p.device).copy_(t)
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise ValueError("loaded state is of an optimizer with amsgrad or maximize, which are not there")
+        super().load_state_dict({**state_dict, "state": {}})
+        for g in self.param_groups:
+            for name, value in self.defaults.items():
+                g.setdefault(name, value)
+        for k, s in loaded.items():
+            self.state[params[k]] = s
+
+    # ------------------------------------------------------------------ step
+    def _scratch(self, device):
+        """(the counter that launches use, {norm, factor}) of a device."""
+        kept = self.__dict__.setdefault("_kept", {})
+        if device not in kept:
+            kept[device] = (torch.zeros(1, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.float32, device=device))
+        return kept[device]
+
+    @property
+    def grad_norm(self) -> Optional[torch.Tensor]:
+        """The norm of all gradients in the last step (before they were clipped), where max_norm is set; None before the first."""
+        return self.__dict__.get("_norm")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls, number = [], -1
+        for group in self.param_groups:
+            lists = {}
+            for p in group["params"]:
+                number += 1
+                if p.grad is None:
+                    continue
+                s = self.state.get(p) or self._start(p)
+                names = self._format(p)
+                params, grads, states, numbers = lists.setdefault((p.device, p.dtype), ([], [], [], []))
+                params.append(p)
+                grads.append(p.grad)
+                states.append([s[name] for name in names])
+                numbers.append(number)
+            calls += [(group, device, dtype, *l) for (device, dtype), l in lists.items()]
+        if not calls:
+            return loss
+        host, norm = _lib.host(), None
+        if self.max_norm is not None:
+            if len({c[1] for c in calls}) > 1:
+                raise ValueError("max_norm takes parameters on one device")
+            ticket, norm = self._scratch(calls[0][1])
+            host.grad_norm([g for c in calls for g in c[4]], self.max_norm, norm, ticket)
+            self._norm = norm[0]
+        for group, device, dtype, params, grads, states, numbers in calls:
+            if device.type != "cuda":
+                raise ValueError("a parameter must be a CUDA tensor (there is no CPU path)")
+            lr, (beta1, beta2) = group["lr"], group["betas"]
+            at = lr if isinstance(lr, torch.Tensor) and lr.is_cuda else None
+            host.adamw(params, grads, states, numbers, self.state_bits, "master" in self._format(params[0]), 0.0 if at is not None else float(lr), at,
+                       float(beta1), float(beta2), float(group["eps"]), float(group["weight_decay"]), group["seed"], norm, self._scratch(device)[0])
+        return loss

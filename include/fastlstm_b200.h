@@ -341,6 +341,54 @@ size_t blstm_rms_norm_grad_workspace(const blstm_norm_desc* d);
 int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* dsum, const void* h, const void* weight,
                         const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
 
+/* One tensor of an AdamW step: param, grad and the states have n elements each, dense, in one order. */
+typedef struct blstm_adamw_item {
+  void* param;
+  const void* grad;              /* of param's type                                                    */
+  void *exp_avg, *exp_avg_sq;    /* 32 bits: fp32 m and v; 8 bits: e4m3 m and sqrt(v), times a scale   */
+  float *exp_avg_scale, *exp_avg_sq_scale;   /* 8 bits: [(n + 255) / 256] each                         */
+  float* master;                 /* 16-bit types: the weight in fp32 (param is it, rounded), all items or none */
+  int64_t* step;                 /* steps so far; the launch adds one                                  */
+  int64_t n;
+  uint32_t number, reserved;     /* 8 bits: the tensor's number in the words that round its states     */
+} blstm_adamw_item;
+
+typedef struct blstm_adamw_desc {
+  int32_t dtype, bits;           /* of param and grad; 32 or 8, of the states                          */
+  int32_t items, reserved;
+  const blstm_adamw_item* item;  /* HOST memory, read during the call                                  */
+  double lr, beta1, beta2, eps, weight_decay;
+  uint64_t seed;
+  const float* lr_at;            /* lr in device memory, read when the kernel runs, or NULL            */
+  const float* factor;           /* of the gradients, in device memory, or NULL: 1.  NaN: nothing changes, no step counts */
+  uint32_t* ticket;              /* one word of 0, which is 0 again behind the launch; of one launch at a time */
+} blstm_adamw_desc;
+
+/* g' = grad factor, m' = beta1 m + (1 - beta1) g', v' = beta2 v + (1 - beta2) g'^2, p' = p (1 - lr weight_decay) - lr m' / (1 - beta1^t) /
+ * (sqrt(v' / (1 - beta2^t)) + eps).  8 bits: a block of 256 elements has the scale (largest magnitude) / 448; numbers between two
+ * e4m3 ones are cut off or rounded up with the probability of what is cut off, by the lower (m) and upper (sqrt v) 16 bits of word
+ * Philox4x32-10(key seed, counter (element / 4, t, number))[element % 4]; a root that is not 0 does not become 0. */
+int blstm_adamw(const blstm_adamw_desc* d, void* stream);
+
+typedef struct blstm_grad_item {
+  const void* grad;
+  int64_t n;
+  int32_t dtype, reserved;
+} blstm_grad_item;
+typedef struct blstm_grad_norm_desc {
+  const blstm_grad_item* item;   /* HOST memory, read during the call                                  */
+  int32_t items;                 /* out is not written where this is 0                                 */
+  float max_norm;
+  float* out;                    /* [2]: the norm; min(1, max_norm / (norm + 1e-6)), NaN where the norm is infinite or NaN */
+  uint32_t* ticket;              /* as above                                                           */
+  void* workspace;               /* 256-byte aligned                                                   */
+  size_t workspace_bytes;
+} blstm_grad_norm_desc;
+
+/* The 2-norm over all elements of all tensors, in an order that the sizes fix. */
+size_t blstm_grad_norm_workspace(int items);
+int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream);
+
 /* Host memory (mapped into the device, four int32: -, status, detail[2]; on an 8-byte boundary both details
  * are always of one report) that the CALLING THREAD's later launches write a device-side error to as well, or
  * NULL (default): a caller that looks there need not read control blocks back.  The status word is written
