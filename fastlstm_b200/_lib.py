@@ -28,6 +28,7 @@ OK = 0
 E_WAIT_TIMEOUT = 6
 E_TOO_LARGE = 8
 E_TOKEN = 9
+E_PARENT = 10
 
 
 class Desc(Structure):
@@ -77,6 +78,15 @@ class GradNormDesc(Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
+class BeamDesc(Structure):
+    _fields_ = [("dtype", c_int32), ("width", c_int32), ("batch", c_int64), ("beams", c_int64), ("vocab", c_int64), ("logits_stride", c_int64 * 2),
+                ("end_token", c_int64), ("length_penalty", c_double)]
+
+
+class ReorderItem(Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("outer", c_int64), ("inner_bytes", c_int64), ("outer_stride", c_int64), ("row_stride", c_int64)]
+
+
 # name -> (restype, argtypes); every symbol include/fastlstm_b200.h declares
 P = c_void_p
 DP = POINTER(Desc)
@@ -114,6 +124,9 @@ SIGNATURES = {
     "blstm_dropout": (c_int, [POINTER(DropoutDesc), P, P, P, P]),
     "blstm_token_log_probs": (c_int, [POINTER(ScoreDesc)] + [P] * 8),
     "blstm_token_log_probs_grad": (c_int, [POINTER(ScoreDesc)] + [P] * 12),
+    "blstm_beam_workspace": (c_size_t, [POINTER(BeamDesc)]),
+    "blstm_beam_step": (c_int, [POINTER(BeamDesc)] + [P] * 10 + [c_size_t, P]),
+    "blstm_reorder": (c_int, [POINTER(ReorderItem), c_int, P, c_int, c_int64, c_int64, c_int64, P]),
     "blstm_adamw": (c_int, [POINTER(AdamWDesc), P]),
     "blstm_grad_norm_workspace": (c_size_t, [c_int]),
     "blstm_grad_norm": (c_int, [POINTER(GradNormDesc), P]),

@@ -17,7 +17,7 @@ import sysconfig
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libfastlstm_b200.so")
-HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_language.cpp", "host_norm.cpp", "host_adamw.cpp")]
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_language.cpp", "host_norm.cpp", "host_adamw.cpp", "host_beam.cpp")]
 HOST_PATH = os.path.join(PKG_DIR, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 HEADERS = glob.glob(os.path.join(PKG_DIR, "..", "include", "*.h"))
 

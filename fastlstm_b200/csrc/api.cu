@@ -201,6 +201,7 @@ const char* blstm_strerror(int code) {
     case BLSTM_E_ARCH: return "device is not sm_100 (B200)";
     case BLSTM_E_TOO_LARGE: return "request exceeds the fixed capacity of this entry point";
     case BLSTM_E_TOKEN: return "token outside of the vocabulary";
+    case BLSTM_E_PARENT: return "parent that is none of the sentence's hypotheses";
   }
   return "unknown status code";
 }

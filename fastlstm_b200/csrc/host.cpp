@@ -421,4 +421,5 @@ PYBIND11_MODULE(_host, m) {
   bind_language(m);
   bind_norm(m);
   bind_adamw(m);
+  bind_beam(m);
 }

@@ -70,6 +70,7 @@ inline void poll(int dev) {
   const int code = m[1], d0 = m[2], d1 = m[3];
   m[1] = 0;
   if (code == BLSTM_E_TOKEN) throw DeviceError{code, "token " + std::to_string(d1) + " at position " + std::to_string((uint32_t)d0)};
+  if (code == BLSTM_E_PARENT) throw DeviceError{code, "parent " + std::to_string(d1) + " at position " + std::to_string((uint32_t)d0)};
   throw DeviceError{code, "recurrence (step " + std::to_string(d0) + ", batch tile " + std::to_string(d1) + ")"};
 }
 
@@ -126,5 +127,6 @@ struct Call {
 void bind_language(py::module_& m);   // host_language.cpp
 void bind_norm(py::module_& m);       // host_norm.cpp
 void bind_adamw(py::module_& m);      // host_adamw.cpp
+void bind_beam(py::module_& m);       // host_beam.cpp
 
 }  // namespace blstm_host

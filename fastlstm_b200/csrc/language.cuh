@@ -35,9 +35,9 @@ struct Tokens {
 // The mailbox that the calling thread has set (blstm_set_mailbox), or null.
 int* current_mailbox();
 
-// A token outside of the vocabulary: one report is kept, position and token in one store, the status word last.  (A mailbox of
-// ints need not lie on 8 bytes: there, position and token of two reports at a time may mix.)
-static __device__ __noinline__ void report_token(int* mailbox, unsigned position, long long token) {
+// A token outside of the vocabulary (or another number that is out of range): one report is kept, position and token in one store, the
+// status word last.  (A mailbox of ints need not lie on 8 bytes: there, position and token of two reports at a time may mix.)
+static __device__ __noinline__ void report_token(int* mailbox, unsigned position, long long token, int code = BLSTM_E_TOKEN) {
   if (!mailbox) return;
   volatile int* m = mailbox;
   const int shown = token > INT32_MAX ? INT32_MAX : token < INT32_MIN ? INT32_MIN : (int)token;
@@ -48,7 +48,7 @@ static __device__ __noinline__ void report_token(int* mailbox, unsigned position
     m[3] = shown;
   }
   __threadfence_system();
-  m[1] = BLSTM_E_TOKEN;
+  m[1] = code;
 }
 
 // VEC elements of T on their natural boundary, as floats.

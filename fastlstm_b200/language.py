@@ -94,3 +94,59 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[t
 
     Values are rounded once, from 32 bits.  A row of zeros has scale 0 and values 0."""
     return EightBitRows(*_lib.host().rms_norm_e4m3(x, weight, residual, float(eps)))
+
+
+class BeamStep(NamedTuple):
+    """What beam_step returns, the best hypothesis of every sentence first; finished and lengths are None where they were not asked for."""
+    scores: torch.Tensor                     # [batch, width] float32: log probabilities of the hypotheses so far
+    parents: torch.Tensor                    # [batch, width] int64: the hypothesis each goes on from
+    tokens: torch.Tensor                     # [batch, width] int64: what it goes on with
+    finished: Optional[torch.Tensor]         # [batch, width] bool: whether it has ended, with this token or before
+    lengths: Optional[torch.Tensor]          # [batch, width] int64: tokens up to its end
+
+
+def beam_step(logits: torch.Tensor, scores: torch.Tensor, *, width: Optional[int] = None, end_token: Optional[int] = None,
+              finished: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None, length_penalty: float = 0.0) -> BeamStep:
+    """The `width` best continuations of every sentence's hypotheses; without gradients.
+
+    logits [batch, hypotheses, vocabulary] are the hypotheses' next predictions, scores [batch, hypotheses] (float32) their log
+    probabilities so far; the first step has one hypothesis of score 0 and a width of its own (at most 32; the number of hypotheses by
+    default).  A continuation's score is its hypothesis' plus the log softmax of the logits.  A hypothesis in `finished` (bool) goes
+    on with end_token alone, at its own score; its logits are not read, nor are those of a hypothesis whose score is -inf.
+    With a length_penalty continuations are ranked by score / length ** length_penalty (scores stay what they are); lengths (int64)
+    counts the tokens of hypotheses, to which a continuation adds one unless its hypothesis is finished.
+
+    Sums are ranked in 64 bits, equal ones in the order of (hypothesis, token).  Where fewer than `width` continuations are possible,
+    impossible ones (score -inf) follow.  NaN or +inf among a hypothesis' logits makes its continuations NaN, which come first."""
+    whole = lambda v, name: None if v is None else _whole(v, name)
+    return BeamStep(*_lib.host().beam_step(logits, scores, whole(width, "width"), whole(end_token, "end_token"), finished, lengths, float(length_penalty)))
+
+
+def reorder_states(states, parents: torch.Tensor, *, dim: int = 1):
+    """What belongs to hypotheses in the order of those that go on: states [..., batch * hypotheses, ...] -> [..., batch * width, ...] along
+    dim, where row b * width + j is row b * hypotheses + parents[b, j].
+
+    states: a tensor or a (nested) list or tuple of tensors of any types, in which `None` stays: the (h, c) [layers, rows, width] of a
+    FastLSTM, several of them, and token histories [steps, rows] in one launch.  parents [batch, width] (int64 or int32) are those of
+    beam_step.  A parent that is none gives zeros, and `check_status()` or a later call raises BlstmError.  Without gradients."""
+    flat = []
+
+    def collect(s):
+        if isinstance(s, torch.Tensor):
+            flat.append(s)
+        elif isinstance(s, (list, tuple)):
+            for t in s:
+                collect(t)
+        elif s is not None:
+            raise ValueError(f"states must be tensors in lists or tuples, got {type(s).__name__}")
+
+    collect(states)
+    moved = iter(_lib.host().reorder(flat, parents, _whole(dim, "dim")))
+
+    def rebuild(s):
+        if s is None or isinstance(s, torch.Tensor):
+            return None if s is None else next(moved)
+        parts = [rebuild(t) for t in s]
+        return parts if isinstance(s, list) else type(s)(*parts) if hasattr(s, "_fields") else tuple(parts)
+
+    return rebuild(states)

@@ -47,7 +47,8 @@ enum {
   BLSTM_E_WAIT_TIMEOUT = 6,    /* device: a bounded cross-CTA wait ran out               */
   BLSTM_E_ARCH = 7,            /* device is not sm_100                                    */
   BLSTM_E_TOO_LARGE = 8,       /* request exceeds a fixed capacity (no-allocation entry) or a grid */
-  BLSTM_E_TOKEN = 9            /* device: a token outside of the vocabulary                */
+  BLSTM_E_TOKEN = 9,           /* device: a token outside of the vocabulary                */
+  BLSTM_E_PARENT = 10          /* device: a hypothesis' parent that is none of its sentence's */
 };
 
 /* blstm_desc.flags */
@@ -388,6 +389,38 @@ typedef struct blstm_grad_norm_desc {
 /* The 2-norm over all elements of all tensors, in an order that the sizes fix. */
 size_t blstm_grad_norm_workspace(int items);
 int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream);
+
+/* A step of beam search over logits [batch, beams, vocab]; everything else is dense, [batch, beams] or [batch, width]. */
+#define BLSTM_MAX_BEAMS 32
+typedef struct blstm_beam_desc {
+  int32_t dtype, width;          /* of logits; hypotheses that are kept, at most BLSTM_MAX_TOP and beams * vocab */
+  int64_t batch, beams, vocab;   /* batch * beams < 2^31, beams <= BLSTM_MAX_BEAMS                     */
+  int64_t logits_stride[2];
+  int64_t end_token;             /* or -1                                                              */
+  double length_penalty;         /* of at least 0; needs lengths where it is not 0                     */
+} blstm_beam_desc;
+
+/* total[k,v] = scores[k] + log softmax(logits[k])[v]; where finished[k] (or NULL: none) scores[k] for end_token and -inf for all others.
+ * The width largest of total / (lengths[k] + 1)^length_penalty (lengths[k]^length_penalty where finished[k]), equal ones by (k, v), NaN
+ * first: out_scores (their totals), parents (k), tokens (v), out_finished (finished[k] or v == end_token), out_lengths (lengths[k], + 1 unless
+ * finished[k]); the last two, or NULL.  Logits of finished hypotheses and of those with scores of -inf are not read; a row of nothing but
+ * -inf continues with -inf.  Totals are compared in 64 bits. */
+size_t blstm_beam_workspace(const blstm_beam_desc* d);
+int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* scores, const uint8_t* finished,
+                    const int64_t* lengths, float* out_scores, int64_t* parents, int64_t* tokens, uint8_t* out_finished,
+                    int64_t* out_lengths, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct blstm_reorder_item {
+  const void* src;               /* [outer, batch*beams] rows of inner_bytes bytes                     */
+  void* dst;                     /* [outer, batch*width, inner_bytes], dense                           */
+  int64_t outer, inner_bytes;
+  int64_t outer_stride, row_stride;   /* of src, in bytes                                              */
+} blstm_reorder_item;
+
+/* dst[o, b*width + j] = src[o, b*beams + parents[b, j]] of every item; parents [batch, width], dense, of 32 or 64 bits.  A parent that is not
+ * in [0, beams) is reported as BLSTM_E_PARENT through the mailbox (detail[0] its place, detail[1] its value) and gives zeros. */
+int blstm_reorder(const blstm_reorder_item* items, int n, const void* parents, int parent_bits, int64_t batch, int64_t beams,
+                  int64_t width, void* stream);
 
 /* Host memory (mapped into the device, four int32: -, status, detail[2]; on an 8-byte boundary both details
  * are always of one report) that the CALLING THREAD's later launches write a device-side error to as well, or

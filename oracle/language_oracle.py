@@ -116,3 +116,43 @@ def e4m3(x):
     a = np.abs(x).astype(np.float64)
     step = 2.0 ** (np.floor(np.log2(np.maximum(a, 2.0 ** -6))) - 3)
     return np.sign(x) * np.rint(a / step) * step
+
+
+# ---------------------------------------------------------------- beam search
+def beam_ranks(logits, scores, end=None, finished=None, lengths=None, penalty=0.0):
+    """(ranks, totals) [B, n, V] of every continuation."""
+    z = logits.astype(np.float64)
+    B, n, V = z.shape
+    scores = scores.astype(np.float64)
+    with np.errstate(all="ignore"):
+        m = z.max(-1, keepdims=True)
+        none = np.isneginf(m)
+        lse = m + np.log(np.exp(z - m).sum(-1, keepdims=True))
+        total = np.where(none, -np.inf, z - np.where(none, 0, lse)) + scores[..., None]
+        total = np.where(np.isneginf(scores)[..., None], -np.inf, total)
+        after = np.ones((B, n)) if lengths is None else lengths.astype(np.float64) + 1
+        if finished is not None:
+            after = after - finished
+            over = np.full((B, n, V), -np.inf)
+            over[..., end] = scores
+            total = np.where(finished[..., None], over, total)
+        return total / (after ** penalty)[..., None], total
+
+
+def beam_step(logits, scores, width, end=None, finished=None, lengths=None, penalty=0.0):
+    """(scores, parents, tokens, finished, lengths) [B, width]."""
+    rank, total = beam_ranks(logits, scores, end, finished, lengths, penalty)
+    B, n, V = rank.shape
+    first = np.where(np.isnan(rank), np.inf, rank).reshape(B, -1)
+    flat = np.stack([np.lexsort((np.arange(n * V), -r))[:width] for r in first])
+    parents, tokens = flat // V, flat % V
+    rows = np.arange(B)[:, None]
+    ended = np.zeros((B, n), bool) if finished is None else finished
+    return (total[rows, parents, tokens], parents, tokens, ended[rows, parents] | (tokens == (-1 if end is None else end)),
+            None if lengths is None else lengths[rows, parents] + ~ended[rows, parents])
+
+
+def reorder(state, parents, dim=1):
+    B, W = parents.shape
+    n = state.shape[dim] // B
+    return np.take(state, (np.arange(B)[:, None] * n + parents).reshape(-1), axis=dim)
