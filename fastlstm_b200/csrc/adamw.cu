@@ -15,12 +15,14 @@
 // 0, which would divide by it.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "language.cuh"
 
 namespace blstm {
 
-constexpr int kChunk = 2048, kAdamThreads = 256;       // elements of a block's turn: 8 a thread, 256 (a scale) a warp
+constexpr int kAdamThreads = 256, kTurn = 8 * kAdamThreads;       // elements of a block's turn: 8 a thread, 256 (a scale) a warp
+constexpr int kChunk = 4 * kTurn;
 
 struct AdamItem {
   void* param;
@@ -43,103 +45,107 @@ struct AdamParams {
   unsigned* ticket;
 };
 
-// Eight elements from i on as floats; those from n on are 0.
+// Eight elements as they lie in memory: in 16-byte pieces where all eight are there and on a boundary (WHOLE), else the first `left` of them one
+// by one, zeros behind.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long long i, long long n, bool wide, float (&z)[8]) {
-  if (wide && i + 8 <= n) {
+struct Raw {
+  static constexpr int N = sizeof(T) / 2;              // 16-byte pieces
+  uint4 v[N];
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const T* p, long long left) {
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int k = 0; k < 8; k += kPer<T>) unpack(*reinterpret_cast<const uint4*>(p + i + k), z + k, T{});
-  } else {
+      for (int k = 0; k < N; ++k) v[k] = reinterpret_cast<const uint4*>(p)[k];
+    } else {
+      float z[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) z[k] = i + k < n ? ld_f(p + i + k) : 0.f;
+      for (int k = 0; k < 8; ++k) z[k] = k < left ? ld_f(p + k) : 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = pack(z + k * kPer<T>, T{});
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, long long i, long long n, bool wide, const float (&z)[8]) {
-  if (wide && i + 8 <= n) {
+  __device__ __forceinline__ void get(float (&z)[8]) const {
 #pragma unroll
-    for (int k = 0; k < 8; k += kPer<T>) *reinterpret_cast<uint4*>(p + i + k) = pack(z + k, T{});
+    for (int k = 0; k < N; ++k) unpack(v[k], z + k * kPer<T>, T{});
+  }
+};
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store8(T* p, long long left, const float (&z)[8]) {
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int k = 0; k < 8; k += kPer<T>) *reinterpret_cast<uint4*>(p + k) = pack(z + k, T{});
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[i + k] = Elem<T>::from_f(z[k]);
+      if (k < left) p[k] = Elem<T>::from_f(z[k]);
   }
 }
-
-// Eight e4m3 numbers as they lie in memory.
-__device__ __forceinline__ uint2 load8_bytes(const uint8_t* p, long long i, long long n, bool wide) {
-  if (wide && i + 8 <= n) return *reinterpret_cast<const uint2*>(p + i);
+template <bool WHOLE>
+__device__ __forceinline__ uint2 load8_bytes(const uint8_t* p, long long left) {
+  if constexpr (WHOLE) return *reinterpret_cast<const uint2*>(p);
   unsigned w[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    if (i + k < n) w[k / 4] |= (unsigned)p[i + k] << k % 4 * 8;
+    if (k < left) w[k / 4] |= (unsigned)p[k] << k % 4 * 8;
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void store8_bytes(uint8_t* p, long long i, long long n, bool wide, uint2 w) {
-  if (wide && i + 8 <= n) {
-    *reinterpret_cast<uint2*>(p + i) = w;
+template <bool WHOLE>
+__device__ __forceinline__ void store8_bytes(uint8_t* p, long long left, uint2 v) {
+  if constexpr (WHOLE) {
+    *reinterpret_cast<uint2*>(p) = v;
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[i + k] = (uint8_t)((k < 4 ? w.x : w.y) >> k % 4 * 8);
+      if (k < left) p[k] = (uint8_t)((k < 4 ? v.x : v.y) >> k % 4 * 8);
   }
 }
-__device__ __forceinline__ void decode8(uint2 w, float scale, float (&z)[8]) {
+__device__ __forceinline__ void decode8(uint2 w, Pair (&z)[4]) {
 #pragma unroll
-  for (int k = 0; k < 8; k += 2) {
-    const unsigned short two = (unsigned short)((k < 4 ? w.x : w.y) >> k % 4 * 8);
+  for (int k = 0; k < 4; ++k) {
+    const unsigned short two = (unsigned short)((k < 2 ? w.x : w.y) >> k % 2 * 16);
     unsigned h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    z[k] = f.x * scale;
-    z[k + 1] = f.y * scale;
+    z[k] = Pair::of(f.x, f.y);
   }
 }
 
-// A magnitude of at most 448 as an e4m3 number, in bits 20 to 27: times 2^-120 its bits are the top bits of the float's, subnormal
-// numbers too, and adding `chance` (20 bits) below them rounds up with the probability of what is cut off.
-__device__ __forceinline__ unsigned encode(float magnitude, unsigned chance) {
-  return min(__float_as_uint(magnitude * 0x1p-120f) + chance, (127u << 20) - 1);
+// A number of at most 448, times 2^-120, as an e4m3 number in bits 20 to 26, its sign where it was: what it is in a float's own bits,
+// subnormal numbers too, and adding `chance` (16 bits, of 20) below it rounds up with the probability of what is cut off.  (The division that
+// makes the largest 448 is off by two in the last place at most, which no chance carries to the next number.)
+__device__ __forceinline__ unsigned encode(float y, unsigned chance) { return __float_as_uint(y) + (chance << 4); }
+// Four of them in their order in memory.
+__device__ __forceinline__ unsigned bytes_of(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x7632) >> 4, __byte_perm(c, d, 0x7632) >> 4, 0x6420);
+}
+__device__ __forceinline__ unsigned signs_of(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410) & 0x80808080u;
 }
 
-// The words of elements 4 block .. 4 block + 7 in step t of tensor `number`: Philox4x32-10 (Salmon, Moraes, Dror, Shaw, 2011) with the seed
+// The words of elements 4 block .. 4 block + 3 in step t of tensor `number`: Philox4x32-10 (Salmon, Moraes, Dror, Shaw, 2011) with the seed
 // as the key and (block, t, number) as the counter.
-__device__ __forceinline__ void draw8(unsigned (&w)[8], const unsigned* keys, unsigned long long block, unsigned t, unsigned number) {
-#pragma unroll
-  for (int b = 0; b < 8; b += 4) {
-    const unsigned long long c = block + b / 4;
-    w[b] = (unsigned)c;
-    w[b + 1] = (unsigned)(c >> 32);
-    w[b + 2] = t;
-    w[b + 3] = number;
-  }
+__device__ __forceinline__ void draw4(unsigned (&w)[4], const unsigned* keys, unsigned long long block, unsigned t, unsigned number) {
+  w[0] = (unsigned)block;
+  w[1] = (unsigned)(block >> 32);
+  w[2] = t;
+  w[3] = number;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-#pragma unroll
-    for (int b = 0; b < 8; b += 4) {
-      const unsigned long long x = (unsigned long long)w[b] * 0xD2511F53u, y = (unsigned long long)w[b + 2] * 0xCD9E8D57u;
-      w[b] = (unsigned)(y >> 32) ^ w[b + 1] ^ keys[2 * r];
-      w[b + 1] = (unsigned)y;
-      w[b + 2] = (unsigned)(x >> 32) ^ w[b + 3] ^ keys[2 * r + 1];
-      w[b + 3] = (unsigned)x;
-    }
+    const unsigned long long x = (unsigned long long)w[0] * 0xD2511F53u, y = (unsigned long long)w[2] * 0xCD9E8D57u;
+    w[0] = (unsigned)(y >> 32) ^ w[1] ^ keys[2 * r];
+    w[1] = (unsigned)y;
+    w[2] = (unsigned)(x >> 32) ^ w[3] ^ keys[2 * r + 1];
+    w[3] = (unsigned)x;
   }
 }
 
-// The largest magnitude of a warp's numbers: the bits of magnitudes have their order, and NaN comes last.
-__device__ __forceinline__ float warp_most(const float (&z)[8]) {
-  unsigned most = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(z[e]) & 0x7fffffffu);
-  return __uint_as_float(__reduce_max_sync(~0u, most));
+__device__ __forceinline__ float max_abs(float m, float v) {      // NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
 }
-// The codes of four numbers in their order in memory, from the bits 20 to 27 of four words.
-__device__ __forceinline__ unsigned bytes_of(unsigned a, unsigned b, unsigned c, unsigned d) {
-  return __byte_perm(__byte_perm(a << 4, b << 4, 0x0073), __byte_perm(c << 4, d << 4, 0x0073), 0x5410);
-}
-__device__ __forceinline__ unsigned signs_of(float a, float b, float c, float d) {
-  return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0073), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0073), 0x5410) & 0x80808080u;
-}
+// The largest of a warp's magnitudes: their bits have their order, and NaN comes last.
+__device__ __forceinline__ float warp_most(float most) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most))); }
 __device__ __forceinline__ float reciprocal_fast(float x) {      // to 2^-23
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -150,6 +156,12 @@ __device__ __forceinline__ float sqrt_fast(float x) {      // to 2^-22
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The same of what is 2^-126 at least; the root of anything less is 2^-63.
+__device__ __forceinline__ float sqrt_clamped(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 0x1p-126f)));
+  return y;
+}
 
 // What a scale and its inverse are for a largest magnitude; magnitudes below 2^-110 are 0 (the inverse would not be a number of 32 bits).
 struct Scale {
@@ -158,98 +170,333 @@ struct Scale {
       : up(most > 0x1p-110f ? 1.f / most * 448.f : 0.f), down(most <= 0x1p-110f ? 0.f : most * (1.f / 448.f)) {}
 };
 
-template <typename T, int BITS, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamParams<CAP> p) {
-  const unsigned tid = threadIdx.x, lane = tid & 31;
-  const float factor = p.factor ? *p.factor : 1.f;
-  if (factor != factor) return;                // gradients that are no numbers: everything stays as it is
-  unsigned k = 0, t = 0;
-  int known = -1;                              // the item that t, c1 and c2 are of
-  float c1 = 0.f, c2 = 0.f;
-  const float lr = p.lr_at ? *p.lr_at : p.lr, decay = lr * p.decay;
-  for (unsigned chunk = blockIdx.x; chunk < p.chunks; chunk += gridDim.x) {
-    while (k + 1 < p.items && chunk >= p.item[k + 1].first) ++k;
-    const AdamItem& a = p.item[k];
-    const bool wide = p.wide[k / 64] >> k % 64 & 1;
-    const long long i = (long long)(chunk - a.first) * kChunk + tid * 8;
-    float g[8], m[8], v[8], x[8];
-    uint2 m8, v8;
-    float m_scale, v_scale;
-    const long long block = i / 256;           // (of a warp)
-    load8(static_cast<const T*>(a.grad), i, a.n, wide, g);
-    if constexpr (BITS == 32) {
-      load8(static_cast<const float*>(a.m), i, a.n, wide, m);
-      load8(static_cast<const float*>(a.v), i, a.n, wide, v);
-    } else {
-      m8 = load8_bytes(static_cast<const uint8_t*>(a.m), i, a.n, wide);
-      v8 = load8_bytes(static_cast<const uint8_t*>(a.v), i, a.n, wide);
-      m_scale = block * 256 < a.n ? a.m_scale[block] : 0.f;
-      v_scale = block * 256 < a.n ? a.v_scale[block] : 0.f;
-    }
-    if constexpr (MASTER) load8(a.master, i, a.n, wide, x);
-    else load8(static_cast<const T*>(a.param), i, a.n, wide, x);
-    if ((int)k != known) {
-      known = (int)k;
-      const long long count = *a.step + 1;
-      t = (unsigned)count;
-      c1 = lr / -expm1f((float)((double)count * p.log_beta1));
-      c2 = rsqrtf(-expm1f((float)((double)count * p.log_beta2)));
-    }
-    if constexpr (BITS == 8) {
-      decode8(m8, m_scale, m);
-      decode8(v8, v_scale, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= v[e];
-    }
-    float u[8];
+// What a step does to eight elements.
+struct AdamStep {
+  float factor, beta1, beta2, one_less1, one_less2, eps, decay, c1, c2;
+
+  __device__ __forceinline__ void operator()(const float (&g)[8], float (&m)[8], float (&v)[8], float (&x)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float ge = g[e] * factor;
-      if constexpr (BITS == 32) {
-        m[e] = fmaf(p.beta1, m[e], p.one_less1 * ge);
-        v[e] = fmaf(p.beta2, v[e], p.one_less2 * (ge * ge));
-        u[e] = sqrt_fast(v[e]);
-      } else {
-        // (each operation rounded by itself, so that what is rounded to 8 bits depends on the formula alone)
-        m[e] = __fadd_rn(__fmul_rn(p.beta1, m[e]), __fmul_rn(p.one_less1, ge));
-        u[e] = __fsqrt_rn(__fadd_rn(__fmul_rn(p.beta2, v[e]), __fmul_rn(p.one_less2, __fmul_rn(ge, ge))));
-      }
-      x[e] -= fmaf(decay, x[e], c1 * m[e] * reciprocal_fast(fmaf(u[e], c2, p.eps)));
-    }
-    if constexpr (MASTER) store8(a.master, i, a.n, wide, x);
-    store8(static_cast<T*>(a.param), i, a.n, wide, x);
-    if constexpr (BITS == 32) {
-      store8(static_cast<float*>(a.m), i, a.n, wide, m);
-      store8(static_cast<float*>(a.v), i, a.n, wide, v);
-    } else {
-      const Scale sm(warp_most(m)), su(warp_most(u));
-      unsigned w[8], cm[8], cu[8];
-      draw8(w, p.keys, (unsigned long long)i / 4, t, a.number);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cm[e] = encode(fabsf(m[e]) * sm.up, w[e] << 4 & 0xffff0u);
-        cu[e] = encode(u[e] * su.up, w[e] >> 12 & 0xffff0u);
-        if (u[e] * su.up > 0.f) cu[e] = max(cu[e], 1u << 20);
-      }
-      store8_bytes(static_cast<uint8_t*>(a.m), i, a.n, wide, make_uint2(bytes_of(cm[0], cm[1], cm[2], cm[3]) | signs_of(m[0], m[1], m[2], m[3]),
-                                                                        bytes_of(cm[4], cm[5], cm[6], cm[7]) | signs_of(m[4], m[5], m[6], m[7])));
-      store8_bytes(static_cast<uint8_t*>(a.v), i, a.n, wide, make_uint2(bytes_of(cu[0], cu[1], cu[2], cu[3]), bytes_of(cu[4], cu[5], cu[6], cu[7])));
-      if (lane == 0 && block * 256 < a.n) {
-        a.m_scale[block] = sm.down;
-        a.v_scale[block] = su.down;
-      }
+      m[e] = fmaf(beta1, m[e], one_less1 * ge);
+      v[e] = fmaf(beta2, v[e], one_less2 * (ge * ge));
+      x[e] -= fmaf(decay, x[e], c1 * m[e] * reciprocal_fast(fmaf(sqrt_fast(v[e]), c2, eps)));
     }
   }
-  // The last block to get here counts the steps, once nobody reads them any more.
+
+  // The same in 8 bits, by a warp with 256 elements: m8 and u8 are theirs and become the new ones, as do the scales.  Two floats an
+  // instruction (it is instructions that bound this).  Moments and scales are rounded operation by operation, so that they depend on the
+  // formula alone; only the roots of elements that are not their block's largest are the fast unit's (2^-22 of them).
+  template <typename F>
+  __device__ __forceinline__ void operator()(const float (&g)[8], uint2& m8, uint2& u8, float& m_scale, float& u_scale, float (&x)[8], F&& words) const {
+    Pair m[4], v[4], u[4];
+    float most_m = 0.f, most_v = 0.f;
+    decode8(m8, m);
+    decode8(u8, v);
+    auto both = [](float a) { return Pair::of(a, a); };
+    const Pair sm = both(m_scale), su = both(u_scale), f = both(factor), b1 = both(beta1), b2 = both(beta2), a1 = both(one_less1), a2 = both(one_less2);
+    const Pair minus = both(-1.f), rate = both(c1), fix = both(c2), e0 = both(eps), wd = both(decay);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const Pair ge = Pair::of(g[2 * k], g[2 * k + 1]) * f, old = v[k] * su;
+      m[k] = b1 * (m[k] * sm) + a1 * ge;
+      v[k] = b2 * (old * old) + a2 * (ge * ge);
+      float lo, hi;
+      m[k].get(lo, hi);
+      most_m = max_abs(max_abs(most_m, lo), hi);
+      v[k].get(lo, hi);
+      most_v = max_abs(max_abs(most_v, lo), hi);
+      u[k] = Pair::of(sqrt_clamped(lo), sqrt_clamped(hi));
+    }
+    const float largest = warp_most(most_v), root = __fsqrt_rn(largest);
+    const Scale ms(warp_most(most_m)), us(root);
+    if (largest < 0x1p-56f)                     // (above it, what is below 2^-126 is 0 next to it)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float lo, hi;
+        v[k].get(lo, hi);
+        u[k] = Pair::of(__fsqrt_rn(lo), __fsqrt_rn(hi));
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float p, q;
+      fma2(u[k], fix, e0).get(p, q);
+      const Pair move = m[k] * rate * Pair::of(reciprocal_fast(p), reciprocal_fast(q)), at = Pair::of(x[2 * k], x[2 * k + 1]);
+      fma2(fma2(at, wd, move), minus, at).get(x[2 * k], x[2 * k + 1]);
+    }
+    const Pair up_m = both(ms.up), up_u = both(us.up), small = both(0x1p-120f);
+    unsigned half_m[2], half_u[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unsigned w[4], cm[4], cu[4], least = ~0u;
+      words(h, w);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float y[2], z[2], q[2];
+        v[2 * h + k].get(q[0], q[1]);
+        u[2 * h + k].get(z[0], z[1]);
+        (m[2 * h + k] * up_m * small).get(y[0], y[1]);
+        (Pair::of(q[0] == largest ? root : z[0], q[1] == largest ? root : z[1]) * up_u * small).get(z[0], z[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int e = 2 * k + i;
+          cm[e] = encode(y[i], w[e] & 0xffffu);
+          cu[e] = encode(z[i], w[e] >> 16);
+          least = min(least, cu[e]);
+        }
+      }
+      if (least < 1u << 20)                     // (a root that is not 0 does not become it)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float lo, hi;
+          v[2 * h + k].get(lo, hi);
+          if (lo > 0.f) cu[2 * k] = max(cu[2 * k], 1u << 20);
+          if (hi > 0.f) cu[2 * k + 1] = max(cu[2 * k + 1], 1u << 20);
+        }
+      half_m[h] = bytes_of(cm[0], cm[1], cm[2], cm[3]) & 0x7f7f7f7fu | signs_of(cm[0], cm[1], cm[2], cm[3]);
+      half_u[h] = bytes_of(cu[0], cu[1], cu[2], cu[3]);
+    }
+    m8 = make_uint2(half_m[0], half_m[1]);
+    u8 = make_uint2(half_u[0], half_u[1]);
+    m_scale = ms.down;
+    u_scale = us.down;
+  }
+};
+
+// A chunk of an item from element `begin` on, of which `left` are there: what a turn needs is fetched while the one before it is worked on.
+template <typename T, int BITS, bool MASTER, bool WHOLE>
+__device__ __forceinline__ void turns(const AdamStep& step, const AdamItem& a, long long begin, long long left, const unsigned* keys, unsigned t) {
+  const unsigned tid = threadIdx.x;
+  const long long i0 = begin + tid * 8;
+  const T* grad = static_cast<const T*>(a.grad) + i0;
+  T* param = static_cast<T*>(a.param) + i0;
+  float *m32 = static_cast<float*>(a.m) + i0, *v32 = static_cast<float*>(a.v) + i0, *w32 = MASTER ? a.master + i0 : nullptr;
+  uint8_t *mb = static_cast<uint8_t*>(a.m) + i0, *ub = static_cast<uint8_t*>(a.v) + i0;
+  float *sm = a.m_scale + i0 / 256, *su = a.v_scale + i0 / 256;        // (of a warp)
+  Raw<T> g, x;
+  Raw<float> m, v, master;
+  uint2 m8, u8;
+  float m_scale = 0.f, u_scale = 0.f;
+  auto fetch = [&](int at, long long rest) {
+    g.template load<WHOLE>(grad + at, rest);
+    if constexpr (BITS == 32) {
+      m.template load<WHOLE>(m32 + at, rest);
+      v.template load<WHOLE>(v32 + at, rest);
+    } else {
+      m8 = load8_bytes<WHOLE>(mb + at, rest);
+      u8 = load8_bytes<WHOLE>(ub + at, rest);
+      if (WHOLE || rest + (tid % 32) * 8 > 0) {
+        m_scale = sm[at / 256];
+        u_scale = su[at / 256];
+      }
+    }
+    if constexpr (MASTER) master.template load<WHOLE>(w32 + at, rest);
+    else x.template load<WHOLE>(param + at, rest);
+  };
+  long long rest = left - tid * 8;              // from this thread's first element on
+  fetch(0, rest);
+  const int end = WHOLE ? kChunk : (int)min(left, (long long)kChunk);
+#pragma unroll 1
+  for (int at = 0; at < end; at += kTurn, rest -= kTurn) {
+    float ge[8], xe[8];
+    g.get(ge);
+    if constexpr (MASTER) master.get(xe);
+    else x.get(xe);
+    if constexpr (BITS == 32) {
+      float me[8], ve[8];
+      m.get(me);
+      v.get(ve);
+      if (at + kTurn < end) fetch(at + kTurn, rest - kTurn);
+      step(ge, me, ve, xe);
+      store8<WHOLE>(m32 + at, rest, me);
+      store8<WHOLE>(v32 + at, rest, ve);
+    } else {
+      uint2 mine = m8, roots = u8;
+      float ms = m_scale, us = u_scale;
+      if (at + kTurn < end) fetch(at + kTurn, rest - kTurn);
+      step(ge, mine, roots, ms, us, xe, [&](int h, unsigned (&w)[4]) { draw4(w, keys, (unsigned long long)(i0 + at) / 4 + h, t, a.number); });
+      store8_bytes<WHOLE>(mb + at, rest, mine);
+      store8_bytes<WHOLE>(ub + at, rest, roots);
+      if (tid % 32 == 0 && (WHOLE || rest > 0)) {
+        sm[at / 256] = ms;
+        su[at / 256] = us;
+      }
+    }
+    if constexpr (MASTER) store8<WHOLE>(w32 + at, rest, xe);
+    store8<WHOLE>(param + at, rest, xe);
+  }
+}
+
+// Which chunk a block is at, and the item that it belongs to.
+template <int CAP>
+struct Cursor {
+  unsigned chunk, k = 0;
+  __device__ __forceinline__ Cursor() : chunk(blockIdx.x) {}
+  __device__ __forceinline__ bool there(const AdamParams<CAP>& p) {
+    if (chunk >= p.chunks) return false;
+    while (k + 1 < p.items && chunk >= p.item[k + 1].first) ++k;
+    return true;
+  }
+  __device__ __forceinline__ long long begin(const AdamParams<CAP>& p) const { return (long long)(chunk - p.item[k].first) * kChunk; }
+  __device__ __forceinline__ bool whole(const AdamParams<CAP>& p) const { return (p.wide[k / 64] >> k % 64 & 1) && p.item[k].n - begin(p) >= kChunk; }
+  __device__ __forceinline__ void next() { chunk += gridDim.x; }
+};
+
+// The coefficients of an item's step, looked up where the item is another than before.
+template <int CAP>
+__device__ __forceinline__ void of_item(AdamStep& step, unsigned& t, int& known, const AdamParams<CAP>& p, unsigned k, float lr) {
+  if ((int)k == known) return;
+  known = (int)k;
+  const long long count = *p.item[k].step + 1;
+  t = (unsigned)count;
+  step.c1 = lr / -expm1f((float)((double)count * p.log_beta1));
+  step.c2 = rsqrtf(-expm1f((float)((double)count * p.log_beta2)));
+}
+
+// The last block to get here counts the steps, once nobody reads them any more.
+template <int CAP>
+__device__ __forceinline__ void count_steps(const AdamParams<CAP>& p) {
   __shared__ bool last;
   __syncthreads();
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
     __threadfence();
     last = atomicInc(p.ticket, gridDim.x - 1) == gridDim.x - 1;      // (back to 0 for the next launch)
   }
   __syncthreads();
   if (last)
-    for (unsigned j = tid; j < p.items; j += kAdamThreads) ++*p.item[j].step;
+    for (unsigned j = threadIdx.x; j < p.items; j += kAdamThreads) ++*p.item[j].step;
+}
+
+template <typename T, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamParams<CAP> p) {
+  const float factor = p.factor ? *p.factor : 1.f;
+  if (factor != factor) return;                // gradients that are no numbers: everything stays as it is
+  const float lr = p.lr_at ? *p.lr_at : p.lr;
+  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, 0.f, 0.f};
+  unsigned t = 0;
+  int known = -1;
+  for (Cursor<CAP> c; c.there(p); c.next()) {
+    of_item(step, t, known, p, c.k, lr);
+    if (c.whole(p)) turns<T, 32, MASTER, true>(step, p.item[c.k], c.begin(p), kChunk, p.keys, t);
+    else turns<T, 32, MASTER, false>(step, p.item[c.k], c.begin(p), p.item[c.k].n - c.begin(p), p.keys, t);
+  }
+  count_steps(p);
+}
+
+// 8 bits: what a turn needs comes into shared memory kStages - 1 turns ahead, every thread's own by itself (in registers it would cost
+// the warps that hide the arithmetic).
+constexpr int kStages = 4;
+template <typename T, bool MASTER>
+struct AdamStage {
+  static constexpr int NG = sizeof(T) / 2, NX = MASTER ? 2 : NG;
+  uint4 g[NG][kAdamThreads], x[NX][kAdamThreads];
+  uint2 m[kAdamThreads], u[kAdamThreads];
+  float scale[2][kAdamThreads / 32];
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const unsigned a = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(from), "n"(BYTES) : "memory");
+}
+
+template <typename T, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kAdamThreads, 2) adamw8_kernel(const __grid_constant__ AdamParams<CAP> p) {
+  extern __shared__ uint4 s_raw[];
+  using Stage = AdamStage<T, MASTER>;
+  using X = std::conditional_t<MASTER, float, T>;
+  Stage* stages = reinterpret_cast<Stage*>(s_raw);
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float factor = p.factor ? *p.factor : 1.f;
+  if (factor != factor) return;
+  const float lr = p.lr_at ? *p.lr_at : p.lr;
+  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, 0.f, 0.f};
+  unsigned t = 0;
+  int known = -1;
+  // the fetching side: whole chunks alone
+  Cursor<CAP> f;
+  int f_at = 0, f_stage = 0;
+  const T* f_grad = nullptr;
+  const X* f_x = nullptr;
+  const uint8_t *f_m = nullptr, *f_u = nullptr;
+  const float* f_scale = nullptr;              // lane 0: m's, lane 1: the root's
+  auto f_open = [&] {                          // the next whole chunk from here on
+    while (f.there(p) && !f.whole(p)) f.next();
+    if (f.chunk >= p.chunks) return;
+    const AdamItem& a = p.item[f.k];
+    const long long i = f.begin(p) + tid * 8;
+    f_grad = static_cast<const T*>(a.grad) + i;
+    f_x = (MASTER ? reinterpret_cast<const X*>(a.master) : static_cast<const X*>(a.param)) + i;
+    f_m = static_cast<const uint8_t*>(a.m) + i;
+    f_u = static_cast<const uint8_t*>(a.v) + i;
+    f_scale = (lane ? a.v_scale : a.m_scale) + i / 256;
+  };
+  auto fetch = [&] {
+    if (f.chunk < p.chunks) {
+      Stage& s = stages[f_stage];
+#pragma unroll
+      for (int k = 0; k < Stage::NG; ++k) copy_async<16>(&s.g[k][tid], reinterpret_cast<const uint4*>(f_grad) + k);
+#pragma unroll
+      for (int k = 0; k < Stage::NX; ++k) copy_async<16>(&s.x[k][tid], reinterpret_cast<const uint4*>(f_x) + k);
+      copy_async<8>(&s.m[tid], f_m);
+      copy_async<8>(&s.u[tid], f_u);
+      if (lane < 2) copy_async<4>(&s.scale[lane][warp], f_scale);
+      f_grad += kTurn; f_x += kTurn; f_m += kTurn; f_u += kTurn; f_scale += kTurn / 256;
+      f_at += kTurn;
+      if (f_at == kChunk) {
+        f_at = 0;
+        f.next();
+        f_open();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+  };
+  f_open();
+#pragma unroll
+  for (int k = 0; k + 1 < kStages; ++k) fetch();
+  int stage = 0;
+  for (Cursor<CAP> c; c.there(p); c.next()) {
+    of_item(step, t, known, p, c.k, lr);
+    const AdamItem& a = p.item[c.k];
+    if (!c.whole(p)) {
+      turns<T, 8, MASTER, false>(step, a, c.begin(p), a.n - c.begin(p), p.keys, t);
+      continue;
+    }
+    const long long i0 = c.begin(p) + tid * 8;
+    T* param = static_cast<T*>(a.param) + i0;
+    float* master = MASTER ? a.master + i0 : nullptr;
+    uint8_t *mb = static_cast<uint8_t*>(a.m) + i0, *ub = static_cast<uint8_t*>(a.v) + i0;
+    float* scale = (lane ? a.v_scale : a.m_scale) + i0 / 256;
+    unsigned long long block = (unsigned long long)i0 / 4;
+#pragma unroll 1
+    for (int at = 0; at < kChunk; at += kTurn, block += kTurn / 4) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();                            // (the scales are other lanes' copies; and this stage's next copies come behind everybody's reads)
+      Stage& s = stages[stage];
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      float ge[8], xe[8];
+      Raw<T> g;
+      Raw<X> x;
+#pragma unroll
+      for (int k = 0; k < Stage::NG; ++k) g.v[k] = s.g[k][tid];
+#pragma unroll
+      for (int k = 0; k < Stage::NX; ++k) x.v[k] = s.x[k][tid];
+      uint2 m8 = s.m[tid], u8 = s.u[tid];
+      float ms = s.scale[0][warp], us = s.scale[1][warp];
+      g.get(ge);
+      x.get(xe);
+      fetch();
+      step(ge, m8, u8, ms, us, xe, [&](int h, unsigned (&w)[4]) { draw4(w, p.keys, block + h, t, a.number); });
+      store8_bytes<true>(mb + at, 8, m8);
+      store8_bytes<true>(ub + at, 8, u8);
+      if (lane < 2) scale[at / 256] = lane ? us : ms;
+      if constexpr (MASTER) store8<true>(master + at, 8, xe);
+      store8<true>(param + at, 8, xe);
+    }
+  }
+  count_steps(p);
 }
 
 // ---------------------------------------------------------------- the norm of all gradients
@@ -270,15 +517,19 @@ struct GradNormParams {
   float* out;                    // norm, factor; null before the last launch
   unsigned* ticket;
 };
-constexpr int kNormChunk = 4 * kChunk;
+constexpr int kNormChunk = 4 * kTurn;
 
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const T* g, long long i, long long n, bool wide) {
   double sum = 0;
 #pragma unroll
-  for (int part = 0; part < kNormChunk / kChunk; ++part) {
+  for (int part = 0; part < kNormChunk / kTurn; ++part) {
     float z[8], t = 0.f;
-    load8(g, i + part * kChunk, n, wide, z);
+    Raw<T> raw;
+    const long long at = i + part * kTurn;
+    if (wide && at + 8 <= n) raw.template load<true>(g + at, 8);
+    else raw.template load<false>(g + at, n - at);
+    raw.get(z);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t = fmaf(z[e], z[e], t);
     sum += t;
@@ -336,6 +587,8 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_co
 // ---------------------------------------------------------------- host
 constexpr int kFew = 32, kMany = 384;          // tensors of a launch, with 2.7 and 31 KB of parameters
 
+// (More blocks than an SM has at a time: SMs are not all as near to all memory, and blocks that are still to come even that out.  138 M bf16
+// weights in 8 bits with 2, 4, 8, 32 blocks an SM: 435, 460, 390, 400 us.)
 static unsigned adam_grid(unsigned chunks) { return std::min(chunks, 8u * (unsigned)plan_sm_count()); }
 
 template <typename T, int BITS, bool MASTER, int CAP>
@@ -363,7 +616,13 @@ static int launch_adamw(const blstm_adamw_desc& d, const blstm_adamw_item* items
   p.eps = (float)d.eps; p.decay = (float)d.weight_decay;
   p.log_beta1 = std::log(d.beta1); p.log_beta2 = std::log(d.beta2);
   p.lr_at = d.lr_at; p.factor = d.factor; p.ticket = d.ticket;
-  adamw_kernel<T, BITS, MASTER, CAP><<<adam_grid(p.chunks), kAdamThreads, 0, st>>>(p);
+  if constexpr (BITS == 32) {
+    adamw_kernel<T, MASTER, CAP><<<adam_grid(p.chunks), kAdamThreads, 0, st>>>(p);
+  } else {
+    constexpr int smem = kStages * (int)sizeof(AdamStage<T, MASTER>);
+    if constexpr (smem > 48 * 1024) BLSTM_CUDA_OK(cudaFuncSetAttribute(adamw8_kernel<T, MASTER, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    adamw8_kernel<T, MASTER, CAP><<<adam_grid(p.chunks), kAdamThreads, smem, st>>>(p);
+  }
   BLSTM_CUDA_OK(cudaGetLastError());
   count_launch();
   return BLSTM_OK;

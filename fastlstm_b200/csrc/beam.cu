@@ -31,6 +31,10 @@ struct BeamParams {
 
 constexpr float kLog2E = 1.4426950408889634f;
 
+// The launch behind this one may begin, as far as begin_behind; there it waits for all of this one.
+__device__ __forceinline__ void let_begin() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void begin_behind() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A hypothesis whose logits count: it has not ended, and it is not dead.
 __device__ __forceinline__ bool goes_on(const BeamParams& p, unsigned r) { return !(p.finished && p.finished[r]) && p.scores[r] != -INFINITY; }
 
@@ -76,6 +80,7 @@ template <typename T, int PPL>
 __global__ void __launch_bounds__(32 * kWarpRows) beam_warp_kernel(const __grid_constant__ BeamParams p) {
   __shared__ unsigned long long s_cand[kWarpRows][kWarpCand];
   const unsigned warp = threadIdx.x >> 5, r = blockIdx.x * kWarpRows + warp;
+  let_begin();
   if (r >= p.batch * p.beams || !goes_on(p, r)) return;
   const WarpRow<T, PPL> w(static_cast<const T*>(p.logits) + p.rows(r), p.vocab);
   Sum a{-INFINITY, 0.f};
@@ -101,6 +106,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const __grid_c
   __shared__ BeamShared<NT> s;
   const unsigned parts = cluster_size(), part = cluster_rank(), r = blockIdx.x / parts;
   const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  let_begin();
   if (!goes_on(p, r)) return;                  // (the same for a whole cluster)
   if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
@@ -177,15 +183,15 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     const float score = p.scores[r];
     const bool ended = p.finished && p.finished[r];
     s_kind[tid] = ended ? 1 : score == -INFINITY ? 2 : 0;
-    double base = score, high = 0;
-    if (s_kind[tid] == 0) {
-      const float2 st = p.stats[r];
-      high = st.x;
-      base = st.y == 0.f ? -INFINITY : (double)score - log((double)st.y);      // (a row of nothing but -inf)
-    }
-    s_base[tid] = base;
-    s_high[tid] = high;
+    s_base[tid] = score;
+    s_high[tid] = 0;
     s_per[tid] = p.penalty != 0.0 ? pow((double)(p.lengths[r] + !ended), p.penalty) : 1.0;
+  }
+  begin_behind();                              // (what does not need the rows' results came before)
+  if (tid < p.beams && s_kind[tid] == 0) {
+    const float2 st = p.stats[b * p.beams + tid];
+    s_high[tid] = st.x;
+    s_base[tid] = st.y == 0.f ? -INFINITY : s_base[tid] - log((double)st.y);      // (a row of nothing but -inf)
   }
   __syncthreads();
   auto total_of = [&](unsigned k, float z) { return s_base[k] == -INFINITY ? -INFINITY : s_base[k] + ((double)z - s_high[k]); };
@@ -245,14 +251,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------- reordering
-constexpr int kReorderItems = 32, kReorderThreads = 256;
+// Rows are moved by groups of 1 to 32 lanes, up to kRowPieces pieces a lane; longer ones in parts.  (A thread for every piece finds its row
+// by divisions: 2 x 2560 rows of 301 fp32 twice and 100 x 2560 numbers 26 us, so 8.)
+constexpr int kReorderItems = 32, kReorderThreads = 256, kRowPieces = 16;
 struct ReorderItem {
   const char* src;
   char* dst;
   long long outer_stride, row_stride;          // of src, in bytes
-  unsigned long long pieces;                   // of dst
-  unsigned per_row, first;                     // pieces of a row; its first block
-  int bytes;                                   // of a piece
+  unsigned long long units;                    // parts of rows
+  unsigned per_row, parts, first;              // pieces of a row, its parts; the item's first block
+  unsigned char lanes, bytes;                  // log2 of the lanes of a unit; of a piece
 };
 struct ReorderParams {
   ReorderItem item[kReorderItems];
@@ -263,35 +271,44 @@ struct ReorderParams {
 };
 
 template <typename V>
-__device__ __forceinline__ void move_piece(const ReorderItem& a, unsigned long long i, unsigned long long outer, long long row, unsigned col) {
-  V v{};
-  if (row >= 0) v = *reinterpret_cast<const V*>(a.src + outer * a.outer_stride + row * a.row_stride + (size_t)col * sizeof(V));
-  reinterpret_cast<V*>(a.dst)[i] = v;
+__device__ __forceinline__ void move_row(const char* src, char* dst, unsigned begin, unsigned end, unsigned lane, unsigned lanes) {
+  for (unsigned i = begin + lane; i < end; i += 8 * lanes) {
+    V v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      v[u] = V{};
+      if (src && i + u * lanes < end) v[u] = reinterpret_cast<const V*>(src)[i + u * lanes];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u * lanes < end) reinterpret_cast<V*>(dst)[i + u * lanes] = v[u];
+  }
 }
+
+__device__ __forceinline__ unsigned long long quotient(unsigned long long a, unsigned b) { return a >> 32 ? a / b : (unsigned)a / b; }
 
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
   unsigned k = 0;
   while (k + 1 < p.items && blockIdx.x >= p.item[k + 1].first) ++k;
   const ReorderItem& a = p.item[k];
-  const unsigned long long i = (unsigned long long)(blockIdx.x - a.first) * kReorderThreads + threadIdx.x;
-  if (i >= a.pieces) return;
+  const unsigned lanes = 1u << a.lanes, lane = threadIdx.x & (lanes - 1);
+  const unsigned long long unit = (unsigned long long)(blockIdx.x - a.first) * (kReorderThreads >> a.lanes) + (threadIdx.x >> a.lanes);
+  if (unit >= a.units) return;
   const unsigned rows = p.batch * p.width;
-  unsigned long long out_row;
-  unsigned col;
-  if (i >> 32) { out_row = i / a.per_row; col = (unsigned)(i - out_row * a.per_row); }
-  else { out_row = (unsigned)i / a.per_row; col = (unsigned)i - (unsigned)out_row * a.per_row; }
-  const unsigned long long outer = out_row >> 32 ? out_row / rows : (unsigned)out_row / rows;
+  const unsigned long long out_row = a.parts == 1 ? unit : quotient(unit, a.parts), outer = quotient(out_row, rows);
+  const unsigned begin = (unsigned)(unit - out_row * a.parts) * (kRowPieces << a.lanes), end = min(a.per_row, begin + (kRowPieces << a.lanes));
   const unsigned at = (unsigned)(out_row - outer * rows), b = at / p.width;
   const long long parent = p.wide ? static_cast<const long long*>(p.parents)[at] : (long long)static_cast<const int*>(p.parents)[at];
   const bool in = parent >= 0 && parent < p.beams;
-  if (!in && outer == 0 && col == 0) report_token(p.mailbox, at, parent, BLSTM_E_PARENT);
-  const long long row = in ? (long long)b * p.beams + parent : -1;
+  if (!in && outer == 0 && begin + lane == 0) report_token(p.mailbox, at, parent, BLSTM_E_PARENT);
+  const char* src = in ? a.src + outer * a.outer_stride + ((long long)b * p.beams + parent) * a.row_stride : nullptr;
+  char* dst = a.dst + out_row * a.per_row * a.bytes;
   switch (a.bytes) {
-    case 16: return move_piece<uint4>(a, i, outer, row, col);
-    case 8: return move_piece<uint2>(a, i, outer, row, col);
-    case 4: return move_piece<unsigned>(a, i, outer, row, col);
-    case 2: return move_piece<unsigned short>(a, i, outer, row, col);
-    default: return move_piece<unsigned char>(a, i, outer, row, col);
+    case 16: return move_row<uint4>(src, dst, begin, end, lane, lanes);
+    case 8: return move_row<uint2>(src, dst, begin, end, lane, lanes);
+    case 4: return move_row<unsigned>(src, dst, begin, end, lane, lanes);
+    case 2: return move_row<unsigned short>(src, dst, begin, end, lane, lanes);
+    default: return move_row<unsigned char>(src, dst, begin, end, lane, lanes);
   }
 }
 
@@ -376,8 +393,16 @@ int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* s
   p.out_finished = out_finished;
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = with_type(d->dtype, [&](auto t) -> int { return launch_rows<decltype(t)>(p, st); })) return rc;
-  beam_merge_kernel<<<p.batch, kMergeThreads, 0, st>>>(p);
-  BLSTM_CUDA_OK(cudaGetLastError());
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = p.batch;
+  cfg.blockDim = kMergeThreads;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, beam_merge_kernel, p));
   count_launch();
   return BLSTM_OK;
 }
@@ -415,12 +440,15 @@ int blstm_reorder(const blstm_reorder_item* items, int n, const void* parents, i
     const int bytes = bits & 1 ? 1 : bits & 2 ? 2 : bits & 4 ? 4 : bits & 8 ? 8 : 16;
     const uint64_t per_row = (uint64_t)s.inner_bytes / bytes, rows = (uint64_t)(batch * width);
     if (per_row > UINT32_MAX || (uint64_t)s.outer > (1ull << 48) / rows / per_row) return BLSTM_E_TOO_LARGE;
-    const uint64_t pieces = (uint64_t)s.outer * rows * per_row, more = (pieces + kReorderThreads - 1) / kReorderThreads;
+    unsigned lanes = 0;
+    while (lanes < 5 && (1ull << lanes) < per_row) ++lanes;
+    const uint64_t parts = (per_row + (kRowPieces << lanes) - 1) / (kRowPieces << lanes), units = (uint64_t)s.outer * rows * parts;
+    const uint64_t more = (units + (kReorderThreads >> lanes) - 1) / (kReorderThreads >> lanes);
     if (more > INT32_MAX) return BLSTM_E_TOO_LARGE;
     if (p.items == kReorderItems || blocks + more > INT32_MAX)
       if (int rc = launch()) return rc;
-    p.item[p.items++] = {static_cast<const char*>(s.src), static_cast<char*>(s.dst), (long long)s.outer_stride, (long long)s.row_stride, pieces,
-                         (unsigned)per_row, (unsigned)blocks, bytes};
+    p.item[p.items++] = {static_cast<const char*>(s.src), static_cast<char*>(s.dst), (long long)s.outer_stride, (long long)s.row_stride, units,
+                         (unsigned)per_row, (unsigned)parts, (unsigned)blocks, (unsigned char)lanes, (unsigned char)bytes};
     blocks += more;
   }
   return launch();

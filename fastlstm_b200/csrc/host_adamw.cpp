@@ -1,6 +1,8 @@
-// Host side of the AdamW step: lists of tensors checked and handed to the C ABI, tensors of one type to a call.
+// Host side of the AdamW step: parameters, gradients and states collected and checked, tensors of one type handed to a call of the C ABI.  (A
+// step over a layer's four tensors took 31 us where Python collected them.)
 #include "host_language.h"
 
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
 namespace {
@@ -30,94 +32,140 @@ float* f32(const Tensor& t, const char* name, const Tensor& param, int64_t n) {
   return static_cast<float*>(t.data_ptr());
 }
 
-// params [k], and of each {exp_avg, exp_avg_sq (8 bits: its root), step [, scale, scale] [, master]}; norm: {norm, factor}, written first
-// where max_norm is positive.
-void adamw(const std::vector<Tensor>& params, const std::vector<Tensor>& grads_in, const std::vector<std::vector<Tensor>>& states,
-           const std::vector<uint32_t>& numbers, int bits, bool masters, double lr, const OptTensor& lr_at, double beta1, double beta2, double eps,
-           double weight_decay, uint64_t seed, const OptTensor& norm, const Tensor& ticket) {
-  py::gil_scoped_release nogil;
-  if (params.empty()) return;
-  const Tensor& first = params[0];
-  on_gpu(first, "a parameter");
-  std::vector<Tensor> grads;
+// The tensors of one call: of a group, a device and a type.
+struct Bucket {
+  std::vector<Tensor> params, grads;           // (grads dense, held until the launch)
   std::vector<blstm_adamw_item> items;
-  grads.reserve(params.size());
-  items.reserve(params.size());
-  blstm_adamw_desc d{};
-  d.dtype = dtype_code(first.scalar_type());
-  const size_t expected = 3 + (bits == 8 ? 2 : 0) + (masters ? 1 : 0);
-  const at::ScalarType state_type = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
-  for (size_t k = 0; k < params.size(); ++k) {
-    const Tensor& p = params[k];
-    beside(p, "a parameter", first);
-    if (p.scalar_type() != first.scalar_type()) throw wrong("parameters of one call have one dtype");
-    if (!p.is_contiguous()) throw wrong("a parameter of shape " + shape_str(p.sizes()) + " must be contiguous");
-    const std::vector<Tensor>& s = states[k];
-    if (s.size() != expected) throw wrong("an optimizer state has other tensors than expected");
-    if (p.numel() == 0) continue;
-    grads.push_back(dense_grad(grads_in[k], p));
-    blstm_adamw_item a{};
-    a.param = p.data_ptr();
-    a.grad = ptr(grads.back());
-    a.exp_avg = flat(s[0], "exp_avg", p, state_type).data_ptr();
-    a.exp_avg_sq = flat(s[1], "exp_avg_sq", p, state_type).data_ptr();
-    beside(s[2], "step", p);
-    if (s[2].scalar_type() != at::kLong || s[2].numel() != 1) throw wrong("step must be one int64 element");
-    a.step = static_cast<int64_t*>(s[2].data_ptr());
-    a.n = p.numel();
-    a.number = numbers[k];
-    if (bits == 8) {
-      a.exp_avg_scale = f32(s[3], "exp_avg_scale", p, (a.n + 255) / 256);
-      a.exp_avg_sq_scale = f32(s[4], "exp_avg_sq_root_scale", p, (a.n + 255) / 256);
-    }
-    if (masters) a.master = f32(flat(s.back(), "master", p, at::kFloat), "master", p, a.n);
-    items.push_back(a);
-  }
-  if (items.empty()) return;
-  if (lr_at) {
-    beside(*lr_at, "lr", first);
-    if (lr_at->scalar_type() != at::kFloat || lr_at->numel() != 1) throw wrong("lr on the GPU must be one float32 element");
-    d.lr_at = static_cast<const float*>(ptr(*lr_at));
-  }
-  d.bits = bits;
-  d.items = (int32_t)items.size();
-  d.item = items.data();
-  d.lr = lr; d.beta1 = beta1; d.beta2 = beta2; d.eps = eps; d.weight_decay = weight_decay;
-  d.seed = seed;
-  if (norm) d.factor = static_cast<const float*>(ptr(*norm)) + 1;
-  d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
-  Call call(first.device());
-  check(blstm_adamw(&d, call.stream), "adamw");
-  for (const Tensor& p : params) torch::autograd::impl::bump_version(p);
+};
+
+PyObject* interned(const char* name) { return PyUnicode_InternFromString(name); }
+
+const Tensor& state_tensor(PyObject* state, PyObject* name) {
+  PyObject* t = PyDict_GetItemWithError(state, name);
+  if (!t || !THPVariable_Check(t)) throw wrong("an optimizer state has no tensor " + std::string(PyUnicode_AsUTF8(name)));
+  return THPVariable_Unpack(t);
 }
 
-void grad_norm(const std::vector<Tensor>& grads_in, double max_norm, const Tensor& out, const Tensor& ticket) {
-  py::gil_scoped_release nogil;
-  std::vector<Tensor> grads;
-  std::vector<blstm_grad_item> items;
-  for (const Tensor& g_in : grads_in) {
-    if (g_in.layout() != at::kStrided) throw wrong("sparse gradients are not there for AdamW");
-    beside(g_in, "a gradient", out);
-    if (g_in.numel() == 0) continue;
-    grads.push_back(g_in.contiguous());
-    blstm_grad_item a{};
-    a.grad = ptr(grads.back());
-    a.n = grads.back().numel();
-    a.dtype = dtype_code(g_in.scalar_type());
-    items.push_back(a);
+double number_of(PyObject* group, PyObject* name) {
+  PyObject* v = PyDict_GetItemWithError(group, name);
+  if (!v) throw wrong("a parameter group has no " + std::string(PyUnicode_AsUTF8(name)));
+  const double d = THPVariable_Check(v) ? THPVariable_Unpack(v).item<double>() : PyFloat_AsDouble(v);
+  if (d == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+  return d;
+}
+
+// A step over the parameter groups of an optimizer (optim.py).  start(p): makes the state of a parameter that has none; scratch(p): the
+// counter of p's device and its {norm, factor}.  Returns {norm, factor} where max_norm is given and there was anything to do.
+std::optional<Tensor> adamw_step(const py::list& groups, const py::dict& state, int bits, bool masters, std::optional<double> max_norm,
+                                 const py::object& start, const py::object& scratch) {
+  static PyObject *const k_params = interned("params"), *const k_m = interned("exp_avg"), *const k_v = interned("exp_avg_sq"),
+                  *const k_u = interned("exp_avg_sq_root"), *const k_ms = interned("exp_avg_scale"), *const k_us = interned("exp_avg_sq_root_scale"),
+                  *const k_step = interned("step"), *const k_master = interned("master"), *const k_lr = interned("lr"), *const k_betas = interned("betas"),
+                  *const k_eps = interned("eps"), *const k_decay = interned("weight_decay"), *const k_seed = interned("seed");
+  const at::ScalarType state_type = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+  std::vector<std::pair<PyObject*, Bucket>> calls;       // with the group of each
+  uint32_t number = 0;
+  for (const py::handle group_in : groups) {
+    PyObject* group = group_in.ptr();
+    const size_t begin = calls.size();
+    const py::list params = py::reinterpret_borrow<py::list>(PyDict_GetItemWithError(group, k_params));
+    for (const py::handle at : params) {
+      const uint32_t mine = number++;
+      if (!THPVariable_Check(at.ptr())) throw wrong("a parameter must be a tensor");
+      const Tensor& p = THPVariable_Unpack(at.ptr());
+      if (!p.grad().defined()) continue;
+      on_gpu(p, "a parameter");
+      dtype_code(p.scalar_type());
+      if (!p.is_contiguous()) throw wrong("a parameter of shape " + shape_str(p.sizes()) + " must be contiguous");
+      PyObject* s = PyDict_GetItemWithError(state.ptr(), at.ptr());
+      py::object made;
+      if (!s || PyDict_GET_SIZE(s) == 0) {
+        made = start(at);
+        s = made.ptr();
+      }
+      Bucket* b = nullptr;
+      for (size_t k = begin; k < calls.size(); ++k)
+        if (calls[k].second.params[0].device() == p.device() && calls[k].second.params[0].scalar_type() == p.scalar_type()) b = &calls[k].second;
+      if (!b) {
+        calls.emplace_back(group, Bucket());
+        b = &calls.back().second;
+      }
+      blstm_adamw_item a{};
+      a.n = p.numel();
+      a.number = mine;
+      a.exp_avg = flat(state_tensor(s, k_m), "exp_avg", p, state_type).data_ptr();
+      a.exp_avg_sq = flat(state_tensor(s, bits == 8 ? k_u : k_v), bits == 8 ? "exp_avg_sq_root" : "exp_avg_sq", p, state_type).data_ptr();
+      const Tensor& step = state_tensor(s, k_step);
+      beside(step, "step", p);
+      if (step.scalar_type() != at::kLong || step.numel() != 1) throw wrong("step must be one int64 element");
+      a.step = static_cast<int64_t*>(step.data_ptr());
+      if (bits == 8) {
+        a.exp_avg_scale = f32(state_tensor(s, k_ms), "exp_avg_scale", p, (a.n + 255) / 256);
+        a.exp_avg_sq_scale = f32(state_tensor(s, k_us), "exp_avg_sq_root_scale", p, (a.n + 255) / 256);
+      }
+      if (masters && p.scalar_type() != at::kFloat) a.master = f32(flat(state_tensor(s, k_master), "master", p, at::kFloat), "master", p, a.n);
+      b->params.push_back(p);
+      b->grads.push_back(dense_grad(p.grad(), p));
+      a.param = p.data_ptr();
+      a.grad = ptr(b->grads.back());
+      if (a.n) b->items.push_back(a);
+    }
   }
-  if (items.empty()) return;
-  Call call(out.device());
-  blstm_grad_norm_desc d{};
-  d.item = items.data();
-  d.items = (int32_t)items.size();
-  d.max_norm = (float)max_norm;
-  d.out = static_cast<float*>(out.data_ptr());
-  d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
-  d.workspace_bytes = blstm_grad_norm_workspace(d.items);
-  const Tensor ws = fresh({(int64_t)d.workspace_bytes}, at::kByte, out);
-  d.workspace = ws.data_ptr();
-  check(blstm_grad_norm(&d, call.stream), "gradient norm");
+  if (calls.empty()) return std::nullopt;
+  auto scratch_of = [&](const Bucket& b) { return scratch(b.params[0].device().index()).cast<std::pair<Tensor, Tensor>>(); };
+  std::optional<Tensor> norm;
+  if (max_norm) {
+    const Bucket& first = calls[0].second;
+    std::vector<blstm_grad_item> items;
+    for (const auto& [group, b] : calls) {
+      if (b.params[0].device() != first.params[0].device()) throw wrong("max_norm takes parameters on one device");
+      for (const blstm_adamw_item& a : b.items) items.push_back({a.grad, a.n, dtype_code(b.params[0].scalar_type()), 0});
+    }
+    const auto [ticket, out] = scratch_of(first);
+    norm = out;
+    if (!items.empty()) {
+      Call call(out.device());
+      blstm_grad_norm_desc d{};
+      d.item = items.data();
+      d.items = (int32_t)items.size();
+      d.max_norm = (float)*max_norm;
+      d.out = static_cast<float*>(out.data_ptr());
+      d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
+      d.workspace_bytes = blstm_grad_norm_workspace(d.items);
+      const Tensor ws = fresh({(int64_t)d.workspace_bytes}, at::kByte, out);
+      d.workspace = ws.data_ptr();
+      check(blstm_grad_norm(&d, call.stream), "gradient norm");
+    }
+  }
+  for (const auto& [group, b] : calls) {
+    if (b.items.empty()) continue;
+    blstm_adamw_desc d{};
+    d.dtype = dtype_code(b.params[0].scalar_type());
+    d.bits = bits;
+    d.items = (int32_t)b.items.size();
+    d.item = b.items.data();
+    PyObject* lr = PyDict_GetItemWithError(group, k_lr);
+    if (lr && THPVariable_Check(lr) && THPVariable_Unpack(lr).is_cuda()) {
+      const Tensor& t = THPVariable_Unpack(lr);
+      beside(t, "lr", b.params[0]);
+      if (t.scalar_type() != at::kFloat || t.numel() != 1) throw wrong("lr on the GPU must be one float32 element");
+      d.lr_at = static_cast<const float*>(ptr(t));
+    } else {
+      d.lr = number_of(group, k_lr);
+    }
+    const auto betas = py::reinterpret_borrow<py::object>(PyDict_GetItemWithError(group, k_betas)).cast<std::pair<double, double>>();
+    d.beta1 = betas.first; d.beta2 = betas.second;
+    d.eps = number_of(group, k_eps);
+    d.weight_decay = number_of(group, k_decay);
+    d.seed = py::reinterpret_borrow<py::object>(PyDict_GetItemWithError(group, k_seed)).cast<uint64_t>();
+    if (norm) d.factor = static_cast<const float*>(ptr(*norm)) + 1;
+    const Tensor ticket = scratch_of(b).first;
+    d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
+    Call call(b.params[0].device());
+    check(blstm_adamw(&d, call.stream), "adamw");
+    for (const Tensor& p : b.params) torch::autograd::impl::bump_version(p);
+  }
+  return norm;
 }
 
 }  // namespace
@@ -125,8 +173,7 @@ void grad_norm(const std::vector<Tensor>& grads_in, double max_norm, const Tenso
 namespace blstm_host {
 
 void bind_adamw(py::module_& m) {
-  m.def("adamw", &adamw);
-  m.def("grad_norm", &grad_norm);
+  m.def("adamw_step", &adamw_step);
 }
 
 }  // namespace blstm_host

@@ -82,6 +82,32 @@ __device__ __forceinline__ unsigned two(float a, float b, __half) { const __half
 template <typename T>
 __device__ __forceinline__ uint4 pack(const float* z, T t) { return make_uint4(two(z[0], z[1], t), two(z[2], z[3], t), two(z[4], z[5], t), two(z[6], z[7], t)); }
 
+// Two 32-bit floats that one instruction works on.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ static Pair of(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+  }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // Whether all addresses are multiples of `bytes`, a power of two.
 template <typename... P>
 bool aligned(size_t bytes, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0; }

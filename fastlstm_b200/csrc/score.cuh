@@ -35,32 +35,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Two 32-bit floats that one instruction works on.
-struct Pair {
-  unsigned long long v;
-  __device__ __forceinline__ static Pair of(float a, float b) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
-    return p;
-  }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-
 // How many of n keys in shared memory come before `key`.
 __device__ __forceinline__ unsigned rank_of(const unsigned long long* keys, unsigned n, unsigned long long key) {
   unsigned before = 0;

@@ -98,6 +98,24 @@ def test_copies_and_groups():
     torch.optim.lr_scheduler.StepLR(o, 1)
 
 
+def test_hooks_and_profilers_are_heard():
+    p = torch.zeros(3, requires_grad=True)
+    o = F.AdamW([p])
+    seen = []
+    handles = [o.register_step_pre_hook(lambda *a: seen.append("before")), o.register_step_post_hook(lambda *a: seen.append("behind"))]
+    assert o.step(lambda: seen.append("closure") or 3) == 3 and seen == ["before", "closure", "behind"]
+    for h in handles:
+        h.remove()
+    assert o.step(lambda: 4) == 4 and len(seen) == 3
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        o.step()
+    assert any("AdamW.step" in e.key for e in prof.key_averages())
+    scheduler = torch.optim.lr_scheduler.StepLR(o, 1, gamma=0.5)
+    o.step()
+    scheduler.step()
+    assert o.param_groups[0]["lr"] == 5e-4
+
+
 def test_descriptor_layouts_match_the_library():
     assert [ctypes.sizeof(c) for c in (_lib.AdamWItem, _lib.AdamWDesc, _lib.GradItem, _lib.GradNormDesc)] == [80, 96, 24, 48]
 
