@@ -3,10 +3,11 @@
 //   total[k,v] = score_k + z_kv - log sum_j exp z_kj       (an ended hypothesis: score_k for the end token, -inf for all others)
 //   rank = total / length^penalty                          the `width` largest, equal ones by (k, v)
 //
-// Two launches.  The first reads every hypothesis' logits once and keeps its softmax's statistics and `width` largest logits: nothing
-// else of it can be among the `width` best of the sentence.  The second joins a sentence's lists.  Bound by memory.  Totals are
-// compared in 64 bits, so that what decides between two hypotheses is the sum's error alone: 2^-24 a term, 2^-22 an exponential, which
-// average out to some 1e-7.
+// Two launches.  The first reads every hypothesis' logits once, in as many parts as there are SMs for, and keeps of each part the softmax's
+// statistics and the largest logits of its threads in groups.  The second has a block for every sentence: the `width`-th largest of the
+// groups' totals, taken over all hypotheses, is a lower bound of the `width`-th largest total, and only the few groups that reach it are read
+// again.  Bound by memory; few sentences are two chains of latencies.  Totals are compared in 64 bits, so that what decides between two
+// hypotheses is the sum's error alone: 2^-24 a term, 2^-22 an exponential, which average out to some 1e-7.
 #include <algorithm>
 
 #include "score.cuh"
@@ -19,11 +20,11 @@ struct BeamParams {
   const float* scores;
   const uint8_t* finished;       // or null
   const long long* lengths;      // or null
-  unsigned batch, beams, vocab, width, top;      // top: min(width, vocab), the length of a list
+  unsigned batch, beams, vocab, width, parts, log_parts;       // parts of a row, a power of two
   long long end;
   double penalty;
-  float2* stats;                 // [batch*beams]: largest logit, sum of exp(z - it)
-  unsigned long long* keys;      // [batch*beams][top]
+  float2* stats;                 // [batch*beams*parts]: largest logit, sum of exp(z - it)
+  float* largest;                // [batch*beams*parts][groups]
   float* out_scores;
   long long *parents, *tokens, *out_lengths;
   uint8_t* out_finished;
@@ -76,88 +77,51 @@ __device__ __forceinline__ void take(Sum& a, const float (&z)[N]) {
   a.s = s0 + s1;
 }
 
-template <typename T, int PPL>
-__global__ void __launch_bounds__(32 * kWarpRows) beam_warp_kernel(const __grid_constant__ BeamParams p) {
-  __shared__ unsigned long long s_cand[kWarpRows][kWarpCand];
-  const unsigned warp = threadIdx.x >> 5, r = blockIdx.x * kWarpRows + warp;
-  let_begin();
-  if (r >= p.batch * p.beams || !goes_on(p, r)) return;
-  const WarpRow<T, PPL> w(static_cast<const T*>(p.logits) + p.rows(r), p.vocab);
-  Sum a{-INFINITY, 0.f};
-  take(a, w.z);
-  const float edge[2] = {w.edge, -INFINITY};
-  take(a, edge);
-  const unsigned mine = value_key(a.m);
-  a.join(32);
-  if (w.lane == 0) p.stats[r] = make_float2(a.m, a.s);
-  warp_top(w, mine, p.top, s_cand[warp], [&](unsigned k, unsigned long long key) { p.keys[(size_t)r * p.top + k] = key; });
-}
-
-template <int NT>
-struct BeamShared {
-  Sum part[NT / 32];
-  Sum peers[kMaxCluster];
-  TopShared<NT> top;
-  unsigned long long all[kMaxCluster * BLSTM_MAX_TOP];
-};
+// NT threads have a part of a row: a warp, or a block.  Their pieces are neighbours in turns of NT; groups of NT / groups threads.
+constexpr int kBlock = 256, kMostGroups = 64, kAhead = 4;
+template <int NT> constexpr int kGroups = NT < kMostGroups ? NT : kMostGroups;
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) beam_rows_kernel(const __grid_constant__ BeamParams p) {
-  __shared__ BeamShared<NT> s;
-  const unsigned parts = cluster_size(), part = cluster_rank(), r = blockIdx.x / parts;
-  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(kBlock) beam_rows_kernel(const __grid_constant__ BeamParams p) {
+  __shared__ Sum s_part[kBlock / 32];
+  constexpr int kEach = kBlock / NT, kLanes = NT / kGroups<NT>;
+  const unsigned seg = blockIdx.x * kEach + threadIdx.x / NT, tid = threadIdx.x % NT, lane = tid & 31;
+  const unsigned r = seg / p.parts, part = seg - r * p.parts;
   let_begin();
-  if (!goes_on(p, r)) return;                  // (the same for a whole cluster)
-  if (parts > 1) cluster_arrive();             // this block has begun: the others may write to it
+  if (r >= p.batch * p.beams || !goes_on(p, r)) return;          // (the same for all NT threads)
   const T* row = static_cast<const T*>(p.logits) + p.rows(r);
-  const Span<T> span(row, p.vocab, part, parts);
+  const Span<T> span(row, p.vocab, part, p.parts);
   const uint4* body = span.body();
-  auto fetch = [&](unsigned i, uint4 (&v)[kUnroll]) {
+  auto fetch = [&](unsigned i, uint4 (&v)[kAhead]) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) v[u] = i + u * NT < span.end ? load_once(body + i + u * NT) : minus_infinity(T{});
+    for (int u = 0; u < kAhead; ++u) v[u] = i + u * NT < span.end ? load_once(body + i + u * NT) : minus_infinity(T{});
   };
-  uint4 next[kUnroll];
+  uint4 next[kAhead];
   fetch(span.begin + tid, next);
   Sum a{-INFINITY, 0.f};
   if (tid < span.edges()) {
     const float z[2] = {ld_f(row + span.edge(tid)), -INFINITY};
     take(a, z);
   }
-  for (unsigned i = span.begin + tid; i < span.end; i += kUnroll * NT) {
-    float z[kUnroll * kPer<T>];
+  for (unsigned i = span.begin + tid; i < span.end; i += kAhead * NT) {
+    float z[kAhead * kPer<T>];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) unpack(next[u], z + u * kPer<T>, T{});
-    fetch(i + kUnroll * NT, next);
+    for (int u = 0; u < kAhead; ++u) unpack(next[u], z + u * kPer<T>, T{});
+    fetch(i + kAhead * NT, next);
     take(a, z);
   }
-  const float thread_max = a.m;
+  float most = a.m;
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) most = max_nan(most, __shfl_xor_sync(~0u, most, o));
+  if (tid % kLanes == 0) p.largest[(size_t)seg * kGroups<NT> + tid / kLanes] = most;
   a.join(32);
-  if (lane == 0) s.part[warp] = a;
-  block_top(s.top, span, thread_max, p.top);
-  a = s.part[lane % (NT / 32)];
-  a.join(NT / 32);
-  if (parts > 1) {
-    cluster_wait();
-    if (tid < parts) {
-      static_assert(sizeof(Sum) == 8, "");
-      store_to(tid, &s.peers[part], (unsigned long long)__float_as_uint(a.s) << 32 | __float_as_uint(a.m));
-    }
-    if (tid < parts * p.top) store_to(tid / p.top, &s.all[part * p.top + tid % p.top], s.top.best[tid % p.top]);
-    cluster_arrive();
-    cluster_wait();
-    a = lane % kMaxCluster < parts ? s.peers[lane % kMaxCluster] : Sum{-INFINITY, 0.f};
-    a.join(kMaxCluster);
-    if (part == 0 && tid == 0) p.stats[r] = make_float2(a.m, a.s);
-    if (tid / kMaxCluster < p.top) {
-      static_assert(NT < 256 || NT == kMaxCluster * BLSTM_MAX_TOP, "clusters have blocks of 256 threads");
-      const unsigned long long key = s.top.best[tid / kMaxCluster];
-      const unsigned before = place_in_lists(s.all, key, parts, p.top);
-      if (tid % kMaxCluster == 0 && key && before < p.top) p.keys[(size_t)r * p.top + before] = key;
-    }
-  } else {
-    if (tid == 0) p.stats[r] = make_float2(a.m, a.s);
-    if (tid < p.top) p.keys[(size_t)r * p.top + tid] = s.top.best[tid];
+  if constexpr (NT > 32) {
+    if (lane == 0) s_part[tid / 32] = a;
+    __syncthreads();
+    a = s_part[lane % (NT / 32)];
+    a.join(NT / 32);
   }
+  if (tid == 0) p.stats[seg] = make_float2(a.m, a.s);
 }
 
 // Larger ranks have larger keys, NaN the largest; no key is 0.
@@ -166,86 +130,225 @@ __device__ __forceinline__ unsigned long long rank_key(double v) {
   const long long b = __double_as_longlong(v + 0.0);
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 1ull << 63;
 }
+__device__ __forceinline__ unsigned rank_key(float v) {
+  if (v != v) return ~0u;
+  const unsigned b = __float_as_uint(v + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+constexpr unsigned long long kImpossible = 0x000fffffffffffffull;      // the key of -inf
+constexpr unsigned kImpossible32 = 0x007fffffu;
 
-constexpr int kMergeThreads = 256, kMost = BLSTM_MAX_BEAMS * BLSTM_MAX_TOP;
+constexpr int kMergeThreads = 1024, kCand = 1024, kWindow = 2048, kTop = 64;
 
-// A sentence's lists as one.  Every list has its `width`-th entry: what is below the largest of those is out; of what is left, eight lanes
-// count what comes before an entry.
+// What is among the best is decided in 64 bits; which groups are looked at, and which of their logits, in 32, with a margin for what those are
+// off.  The block's code runs once, and fetching it takes most of its time (some 240 clocks for eight instructions): so many threads, few
+// instructions, and loops that stay loops.
+struct MergeShared {
+  double base[BLSTM_MAX_BEAMS], weight[BLSTM_MAX_BEAMS];         // total = base + (z - high), rank = total weight
+  float base32[BLSTM_MAX_BEAMS], weight32[BLSTM_MAX_BEAMS], high[BLSTM_MAX_BEAMS];
+  int kind[BLSTM_MAX_BEAMS];                   // 0 goes on, 1 has ended, 2 is dead
+  alignas(16) unsigned top[kTop];
+  unsigned from;
+  unsigned long long bound, place;
+  unsigned long long keys[kCand], places[kCand];         // candidates: ranks, and (hypothesis, token); what comes first has the larger key, or
+  float z[kCand];                                        // the smaller place
+  unsigned owner[kWindow], owners, count;
+
+  __device__ __forceinline__ double total(unsigned k, float at) const { return base[k] == -INFINITY ? -INFINITY : base[k] + ((double)at - (double)high[k]); }
+  // The rank in 32 bits, less or more (side -1, 1) than what it may be off; one that is finite stays it.
+  __device__ __forceinline__ float rank32(unsigned k, float at, float side) const {
+    const float d = at - high[k], off = 2e-6f * (fabsf(base32[k]) + fabsf(d));
+    return at == -INFINITY ? at : fminf(max_nan(max_nan(base32[k] + d + side * off, kLowest) * weight32[k], kLowest), -kLowest);
+  }
+  // A continuation that may be among the best.
+  __device__ __noinline__ void offer(unsigned k, unsigned token, float at) {
+    const unsigned long long rank = rank_key((kind[k] == 1 ? base[k] : total(k, at)) * weight[k]), at_place = (unsigned long long)k << 32 | token;
+    if (rank <= kImpossible || rank < bound || (rank == bound && at_place > place)) return;
+    const unsigned i = atomicAdd(&count, 1u);
+    if (i >= kCand) return;
+    keys[i] = rank;
+    places[i] = at_place;
+    z[i] = at;
+  }
+};
+
+template <typename T, int NT>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamParams p) {
-  __shared__ double s_base[BLSTM_MAX_BEAMS], s_high[BLSTM_MAX_BEAMS], s_per[BLSTM_MAX_BEAMS];
-  __shared__ int s_kind[BLSTM_MAX_BEAMS];      // 0 goes on, 1 has ended, 2 is dead
-  __shared__ unsigned long long s_key[kMost], s_bound;
-  __shared__ unsigned s_token[kMost], s_kept[kMost], s_count;
-  const unsigned b = blockIdx.x, tid = threadIdx.x, total = p.beams * p.top;
-  if (tid == 0) { s_bound = 0; s_count = 0; }
-  if (tid < p.beams) {
-    const unsigned r = b * p.beams + tid;
-    const float score = p.scores[r];
-    const bool ended = p.finished && p.finished[r];
-    s_kind[tid] = ended ? 1 : score == -INFINITY ? 2 : 0;
-    s_base[tid] = score;
-    s_high[tid] = 0;
-    s_per[tid] = p.penalty != 0.0 ? pow((double)(p.lengths[r] + !ended), p.penalty) : 1.0;
+  __shared__ MergeShared s;
+  constexpr int kLanes = NT / kGroups<NT>;
+  const unsigned b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r0 = b * p.beams, segs = p.beams * p.parts;
+  // eight lanes have a hypothesis
+  static_assert(kMergeThreads >= 8 * BLSTM_MAX_BEAMS && kMergeThreads == 16 * kTop, "");
+  const unsigned mine = tid / 8;
+  float score = -INFINITY;
+  bool ended = false;
+  if (mine < p.beams) {
+    score = p.scores[r0 + mine];
+    ended = p.finished && p.finished[r0 + mine];
   }
+  const bool live = !ended && score != -INFINITY;
+  if (mine < p.beams && tid % 8 == 0) {
+    s.kind[mine] = ended ? 1 : live ? 0 : 2;
+    const double weight = p.penalty != 0.0 ? 1.0 / pow((double)(p.lengths[r0 + mine] + !ended), p.penalty) : 1.0;
+    s.weight[mine] = weight;
+    s.weight32[mine] = (float)weight;
+  }
+  if (tid < kTop) s.top[tid] = 0;
+  if (tid == 0) { s.bound = 0; s.place = ~0ull; s.count = 0; s.from = ~0u; }
+  let_begin();
   begin_behind();                              // (what does not need the rows' results came before)
-  if (tid < p.beams && s_kind[tid] == 0) {
-    const float2 st = p.stats[b * p.beams + tid];
-    s_high[tid] = st.x;
-    s_base[tid] = st.y == 0.f ? -INFINITY : s_base[tid] - log((double)st.y);      // (a row of nothing but -inf)
-  }
-  __syncthreads();
-  auto total_of = [&](unsigned k, float z) { return s_base[k] == -INFINITY ? -INFINITY : s_base[k] + ((double)z - s_high[k]); };
-  for (unsigned c = tid; c < total; c += kMergeThreads) {
-    const unsigned k = c / p.top, i = c - k * p.top;
-    unsigned token = i;
-    double v = -INFINITY;
-    if (s_kind[k] == 0) {
-      const unsigned long long key = p.keys[(size_t)(b * p.beams + k) * p.top + i];
-      token = 0xffffffffu - (unsigned)key;
-      v = total_of(k, key_value((unsigned)(key >> 32)));
-    } else if (s_kind[k] == 1 && s_base[k] != -INFINITY) {
-      if (i == 0) { token = (unsigned)p.end; v = s_base[k]; }
-      else token = i <= p.end ? i - 1 : i;
+  Sum a{-INFINITY, 0.f};
+  if (live)
+#pragma unroll 1
+    for (unsigned q = tid % 8; q < p.parts; q += 8) {
+      const float2 st = p.stats[(size_t)(r0 + mine) * p.parts + q];
+      Sum o{st.x, st.y};
+      const float m = max_nan(a.m, o.m), to = max_nan(m, kLowest);
+      a.rescale(to);
+      o.rescale(to);
+      a = Sum{m, a.s + o.s};
     }
-    const unsigned long long key = rank_key(v / s_per[k]);
-    s_key[c] = key;
-    s_token[c] = token;
-    if (i + 1 == p.width) atomicMax(&s_bound, key);
+  a.join(8);
+  if (mine < p.beams && tid % 8 == 0) {
+    const double base = !live ? (double)score : a.s == 0.f ? -INFINITY : (double)score - log((double)a.s);      // (a row of nothing but -inf)
+    s.base[mine] = base;
+    s.base32[mine] = base == -INFINITY ? -INFINITY : max_nan((float)base, kLowest);                // (-inf alone stands for none)
+    s.high[mine] = live ? a.m : 0.f;
   }
   __syncthreads();
-  const unsigned long long bound = s_bound;
-  for (unsigned c = tid; c < total; c += kMergeThreads)
-    if (s_key[c] >= bound) s_kept[atomicAdd(&s_count, 1u)] = c;
+  // the groups of all parts of all hypotheses by their number, without those of hypotheses that do not go on
+  const float* largest = p.largest + (size_t)r0 * p.parts * kGroups<NT>;
+  const unsigned all = segs * kGroups<NT>;
+  auto group_key = [&](unsigned i, float side) {
+    const unsigned k = i / kGroups<NT> >> p.log_parts;
+    return s.kind[k] == 0 && s.base32[k] != -INFINITY ? rank_key(s.rank32(k, largest[i], side)) : 0u;
+  };
+  // the `width`-th largest of what they come to
+  {
+    unsigned most = 0;
+#pragma unroll 1
+    for (unsigned i = tid; i < all; i += kMergeThreads) most = max(most, group_key(i, -1.f));
+    atomicMax(&s.top[tid % kTop], most);
+    if (tid < p.beams && s.kind[tid] == 1) atomicMax(&s.top[tid % kTop], rank_key(s.rank32(tid, 0.f, -1.f)));
+  }
   __syncthreads();
-  const unsigned count = s_count, lane = tid & 7;
-  for (unsigned i0 = 0; i0 < count; i0 += kMergeThreads / 8) {
-    const unsigned i = i0 + tid / 8;
-    unsigned c = 0, before = 0;
-    if (i < count) {
-      c = s_kept[i];
-      const unsigned long long key = s_key[c];
-      const unsigned long long place = (unsigned long long)(c / p.top) << 32 | s_token[c];
-      for (unsigned j = lane; j < count; j += 8) {
-        const unsigned o = s_kept[j];
-        const unsigned long long other = s_key[o];
-        before += other > key || (other == key && ((unsigned long long)(o / p.top) << 32 | s_token[o]) < place);
+  {
+    // the smallest that fewer than `width` are above (equal ones count alike): sixteen lanes have one
+    const unsigned g = s.top[tid / 16];
+    const uint4 v = *reinterpret_cast<const uint4*>(s.top + tid % 16 * 4);
+    unsigned above = (v.x > g) + (v.y > g) + (v.z > g) + (v.w > g);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) above += __shfl_xor_sync(~0u, above, o);
+    if (tid % 16 == 0 && above < p.width) atomicMin(&s.from, g);
+  }
+  __syncthreads();
+  unsigned from = s.from;
+  // what a group has of a part is looked at by warps, kRows turns of NT pieces at a time
+  constexpr unsigned kRows = 32 / kLanes;
+  const unsigned looks = ((p.vocab / kPer<T> >> p.log_parts) + kRows * NT) / (kRows * NT);      // (turns of a part: pieces / parts, rounded up, / NT)
+  for (;;) {
+    // the least rank that is looked at (-inf: all that is possible)
+    const float rank = from <= kImpossible32 ? -INFINITY : __uint_as_float(from & 0x80000000u ? from & 0x7fffffffu : ~from);
+    const unsigned least_key = max(from, kImpossible32 + 1);
+    if (tid < p.beams && s.kind[tid] == 1) s.offer(tid, (unsigned)p.end, 0.f);
+    for (unsigned w0 = 0; w0 < all; w0 += kWindow) {
+      if (tid == 0) s.owners = 0;
+      __syncthreads();
+      const unsigned w1 = min(all, w0 + kWindow);
+#pragma unroll 1
+      for (unsigned i = w0 + tid; i < w1; i += kMergeThreads)
+        if (group_key(i, 1.f) >= least_key) s.owner[atomicAdd(&s.owners, 1u)] = i;
+      __syncthreads();
+      const unsigned owners = s.owners;
+#pragma unroll 1
+      for (unsigned o = warp; o < owners * looks; o += kMergeThreads / 32) {
+        const unsigned look = o / owners, i = s.owner[o - look * owners], seg = i / kGroups<NT>, group = i % kGroups<NT>, k = seg >> p.log_parts;
+        const T* row = static_cast<const T*>(p.logits) + p.rows(r0 + k);
+        const Span<T> span(row, p.vocab, seg & (p.parts - 1), p.parts);
+        const unsigned piece = span.begin + (look * kRows + lane / kLanes) * NT + group * kLanes + lane % kLanes;
+        const uint4 v = piece < span.end ? span.body()[piece] : minus_infinity(T{});
+        // the least logit that is looked at
+        const float total = rank / s.weight32[k], need = total - s.base32[k] + s.high[k];
+        const float off = 4e-6f * (fabsf(total) + fabsf(s.base32[k]) + fabsf(s.high[k])) + 1e-30f, least = need - off > kLowest ? need - off : -INFINITY;
+        float z[kPer<T>], m;
+        unpack(v, z, T{});
+        m = z[0];
+#pragma unroll
+        for (int e = 1; e < kPer<T>; ++e) m = max_nan(m, z[e]);
+        unsigned token = span.number(piece), last = m < least || m == -INFINITY ? token : token + kPer<T>;
+        if (look == 0) {                       // thread `edge` of the part had one of its edges
+          const unsigned edge = group * kLanes + lane;
+          if (lane < kLanes && edge < span.edges()) s.offer(k, span.edge(edge), ld_f(row + span.edge(edge)));
+        }
+#pragma unroll 1
+        for (; token < last; ++token) {        // (few, so in little code)
+          const float at = ld_f(row + token);
+          if (!(at < least)) s.offer(k, token, at);
+        }
       }
+      __syncthreads();
+    }
+    if (s.count <= kCand) break;
+    // (many equal ones) a higher bound, the `width`-th of some of them, until they fit
+    unsigned long long key = 0, at = 0;
+    bool is = false;
+    for (unsigned i = tid; i < kCand; i += kMergeThreads) {
+      unsigned before = 0;
+#pragma unroll 1
+      for (unsigned j = 0; j < kCand; ++j) before += s.keys[j] > s.keys[i] || (s.keys[j] == s.keys[i] && s.places[j] < s.places[i]);
+      if (before + 1 == p.width) { key = s.keys[i]; at = s.places[i]; is = true; }
+    }
+    __syncthreads();
+    if (is) { s.bound = key; s.place = at; }
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    const unsigned long long high = s.bound;
+    // (groups that hold NaN or infinity have the largest rank that is finite)
+    const double raised = __longlong_as_double((long long)(high >> 63 ? high & ~(1ull << 63) : ~high));
+    from = max(from, rank_key(raised != raised ? -kLowest : fminf(fmaxf(__double2float_rd(raised), kLowest), -kLowest)));
+  }
+  const unsigned count = s.count;
+  auto put = [&](unsigned place, unsigned k, unsigned token, double total) {
+    const size_t at = (size_t)b * p.width + place;
+    const bool ended = s.kind[k] == 1 || (s.kind[k] == 2 && p.finished && p.finished[r0 + k]);
+    p.out_scores[at] = (float)total;
+    p.parents[at] = k;
+    p.tokens[at] = token;
+    if (p.out_finished) p.out_finished[at] = ended || token == p.end;
+    if (p.out_lengths) p.out_lengths[at] = p.lengths[r0 + k] + !ended;
+  };
+  for (unsigned i0 = 0; i0 < count; i0 += kMergeThreads / 8) {         // eight lanes count what comes before a candidate
+    const unsigned i = i0 + tid / 8;
+    unsigned before = 0;
+    if (i < count) {
+      const unsigned long long key = s.keys[i], place = s.places[i];
+#pragma unroll 1
+      for (unsigned j = tid % 8; j < count; j += 8) before += s.keys[j] > key || (s.keys[j] == key && s.places[j] < place);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) before += __shfl_xor_sync(~0u, before, o);
-    if (i < count && lane == 0 && before < p.width) {
-      const unsigned k = c / p.top, token = s_token[c];
-      const size_t at = (size_t)b * p.width + before;
-      const unsigned r = b * p.beams + k;
+    if (i < count && tid % 8 == 0 && before < p.width) {
+      const unsigned k = (unsigned)(s.places[i] >> 32);
+      put(before, k, (unsigned)s.places[i], s.kind[k] == 1 ? s.base[k] : s.total(k, s.z[i]));
+    }
+  }
+  if (count >= p.width) return;
+  // Too few that are possible: impossible ones follow, the first of them (no more than `count` possible ones lie between).
+  if (warp == 0) {
+    unsigned found = count;
+    for (unsigned long long i0 = 0; found < p.width && i0 < (unsigned long long)p.beams * p.vocab; i0 += 32) {
+      const unsigned long long i = i0 + lane;
+      const unsigned k = (unsigned)(i / p.vocab), token = (unsigned)(i - (unsigned long long)k * p.vocab);
+      bool is = k < p.beams;
       double v = -INFINITY;
-      if (s_kind[k] == 0) v = total_of(k, key_value((unsigned)(p.keys[(size_t)r * p.top + (c - k * p.top)] >> 32)));
-      else if (s_kind[k] == 1 && c == k * p.top) v = s_base[k];
-      p.out_scores[at] = (float)v;
-      p.parents[at] = k;
-      p.tokens[at] = token;
-      const bool ended = p.finished && p.finished[r];
-      if (p.out_finished) p.out_finished[at] = ended || token == p.end;
-      if (p.out_lengths) p.out_lengths[at] = p.lengths[r] + !ended;
+      if (is && s.base[k] != -INFINITY) {
+        if (s.kind[k] == 0) v = s.total(k, ld_f(static_cast<const T*>(p.logits) + p.rows(r0 + k) + token));
+        else if (token == p.end) v = s.base[k];
+      }
+      if (is) is = rank_key(v * s.weight[k]) <= kImpossible;
+      const unsigned who = __ballot_sync(~0u, is), place = found + __popc(who & ((1u << lane) - 1));
+      if (is && place < p.width) put(place, k, token, v);
+      found += __popc(who);
     }
   }
 }
@@ -298,6 +401,8 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
   const unsigned long long out_row = a.parts == 1 ? unit : quotient(unit, a.parts), outer = quotient(out_row, rows);
   const unsigned begin = (unsigned)(unit - out_row * a.parts) * (kRowPieces << a.lanes), end = min(a.per_row, begin + (kRowPieces << a.lanes));
   const unsigned at = (unsigned)(out_row - outer * rows), b = at / p.width;
+  let_begin();
+  begin_behind();                              // (a step of beam search, or whatever the stream has in front)
   const long long parent = p.wide ? static_cast<const long long*>(p.parents)[at] : (long long)static_cast<const int*>(p.parents)[at];
   const bool in = parent >= 0 && parent < p.beams;
   if (!in && outer == 0 && begin + lane == 0) report_token(p.mailbox, at, parent, BLSTM_E_PARENT);
@@ -321,39 +426,46 @@ static int check_beam(const blstm_beam_desc* d) {
   return BLSTM_OK;
 }
 
-static unsigned list_length(const blstm_beam_desc& d) { return (unsigned)std::min<int64_t>(d.width, d.vocab); }
-static size_t stats_bytes(const blstm_beam_desc& d) { return round_up((size_t)d.batch * d.beams * sizeof(float2), 256); }
-
 // 16-byte pieces of a row: what they are at least, and at most where it does not begin on a boundary.
-static unsigned beam_pieces(const BeamParams& p, size_t element) { return (unsigned)((unsigned long long)p.vocab * element / 16); }
+static unsigned beam_pieces(const blstm_beam_desc& d) { return (unsigned)((uint64_t)d.vocab * dtype_bytes(d.dtype) / 16); }
 
-template <typename T>
-static int launch_rows(const BeamParams& p, cudaStream_t st) {
-  const unsigned n = p.batch * p.beams, pieces = beam_pieces(p, sizeof(T));
-  constexpr int kMostPieces = sizeof(T) == 2 ? 128 : 256;
-  if (pieces <= kMostPieces) {
-    const unsigned grid = (n + kWarpRows - 1) / kWarpRows, block = 32 * kWarpRows;
-    if (pieces <= 32) beam_warp_kernel<T, 1><<<grid, block, 0, st>>>(p);
-    else if (pieces <= 64) beam_warp_kernel<T, 2><<<grid, block, 0, st>>>(p);
-    else if (pieces <= 128) beam_warp_kernel<T, 4><<<grid, block, 0, st>>>(p);
-    else if constexpr (kMostPieces > 128) beam_warp_kernel<T, 8><<<grid, block, 0, st>>>(p);
-    BLSTM_CUDA_OK(cudaGetLastError());
-  } else {
-    unsigned parts = 1;
-    while (parts < kMaxCluster && (unsigned long long)n * parts * 2 <= 4ull * plan_sm_count() && pieces / (parts * 2) >= 256) parts *= 2;
-    if ((unsigned long long)n * parts > INT32_MAX) return BLSTM_E_TOO_LARGE;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {parts, 1, 1};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = n * parts;
-    cfg.blockDim = 256;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = parts > 1 ? 1 : 0;
-    BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, beam_rows_kernel<T, 256>, p));
-  }
-  count_launch();
+// Threads of a part, and parts of a row: warps have short rows; else as many parts (a power of two) as give kPartBlocks blocks to an SM, with
+// kPartPieces pieces at least for each thread.
+constexpr unsigned kShortPieces = 256, kPartBlocks = 16, kPartPieces = 4, kMostParts = 16;
+static unsigned beam_threads(const blstm_beam_desc& d) { return beam_pieces(d) <= kShortPieces ? 32 : kBlock; }
+static unsigned beam_parts(const blstm_beam_desc& d) {
+  unsigned parts = 1;
+  if (beam_threads(d) == kBlock)
+    while (parts < kMostParts && (uint64_t)d.batch * d.beams * parts * 2 <= (uint64_t)kPartBlocks * plan_sm_count() && beam_pieces(d) / (parts * 2) >= kPartPieces * kBlock)
+      parts *= 2;
+  return parts;
+}
+static uint64_t beam_segs(const blstm_beam_desc& d) { return (uint64_t)d.batch * d.beams * beam_parts(d); }
+static size_t stats_bytes(const blstm_beam_desc& d) { return round_up(beam_segs(d) * sizeof(float2), 256); }
+
+// A launch that may begin while the one in front of it ends (and waits for it in begin_behind).
+template <typename P>
+static cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned block, cudaStream_t st, const P& p) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, int NT>
+static int launch_beam(const BeamParams& p, cudaStream_t st) {
+  const uint64_t segs = (uint64_t)p.batch * p.beams * p.parts, grid = (segs + kBlock / NT - 1) / (kBlock / NT);
+  if (grid > INT32_MAX) return BLSTM_E_TOO_LARGE;
+  beam_rows_kernel<T, NT><<<(unsigned)grid, kBlock, 0, st>>>(p);
+  BLSTM_CUDA_OK(cudaGetLastError());
+  BLSTM_CUDA_OK(launch_behind(beam_merge_kernel<T, NT>, p.batch, kMergeThreads, st, p));
+  count_launch(2);
   return BLSTM_OK;
 }
 
@@ -365,7 +477,7 @@ extern "C" {
 
 size_t blstm_beam_workspace(const blstm_beam_desc* d) {
   if (check_beam(d) || d->batch == 0) return 0;
-  return round_up(stats_bytes(*d) + (size_t)d->batch * d->beams * list_length(*d) * 8, 256);
+  return round_up(stats_bytes(*d) + beam_segs(*d) * std::min<size_t>(beam_threads(*d), kMostGroups) * sizeof(float), 256);
 }
 
 int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* scores, const uint8_t* finished, const int64_t* lengths,
@@ -382,29 +494,20 @@ int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* s
   p.rows = row_map(d->batch, d->beams, d->logits_stride);
   p.scores = scores; p.finished = finished;
   p.lengths = reinterpret_cast<const long long*>(lengths);
-  p.batch = (unsigned)d->batch; p.beams = (unsigned)d->beams; p.vocab = (unsigned)d->vocab; p.width = (unsigned)d->width; p.top = list_length(*d);
+  p.batch = (unsigned)d->batch; p.beams = (unsigned)d->beams; p.vocab = (unsigned)d->vocab; p.width = (unsigned)d->width; p.parts = beam_parts(*d);
+  while (1u << p.log_parts < p.parts) ++p.log_parts;
   p.end = d->end_token;
   p.penalty = d->length_penalty;
   p.stats = static_cast<float2*>(workspace);
-  p.keys = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + stats_bytes(*d));
+  p.largest = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(*d));
   p.out_scores = out_scores;
   p.parents = reinterpret_cast<long long*>(parents); p.tokens = reinterpret_cast<long long*>(tokens);
   p.out_lengths = reinterpret_cast<long long*>(out_lengths);
   p.out_finished = out_finished;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = with_type(d->dtype, [&](auto t) -> int { return launch_rows<decltype(t)>(p, st); })) return rc;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = p.batch;
-  cfg.blockDim = kMergeThreads;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  BLSTM_CUDA_OK(cudaLaunchKernelEx(&cfg, beam_merge_kernel, p));
-  count_launch();
-  return BLSTM_OK;
+  return with_type(d->dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    return beam_threads(*d) == 32 ? launch_beam<T, 32>(p, (cudaStream_t)stream) : launch_beam<T, kBlock>(p, (cudaStream_t)stream);
+  });
 }
 
 int blstm_reorder(const blstm_reorder_item* items, int n, const void* parents, int parent_bits, int64_t batch, int64_t beams, int64_t width,
@@ -425,8 +528,7 @@ int blstm_reorder(const blstm_reorder_item* items, int n, const void* parents, i
   unsigned long long blocks = 0;
   auto launch = [&]() -> int {
     if (p.items == 0) return BLSTM_OK;
-    reorder_kernel<<<(unsigned)blocks, kReorderThreads, 0, (cudaStream_t)stream>>>(p);
-    BLSTM_CUDA_OK(cudaGetLastError());
+    BLSTM_CUDA_OK(launch_behind(reorder_kernel, (unsigned)blocks, kReorderThreads, (cudaStream_t)stream, p));
     count_launch();
     p.items = 0;
     blocks = 0;

@@ -1,6 +1,8 @@
 // Host side of beam search: argument checks, buffers, the calls of the C ABI.
 #include "host_language.h"
 
+#include <torch/csrc/autograd/python_variable.h>
+
 namespace {
 
 using namespace blstm_host;
@@ -85,7 +87,7 @@ bool in_pieces(const Tensor& t, int64_t dim, int64_t& outer_stride) {
 }
 
 // [.., batch * hypotheses along dim, ..] of each tensor -> [.., batch * width, ..]
-std::vector<Tensor> reorder(const std::vector<Tensor>& states, const Tensor& parents_in, int64_t dim_in) {
+std::vector<Tensor> reorder_flat(const std::vector<Tensor>& states, const Tensor& parents_in, int64_t dim_in) {
   py::gil_scoped_release nogil;
   on_gpu(parents_in, "parents");
   token_bits(parents_in);
@@ -137,6 +139,38 @@ std::vector<Tensor> reorder(const std::vector<Tensor>& states, const Tensor& par
                       call.stream),
         "reorder_states");
   return out;
+}
+
+// Tensors in (nested) lists and tuples, None among them, as one list; and one list in their place again.
+void collect(PyObject* s, std::vector<Tensor>& flat) {
+  if (THPVariable_Check(s)) flat.push_back(THPVariable_Unpack(s));
+  else if (PyList_Check(s) || PyTuple_Check(s)) {
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(s);
+    for (Py_ssize_t i = 0; i < n; ++i) collect(PySequence_Fast_GET_ITEM(s, i), flat);
+  } else if (s != Py_None) {
+    throw wrong(std::string("states must be tensors in lists or tuples, got ") + Py_TYPE(s)->tp_name);
+  }
+}
+py::object rebuild(PyObject* s, const std::vector<Tensor>& flat, size_t& at) {
+  if (THPVariable_Check(s)) return py::cast(flat[at++]);
+  if (s == Py_None) return py::none();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(s);
+  if (PyList_Check(s)) {
+    py::list r(n);
+    for (Py_ssize_t i = 0; i < n; ++i) r[i] = rebuild(PySequence_Fast_GET_ITEM(s, i), flat, at);
+    return r;
+  }
+  py::tuple r(n);
+  for (Py_ssize_t i = 0; i < n; ++i) r[i] = rebuild(PySequence_Fast_GET_ITEM(s, i), flat, at);
+  return PyTuple_CheckExact(s) ? py::object(r) : py::reinterpret_borrow<py::object>((PyObject*)Py_TYPE(s))(*r);     // (a named tuple)
+}
+
+py::object reorder(const py::object& states, const Tensor& parents, int64_t dim) {
+  std::vector<Tensor> flat;
+  collect(states.ptr(), flat);
+  const std::vector<Tensor> moved = reorder_flat(flat, parents, dim);
+  size_t at = 0;
+  return rebuild(states.ptr(), moved, at);
 }
 
 }  // namespace

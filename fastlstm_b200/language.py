@@ -129,24 +129,4 @@ def reorder_states(states, parents: torch.Tensor, *, dim: int = 1):
     states: a tensor or a (nested) list or tuple of tensors of any types, in which `None` stays: the (h, c) [layers, rows, width] of a
     FastLSTM, several of them, and token histories [steps, rows] in one launch.  parents [batch, width] (int64 or int32) are those of
     beam_step.  A parent that is none gives zeros, and `check_status()` or a later call raises BlstmError.  Without gradients."""
-    flat = []
-
-    def collect(s):
-        if isinstance(s, torch.Tensor):
-            flat.append(s)
-        elif isinstance(s, (list, tuple)):
-            for t in s:
-                collect(t)
-        elif s is not None:
-            raise ValueError(f"states must be tensors in lists or tuples, got {type(s).__name__}")
-
-    collect(states)
-    moved = iter(_lib.host().reorder(flat, parents, _whole(dim, "dim")))
-
-    def rebuild(s):
-        if s is None or isinstance(s, torch.Tensor):
-            return None if s is None else next(moved)
-        parts = [rebuild(t) for t in s]
-        return parts if isinstance(s, list) else type(s)(*parts) if hasattr(s, "_fields") else tuple(parts)
-
-    return rebuild(states)
+    return _lib.host().reorder(states, parents, _whole(dim, "dim"))

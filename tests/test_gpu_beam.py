@@ -254,6 +254,10 @@ def test_reorder_layouts_and_nests():
     assert isinstance(got, list) and isinstance(got[0], tuple) and isinstance(got[1], list) and got[1][1] is None
     for a, b in zip((got[0][0], got[0][1], got[1][0], got[2]), views):
         assert torch.equal(a, b[:, rows])
+    from collections import namedtuple
+    Pair = namedtuple("Pair", "h c")
+    pair = F.reorder_states([Pair(views[0], None)], parents)[0]
+    assert type(pair) is Pair and torch.equal(pair.h, got[0][0]) and pair.c is None
     many = [make_state(1 + k % 3, B * n, 1 + k % 5) for k in range(100)]
     for a, b in zip(F.reorder_states(many, parents.t().contiguous().t()), many):
         assert torch.equal(a, b[:, rows])
