@@ -520,19 +520,30 @@ struct GradNormParams {
 constexpr int kNormChunk = 4 * kTurn;
 
 template <typename T>
+__device__ __forceinline__ float squares(const Raw<T>& raw) {
+  float z[8], t = 0.f;
+  raw.get(z);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t = fmaf(z[e], z[e], t);
+  return t;
+}
+template <typename T>
 __device__ __forceinline__ double chunk_squares(const T* g, long long i, long long n, bool wide) {
+  constexpr int kParts = kNormChunk / kTurn;
   double sum = 0;
+  if (wide && i - threadIdx.x * 8 + kNormChunk <= n) {
+    Raw<T> raw[kParts];
 #pragma unroll
-  for (int part = 0; part < kNormChunk / kTurn; ++part) {
-    float z[8], t = 0.f;
-    Raw<T> raw;
-    const long long at = i + part * kTurn;
-    if (wide && at + 8 <= n) raw.template load<true>(g + at, 8);
-    else raw.template load<false>(g + at, n - at);
-    raw.get(z);
+    for (int part = 0; part < kParts; ++part) raw[part].template load<true>(g + i + part * kTurn, 8);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t = fmaf(z[e], z[e], t);
-    sum += t;
+    for (int part = 0; part < kParts; ++part) sum += squares(raw[part]);
+  } else {
+#pragma unroll 1
+    for (long long at = i; at < n && at < i + kNormChunk; at += kTurn) {
+      Raw<T> raw;
+      raw.template load<false>(g + at, n - at);
+      sum += squares(raw);
+    }
   }
   return sum;
 }

@@ -87,7 +87,7 @@ template <typename T>
 __device__ __forceinline__ const uint4* piece_at(const T* row, unsigned j) { return reinterpret_cast<const uint4*>(row + j); }
 
 template <typename T, int P, int G, bool EDGES>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) norm_kernel(const __grid_constant__ NormParams p) {
   constexpr int NT = G < 128 ? 128 : G, ROWS = NT / G, K = kPer<T>;
   __shared__ float s[2][G / 32];
   unsigned turn = 0;
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(const __grid_co
 // The gradient of the weight is added up over a block's rows, in registers where a thread has the same columns in every row, else in
 // shared memory (a word of padding a piece, so that neighbours meet no bank twice), and once more over the blocks by sum_parts_kernel.
 template <typename T, int P, int G, bool EDGES>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_grad_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) norm_grad_kernel(const __grid_constant__ NormParams p) {
   constexpr int NT = G < 128 ? 128 : G, ROWS = NT / G, K = kPer<T>, COLS = (P * G + (EDGES ? 1 : 0)) * K, PADDED = COLS / K * (K + 1);
   __shared__ float s[2][G / 32];
   extern __shared__ float s_dw[];               // [ROWS][PADDED]
@@ -416,8 +416,10 @@ static unsigned norm_blocks(const NormPlan& c, unsigned n, unsigned each) {
   const unsigned rows = (unsigned)(std::max(c.group, 128) / c.group);
   return std::min((n + rows - 1) / rows, each * (unsigned)plan_sm_count());
 }
-// Blocks of an SM in the gradient: fewer parts to add up than there could be blocks.
-static unsigned grad_blocks(const NormPlan& c, unsigned n) { return norm_blocks(c, n, c.group == 32 ? 8 : c.group == 128 ? 6 : 2); }
+// Blocks of an SM in the gradient: two turns of those that it has at a time, which evens out that not all memory is as near to every SM,
+// and few parts to add up.  (256 x 512 x 512 bf16, forward and backward with 8 and 5, 64 and 5, 64 and 10, 32 and 24 blocks an SM: 184, 206,
+// 175, 190 us.)
+static unsigned grad_blocks(const NormPlan& c, unsigned n) { return norm_blocks(c, n, c.group == 32 ? 10 : c.group == 128 ? 6 : 2); }
 static unsigned grad_parts(const NormPlan& c, unsigned n) { return grad_blocks(c, n) * (c.pieces ? 1 : (unsigned)(std::max(c.group, 128) / c.group)); }
 
 template <int P_, int G_>
@@ -462,7 +464,7 @@ static NormParams norm_params(const blstm_norm_desc& d, const void* x, const voi
 static int run_norm(const blstm_norm_desc& d, NormParams p, cudaStream_t st) {
   const bool alike = like_dense(d, p.x, d.x_stride) && like_dense(d, p.r, d.residual_stride) && aligned(16, p.y, p.h) && aligned(8, p.q);
   const NormPlan c = norm_plan(d.width, dtype_bytes(d.dtype), alike, whole_rows(d, p.w));
-  const unsigned grid = norm_blocks(c, p.n, c.group == 32 ? 16 : c.group == 128 ? 16 : 4);
+  const unsigned grid = norm_blocks(c, p.n, c.group == 32 ? 64 : c.group == 128 ? 16 : 4);
   return with_type(d.dtype, [&](auto t) -> int {
     using T = decltype(t);
     if (c.pieces == 0) {
