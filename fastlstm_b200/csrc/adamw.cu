@@ -156,13 +156,6 @@ __device__ __forceinline__ float sqrt_fast(float x) {      // to 2^-22
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// The same of what is 2^-126 at least; the root of anything less is 2^-63.
-__device__ __forceinline__ float sqrt_clamped(float x) {
-  float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(x, 0x1p-126f)));
-  return y;
-}
-
 // What a scale and its inverse are for a largest magnitude; magnitudes below 2^-110 are 0 (the inverse would not be a number of 32 bits).
 struct Scale {
   float up, down;
@@ -185,8 +178,8 @@ struct AdamStep {
   }
 
   // The same in 8 bits, by a warp with 256 elements: m8 and u8 are theirs and become the new ones, as do the scales.  Two floats an
-  // instruction (it is instructions that bound this).  Moments and scales are rounded operation by operation, so that they depend on the
-  // formula alone; only the roots of elements that are not their block's largest are the fast unit's (2^-22 of them).
+  // instruction (it is instructions that bound this).  Moments, roots and scales are rounded operation by operation, so that they depend on
+  // the formula alone: between small numbers a step of e4m3 is half of what it is taken from, and the next step's quotient goes by it.
   template <typename F>
   __device__ __forceinline__ void operator()(const float (&g)[8], uint2& m8, uint2& u8, float& m_scale, float& u_scale, float (&x)[8], F&& words) const {
     Pair m[4], v[4], u[4];
@@ -206,17 +199,9 @@ struct AdamStep {
       most_m = max_abs(max_abs(most_m, lo), hi);
       v[k].get(lo, hi);
       most_v = max_abs(max_abs(most_v, lo), hi);
-      u[k] = Pair::of(sqrt_clamped(lo), sqrt_clamped(hi));
+      u[k] = Pair::of(__fsqrt_rn(lo), __fsqrt_rn(hi));
     }
-    const float largest = warp_most(most_v), root = __fsqrt_rn(largest);
-    const Scale ms(warp_most(most_m)), us(root);
-    if (largest < 0x1p-56f)                     // (above it, what is below 2^-126 is 0 next to it)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float lo, hi;
-        v[k].get(lo, hi);
-        u[k] = Pair::of(__fsqrt_rn(lo), __fsqrt_rn(hi));
-      }
+    const Scale ms(warp_most(most_m)), us(__fsqrt_rn(warp_most(most_v)));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       float p, q;
@@ -232,11 +217,9 @@ struct AdamStep {
       words(h, w);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float y[2], z[2], q[2];
-        v[2 * h + k].get(q[0], q[1]);
-        u[2 * h + k].get(z[0], z[1]);
+        float y[2], z[2];
         (m[2 * h + k] * up_m * small).get(y[0], y[1]);
-        (Pair::of(q[0] == largest ? root : z[0], q[1] == largest ? root : z[1]) * up_u * small).get(z[0], z[1]);
+        (u[2 * h + k] * up_u * small).get(z[0], z[1]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int e = 2 * k + i;
@@ -249,7 +232,7 @@ struct AdamStep {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float lo, hi;
-          v[2 * h + k].get(lo, hi);
+          u[2 * h + k].get(lo, hi);
           if (lo > 0.f) cu[2 * k] = max(cu[2 * k], 1u << 20);
           if (hi > 0.f) cu[2 * k + 1] = max(cu[2 * k + 1], 1u << 20);
         }
@@ -402,7 +385,7 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 }
 
 template <typename T, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kAdamThreads, 2) adamw8_kernel(const __grid_constant__ AdamParams<CAP> p) {
+__global__ void __launch_bounds__(kAdamThreads, 3) adamw8_kernel(const __grid_constant__ AdamParams<CAP> p) {
   extern __shared__ uint4 s_raw[];
   using Stage = AdamStage<T, MASTER>;
   using X = std::conditional_t<MASTER, float, T>;
@@ -517,7 +500,7 @@ struct GradNormParams {
   float* out;                    // norm, factor; null before the last launch
   unsigned* ticket;
 };
-constexpr int kNormChunk = 4 * kTurn;
+constexpr int kNormChunk = 2 * kTurn;
 
 template <typename T>
 __device__ __forceinline__ float squares(const Raw<T>& raw) {
