@@ -39,7 +39,7 @@ struct AdamParams {
   unsigned items, chunks;
   unsigned long long wide[(CAP + 63) / 64];            // items whose addresses are multiples of 16
   unsigned keys[20];
-  float lr, beta1, beta2, one_less1, one_less2, eps, decay;
+  float lr, beta1, beta2, one_less1, one_less2, eps, decay, one;       // one: 1 (see AdamStep)
   double log_beta1, log_beta2;
   const float *lr_at, *factor;
   unsigned* ticket;
@@ -165,7 +165,7 @@ struct Scale {
 
 // What a step does to eight elements.
 struct AdamStep {
-  float factor, beta1, beta2, one_less1, one_less2, eps, decay, c1, c2;
+  float factor, beta1, beta2, one_less1, one_less2, eps, decay, one, c1, c2;
 
   __device__ __forceinline__ void operator()(const float (&g)[8], float (&m)[8], float (&v)[8], float (&x)[8]) const {
 #pragma unroll
@@ -188,12 +188,14 @@ struct AdamStep {
     decode8(u8, v);
     auto both = [](float a) { return Pair::of(a, a); };
     const Pair sm = both(m_scale), su = both(u_scale), f = both(factor), b1 = both(beta1), b2 = both(beta2), a1 = both(one_less1), a2 = both(one_less2);
-    const Pair minus = both(-1.f), rate = both(c1), fix = both(c2), e0 = both(eps), wd = both(decay);
+    // (a sum as a product with a 1 that the compiler does not know: it makes one rounding of a product and a sum, also of those that say how
+    // they round)
+    const Pair same = both(one), minus = both(-1.f), rate = both(c1), fix = both(c2), e0 = both(eps), wd = both(decay);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const Pair ge = Pair::of(g[2 * k], g[2 * k + 1]) * f, old = v[k] * su;
-      m[k] = b1 * (m[k] * sm) + a1 * ge;
-      v[k] = b2 * (old * old) + a2 * (ge * ge);
+      m[k] = fma2(b1 * (m[k] * sm), same, a1 * ge);
+      v[k] = fma2(b2 * (old * old), same, a2 * (ge * ge));
       float lo, hi;
       m[k].get(lo, hi);
       most_m = max_abs(max_abs(most_m, lo), hi);
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   const float factor = p.factor ? *p.factor : 1.f;
   if (factor != factor) return;                // gradients that are no numbers: everything stays as it is
   const float lr = p.lr_at ? *p.lr_at : p.lr;
-  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, 0.f, 0.f};
+  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, p.one, 0.f, 0.f};
   unsigned t = 0;
   int known = -1;
   for (Cursor<CAP> c; c.there(p); c.next()) {
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw8_kernel(const __grid_co
   const float factor = p.factor ? *p.factor : 1.f;
   if (factor != factor) return;
   const float lr = p.lr_at ? *p.lr_at : p.lr;
-  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, 0.f, 0.f};
+  AdamStep step{factor, p.beta1, p.beta2, p.one_less1, p.one_less2, p.eps, lr * p.decay, p.one, 0.f, 0.f};
   unsigned t = 0;
   int known = -1;
   // the fetching side: whole chunks alone
@@ -503,11 +505,12 @@ struct GradNormParams {
 constexpr int kNormChunk = 2 * kTurn;
 
 template <typename T>
-__device__ __forceinline__ float squares(const Raw<T>& raw) {
-  float z[8], t = 0.f;
+__device__ __forceinline__ double squares(const Raw<T>& raw) {
+  float z[8];
+  double t = 0;
   raw.get(z);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) t = fmaf(z[e], z[e], t);
+  for (int e = 0; e < 8; ++e) t = fma((double)z[e], (double)z[e], t);
   return t;
 }
 template <typename T>
@@ -531,7 +534,7 @@ __device__ __forceinline__ double chunk_squares(const T* g, long long i, long lo
   return sum;
 }
 
-// Squares of eight neighbours are added up in 32 bits, what they come to in 64.
+// In 64 bits throughout: the factor is the same whatever the order, but for one rounding to 32 bits.
 template <int CAP>
 __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_constant__ GradNormParams<CAP> p) {
   __shared__ double s[kAdamThreads / 32];
@@ -608,6 +611,7 @@ static int launch_adamw(const blstm_adamw_desc& d, const blstm_adamw_item* items
   p.lr = (float)d.lr; p.beta1 = (float)d.beta1; p.beta2 = (float)d.beta2;
   p.one_less1 = (float)(1 - d.beta1); p.one_less2 = (float)(1 - d.beta2);
   p.eps = (float)d.eps; p.decay = (float)d.weight_decay;
+  p.one = 1.f;
   p.log_beta1 = std::log(d.beta1); p.log_beta2 = std::log(d.beta2);
   p.lr_at = d.lr_at; p.factor = d.factor; p.ticket = d.ticket;
   if constexpr (BITS == 32) {

@@ -386,7 +386,7 @@ typedef struct blstm_grad_norm_desc {
   size_t workspace_bytes;
 } blstm_grad_norm_desc;
 
-/* The 2-norm over all elements of all tensors, in an order that the sizes fix. */
+/* The 2-norm over all elements of all tensors, added up in 64 bits in an order that the sizes fix. */
 size_t blstm_grad_norm_workspace(int items);
 int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream);
 
