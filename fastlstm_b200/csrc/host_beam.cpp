@@ -119,10 +119,10 @@ std::vector<Tensor> reorder_flat(const std::vector<Tensor>& states, const Tensor
     out.push_back(fresh(sizes, t.scalar_type(), t));
     if (out.back().numel() == 0) continue;
     const int64_t outer = c10::multiply_integers(t.sizes().slice(0, dim)), inner = c10::multiply_integers(t.sizes().slice(dim + 1));
-    Tensor v = t;
+    Tensor v = t.resolve_conj().resolve_neg();
     int64_t outer_stride;
     if (!in_pieces(v, dim, outer_stride)) {
-      v = t.contiguous();
+      v = v.contiguous();
       in_pieces(v, dim, outer_stride);
     }
     held.push_back(v);

@@ -258,6 +258,9 @@ def test_reorder_layouts_and_nests():
     Pair = namedtuple("Pair", "h c")
     pair = F.reorder_states([Pair(views[0], None)], parents)[0]
     assert type(pair) is Pair and torch.equal(pair.h, got[0][0]) and pair.c is None
+    z = torch.view_as_complex(make_state(2, B * n, 8, 2))
+    for lazy in (z.conj(), z.conj().imag):               # (numbers whose signs are still to be turned)
+        assert torch.equal(F.reorder_states(lazy, parents), lazy[:, rows])
     many = [make_state(1 + k % 3, B * n, 1 + k % 5) for k in range(100)]
     for a, b in zip(F.reorder_states(many, parents.t().contiguous().t()), many):
         assert torch.equal(a, b[:, rows])
