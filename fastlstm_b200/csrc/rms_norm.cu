@@ -21,6 +21,7 @@ struct NormParams {
   uint8_t* q;
   float *scales, *rstd, *dw;     // dw: the blocks' parts [parts][width], or the result where one block has all rows
   unsigned n, width, parts;
+  bool x_alike, r_alike, dy_alike;       // rows on the same addresses modulo 16 as those of the results
   float eps, per_width;
 };
 
@@ -67,13 +68,15 @@ __device__ __forceinline__ float over_row(float v, float (*s)[G / 32], unsigned&
   return v;
 }
 
-// What a thread has of a row of `width` elements that G threads share in 16-byte pieces: up to P of them, and where rows do not begin
-// on a boundary (EDGES) one of the elements in front of the first piece and behind the last.  The threads' pieces are neighbours.
+// What a thread has of a row of `width` elements that G threads share in 16-byte pieces of the results: up to P of them, and where rows
+// do not begin on a boundary (EDGES) one of the elements in front of the first piece and behind the last.  The threads' pieces are
+// neighbours.  A group's rows are a multiple of eight apart, so all of them begin alike: what belongs to columns stays in registers.
 template <typename T, int G, bool EDGES>
 struct Cut {
   unsigned head, pieces, edges, at;
-  __device__ __forceinline__ Cut(const T* row, unsigned width) : at(threadIdx.x % G) {
-    head = EDGES ? min(width, (unsigned)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (unsigned)sizeof(T)) : 0;
+  __device__ __forceinline__ Cut(unsigned row, unsigned width) : at(threadIdx.x % G) {
+    const unsigned off = (unsigned)((size_t)row * width % kPer<T>);      // of results that begin on a boundary
+    head = EDGES ? min(width, (kPer<T> - off) % kPer<T>) : 0;
     pieces = (width - head) / kPer<T>;
     edges = EDGES ? width - pieces * kPer<T> : 0;
   }
@@ -83,8 +86,28 @@ struct Cut {
   __device__ __forceinline__ unsigned edge() const { return at < head ? at : at + pieces * kPer<T>; }
 };
 
+// A piece from anywhere: in one load where it lies on a boundary, else in narrow ones.
 template <typename T>
-__device__ __forceinline__ const uint4* piece_at(const T* row, unsigned j) { return reinterpret_cast<const uint4*>(row + j); }
+__device__ __forceinline__ uint4 load_piece(const T* p, bool whole) {
+  if (whole) return load_stream(reinterpret_cast<const uint4*>(p));
+  uint4 v;
+  if (sizeof(T) == 4 || (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+    const unsigned* w = reinterpret_cast<const unsigned*>(p);
+    v = make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+  } else {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    unsigned w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __ldg(h + 2 * k) | (unsigned)__ldg(h + 2 * k + 1) << 16;
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+template <typename T, int P, typename C>
+__device__ __forceinline__ void load_row(uint4 (&v)[P], const T* row, const C& c, bool whole) {
+#pragma unroll
+  for (int u = 0; u < P; ++u) v[u] = c.has(u) ? load_piece(row + c.first(u), whole) : make_uint4(0, 0, 0, 0);
+}
 
 template <typename T, int P, int G, bool EDGES>
 __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) norm_kernel(const __grid_constant__ NormParams p) {
@@ -92,26 +115,22 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) 
   __shared__ float s[2][G / 32];
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
+  unsigned row = blockIdx.x * ROWS + threadIdx.x / G;
+  const Cut<T, G, EDGES> c(row, p.width);
   uint4 weight[P];
-  if constexpr (!EDGES) {
-    const Cut<T, G, EDGES> c(w, p.width);
-#pragma unroll
-    for (int u = 0; u < P; ++u) weight[u] = c.has(u) ? *piece_at(w, c.first(u)) : make_uint4(0, 0, 0, 0);
-  }
-  for (unsigned row = blockIdx.x * ROWS + threadIdx.x / G; row < p.n; row += gridDim.x * ROWS) {
+  load_row(weight, w, c, !EDGES);
+  const float edge_weight = c.has_edge() ? ld_f(w + c.edge()) : 0.f;
+  for (; row < p.n; row += gridDim.x * ROWS) {
     const T* x = static_cast<const T*>(p.x) + p.x_map(row);
-    const Cut<T, G, EDGES> c(x, p.width);
     uint4 v[P];
     float edge = 0.f, sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < P; ++u) v[u] = c.has(u) ? load_stream(piece_at(x, c.first(u))) : make_uint4(0, 0, 0, 0);
+    load_row(v, x, c, p.x_alike);
     if (c.has_edge()) edge = ld_f(x + c.edge());
     if (p.r) {
       const T* r = static_cast<const T*>(p.r) + p.r_map(row);
       T* h = static_cast<T*>(p.h) + (size_t)row * p.width;
       uint4 b[P];
-#pragma unroll
-      for (int u = 0; u < P; ++u) b[u] = c.has(u) ? load_stream(piece_at(r, c.first(u))) : make_uint4(0, 0, 0, 0);
+      load_row(b, r, c, p.r_alike);
       if (c.has_edge()) {
         const T e = Elem<T>::from_f(edge + ld_f(r + c.edge()));
         h[c.edge()] = e;
@@ -139,18 +158,13 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) 
     const float i = rsqrtf(fmaf(sum, p.per_width, p.eps));
     if (p.rstd && c.at == 0) p.rstd[row] = i;
     auto normed = [&](int u, float (&z)[K]) {
-      unpack(v[u], z, T{});
       float o[K];
-      if constexpr (EDGES) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) o[k] = c.has(u) ? ld_f(w + c.first(u) + k) : 0.f;
-      } else {
-        unpack(weight[u], o, T{});
-      }
+      unpack(v[u], z, T{});
+      unpack(weight[u], o, T{});
 #pragma unroll
       for (int k = 0; k < K; ++k) z[k] = z[k] * i * o[k];
     };
-    if (c.has_edge()) edge = edge * i * ld_f(w + c.edge());
+    edge = edge * i * edge_weight;
     if (p.q) {
       float most = fabsf(edge);
 #pragma unroll
@@ -189,8 +203,8 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) 
   }
 }
 
-// The gradient of the weight is added up over a block's rows, in registers where a thread has the same columns in every row, else in
-// shared memory (a word of padding a piece, so that neighbours meet no bank twice), and once more over the blocks by sum_parts_kernel.
+// The gradient of the weight is added up over a group's rows in registers, over a block's groups in shared memory (a word of padding a
+// piece, so that neighbours meet no bank twice), and over the blocks by sum_parts_kernel.
 template <typename T, int P, int G, bool EDGES>
 __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) norm_grad_kernel(const __grid_constant__ NormParams p) {
   constexpr int NT = G < 128 ? 128 : G, ROWS = NT / G, K = kPer<T>, COLS = (P * G + (EDGES ? 1 : 0)) * K, PADDED = COLS / K * (K + 1);
@@ -198,34 +212,28 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
   extern __shared__ float s_dw[];               // [ROWS][PADDED]
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
+  unsigned row = blockIdx.x * ROWS + threadIdx.x / G;
+  const Cut<T, G, EDGES> c(row, p.width);
   uint4 weight[P];
-  float acc[EDGES ? 1 : P * K];
-  auto cell = [&](unsigned j) -> float& { return s_dw[threadIdx.x / G * PADDED + j + j / K]; };
-  if constexpr (!EDGES) {
-    const Cut<T, G, EDGES> c(w, p.width);
+  load_row(weight, w, c, !EDGES);
+  const float edge_weight = c.has_edge() ? ld_f(w + c.edge()) : 0.f;
+  float acc[P * K], edge_acc = 0.f;
 #pragma unroll
-    for (int u = 0; u < P; ++u) weight[u] = c.has(u) ? *piece_at(w, c.first(u)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int k = 0; k < P * K; ++k) acc[k] = 0.f;
-  } else {
-    for (unsigned j = threadIdx.x; j < ROWS * PADDED; j += NT) s_dw[j] = 0.f;
-    __syncthreads();
-  }
-  for (unsigned row = blockIdx.x * ROWS + threadIdx.x / G; row < p.n; row += gridDim.x * ROWS) {
+  for (int k = 0; k < P * K; ++k) acc[k] = 0.f;
+  for (; row < p.n; row += gridDim.x * ROWS) {
     const T *h = static_cast<const T*>(p.x) + p.x_map(row), *dy = static_cast<const T*>(p.dy) + p.dy_map(row);
-    const Cut<T, G, EDGES> c(h, p.width);
     uint4 v[P], g[P], b[P];
-#pragma unroll
-    for (int u = 0; u < P; ++u) {
-      v[u] = c.has(u) ? load_stream(piece_at(h, c.first(u))) : make_uint4(0, 0, 0, 0);
-      g[u] = c.has(u) ? load_stream(piece_at(dy, c.first(u))) : make_uint4(0, 0, 0, 0);
-    }
+    load_row(v, h, c, p.x_alike);
+    load_row(g, dy, c, p.dy_alike);
     const float i = p.rstd[row];
-    float h_edge = 0.f, n_edge = 0.f, b_edge = 0.f;
+    float h_edge = 0.f, g_edge = 0.f, b_edge = 0.f;
+    if (c.has_edge()) {
+      h_edge = ld_f(h + c.edge());
+      g_edge = ld_f(dy + c.edge());
+    }
     if (p.r) {
       const T* r = static_cast<const T*>(p.r) + p.r_map(row);
-#pragma unroll
-      for (int u = 0; u < P; ++u) b[u] = c.has(u) ? load_stream(piece_at(r, c.first(u))) : make_uint4(0, 0, 0, 0);
+      load_row(b, r, c, p.r_alike);
       if (c.has_edge()) b_edge = ld_f(r + c.edge());
     } else {
 #pragma unroll
@@ -234,23 +242,13 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
     auto weighed = [&](int u, float (&n)[K]) {         // dy w
       float o[K];
       unpack(g[u], n, T{});
-      if constexpr (EDGES) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) o[k] = c.has(u) ? ld_f(w + c.first(u) + k) : 0.f;
-      } else {
-        unpack(weight[u], o, T{});
-      }
+      unpack(weight[u], o, T{});
 #pragma unroll
       for (int k = 0; k < K; ++k) n[k] *= o[k];
     };
-    float sum = 0.f;
-    if (c.has_edge()) {
-      const float e = ld_f(dy + c.edge());
-      h_edge = ld_f(h + c.edge());
-      if constexpr (EDGES) cell(c.edge()) += e * (h_edge * i);
-      n_edge = e * ld_f(w + c.edge());
-      sum = n_edge * h_edge;
-    }
+    edge_acc = fmaf(g_edge, h_edge * i, edge_acc);
+    const float n_edge = g_edge * edge_weight;
+    float sum = n_edge * h_edge;
 #pragma unroll
     for (int u = 0; u < P; ++u) {
       float n[K], z[K], e[K];
@@ -260,13 +258,10 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         sum = fmaf(n[k], z[k], sum);
-        const float d = z[k] * i;
-        if constexpr (!EDGES) acc[u * K + k] = fmaf(e[k], d, acc[u * K + k]);
-        else if (c.has(u)) cell(c.first(u) + k) += e[k] * d;
+        acc[u * K + k] = fmaf(e[k], z[k] * i, acc[u * K + k]);
       }
     }
     sum = over_row<G>(sum, s, turn, Add());
-    if constexpr (EDGES) __syncwarp();          // (a column's cell has another thread in the next row)
     const float by = sum * p.per_width * i * i;
     T* dx = static_cast<T*>(p.y) + (size_t)row * p.width;
 #pragma unroll
@@ -282,14 +277,13 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
     if (c.has_edge()) dx[c.edge()] = Elem<T>::from_f(fmaf(i, fmaf(-h_edge, by, n_edge), b_edge));
   }
   if (!p.dw) return;
-  if constexpr (!EDGES) {
-    const Cut<T, G, EDGES> c(w, p.width);
+  auto cell = [&](unsigned j) -> float& { return s_dw[threadIdx.x / G * PADDED + j + j / K]; };
 #pragma unroll
-    for (int u = 0; u < P; ++u)
-      if (c.has(u))
+  for (int u = 0; u < P; ++u)
+    if (c.has(u))
 #pragma unroll
-        for (int k = 0; k < K; ++k) cell(c.first(u) + k) = acc[u * K + k];
-  }
+      for (int k = 0; k < K; ++k) cell(c.first(u) + k) = acc[u * K + k];
+  if (c.has_edge()) cell(c.edge()) = edge_acc;
   __syncthreads();
   for (unsigned j = threadIdx.x; j < p.width; j += NT) {
     float t = s_dw[j + j / K];
@@ -402,11 +396,11 @@ struct NormPlan {
   bool edges;
 };
 
-// Rows stay in registers up to 512 threads with two pieces each where every tensor's rows begin on the same address modulo 16.
-static NormPlan norm_plan(int64_t width, int element, bool alike, bool whole) {
+// Rows stay in registers up to 512 threads with two pieces each, where the results begin on boundaries (`whole`: all of their rows do).
+static NormPlan norm_plan(int64_t width, int element, bool results, bool whole) {
   const int64_t pieces = width / (16 / element);
   NormPlan c{width <= 1024 ? 32 : 512, 0, false};
-  if (!alike || pieces == 0 || pieces > 1024) return c;
+  if (!results || pieces == 0 || pieces > 1024) return c;
   c.edges = !whole;
   c.group = pieces <= 128 ? 32 : pieces <= 512 ? 128 : 512;
   c.pieces = c.group == 32 ? (pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4) : c.group == 128 ? (pieces <= 256 ? 2 : 4) : 2;
@@ -414,7 +408,7 @@ static NormPlan norm_plan(int64_t width, int element, bool alike, bool whole) {
 }
 static unsigned norm_blocks(const NormPlan& c, unsigned n, unsigned each) {
   const unsigned rows = (unsigned)(std::max(c.group, 128) / c.group);
-  return std::min((n + rows - 1) / rows, each * (unsigned)plan_sm_count());
+  return std::min((n + rows - 1) / rows, each * (unsigned)plan_sm_count() / 8 * 8);      // (a group with several rows has them multiples of eight apart)
 }
 // Blocks of an SM in the gradient: two turns of those that it has at a time, which evens out that not all memory is as near to every SM,
 // and few parts to add up.  (256 x 512 x 512 bf16, forward and backward with 8 and 5, 64 and 5, 64 and 10, 32 and 24 blocks an SM: 184, 206,
@@ -462,8 +456,9 @@ static NormParams norm_params(const blstm_norm_desc& d, const void* x, const voi
 }
 
 static int run_norm(const blstm_norm_desc& d, NormParams p, cudaStream_t st) {
-  const bool alike = like_dense(d, p.x, d.x_stride) && like_dense(d, p.r, d.residual_stride) && aligned(16, p.y, p.h) && aligned(8, p.q);
-  const NormPlan c = norm_plan(d.width, dtype_bytes(d.dtype), alike, whole_rows(d, p.w));
+  p.x_alike = like_dense(d, p.x, d.x_stride);
+  p.r_alike = like_dense(d, p.r, d.residual_stride);
+  const NormPlan c = norm_plan(d.width, dtype_bytes(d.dtype), aligned(16, p.y, p.h) && aligned(8, p.q), whole_rows(d, p.w));
   const unsigned grid = norm_blocks(c, p.n, c.group == 32 ? 64 : c.group == 128 ? 16 : 4);
   return with_type(d.dtype, [&](auto t) -> int {
     using T = decltype(t);
@@ -511,12 +506,12 @@ int blstm_rms_norm_e4m3(const blstm_norm_desc* d, const void* x, const void* res
   return run_norm(*d, p, (cudaStream_t)stream);
 }
 
-// (the workspace of whichever cut has the more parts: pointers decide which one runs)
+// (the workspace of whichever cut has the more parts: where dx lies decides which one runs)
 size_t blstm_rms_norm_grad_workspace(const blstm_norm_desc* d) {
   if (check_norm(d, reinterpret_cast<const void*>(16), reinterpret_cast<const void*>(16)) || d->n0 == 0 || d->n1 == 0) return 0;
   const unsigned n = (unsigned)(d->n0 * d->n1);
   unsigned parts = 1;
-  for (const bool alike : {false, true}) parts = std::max(parts, grad_parts(norm_plan(d->width, dtype_bytes(d->dtype), alike, true), n));
+  for (const bool results : {false, true}) parts = std::max(parts, grad_parts(norm_plan(d->width, dtype_bytes(d->dtype), results, true), n));
   return round_up((size_t)parts * d->width * 4, 256);
 }
 
@@ -535,8 +530,10 @@ int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* ds
   NormParams p = norm_params(*d, h, dsum, weight);
   p.dy = dy; p.y = dx;
   p.rstd = const_cast<float*>(rstd);
-  const bool alike = like_dense(*d, h, d->x_stride) && like_dense(*d, dsum, d->residual_stride) && like_dense(*d, dy, d->dy_stride) && aligned(16, dx);
-  const NormPlan c = norm_plan(d->width, (int)e, alike, whole_rows(*d, weight));
+  p.x_alike = like_dense(*d, h, d->x_stride);
+  p.r_alike = like_dense(*d, dsum, d->residual_stride);
+  p.dy_alike = like_dense(*d, dy, d->dy_stride);
+  const NormPlan c = norm_plan(d->width, (int)e, aligned(16, dx), whole_rows(*d, weight));
   const unsigned grid = grad_blocks(c, p.n);
   p.parts = grad_parts(c, p.n);
   return with_type(d->dtype, [&](auto t) -> int {
