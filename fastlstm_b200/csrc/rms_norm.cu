@@ -52,10 +52,12 @@ struct AbsMax {
 
 // A value over the G threads of a row, in each of them.  Groups of more than a warp are whole blocks; `s` has two sets of words that
 // successive calls take in turn, so that one barrier a call does.
+template <int G> constexpr int kWarps = G < 32 ? 1 : G / 32;
 template <int G, typename F>
-__device__ __forceinline__ float over_row(float v, float (*s)[G / 32], unsigned& turn, F f) {
+__device__ __forceinline__ float over_row(float v, float (*s)[kWarps<G>], unsigned& turn, F f) {
+  const unsigned group = G < 32 ? ((1u << (G & 31)) - 1) << (threadIdx.x & 31 & ~(G - 1)) : ~0u;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(~0u, v, o));
+  for (int o = G < 32 ? G / 2 : 16; o; o >>= 1) v = f(v, __shfl_xor_sync(group, v, o));
   if constexpr (G > 32) {
     float* w = s[turn & 1];
     ++turn;
@@ -110,9 +112,9 @@ __device__ __forceinline__ void load_row(uint4 (&v)[P], const T* row, const C& c
 }
 
 template <typename T, int P, int G, bool EDGES>
-__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 ? (P <= 2 ? 8 : 1) : G == 128 ? (P <= 2 ? 8 : 5) : 1) norm_kernel(const __grid_constant__ NormParams p) {
   constexpr int NT = G < 128 ? 128 : G, ROWS = NT / G, K = kPer<T>;
-  __shared__ float s[2][G / 32];
+  __shared__ float s[2][kWarps<G>];
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
   unsigned row = blockIdx.x * ROWS + threadIdx.x / G;
@@ -124,13 +126,13 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) 
     const T* x = static_cast<const T*>(p.x) + p.x_map(row);
     uint4 v[P];
     float edge = 0.f, sum = 0.f;
-    load_row(v, x, c, p.x_alike);
+    load_row(v, x, c, !EDGES || p.x_alike);
     if (c.has_edge()) edge = ld_f(x + c.edge());
     if (p.r) {
       const T* r = static_cast<const T*>(p.r) + p.r_map(row);
       T* h = static_cast<T*>(p.h) + (size_t)row * p.width;
       uint4 b[P];
-      load_row(b, r, c, p.r_alike);
+      load_row(b, r, c, !EDGES || p.r_alike);
       if (c.has_edge()) {
         const T e = Elem<T>::from_f(edge + ld_f(r + c.edge()));
         h[c.edge()] = e;
@@ -206,9 +208,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 8 : 1) 
 // The gradient of the weight is added up over a group's rows in registers, over a block's groups in shared memory (a word of padding a
 // piece, so that neighbours meet no bank twice), and over the blocks by sum_parts_kernel.
 template <typename T, int P, int G, bool EDGES>
-__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) norm_grad_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 ? (P <= 2 ? 5 : 1) : G == 128 ? (P <= 2 ? 5 : 3) : 1) norm_grad_kernel(const __grid_constant__ NormParams p) {
   constexpr int NT = G < 128 ? 128 : G, ROWS = NT / G, K = kPer<T>, COLS = (P * G + (EDGES ? 1 : 0)) * K, PADDED = COLS / K * (K + 1);
-  __shared__ float s[2][G / 32];
+  __shared__ float s[2][kWarps<G>];
   extern __shared__ float s_dw[];               // [ROWS][PADDED]
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
@@ -223,8 +225,8 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
   for (; row < p.n; row += gridDim.x * ROWS) {
     const T *h = static_cast<const T*>(p.x) + p.x_map(row), *dy = static_cast<const T*>(p.dy) + p.dy_map(row);
     uint4 v[P], g[P], b[P];
-    load_row(v, h, c, p.x_alike);
-    load_row(g, dy, c, p.dy_alike);
+    load_row(v, h, c, !EDGES || p.x_alike);
+    load_row(g, dy, c, !EDGES || p.dy_alike);
     const float i = p.rstd[row];
     float h_edge = 0.f, g_edge = 0.f, b_edge = 0.f;
     if (c.has_edge()) {
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
     }
     if (p.r) {
       const T* r = static_cast<const T*>(p.r) + p.r_map(row);
-      load_row(b, r, c, p.r_alike);
+      load_row(b, r, c, !EDGES || p.r_alike);
       if (c.has_edge()) b_edge = ld_f(r + c.edge());
     } else {
 #pragma unroll
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 && P <= 2 ? 5 : 1) 
 template <typename T, int G>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_any_kernel(const __grid_constant__ NormParams p) {
   constexpr int ROWS = (G < 128 ? 128 : G) / G;
-  __shared__ float s[2][G / 32];
+  __shared__ float s[2][kWarps<G>];
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
   const unsigned at = threadIdx.x % G;
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_any_kernel(const __gri
 template <typename T, int G>
 __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_any_grad_kernel(const __grid_constant__ NormParams p) {
   constexpr int ROWS = (G < 128 ? 128 : G) / G;
-  __shared__ float s[2][G / 32];
+  __shared__ float s[2][kWarps<G>];
   unsigned turn = 0;
   const T* w = static_cast<const T*>(p.w);
   const unsigned at = threadIdx.x % G, group = blockIdx.x * ROWS + threadIdx.x / G;
@@ -396,14 +398,14 @@ struct NormPlan {
   bool edges;
 };
 
-// Rows stay in registers up to 512 threads with two pieces each, where the results begin on boundaries (`whole`: all of their rows do).
+// Rows stay in registers up to 512 threads with two pieces each, where the results begin on boundaries (`whole`: all rows of everything do).
 static NormPlan norm_plan(int64_t width, int element, bool results, bool whole) {
   const int64_t pieces = width / (16 / element);
   NormPlan c{width <= 1024 ? 32 : 512, 0, false};
   if (!results || pieces == 0 || pieces > 1024) return c;
   c.edges = !whole;
-  c.group = pieces <= 128 ? 32 : pieces <= 512 ? 128 : 512;
-  c.pieces = c.group == 32 ? (pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4) : c.group == 128 ? (pieces <= 256 ? 2 : 4) : 2;
+  c.group = pieces <= 16 ? 16 : pieces <= 128 ? 32 : pieces <= 512 ? 128 : 512;
+  c.pieces = c.group == 16 ? 1 : c.group == 32 ? (pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4) : c.group == 128 ? (pieces <= 256 ? 2 : 4) : 2;
   return c;
 }
 static unsigned norm_blocks(const NormPlan& c, unsigned n, unsigned each) {
@@ -413,7 +415,7 @@ static unsigned norm_blocks(const NormPlan& c, unsigned n, unsigned each) {
 // Blocks of an SM in the gradient: two turns of those that it has at a time, which evens out that not all memory is as near to every SM,
 // and few parts to add up.  (256 x 512 x 512 bf16, forward and backward with 8 and 5, 64 and 5, 64 and 10, 32 and 24 blocks an SM: 184, 206,
 // 175, 190 us.)
-static unsigned grad_blocks(const NormPlan& c, unsigned n) { return norm_blocks(c, n, c.group == 32 ? 10 : c.group == 128 ? 6 : 2); }
+static unsigned grad_blocks(const NormPlan& c, unsigned n) { return norm_blocks(c, n, c.group <= 128 ? 10 : 2); }
 static unsigned grad_parts(const NormPlan& c, unsigned n) { return grad_blocks(c, n) * (c.pieces ? 1 : (unsigned)(std::max(c.group, 128) / c.group)); }
 
 template <int P_, int G_>
@@ -423,6 +425,7 @@ struct NormCut {
 // f(NormCut<pieces, group>) of a plan.
 template <typename F>
 static int with_cut(const NormPlan& c, F&& f) {
+  if (c.group == 16) return f(NormCut<1, 16>());
   if (c.group == 32) return c.pieces == 1 ? f(NormCut<1, 32>()) : c.pieces == 2 ? f(NormCut<2, 32>()) : f(NormCut<4, 32>());
   if (c.group == 128) return c.pieces == 2 ? f(NormCut<2, 128>()) : f(NormCut<4, 128>());
   return f(NormCut<2, 512>());
@@ -458,8 +461,8 @@ static NormParams norm_params(const blstm_norm_desc& d, const void* x, const voi
 static int run_norm(const blstm_norm_desc& d, NormParams p, cudaStream_t st) {
   p.x_alike = like_dense(d, p.x, d.x_stride);
   p.r_alike = like_dense(d, p.r, d.residual_stride);
-  const NormPlan c = norm_plan(d.width, dtype_bytes(d.dtype), aligned(16, p.y, p.h) && aligned(8, p.q), whole_rows(d, p.w));
-  const unsigned grid = norm_blocks(c, p.n, c.group == 32 ? 64 : c.group == 128 ? 16 : 4);
+  const NormPlan c = norm_plan(d.width, dtype_bytes(d.dtype), aligned(16, p.y, p.h) && aligned(8, p.q), whole_rows(d, p.w) && p.x_alike && p.r_alike);
+  const unsigned grid = norm_blocks(c, p.n, c.group <= 128 ? 64 : 4);
   return with_type(d.dtype, [&](auto t) -> int {
     using T = decltype(t);
     if (c.pieces == 0) {
@@ -533,7 +536,7 @@ int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* ds
   p.x_alike = like_dense(*d, h, d->x_stride);
   p.r_alike = like_dense(*d, dsum, d->residual_stride);
   p.dy_alike = like_dense(*d, dy, d->dy_stride);
-  const NormPlan c = norm_plan(d->width, (int)e, aligned(16, dx), whole_rows(*d, weight));
+  const NormPlan c = norm_plan(d->width, (int)e, aligned(16, dx), whole_rows(*d, weight) && p.x_alike && p.r_alike && p.dy_alike);
   const unsigned grid = grad_blocks(c, p.n);
   p.parts = grad_parts(c, p.n);
   return with_type(d->dtype, [&](auto t) -> int {
