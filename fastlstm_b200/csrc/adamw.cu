@@ -156,6 +156,17 @@ __device__ __forceinline__ float sqrt_fast(float x) {      // to 2^-22
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two square roots by a step of Newton's iteration from v r, r the fast unit's 1 / sqrt(v) to 2^-22: the residual v - u^2 is exact in a
+// fused product, so what is left is the last rounding, and 2^-44.  0 is 0; below 2^-126 (where r is held) it is no root.
+__device__ __forceinline__ Pair roots(Pair v, Pair half) {
+  float lo, hi, a, b;
+  v.get(lo, hi);
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi));
+  const Pair r = Pair::of(fminf(a, 0x1p63f), fminf(b, 0x1p63f)), u = v * r;
+  return fma2(fma2(u * Pair::of(-1.f, -1.f), u, v), r * half, u);
+}
+
 // What a scale and its inverse are for a largest magnitude; magnitudes below 2^-110 are 0 (the inverse would not be a number of 32 bits).
 struct Scale {
   float up, down;
@@ -201,9 +212,17 @@ struct AdamStep {
       most_m = max_abs(max_abs(most_m, lo), hi);
       v[k].get(lo, hi);
       most_v = max_abs(max_abs(most_v, lo), hi);
-      u[k] = Pair::of(__fsqrt_rn(lo), __fsqrt_rn(hi));
+      u[k] = roots(v[k], both(0.5f));
     }
-    const Scale ms(warp_most(most_m)), us(__fsqrt_rn(warp_most(most_v)));
+    const float largest = warp_most(most_v);
+    if (largest < 0x1p-56f)                     // (above it, what has a square below 2^-126 is nothing next to the scale)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float lo, hi;
+        v[k].get(lo, hi);
+        u[k] = Pair::of(__fsqrt_rn(lo), __fsqrt_rn(hi));
+      }
+    const Scale ms(warp_most(most_m)), us(__fsqrt_rn(largest));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       float p, q;
