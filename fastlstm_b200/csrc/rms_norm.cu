@@ -372,22 +372,28 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_any_grad_kernel(const 
   }
 }
 
-// dw = the sum of the parts, 32 columns a block.
+// dw = the sum of the parts, 32 columns a block, sixteen rows of them on their way to each of its warps (1480 parts of 512 columns with half the
+// warps and eight rows 12.8 us, so 9; caches cold).
+constexpr int kSumWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(512) sum_parts_kernel(const float* parts, T* dw, unsigned n, unsigned width) {
-  __shared__ float s[16][33];
+__global__ void __launch_bounds__(32 * kSumWarps) sum_parts_kernel(const float* parts, T* dw, unsigned n, unsigned width) {
+  __shared__ float s[kSumWarps][33];
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
   float t = 0.f;
-  if (j < width)
-#pragma unroll 8
-    for (unsigned k = warp; k < n; k += 16) t += parts[(size_t)k * width + j];
+  for (unsigned k0 = warp; k0 < n; k0 += 16 * kSumWarps) {
+    float z[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) z[k] = j < width && k0 + k * kSumWarps < n ? __ldg(parts + (size_t)(k0 + k * kSumWarps) * width + j) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += z[k];
+  }
   s[warp][lane] = t;
   __syncthreads();
-  if (warp == 0 && j < width) {
+  // a warp has a column, whose parts its lanes hold
+  t = s[lane][warp];
 #pragma unroll
-    for (int k = 1; k < 16; ++k) t += s[k][lane];
-    dw[j] = Elem<T>::from_f(t);
-  }
+  for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < width) dw[blockIdx.x * 32 + warp] = Elem<T>::from_f(t);
 }
 
 // ---------------------------------------------------------------- host
@@ -559,7 +565,7 @@ int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* ds
     BLSTM_CUDA_OK(cudaGetLastError());
     count_launch();
     if (dweight && (p.parts > 1 || c.pieces == 0)) {
-      sum_parts_kernel<T><<<(p.width + 31) / 32, 512, 0, st>>>(static_cast<const float*>(workspace), static_cast<T*>(dweight), p.parts, p.width);
+      sum_parts_kernel<T><<<(p.width + 31) / 32, 32 * kSumWarps, 0, st>>>(static_cast<const float*>(workspace), static_cast<T*>(dweight), p.parts, p.width);
       BLSTM_CUDA_OK(cudaGetLastError());
       count_launch();
     }
