@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   const unsigned count = s.count;
   auto put = [&](unsigned place, unsigned k, unsigned token, double total) {
     const size_t at = (size_t)b * p.width + place;
-    const bool ended = s.kind[k] == 1 || (s.kind[k] == 2 && p.finished && p.finished[r0 + k]);
+    const bool ended = s.kind[k] == 1;
     p.out_scores[at] = (float)total;
     p.parents[at] = k;
     p.tokens[at] = token;

@@ -130,6 +130,35 @@ def test_ties(V, kind):
     assert check(logits, spread, 9)[1]
 
 
+@pytest.mark.parametrize("V", [40, 3001, 40000])
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e30, torch.finfo(torch.float32).min])
+def test_scores_that_stand_for_dead_hypotheses(V, low):
+    """First steps with one hypothesis of score 0 and others that are out by their scores; sentences of nothing but those, whose totals may
+    all be one number: the first hypothesis, the first tokens."""
+    g = gen(V)
+    logits, scores = make(g, 4, 5, V)
+    scores[0], scores[1], scores[2, 1:] = low, low, low
+    scores[0, 3] = 0
+    r, _ = check(logits, scores)
+    assert (r.parents[0] == 3).all() and (r.parents[2] == 0).all()
+    if low <= -1e30:
+        assert (r.parents[1] == 0).all() and r.tokens[1].tolist() == list(range(5))
+    lengths = torch.randint(1, 9, (4, 5), generator=g, device="cuda")
+    if low > -1e30:
+        check(logits, scores, 7, 1, None, lengths, 0.7)
+
+
+@pytest.mark.parametrize("scale", [1e3, 1e6])
+def test_scores_of_any_size_and_sign(scale):
+    """Scores that cancel against what the logits come to."""
+    g = gen(9)
+    logits, scores = make(g, 3, 6, 9001, "fp32")
+    logits[1] *= 40
+    scores = torch.randn(3, 6, generator=g, device="cuda") * scale
+    check(logits, scores)
+    check(logits, scores - scores.amax(1, keepdim=True) + logits.amax(-1), 4)
+
+
 @pytest.mark.parametrize("V", [100, 2000, 20000])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_not_a_number_and_infinity_come_first(V, bad):
