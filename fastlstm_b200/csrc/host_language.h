@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 
@@ -56,10 +57,24 @@ struct Lead {
 
 inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& like) { return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt); }
 
+// A leaf whose gradients are added up on another stream than the one that is captured, because a graph from before the capture lives: its backward
+// cannot be captured, and trying ends the process.
+inline void check_capture(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto adds = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!adds || adds->num_inputs() == 0) return;
+  const auto here = at::cuda::getCurrentCUDAStream(t.device().index());
+  cudaStreamCaptureStatus status;
+  cuda_ok(cudaStreamIsCapturing(here.stream(), &status), "cudaStreamIsCapturing");
+  TORCH_CHECK(status == cudaStreamCaptureStatusNone || adds->input_metadata(0).stream() == here.unwrap(),
+              "fastlstm_b200: a graph of this leaf from before the capture lives, on another stream; free it (or warm up on the captured stream) first");
+}
+
 // A node of the graph that an operator's gradient is, with what it needs as members (a torch::autograd::Function keeps that in a
 // dictionary: 4 us a call).  Backward goes through it once.
 template <typename N, typename... I>
 std::shared_ptr<N> make_node(const I&... inputs) {
+  (check_capture(inputs), ...);
   std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
   return node;

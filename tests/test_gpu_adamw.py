@@ -341,6 +341,28 @@ def test_captured_and_replayed(bits):
     assert float(o.grad_norm) == float(ref.grad_norm)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizers_at_once(bits):
+    """Two optimizers on two streams side by side."""
+    def run(streams):
+        sides = []
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                params = model([(300,), (70001,)], "bf16", 40 + k)
+                sides.append((params, F.AdamW(params, **HYPER, state_bits=bits, max_norm=0.3)))
+        for _ in range(10):
+            for s, (_, o) in zip(streams, sides):
+                with torch.cuda.stream(s):
+                    o.step()
+        torch.cuda.synchronize()
+        return sides
+    here = torch.cuda.current_stream()
+    for (p, o), (q, n) in zip(run([here, here]), run([torch.cuda.Stream(), torch.cuda.Stream()])):
+        assert float(o.grad_norm) == float(n.grad_norm)
+        for a, b in zip(p, q):
+            assert torch.equal(a, b) and all(torch.equal(o.state[a][k].float(), n.state[b][k].float()) for k in o.state[a])
+
+
 def test_a_step_is_a_change_in_place():
     w = torch.randn(8, device="cuda", requires_grad=True)
     y = (w * w).sum()

@@ -234,6 +234,29 @@ def test_captured_and_replayed_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(r[:3], want[:3])) and torch.equal(moved, F.reorder_states(state, want.parents))
 
 
+def test_calls_at_once():
+    """Searches and reorderings on two streams side by side, and two layers' states behind each."""
+    g = gen(12)
+    data = [(*make(g, 7, 6, 9001), torch.randn(2, 42, 96, generator=g, device="cuda")) for _ in range(2)]
+
+    def step(logits, scores, state):
+        r = F.beam_step(logits, scores)
+        again = F.beam_step(logits, r.scores)
+        return [*r[:3], *again[:3], *F.reorder_states((state, r.tokens.view(1, -1)), again.parents)]
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(20):
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+    torch.cuda.synchronize()
+    for k, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[k % 2]))
+
+
 def test_logits_beyond_32_bits():
     """More than 2^31 logits (4.4 GB): the last sentence is what it is alone."""
     B, n, V = 66, 32, 2 ** 20 + 3

@@ -239,6 +239,47 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    x, w = torch.randn(9, 40, device="cuda", requires_grad=True), torch.ones(40, device="cuda", requires_grad=True)
+    eager = F.rms_norm(x, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: F.rms_norm(x, w), lambda: F.rms_norm(x.detach(), w), lambda: F.dropout(x, 0.5, 1),
+                     lambda: F.embedding(torch.zeros(3, dtype=torch.long, device="cuda"), x),
+                     lambda: F.token_log_probs(x, torch.zeros(9, dtype=torch.long, device="cuda"))):
+            with pytest.raises(RuntimeError, match="before the capture lives"):
+                call()
+    want = torch.autograd.grad(eager.sum(), (x, w))
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(F.rms_norm(x, w).sum(), (x, w))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_at_once():
+    """Forward and backward on two streams side by side."""
+    g = gen(11)
+    data = [[rows(g, 3001, 520), rows(g, 520), rows(g, 3001, 520)] for _ in range(2)]
+
+    def step(x, w, up):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(F.rms_norm(a, b), (a, b), up)
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(8):
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+    torch.cuda.synchronize()
+    for k, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[k % 2]))
+
+
 def test_another_stream():
     g = gen(9)
     x, w = rows(g, 513, 640), rows(g, 640)
