@@ -429,10 +429,14 @@ static int check_beam(const blstm_beam_desc* d) {
 // 16-byte pieces of a row: what they are at least, and at most where it does not begin on a boundary.
 static unsigned beam_pieces(const blstm_beam_desc& d) { return (unsigned)((uint64_t)d.vocab * dtype_bytes(d.dtype) / 16); }
 
-// Threads of a part, and parts of a row: warps have short rows; else as many parts (a power of two) as give kPartBlocks blocks to an SM, with
-// kPartPieces pieces at least for each thread.
-constexpr unsigned kShortPieces = 256, kPartBlocks = 16, kPartPieces = 4, kMostParts = 16;
-static unsigned beam_threads(const blstm_beam_desc& d) { return beam_pieces(d) <= kShortPieces ? 32 : kBlock; }
+// Threads of a part, and parts of a row: warps have short rows, longer ones too where there are many; else as many parts (a power of
+// two) as give kPartBlocks blocks to an SM, with kPartPieces pieces at least for each thread.  (132 x 24 x 5288 bf16 with a block and with
+// a warp for each row 33 and 29 us, 256 x 4 x 2500 14.8 and 12.7, 64 x 16 x 20000 25.8 and 27.6.)
+constexpr unsigned kShortPieces = 256, kManyPieces = 1024, kManyRows = 4, kPartBlocks = 16, kPartPieces = 4, kMostParts = 16;
+static unsigned beam_threads(const blstm_beam_desc& d) {
+  const bool many = (uint64_t)d.batch * d.beams >= (uint64_t)kManyRows * plan_sm_count();
+  return beam_pieces(d) <= (many ? kManyPieces : kShortPieces) ? 32 : kBlock;
+}
 static unsigned beam_parts(const blstm_beam_desc& d) {
   unsigned parts = 1;
   if (beam_threads(d) == kBlock)
