@@ -45,15 +45,15 @@ struct AdamParams {
   unsigned* ticket;
 };
 
-// Eight elements as they lie in memory: in 16-byte pieces where all eight are there and on a boundary (WHOLE), else the first `left` of them one
-// by one, zeros behind.
+// Eight elements as they lie in memory: in 16-byte pieces where all eight are there and on a boundary (WHOLE, or as `wide` and `left` say), else the
+// first `left` of them one by one, zeros behind.
 template <typename T>
 struct Raw {
   static constexpr int N = sizeof(T) / 2;              // 16-byte pieces
   uint4 v[N];
   template <bool WHOLE>
-  __device__ __forceinline__ void load(const T* p, long long left) {
-    if constexpr (WHOLE) {
+  __device__ __forceinline__ void load(const T* p, long long left, bool wide) {
+    if (WHOLE || (wide && left >= 8)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) v[k] = reinterpret_cast<const uint4*>(p)[k];
     } else {
@@ -70,8 +70,8 @@ struct Raw {
   }
 };
 template <bool WHOLE, typename T>
-__device__ __forceinline__ void store8(T* p, long long left, const float (&z)[8]) {
-  if constexpr (WHOLE) {
+__device__ __forceinline__ void store8(T* p, long long left, bool wide, const float (&z)[8]) {
+  if (WHOLE || (wide && left >= 8)) {
 #pragma unroll
     for (int k = 0; k < 8; k += kPer<T>) *reinterpret_cast<uint4*>(p + k) = pack(z + k, T{});
   } else {
@@ -81,8 +81,8 @@ __device__ __forceinline__ void store8(T* p, long long left, const float (&z)[8]
   }
 }
 template <bool WHOLE>
-__device__ __forceinline__ uint2 load8_bytes(const uint8_t* p, long long left) {
-  if constexpr (WHOLE) return *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ uint2 load8_bytes(const uint8_t* p, long long left, bool wide) {
+  if (WHOLE || (wide && left >= 8)) return *reinterpret_cast<const uint2*>(p);
   unsigned w[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 8; ++k)
@@ -90,8 +90,8 @@ __device__ __forceinline__ uint2 load8_bytes(const uint8_t* p, long long left) {
   return make_uint2(w[0], w[1]);
 }
 template <bool WHOLE>
-__device__ __forceinline__ void store8_bytes(uint8_t* p, long long left, uint2 v) {
-  if constexpr (WHOLE) {
+__device__ __forceinline__ void store8_bytes(uint8_t* p, long long left, bool wide, uint2 v) {
+  if (WHOLE || (wide && left >= 8)) {
     *reinterpret_cast<uint2*>(p) = v;
   } else {
 #pragma unroll
@@ -269,7 +269,7 @@ struct AdamStep {
 
 // A chunk of an item from element `begin` on, of which `left` are there: what a turn needs is fetched while the one before it is worked on.
 template <typename T, int BITS, bool MASTER, bool WHOLE>
-__device__ __forceinline__ void turns(const AdamStep& step, const AdamItem& a, long long begin, long long left, const unsigned* keys, unsigned t) {
+__device__ __forceinline__ void turns(const AdamStep& step, const AdamItem& a, long long begin, long long left, bool wide, const unsigned* keys, unsigned t) {
   const unsigned tid = threadIdx.x;
   const long long i0 = begin + tid * 8;
   const T* grad = static_cast<const T*>(a.grad) + i0;
@@ -282,20 +282,20 @@ __device__ __forceinline__ void turns(const AdamStep& step, const AdamItem& a, l
   uint2 m8, u8;
   float m_scale = 0.f, u_scale = 0.f;
   auto fetch = [&](int at, long long rest) {
-    g.template load<WHOLE>(grad + at, rest);
+    g.template load<WHOLE>(grad + at, rest, wide);
     if constexpr (BITS == 32) {
-      m.template load<WHOLE>(m32 + at, rest);
-      v.template load<WHOLE>(v32 + at, rest);
+      m.template load<WHOLE>(m32 + at, rest, wide);
+      v.template load<WHOLE>(v32 + at, rest, wide);
     } else {
-      m8 = load8_bytes<WHOLE>(mb + at, rest);
-      u8 = load8_bytes<WHOLE>(ub + at, rest);
+      m8 = load8_bytes<WHOLE>(mb + at, rest, wide);
+      u8 = load8_bytes<WHOLE>(ub + at, rest, wide);
       if (WHOLE || rest + (tid % 32) * 8 > 0) {
         m_scale = sm[at / 256];
         u_scale = su[at / 256];
       }
     }
-    if constexpr (MASTER) master.template load<WHOLE>(w32 + at, rest);
-    else x.template load<WHOLE>(param + at, rest);
+    if constexpr (MASTER) master.template load<WHOLE>(w32 + at, rest, wide);
+    else x.template load<WHOLE>(param + at, rest, wide);
   };
   long long rest = left - tid * 8;              // from this thread's first element on
   fetch(0, rest);
@@ -312,22 +312,22 @@ __device__ __forceinline__ void turns(const AdamStep& step, const AdamItem& a, l
       v.get(ve);
       if (at + kTurn < end) fetch(at + kTurn, rest - kTurn);
       step(ge, me, ve, xe);
-      store8<WHOLE>(m32 + at, rest, me);
-      store8<WHOLE>(v32 + at, rest, ve);
+      store8<WHOLE>(m32 + at, rest, wide, me);
+      store8<WHOLE>(v32 + at, rest, wide, ve);
     } else {
       uint2 mine = m8, roots = u8;
       float ms = m_scale, us = u_scale;
       if (at + kTurn < end) fetch(at + kTurn, rest - kTurn);
       step(ge, mine, roots, ms, us, xe, [&](int h, unsigned (&w)[4]) { draw4(w, keys, (unsigned long long)(i0 + at) / 4 + h, t, a.number); });
-      store8_bytes<WHOLE>(mb + at, rest, mine);
-      store8_bytes<WHOLE>(ub + at, rest, roots);
+      store8_bytes<WHOLE>(mb + at, rest, wide, mine);
+      store8_bytes<WHOLE>(ub + at, rest, wide, roots);
       if (tid % 32 == 0 && (WHOLE || rest > 0)) {
         sm[at / 256] = ms;
         su[at / 256] = us;
       }
     }
-    if constexpr (MASTER) store8<WHOLE>(w32 + at, rest, xe);
-    store8<WHOLE>(param + at, rest, xe);
+    if constexpr (MASTER) store8<WHOLE>(w32 + at, rest, wide, xe);
+    store8<WHOLE>(param + at, rest, wide, xe);
   }
 }
 
@@ -342,7 +342,8 @@ struct Cursor {
     return true;
   }
   __device__ __forceinline__ long long begin(const AdamParams<CAP>& p) const { return (long long)(chunk - p.item[k].first) * kChunk; }
-  __device__ __forceinline__ bool whole(const AdamParams<CAP>& p) const { return (p.wide[k / 64] >> k % 64 & 1) && p.item[k].n - begin(p) >= kChunk; }
+  __device__ __forceinline__ bool wide(const AdamParams<CAP>& p) const { return p.wide[k / 64] >> k % 64 & 1; }
+  __device__ __forceinline__ bool whole(const AdamParams<CAP>& p) const { return wide(p) && p.item[k].n - begin(p) >= kChunk; }
   __device__ __forceinline__ void next() { chunk += gridDim.x; }
 };
 
@@ -381,8 +382,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_consta
   int known = -1;
   for (Cursor<CAP> c; c.there(p); c.next()) {
     of_item(step, t, known, p, c.k, lr);
-    if (c.whole(p)) turns<T, 32, MASTER, true>(step, p.item[c.k], c.begin(p), kChunk, p.keys, t);
-    else turns<T, 32, MASTER, false>(step, p.item[c.k], c.begin(p), p.item[c.k].n - c.begin(p), p.keys, t);
+    if (c.whole(p)) turns<T, 32, MASTER, true>(step, p.item[c.k], c.begin(p), kChunk, true, p.keys, t);
+    else turns<T, 32, MASTER, false>(step, p.item[c.k], c.begin(p), p.item[c.k].n - c.begin(p), c.wide(p), p.keys, t);
   }
   count_steps(p);
 }
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw8_kernel(const __grid_co
     of_item(step, t, known, p, c.k, lr);
     const AdamItem& a = p.item[c.k];
     if (!c.whole(p)) {
-      turns<T, 8, MASTER, false>(step, a, c.begin(p), a.n - c.begin(p), p.keys, t);
+      turns<T, 8, MASTER, false>(step, a, c.begin(p), a.n - c.begin(p), c.wide(p), p.keys, t);
       continue;
     }
     const long long i0 = c.begin(p) + tid * 8;
@@ -493,11 +494,11 @@ __global__ void __launch_bounds__(kAdamThreads, 3) adamw8_kernel(const __grid_co
       x.get(xe);
       fetch();
       step(ge, m8, u8, ms, us, xe, [&](int h, unsigned (&w)[4]) { draw4(w, p.keys, block + h, t, a.number); });
-      store8_bytes<true>(mb + at, 8, m8);
-      store8_bytes<true>(ub + at, 8, u8);
+      store8_bytes<true>(mb + at, 8, true, m8);
+      store8_bytes<true>(ub + at, 8, true, u8);
       if (lane < 2) scale[at / 256] = lane ? us : ms;
-      if constexpr (MASTER) store8<true>(master + at, 8, xe);
-      store8<true>(param + at, 8, xe);
+      if constexpr (MASTER) store8<true>(master + at, 8, true, xe);
+      store8<true>(param + at, 8, true, xe);
     }
   }
   count_steps(p);
@@ -539,14 +540,14 @@ __device__ __forceinline__ double chunk_squares(const T* g, long long i, long lo
   if (wide && i - threadIdx.x * 8 + kNormChunk <= n) {
     Raw<T> raw[kParts];
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) raw[part].template load<true>(g + i + part * kTurn, 8);
+    for (int part = 0; part < kParts; ++part) raw[part].template load<true>(g + i + part * kTurn, 8, true);
 #pragma unroll
     for (int part = 0; part < kParts; ++part) sum += squares(raw[part]);
   } else {
 #pragma unroll 1
     for (long long at = i; at < n && at < i + kNormChunk; at += kTurn) {
       Raw<T> raw;
-      raw.template load<false>(g + at, n - at);
+      raw.template load<false>(g + at, n - at, wide);
       sum += squares(raw);
     }
   }
