@@ -604,9 +604,9 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_co
 // ---------------------------------------------------------------- host
 constexpr int kFew = 32, kMany = 384;          // tensors of a launch, with 2.7 and 31 KB of parameters
 
-// (More blocks than an SM has at a time: SMs are not all as near to all memory, and blocks that are still to come even that out.  138 M bf16
-// weights in 8 bits with 2, 4, 8, 32 blocks an SM: 435, 460, 390, 400 us.)
-static unsigned adam_grid(unsigned chunks) { return std::min(chunks, 8u * (unsigned)plan_sm_count()); }
+// (More blocks than an SM has at a time: SMs are not all as near to all memory, and blocks that are still to come even that out.  3, 4, 8, 16,
+// 32 blocks an SM: 29.8 M bf16 weights with masters, clipped, 177, 183, 155, 151, 155 us; 151 M in 8 bits 403, 403, 391, 391, 392.)
+static unsigned adam_grid(unsigned chunks) { return std::min(chunks, 16u * (unsigned)plan_sm_count()); }
 
 template <typename T, int BITS, bool MASTER, int CAP>
 static int launch_adamw(const blstm_adamw_desc& d, const blstm_adamw_item* items, int n, cudaStream_t st) {
