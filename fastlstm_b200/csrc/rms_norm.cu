@@ -38,6 +38,11 @@ __device__ __forceinline__ unsigned e4m3_two(float a, float b) {
   return r;
 }
 
+// What a row is multiplied by, and its scale, from its largest magnitude.  (At most 2^-110 counts as 0: 448 over it would pass the largest
+// float soon after, and the scale would lose its bits.)
+__device__ __forceinline__ float row_up(float most) { return most > 0x1p-110f ? 448.f / most : 0.f; }
+__device__ __forceinline__ float row_scale(float most) { return most <= 0x1p-110f ? 0.f : most / 448.f; }
+
 __device__ __forceinline__ float abs_max(float m, float v) {      // NaN stays
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
@@ -177,9 +182,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 ? (P <= 2 ? 8 : 1) 
         for (int k = 0; k < K; ++k) most = abs_max(most, z[k]);
       }
       most = over_row<G>(most, s, turn, AbsMax());
-      const float up = most > 0.f ? 448.f / most : 0.f;
+      const float up = row_up(most);
       uint8_t* q = p.q + (size_t)row * p.width;
-      if (c.at == 0) p.scales[row] = most / 448.f;
+      if (c.at == 0) p.scales[row] = row_scale(most);
 #pragma unroll
       for (int u = 0; u < P; ++u) {
         if (!c.has(u)) continue;
@@ -329,8 +334,8 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) norm_any_kernel(const __gri
 #pragma unroll 4
       for (unsigned j = at; j < p.width; j += G) most = abs_max(most, ld_f(x + j) * i * ld_f(w + j));
       most = over_row<G>(most, s, turn, AbsMax());
-      const float up = most > 0.f ? 448.f / most : 0.f;
-      if (at == 0) p.scales[row] = most / 448.f;
+      const float up = row_up(most);
+      if (at == 0) p.scales[row] = row_scale(most);
 #pragma unroll 4
       for (unsigned j = at; j < p.width; j += G) p.q[(size_t)row * p.width + j] = (uint8_t)e4m3_two(ld_f(x + j) * i * ld_f(w + j) * up, 0.f);
     } else {

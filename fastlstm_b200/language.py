@@ -85,14 +85,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
 class EightBitRows(NamedTuple):
     """What rms_norm_e4m3 returns: values * scales[..., None] is the norm; sum is None where there was no residual."""
     values: torch.Tensor                     # [..., width] float8_e4m3fn
-    scales: torch.Tensor                     # [...]        float32: the row's largest magnitude / 448
+    scales: torch.Tensor                     # [...]        float32: the row's largest magnitude / 448, or 0
     sum: Optional[torch.Tensor]              # [..., width] x + residual
 
 
 def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> EightBitRows:
     """rms_norm with its output in 8 bits and a scale for every row, for products of 8-bit operands; without gradients.
 
-    Values are rounded once, from 32 bits.  A row of zeros has scale 0 and values 0."""
+    Values are rounded once, from 32 bits.  A row of zeros, or of magnitudes up to 2^-110, has scale 0 and values 0."""
     return EightBitRows(*_lib.host().rms_norm_e4m3(x, weight, residual, float(eps)))
 
 

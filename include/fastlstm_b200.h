@@ -332,7 +332,8 @@ typedef struct blstm_norm_desc {
 int blstm_rms_norm(const blstm_norm_desc* d, const void* x, const void* residual, const void* weight, void* y, void* sum,
                    float* rstd, void* stream);
 
-/* The same in 8 bits: values [n0,n1,width] = e4m3(h i weight / scale), scales [n0*n1] = the row's largest magnitude / 448. */
+/* The same in 8 bits: values [n0,n1,width] = e4m3(h i weight / scale), scales [n0*n1] = the row's largest magnitude / 448,
+ * both 0 where that magnitude is at most 2^-110. */
 int blstm_rms_norm_e4m3(const blstm_norm_desc* d, const void* x, const void* residual, const void* weight, void* values,
                         float* scales, void* sum, void* stream);
 

@@ -72,6 +72,25 @@ def test_sizes(dtype, n, width, residual):
     check(rows(g, n, width, dtype=dtype), 1 + rows(g, width, dtype=dtype, std=0.3), dtype, rows(g, n, width, dtype=dtype) if residual else None)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [7, 64, 301, 512, 2053, 16400])
+def test_eight_bits_of_tiny_rows(dtype, width):
+    """448 over a magnitude below 2^-119 is infinite: such rows are zeros; those above 2^-110 have their values as ever."""
+    x = rows(gen(width), 5, width, dtype=dtype)
+    x[:, 0] = 0
+    x[1] = 0
+    q = F.rms_norm_e4m3(x, torch.full((width,), 2.0 ** -122, dtype=DT[dtype], device="cuda"))
+    assert (q.scales == 0).all() and (q.values.float() == 0).all()
+    w = torch.full((width,), 2.0 ** -105, dtype=DT[dtype], device="cuda")
+    q = F.rms_norm_e4m3(x, w)
+    C = width / 32 + 50
+    want, _ = O.rms_norm(np64(x), np64(w), 1e-6)
+    most = np.abs(want).max(-1) / 448
+    within(np64(q.scales), most, (C / 2 + 8) * U * most, "scales")
+    scale = np64(q.scales)[..., None]
+    within(np64(q.values) * scale, want, (2.0 ** -4 + (C / 2 + 12) * U) * np.abs(want) + 2.0 ** -10 * scale, "values")
+
+
 @pytest.mark.parametrize("dtype,n,width", [("bf16", 20011, 64), ("fp32", 7001, 301), ("fp16", 5003, 515), ("bf16", 3001, 1536), ("bf16", 1201, 7000)])
 def test_many_rows(dtype, n, width):
     """More rows than blocks, so that each has several."""
