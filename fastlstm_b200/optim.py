@@ -12,6 +12,7 @@ import torch.optim.optimizer as _global_hooks
 from . import _lib
 from .language import _whole
 
+_CAPTURE = "AdamW: take a step or load a state before a capture, which would begin with new states at every replay"
 BLOCK = 256                  # elements of a tensor, in row-major order, that share a scale in 8-bit states
 
 
@@ -75,7 +76,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _start(self, p):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: take a step or load a state before a capture, which would begin with new states at every replay")
+            raise RuntimeError(_CAPTURE)
         self.state[p] = {name: p.detach().float() if name == "master" else torch.zeros(shape, dtype=dtype, device=p.device)
                          for name, (shape, dtype) in self._format(p).items()}
         return self.state[p]
@@ -111,12 +112,16 @@ class AdamW(torch.optim.Optimizer):
                 g.setdefault(name, value)
         for k, s in loaded.items():
             self.state[params[k]] = s
+            if params[k].is_cuda:
+                self._scratch(params[k].device.index)
 
     # ------------------------------------------------------------------ step
     def _scratch(self, device):
         """(the counter that launches use, {norm, factor}) of a device."""
         kept = self.__dict__.setdefault("_kept", {})
         if device not in kept:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(_CAPTURE)
             at = torch.device("cuda", device)
             kept[device] = (torch.zeros(1, dtype=torch.int32, device=at), torch.zeros(2, dtype=torch.float32, device=at))
         return kept[device]

@@ -6,6 +6,8 @@ adds 4 u where gradients are clipped.  The step that is taken from p is m' throu
 corrections (exponentials to 2^-22, a reciprocal root to 2^-22): below 2^-19 of its magnitude, taken with the magnitudes that m' is the sum
 of; p' has one rounding besides, 2 u of p, and e.  8 bits: an element's place among the e4m3 numbers is known to 16 u of its place and to the
 error of m', in steps of the numbers' distance; where a rounding border is not nearer than that the number is the oracle's."""
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -339,6 +341,43 @@ def test_captured_and_replayed(bits):
     for p, q in zip(params, twin):
         assert torch.equal(p, q) and all(torch.equal(o.state[p][k].float(), ref.state[q][k].float()) for k in o.state[p])
     assert float(o.grad_norm) == float(ref.grad_norm)
+
+
+def test_first_step_captured():
+    """After a state was loaded the first step may be a captured one, and steps one by one go on before its replays: what launches use lies
+    outside of the graph's memory, which holds something else until then."""
+    params = model([(300,), (4000,)], "bf16", 18)
+    twin = model([(300,), (4000,)], "bf16", 18)
+    ref = F.AdamW(twin, lr=0.01, max_norm=0.5)
+    ref.step()
+    o = F.AdamW(params, lr=0.01, max_norm=0.5)
+    o.load_state_dict(ref.state_dict())
+    with torch.no_grad():
+        for p, q in zip(params, twin):
+            p.copy_(q)
+    pool = torch.cuda.graph_pool_handle()
+    other, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other, pool=pool):
+        full = [torch.full((4,), 12345, dtype=torch.int32, device="cuda") for _ in range(64)]
+        del full
+    other.replay()
+    with torch.cuda.graph(graph, pool=pool):
+        o.step()
+    for k in range(2):
+        o.step() if k == 0 else graph.replay()
+        ref.step()
+        for p, q in zip(params, twin):
+            assert torch.equal(p, q) and int(o.state[p]["step"]) == int(ref.state[q]["step"]) == k + 2
+    # one that was never used has no place for it
+    copy = pickle.loads(pickle.dumps(o))
+    for p in copy.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device="cuda")
+        with pytest.raises(RuntimeError, match="before a capture"):
+            copy.step()
+    copy.step()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
