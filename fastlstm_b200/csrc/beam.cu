@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   const bool live = !ended && score != -INFINITY;
   if (mine < p.beams && tid % 8 == 0) {
     s.kind[mine] = ended ? 1 : live ? 0 : 2;
-    const double weight = p.penalty != 0.0 ? 1.0 / pow((double)(p.lengths[r0 + mine] + !ended), p.penalty) : 1.0;
+    // (from 1 to 2^24, so that a weight of 32 bits is between 2^-96 and 1 and products with it have all of their bits)
+    const double weight = p.penalty != 0.0 ? 1.0 / pow((double)max(min(p.lengths[r0 + mine], (1ll << 24) - !ended) + !ended, 1ll), p.penalty) : 1.0;
     s.weight[mine] = weight;
     s.weight32[mine] = (float)weight;
   }
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 static int check_beam(const blstm_beam_desc* d) {
   if (!d || !valid_dtype(d->dtype) || !valid_rows(d->batch, d->beams) || d->beams <= 0 || d->beams > BLSTM_MAX_BEAMS || d->width <= 0 ||
       d->width > BLSTM_MAX_TOP || d->vocab <= 0 || d->vocab >= INT32_MAX || d->width > d->beams * d->vocab || d->end_token < -1 ||
-      d->end_token >= d->vocab || !(d->length_penalty >= 0 && d->length_penalty < INFINITY) || d->batch > INT32_MAX / BLSTM_MAX_TOP)
+      d->end_token >= d->vocab || !(d->length_penalty >= 0 && d->length_penalty <= BLSTM_MAX_LENGTH_PENALTY) || d->batch > INT32_MAX / BLSTM_MAX_TOP)
     return BLSTM_E_INVALID_ARG;
   return BLSTM_OK;
 }

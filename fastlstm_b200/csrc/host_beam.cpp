@@ -41,7 +41,8 @@ py::tuple beam_step(const Tensor& logits_in, const Tensor& scores_in, std::optio
       beside(*lengths_in, "lengths", logits_in);
       same(*lengths_in, "lengths", at::kLong, shape);
     }
-    if (!(length_penalty >= 0 && std::isfinite(length_penalty))) throw wrong("length_penalty must be at least 0 and finite");
+    if (!(length_penalty >= 0 && length_penalty <= BLSTM_MAX_LENGTH_PENALTY))
+      throw wrong("length_penalty must be between 0 and " + std::to_string(BLSTM_MAX_LENGTH_PENALTY));
     if (length_penalty != 0 && !lengths_in) throw wrong("length_penalty needs lengths");
     d.length_penalty = length_penalty;
     without_grad(logits_in, "beam_step");

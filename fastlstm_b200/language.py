@@ -113,8 +113,9 @@ def beam_step(logits: torch.Tensor, scores: torch.Tensor, *, width: Optional[int
     probabilities so far; the first step has one hypothesis of score 0 and a width of its own (at most 32; the number of hypotheses by
     default).  A continuation's score is its hypothesis' plus the log softmax of the logits.  A hypothesis in `finished` (bool) goes
     on with end_token alone, at its own score; its logits are not read, nor are those of a hypothesis whose score is -inf.
-    With a length_penalty continuations are ranked by score / length ** length_penalty (scores stay what they are); lengths (int64)
-    counts the tokens of hypotheses, to which a continuation adds one unless its hypothesis is finished.
+    With a length_penalty (0 to 4) continuations are ranked by score / length ** length_penalty (scores stay what they are); lengths
+    (int64) counts the tokens of hypotheses, to which a continuation adds one unless its hypothesis is finished; in ranks they count
+    as 1 at least and 2 ** 24 at most.
 
     Sums are ranked in 64 bits, equal ones in the order of (hypothesis, token).  Where fewer than `width` continuations are possible,
     impossible ones (score -inf) follow.  NaN or +inf among a hypothesis' logits makes its continuations NaN, which come first."""

@@ -393,18 +393,19 @@ int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream);
 
 /* A step of beam search over logits [batch, beams, vocab]; everything else is dense, [batch, beams] or [batch, width]. */
 #define BLSTM_MAX_BEAMS 32
+#define BLSTM_MAX_LENGTH_PENALTY 4
 typedef struct blstm_beam_desc {
   int32_t dtype, width;          /* of logits; hypotheses that are kept, at most BLSTM_MAX_TOP and beams * vocab */
   int64_t batch, beams, vocab;   /* batch * beams < 2^31, beams <= BLSTM_MAX_BEAMS                     */
   int64_t logits_stride[2];
   int64_t end_token;             /* or -1                                                              */
-  double length_penalty;         /* of at least 0; needs lengths where it is not 0                     */
+  double length_penalty;         /* 0 to BLSTM_MAX_LENGTH_PENALTY; needs lengths where it is not 0     */
 } blstm_beam_desc;
 
 /* total[k,v] = scores[k] + log softmax(logits[k])[v]; where finished[k] (or NULL: none) scores[k] for end_token and -inf for all others.
  * The width largest of total / (lengths[k] + 1)^length_penalty (lengths[k]^length_penalty where finished[k]), equal ones by (k, v), NaN
  * first: out_scores (their totals), parents (k), tokens (v), out_finished (finished[k] or v == end_token), out_lengths (lengths[k], + 1 unless
- * finished[k]); the last two, or NULL.  Logits of finished hypotheses and of those with scores of -inf are not read; a row of nothing but
+ * finished[k]); the last two, or NULL.  Lengths below 1 rank like 1, those above 2^24 like 2^24.  Logits of finished hypotheses and of those with scores of -inf are not read; a row of nothing but
  * -inf continues with -inf.  Totals are compared in 64 bits. */
 size_t blstm_beam_workspace(const blstm_beam_desc* d);
 int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* scores, const uint8_t* finished,

@@ -136,7 +136,7 @@ def beam_ranks(logits, scores, end=None, finished=None, lengths=None, penalty=0.
             over = np.full((B, n, V), -np.inf)
             over[..., end] = scores
             total = np.where(finished[..., None], over, total)
-        return total / (after ** penalty)[..., None], total
+        return total / (np.clip(after, 1, 2.0 ** 24) ** penalty)[..., None], total
 
 
 def beam_step(logits, scores, width, end=None, finished=None, lengths=None, penalty=0.0):

@@ -59,7 +59,7 @@ BEAM = dict(dtype=_lib.BF16, width=4, batch=2, beams=3, vocab=10, logits_stride=
 
 @pytest.mark.parametrize("change", [dict(dtype=4), dict(width=0), dict(width=33, vocab=100), dict(width=31), dict(batch=-1), dict(batch=2 ** 30), dict(beams=0),
                                     dict(beams=33), dict(vocab=0), dict(vocab=2 ** 31), dict(end_token=-2), dict(end_token=10),
-                                    dict(length_penalty=-1.0), dict(length_penalty=float("nan")), dict(length_penalty=float("inf"))])
+                                    dict(length_penalty=-1.0), dict(length_penalty=float("nan")), dict(length_penalty=float("inf")), dict(length_penalty=4.001)])
 def test_descriptors_refused(change):
     lib, d = _lib.load(), _desc(_lib.BeamDesc, **{**BEAM, **change})
     assert lib.blstm_beam_step(d, *[PTR] * 10, 1 << 30, None) == 1

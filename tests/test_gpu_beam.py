@@ -207,6 +207,23 @@ def test_no_sentences_and_refusals():
         F.beam_step(z, s)
 
 
+@pytest.mark.parametrize("penalty", [0.6, 4.0])
+@pytest.mark.parametrize("V", [3, 60, 5003])
+def test_lengths_that_are_none(V, penalty):
+    """Lengths of zero, below it and far above any, of hypotheses that go on, have ended or are dead: nothing is divided by 0, and what
+    is impossible comes behind."""
+    g = gen(V)
+    logits, scores = make(g, 4, 6, V)
+    finished = torch.zeros(4, 6, dtype=torch.bool, device="cuda")
+    finished[:, 1] = finished[:, 3] = True
+    scores[0, 2:], scores[1, 1:], scores[2, :5], scores[3, 3] = -torch.inf, -torch.inf, -torch.inf, 0
+    lengths = torch.tensor([0, 0, -7, -1, 2 ** 62, 12], device="cuda").repeat(4, 1)
+    lengths[1], lengths[2] = -1, 1 << 40
+    check(logits, scores, 9, 1, finished, lengths, penalty)
+    with pytest.raises(ValueError, match="length_penalty"):
+        F.beam_step(logits, scores, lengths=lengths, length_penalty=4.5)
+
+
 def test_captured_and_replayed_and_on_another_stream():
     g = gen(3)
     logits, scores = make(g, 4, 5, 9000)
