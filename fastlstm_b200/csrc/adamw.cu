@@ -604,9 +604,12 @@ __global__ void __launch_bounds__(kAdamThreads) grad_norm_kernel(const __grid_co
 // ---------------------------------------------------------------- host
 constexpr int kFew = 32, kMany = 384;          // tensors of a launch, with 2.7 and 31 KB of parameters
 
-// (More blocks than an SM has at a time: SMs are not all as near to all memory, and blocks that are still to come even that out.  3, 4, 8, 16,
-// 32 blocks an SM: 29.8 M bf16 weights with masters, clipped, 177, 183, 155, 151, 155 us; 151 M in 8 bits 403, 403, 391, 391, 392.)
-static unsigned adam_grid(unsigned chunks) { return std::min(chunks, 16u * (unsigned)plan_sm_count()); }
+// (More blocks than an SM has at a time: SMs are not all as near to all memory, and blocks that are still to come even that out.  Of steps
+// with 32 bits, 3, 4, 8, 16, 32 blocks an SM: 29.8 M bf16 weights with masters, clipped, 177, 183, 155, 151, 155 us.  With 8 bits a block
+// fills its stages first, which fewer chunks for each make dearer: 151 M bf16 weights 403, 403, 391, 391, 392, 14 M fp32 ones with 8 and 16
+// 80 and 85.  Norms of gradients with 4, 8, 16: the 29.8 M 151, 147, 149.)
+constexpr unsigned kStepBlocks = 16, kFewBlocks = 8;
+static unsigned adam_grid(unsigned chunks, unsigned each) { return std::min(chunks, each * (unsigned)plan_sm_count()); }
 
 template <typename T, int BITS, bool MASTER, int CAP>
 static int launch_adamw(const blstm_adamw_desc& d, const blstm_adamw_item* items, int n, cudaStream_t st) {
@@ -635,11 +638,11 @@ static int launch_adamw(const blstm_adamw_desc& d, const blstm_adamw_item* items
   p.log_beta1 = std::log(d.beta1); p.log_beta2 = std::log(d.beta2);
   p.lr_at = d.lr_at; p.factor = d.factor; p.ticket = d.ticket;
   if constexpr (BITS == 32) {
-    adamw_kernel<T, MASTER, CAP><<<adam_grid(p.chunks), kAdamThreads, 0, st>>>(p);
+    adamw_kernel<T, MASTER, CAP><<<adam_grid(p.chunks, kStepBlocks), kAdamThreads, 0, st>>>(p);
   } else {
     constexpr int smem = kStages * (int)sizeof(AdamStage<T, MASTER>);
     if constexpr (smem > 48 * 1024) BLSTM_CUDA_OK(cudaFuncSetAttribute(adamw8_kernel<T, MASTER, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    adamw8_kernel<T, MASTER, CAP><<<adam_grid(p.chunks), kAdamThreads, smem, st>>>(p);
+    adamw8_kernel<T, MASTER, CAP><<<adam_grid(p.chunks, kFewBlocks), kAdamThreads, smem, st>>>(p);
   }
   BLSTM_CUDA_OK(cudaGetLastError());
   count_launch();
@@ -666,7 +669,7 @@ static int launch_grad_norm(const blstm_grad_norm_desc& d, int at, int n, unsign
     chunks += (unsigned long long)((s.n + kNormChunk - 1) / kNormChunk);
     if (chunks > INT32_MAX) return BLSTM_E_TOO_LARGE;
   }
-  const unsigned grid = adam_grid((unsigned)chunks);
+  const unsigned grid = adam_grid((unsigned)chunks, kFewBlocks);
   double* all = static_cast<double*>(d.workspace);
   p.items = (unsigned)n; p.chunks = (unsigned)chunks;
   p.partial = all + blocks; p.all = all;
@@ -712,7 +715,7 @@ int blstm_adamw(const blstm_adamw_desc* d, void* stream) {
 }
 
 size_t blstm_grad_norm_workspace(int items) {
-  return items <= 0 ? 256 : round_up((size_t)((items + kMany - 1) / kMany) * adam_grid(UINT32_MAX) * sizeof(double), 256);
+  return items <= 0 ? 256 : round_up((size_t)((items + kMany - 1) / kMany) * adam_grid(UINT32_MAX, kFewBlocks) * sizeof(double), 256);
 }
 
 int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream) {

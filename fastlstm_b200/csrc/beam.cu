@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 
 // ---------------------------------------------------------------- reordering
 // Rows are moved by groups of 1 to 32 lanes, up to kRowPieces pieces a lane; longer ones in parts.  (A thread for every piece finds its row
-// by divisions: 2 x 2560 rows of 301 fp32 twice and 100 x 2560 numbers 26 us, so 8.)
+// by divisions: 2 x 2560 rows of 301 fp32 twice and 100 x 2560 numbers 26 us, so 8, from the L2.)
 constexpr int kReorderItems = 32, kReorderThreads = 256, kRowPieces = 16;
 struct ReorderItem {
   const char* src;
