@@ -154,11 +154,15 @@ struct MergeShared {
   float z[kCand];                                        // the smaller place
   unsigned owner[kWindow], owners, count;
 
+  // A hypothesis whose continuations all come first (NaN, or +inf and, where a logit is -inf, NaN): every token of it counts.
+  __device__ __forceinline__ bool first(unsigned k) const { return !(base32[k] < INFINITY); }
   __device__ __forceinline__ double total(unsigned k, float at) const { return base[k] == -INFINITY ? -INFINITY : base[k] + ((double)at - (double)high[k]); }
-  // The rank in 32 bits, less or more (side -1, 1) than what it may be off; one that is finite stays it.
+  // The rank in 32 bits, less or more (side -1, 1) than what it may be off; one that is finite stays it.  (Where nothing but -inf was found
+  // there may be no token at all: as little as -inf, and where all tokens count as much as any.)
   __device__ __forceinline__ float rank32(unsigned k, float at, float side) const {
     const float d = at - high[k], off = 2e-6f * (fabsf(base32[k]) + fabsf(d));
-    return at == -INFINITY ? at : fminf(max_nan(max_nan(base32[k] + d + side * off, kLowest) * weight32[k], kLowest), -kLowest);
+    if (at == -INFINITY) return side > 0.f && first(k) ? -kLowest : at;
+    return fminf(max_nan(max_nan(base32[k] + d + side * off, kLowest) * weight32[k], kLowest), -kLowest);
   }
   // A continuation that may be among the best.
   __device__ __noinline__ void offer(unsigned k, unsigned token, float at) {
@@ -211,7 +215,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     }
   a.join(8);
   if (mine < p.beams && tid % 8 == 0) {
-    const double base = !live ? (double)score : a.s == 0.f ? -INFINITY : (double)score - log((double)a.s);      // (a row of nothing but -inf)
+    const double base = !live ? (double)score : a.s == 0.f && score < INFINITY ? -INFINITY : (double)score - log((double)a.s);      // (a row of nothing but -inf)
     s.base[mine] = base;
     s.base32[mine] = base == -INFINITY ? -INFINITY : max_nan((float)base, kLowest);                // (-inf alone stands for none)
     s.high[mine] = live ? a.m : 0.f;
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         m = z[0];
 #pragma unroll
         for (int e = 1; e < kPer<T>; ++e) m = max_nan(m, z[e]);
-        unsigned token = span.number(piece), last = m < least || m == -INFINITY ? token : token + kPer<T>;
+        unsigned token = span.number(piece), last = piece < span.end && (s.first(k) || !(m < least || m == -INFINITY)) ? token + kPer<T> : token;
         if (look == 0) {                       // thread `edge` of the part had one of its edges
           const unsigned edge = group * kLanes + lane;
           if (lane < kLanes && edge < span.edges()) s.offer(k, span.edge(edge), ld_f(row + span.edge(edge)));

@@ -143,8 +143,7 @@ def beam_step(logits, scores, width, end=None, finished=None, lengths=None, pena
     """(scores, parents, tokens, finished, lengths) [B, width]."""
     rank, total = beam_ranks(logits, scores, end, finished, lengths, penalty)
     B, n, V = rank.shape
-    first = np.where(np.isnan(rank), np.inf, rank).reshape(B, -1)
-    flat = np.stack([np.lexsort((np.arange(n * V), -r))[:width] for r in first])
+    flat = np.stack([np.lexsort((np.arange(n * V), -r, ~np.isnan(r)))[:width] for r in rank.reshape(B, -1)])      # (NaN comes first)
     parents, tokens = flat // V, flat % V
     rows = np.arange(B)[:, None]
     ended = np.zeros((B, n), bool) if finished is None else finished

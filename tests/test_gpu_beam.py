@@ -174,6 +174,70 @@ def test_not_a_number_and_infinity_come_first(V, bad):
         assert torch.equal(a[[0, 2]], b[[0, 2]])
 
 
+def spoiled(call):
+    """A call whose results lie in memory that holds something else; what it returns twice is the same, bit by bit."""
+    results = []
+    for fill in (-7, 13):
+        junk = [torch.full((n,), fill, dtype=torch.int64, device="cuda") for n in (8, 64, 128, 192, 256, 512) for _ in range(8)]
+        del junk
+        results.append(call())
+    F.check_status()
+    for a, b in zip(*results):
+        assert (a is None and b is None) or torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    return results[0]
+
+
+@pytest.mark.parametrize("V", [9, 40, 600, 4000, 40000])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_not_a_number_and_infinity_beside_masked_logits(V, dtype, bad):
+    """A bad logit makes all of its hypothesis' continuations NaN, the masked ones too: they come first, in the order of (hypothesis, token),
+    and what is possible behind them.  (One healthy hypothesis a sentence: its order is that of its logits.)"""
+    g = gen(V)
+    inf = float("inf")
+    for W in (1, 2, 8, 31, 32):
+        for at in (0, V // 3, V - 1):
+            n = 4
+            logits, scores = make(g, 6, n, V, dtype)
+            logits[:, 1:] = -inf
+            scores[:, 3] = -inf                          # (dead)
+            logits[0, 1, at] = bad                       # one bad logit, nothing else possible; the healthy one in front
+            logits[1, 0] = -inf
+            logits[1, 0, at] = bad                       # the same in the first hypothesis; the second has nothing possible
+            logits[2, 2] = make(g, 1, 1, V, dtype)[0][0, 0]
+            logits[2, 2, torch.rand(V, generator=g, device="cuda") < 0.9] = -inf
+            logits[2, 2, at] = bad                       # some finite ones besides
+            logits[3, 1:3, at] = bad                     # two bad hypotheses
+            logits[4, 2, at:] = bad
+            scores[5, 0] = bad                           # a bad score over logits of which some are masked
+            logits[5, 0, ::2] = -inf
+            w = min(W, n * V)
+            finished = torch.zeros(6, n, dtype=torch.bool, device="cuda")
+            finished[4, 1], scores[4, 1] = True, 0       # (ended, in front of all that go on)
+            lengths = torch.randint(1, 9, (6, n), generator=g, device="cuda")
+            for kw in (dict(), dict(end_token=V // 2, finished=finished, lengths=lengths, length_penalty=0.7)):
+                r = spoiled(lambda: F.beam_step(logits, scores, width=w, **kw))
+                z, s = np64(logits), np64(scores)
+                f, l = (host(finished), host(lengths)) if kw else (None, None)
+                want_s, want_p, want_t, want_f, want_l = O.beam_step(z, s, w, V // 2 if kw else None, f, l, kw.get("length_penalty", 0.0))
+                assert (host(r.parents) == want_p).all() and (host(r.tokens) == want_t).all()
+                got = np64(r.scores)
+                assert (np.isnan(got) == np.isnan(want_s)).all()
+                sure = np.isfinite(want_s)
+                assert (got[~sure & ~np.isnan(got)] == want_s[~sure & ~np.isnan(got)]).all()
+                assert (np.abs(got[sure] - want_s[sure]) <= (4 * 160 + 16 + V / 64) * U + U * np.abs(want_s[sure])).all()
+                if kw:
+                    assert (host(r.finished) == want_f).all() and (host(r.lengths) == want_l).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_scores_of_hypotheses_that_cannot_go_on(bad):
+    """A score of NaN or +inf over logits of nothing but -inf: NaN, not a quiet end."""
+    logits, scores = torch.full((1, 2, 700), -float("inf"), device="cuda"), torch.tensor([[-1.0, bad]], device="cuda")
+    r = spoiled(lambda: F.beam_step(logits, scores, width=5))
+    assert r.scores.isnan().all() and r.parents.tolist() == [[1] * 5] and r.tokens.tolist() == [list(range(5))]
+
+
 @pytest.mark.parametrize("V", [77, 512, 1300, 6007, 40003])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_layouts(V, dtype):
