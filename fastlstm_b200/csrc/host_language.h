@@ -57,17 +57,18 @@ struct Lead {
 
 inline Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& like) { return at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt); }
 
-// A leaf whose gradients are added up on another stream than the one that is captured, because a graph from before the capture lives: its backward
-// cannot be captured, and trying ends the process.
+// A leaf whose gradients are added up on the default stream, because a graph from before the capture lives: that stream cannot wait for a captured
+// one, so the backward pass cannot be captured, and trying ends the process.  (Other streams are joined into the capture.)
 inline void check_capture(const Tensor& t) {
   if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
   const auto adds = torch::autograd::impl::try_get_grad_accumulator(t);
   if (!adds || adds->num_inputs() == 0) return;
-  const auto here = at::cuda::getCurrentCUDAStream(t.device().index());
+  const auto device = t.device().index();
+  if (adds->input_metadata(0).stream() != at::cuda::getDefaultCUDAStream(device).unwrap()) return;
   cudaStreamCaptureStatus status;
-  cuda_ok(cudaStreamIsCapturing(here.stream(), &status), "cudaStreamIsCapturing");
-  TORCH_CHECK(status == cudaStreamCaptureStatusNone || adds->input_metadata(0).stream() == here.unwrap(),
-              "fastlstm_b200: a graph of this leaf from before the capture lives, on another stream; free it (or warm up on the captured stream) first");
+  cuda_ok(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream(device).stream(), &status), "cudaStreamIsCapturing");
+  TORCH_CHECK(status == cudaStreamCaptureStatusNone,
+              "fastlstm_b200: a graph of this leaf from before the capture lives, on the default stream; free it (or warm up on another stream) first");
 }
 
 // A node of the graph that an operator's gradient is, with what it needs as members (a torch::autograd::Function keeps that in a

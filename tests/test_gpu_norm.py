@@ -277,6 +277,57 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+class Around(torch.nn.Module):
+    """Every operator with a gradient, on leaves."""
+
+    def __init__(self, seed):
+        super().__init__()
+        g = gen(seed)
+        self.table = torch.nn.Parameter(torch.randn(50, 40, generator=g, device="cuda"))
+        self.weight = torch.nn.Parameter(1 + 0.1 * torch.randn(40, generator=g, device="cuda"))
+        self.tokens = torch.randint(0, 50, (9,), generator=g, device="cuda")
+
+    def forward(self, x):
+        y, h = F.rms_norm(F.dropout(x, 0.25, 7), self.weight, residual=F.embedding(self.tokens, self.table))
+        r = F.token_log_probs(F.rms_norm(h, self.weight), self.tokens % 40, top=2)
+        return r.log_probs.sum() + r.entropy.sum() + r.top_log_probs.sum() + y.sum()
+
+
+def test_captures_beside_graphs_of_side_streams():
+    """A graph from a side stream may live: its leaves' gradients are joined into the capture (torch.cuda.make_graphed_callables warms up on
+    such a stream and keeps its last outputs)."""
+    model, plain = Around(1), Around(1)
+    x = torch.randn(9, 40, generator=gen(2), device="cuda", requires_grad=True)
+    graphed = torch.cuda.make_graphed_callables(model, (x.detach().clone().requires_grad_(),))
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(9, 40, generator=gen(3 + k), device="cuda"))
+        got = torch.autograd.grad(graphed(x), [x, *model.parameters()])
+        want = torch.autograd.grad(plain(x), [x, *plain.parameters()])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_backward_captured_beside_a_graph_of_a_side_stream():
+    """The same with gradients that are added up in the leaves."""
+    model, plain = Around(4), Around(4)
+    x = torch.randn(9, 40, generator=gen(5), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kept = model(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        model(x).backward()
+    graph.replay()
+    plain(x).backward()
+    for a, b in zip(model.parameters(), plain.parameters()):
+        assert torch.equal(a.grad, b.grad)
+    kept.backward()
+    for a, b in zip(model.parameters(), plain.parameters()):
+        assert torch.equal(a.grad, 2 * b.grad)
+
+
 def test_calls_at_once():
     """Forward and backward on two streams side by side."""
     g = gen(11)
