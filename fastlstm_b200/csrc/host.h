@@ -109,13 +109,13 @@ inline void require(const OptTensor& t, const char* name, at::ScalarType dt, con
 inline const void* ptr(const Tensor& t) { return t.const_data_ptr(); }
 inline const void* ptr(const OptTensor& t) { return t ? t->const_data_ptr() : nullptr; }
 
-// What every call does around its launches.
+// What every call does around its launches.  (`listen`: whether it throws what an earlier launch has left; not in the middle of several.)
 struct Call {
   c10::cuda::CUDAGuard guard;
   int dev;
   void* stream;
-  explicit Call(const at::Device& d) : guard(d), dev(d.index()), stream(at::cuda::getCurrentCUDAStream(d.index()).stream()) {
-    poll(dev);
+  explicit Call(const at::Device& d, bool listen = true) : guard(d), dev(d.index()), stream(at::cuda::getCurrentCUDAStream(d.index()).stream()) {
+    if (listen) poll(dev);
     blstm_set_mailbox(mailbox(dev));
   }
   ~Call() { blstm_set_mailbox(nullptr); }

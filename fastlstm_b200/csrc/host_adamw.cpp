@@ -36,6 +36,8 @@ float* f32(const Tensor& t, const char* name, const Tensor& param, int64_t n) {
 struct Bucket {
   std::vector<Tensor> params, grads;           // (grads dense, held until the launch)
   std::vector<blstm_adamw_item> items;
+  blstm_adamw_desc d{};
+  Tensor ticket;
 };
 
 PyObject* interned(const char* name) { return PyUnicode_InternFromString(name); }
@@ -46,12 +48,29 @@ const Tensor& state_tensor(PyObject* state, PyObject* name) {
   return THPVariable_Unpack(t);
 }
 
-double number_of(PyObject* group, PyObject* name) {
+py::handle entry(PyObject* group, PyObject* name) {
   PyObject* v = PyDict_GetItemWithError(group, name);
   if (!v) throw wrong("a parameter group has no " + std::string(PyUnicode_AsUTF8(name)));
+  return v;
+}
+
+// A finite number of 32 bits, `low` or more.
+double number_of(PyObject* group, PyObject* name, double low) {
+  PyObject* v = entry(group, name).ptr();
   const double d = THPVariable_Check(v) ? THPVariable_Unpack(v).item<double>() : PyFloat_AsDouble(v);
   if (d == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+  if (!(d >= low && std::isfinite((float)d)))
+    throw wrong(std::string(PyUnicode_AsUTF8(name)) + " must be " + (low == 0 ? "at least 0 and " : "") + "finite in 32 bits, got " + std::to_string(d));
   return d;
+}
+
+template <typename T>
+T cast(PyObject* group, PyObject* name, const char* what) {
+  try {
+    return entry(group, name).cast<T>();
+  } catch (const py::cast_error&) {
+    throw wrong(std::string(PyUnicode_AsUTF8(name)) + " must be " + what);
+  }
 }
 
 // A step over the parameter groups of an optimizer (optim.py).  start(p): makes the state of a parameter that has none; scratch(p): the
@@ -112,58 +131,70 @@ std::optional<Tensor> adamw_step(const py::list& groups, const py::dict& state, 
     }
   }
   if (calls.empty()) return std::nullopt;
+  // Everything that can be refused is, before the first launch: groups and types are launched one by one, and a step is taken by all of
+  // them or by none.
   auto scratch_of = [&](const Bucket& b) { return scratch(b.params[0].device().index()).cast<std::pair<Tensor, Tensor>>(); };
   std::optional<Tensor> norm;
+  blstm_grad_norm_desc n{};
+  std::vector<blstm_grad_item> grads;
+  Tensor ws;
   if (max_norm) {
     const Bucket& first = calls[0].second;
-    std::vector<blstm_grad_item> items;
     for (const auto& [group, b] : calls) {
       if (b.params[0].device() != first.params[0].device()) throw wrong("max_norm takes parameters on one device");
-      for (const blstm_adamw_item& a : b.items) items.push_back({a.grad, a.n, dtype_code(b.params[0].scalar_type()), 0});
+      for (const blstm_adamw_item& a : b.items) grads.push_back({a.grad, a.n, dtype_code(b.params[0].scalar_type()), 0});
     }
     const auto [ticket, out] = scratch_of(first);
     norm = out;
-    if (!items.empty()) {
-      Call call(out.device());
-      blstm_grad_norm_desc d{};
-      d.item = items.data();
-      d.items = (int32_t)items.size();
-      d.max_norm = (float)*max_norm;
-      d.out = static_cast<float*>(out.data_ptr());
-      d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
-      d.workspace_bytes = blstm_grad_norm_workspace(d.items);
-      const Tensor ws = fresh({(int64_t)d.workspace_bytes}, at::kByte, out);
-      d.workspace = ws.data_ptr();
-      check(blstm_grad_norm(&d, call.stream), "gradient norm");
-    }
+    n.item = grads.data();
+    n.items = (int32_t)grads.size();
+    n.max_norm = (float)*max_norm;
+    n.out = static_cast<float*>(out.data_ptr());
+    n.ticket = static_cast<uint32_t*>(ticket.data_ptr());
+    n.workspace_bytes = blstm_grad_norm_workspace(n.items);
+    ws = fresh({(int64_t)n.workspace_bytes}, at::kByte, out);
+    n.workspace = ws.data_ptr();
   }
-  for (const auto& [group, b] : calls) {
+  for (auto& [group, b] : calls) {
     if (b.items.empty()) continue;
-    blstm_adamw_desc d{};
+    blstm_adamw_desc& d = b.d;
     d.dtype = dtype_code(b.params[0].scalar_type());
     d.bits = bits;
     d.items = (int32_t)b.items.size();
     d.item = b.items.data();
-    PyObject* lr = PyDict_GetItemWithError(group, k_lr);
-    if (lr && THPVariable_Check(lr) && THPVariable_Unpack(lr).is_cuda()) {
+    PyObject* lr = entry(group, k_lr).ptr();
+    if (THPVariable_Check(lr) && THPVariable_Unpack(lr).is_cuda()) {
       const Tensor& t = THPVariable_Unpack(lr);
       beside(t, "lr", b.params[0]);
       if (t.scalar_type() != at::kFloat || t.numel() != 1) throw wrong("lr on the GPU must be one float32 element");
       d.lr_at = static_cast<const float*>(ptr(t));
     } else {
-      d.lr = number_of(group, k_lr);
+      d.lr = number_of(group, k_lr, -HUGE_VAL);
     }
-    const auto betas = py::reinterpret_borrow<py::object>(PyDict_GetItemWithError(group, k_betas)).cast<std::pair<double, double>>();
+    const auto betas = cast<std::pair<double, double>>(group, k_betas, "two numbers");
+    for (const double beta : {betas.first, betas.second})
+      if (!(beta >= 0 && beta < 1)) throw wrong("betas must be in [0, 1), got " + std::to_string(beta));
     d.beta1 = betas.first; d.beta2 = betas.second;
-    d.eps = number_of(group, k_eps);
-    d.weight_decay = number_of(group, k_decay);
-    d.seed = py::reinterpret_borrow<py::object>(PyDict_GetItemWithError(group, k_seed)).cast<uint64_t>();
+    d.eps = number_of(group, k_eps, 0);
+    d.weight_decay = number_of(group, k_decay, -HUGE_VAL);
+    d.seed = cast<uint64_t>(group, k_seed, "a whole number in [0, 2^64)");
     if (norm) d.factor = static_cast<const float*>(ptr(*norm)) + 1;
-    const Tensor ticket = scratch_of(b).first;
-    d.ticket = static_cast<uint32_t*>(ticket.data_ptr());
-    Call call(b.params[0].device());
-    check(blstm_adamw(&d, call.stream), "adamw");
-    for (const Tensor& p : b.params) torch::autograd::impl::bump_version(p);
+    b.ticket = scratch_of(b).first;
+    d.ticket = static_cast<uint32_t*>(b.ticket.data_ptr());
+  }
+  for (const auto& [group, b] : calls) {
+    const Call heard(b.params[0].device());     // (throws what an earlier launch has left)
+    if (!b.items.empty())
+      for (const Tensor& p : b.params) torch::autograd::impl::bump_version(p);
+  }
+  if (!grads.empty()) {
+    const Call call(norm->device(), false);
+    check(blstm_grad_norm(&n, call.stream), "gradient norm");
+  }
+  for (const auto& [group, b] : calls) {
+    if (b.items.empty()) continue;
+    const Call call(b.params[0].device(), false);
+    check(blstm_adamw(&b.d, call.stream), "adamw");
   }
   return norm;
 }

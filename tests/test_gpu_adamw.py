@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import fastlstm_b200 as F
+from fastlstm_b200._lib import BlstmError
 from oracle import adamw_oracle as A
 
 from test_gpu_language import DT, EPS, TINY, U, gen, np64, within
@@ -463,3 +464,38 @@ def test_offsets_beyond_32_bits():
         assert float((p.detach()[s].float() - q.detach().float()).abs().max()) <= 2.0 ** -8 * 4.5
         assert float((o.state[p]["exp_avg"][s] - small.state[q]["exp_avg"]).abs().max()) <= 1e-6
     assert not p.detach()[2 ** 20:2 ** 30].any() and int(o.state[p]["step"]) == 1
+
+
+def test_a_refused_step_changes_nothing():
+    """Groups and types are launched one by one, but checked before the first of them: weights, states and counts stay what they are."""
+    params = model([(300,), (4000,)], "fp32", 50) + model([(77,)], "bf16", 51) + model([(300,)], "fp32", 52)
+    groups = [dict(params=params[:3]), dict(params=params[3:], lr=0.5)]
+    good = dict(lr=0.5, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1, seed=0)
+    for max_norm in (None, 1.0):
+        o = F.AdamW(groups, **HYPER, max_norm=max_norm)
+        o.step()
+        keep = [p.detach().clone() for p in params] + [t.clone() for p in params for t in o.state[p].values()]
+
+        def unchanged():
+            torch.cuda.synchronize()
+            now = [p.detach() for p in params] + [t for p in params for t in o.state[p].values()]
+            return all(torch.equal(a, b) for a, b in zip(keep, now))
+        for bad in (dict(lr=torch.zeros(1, device="cuda", dtype=torch.float64)), dict(lr=float("nan")), dict(lr="fast"), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)),
+                    dict(betas=0.9), dict(eps=-1.0), dict(eps=float("inf")), dict(weight_decay=float("nan")), dict(seed=2 ** 64), dict(seed=-1),
+                    dict(seed=0.5)):
+            o.param_groups[1].update({**good, **bad})
+            with pytest.raises((ValueError, TypeError)):
+                o.step()
+            assert unchanged(), bad
+        o.param_groups[1].update(good)
+        del o.param_groups[1]["betas"]
+        with pytest.raises(ValueError, match="betas"):
+            o.step()
+        o.param_groups[1].update(good)
+        F.reorder_states(torch.zeros(1, 2, 3, device="cuda"), torch.tensor([[0, 5]], device="cuda"))      # a report that is still to be heard
+        torch.cuda.synchronize()
+        with pytest.raises(BlstmError):
+            o.step()
+        assert unchanged()
+        o.step()
+        assert not unchanged() and [int(o.state[p]["step"]) for p in params] == [2] * 4
