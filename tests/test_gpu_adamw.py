@@ -499,3 +499,39 @@ def test_a_refused_step_changes_nothing():
         assert unchanged()
         o.step()
         assert not unchanged() and [int(o.state[p]["step"]) for p in params] == [2] * 4
+
+
+def test_gradient_norm_is_added_up_in_64_bits():
+    """Seven small squares behind a large one, each below half a step of 32 bits: summed in 32 bits the norm is 1.6 u too small, in 64 it has the
+    one rounding to its own 32 bits."""
+    small = (0.9 * 2.0 ** -25) ** 0.5
+    for dtype, n in (("fp32", 4096), ("fp32", 70000), ("bf16", 4096)):
+        g = torch.full((n,), small, device="cuda")
+        g[::8] = 1
+        p = torch.zeros(n, device="cuda", dtype=DT[dtype], requires_grad=True)
+        p.grad = g.to(DT[dtype])
+        total = np.sqrt((np64(p.grad) ** 2).sum())
+        o = F.AdamW([p], max_norm=1e6)
+        o.step()
+        assert abs(float(o.grad_norm) - total) <= 1.001 * U * total
+
+
+@pytest.mark.parametrize("dtype,master", [("fp32", False), ("bf16", True), ("fp16", False)])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_chunks_than_blocks(dtype, master, bits):
+    """Blocks that go on from chunk to chunk and from tensor to tensor, past chunks that are not whole and a tensor on another boundary, with
+    copies of the next ones under way."""
+    sizes = [700 * 8192 + 100, 3 * 8192 - 5, 8192, 50 * 8192, 300 * 8192, 17, 900 * 8192 + 8191, 40 * 8192]
+    made = [0]
+
+    def odd(p):
+        made[0] += 1
+        if made[0] != 4:
+            return p
+        flat = torch.zeros(p.numel() + 1, device="cuda", dtype=p.dtype)
+        flat[1:] = p
+        return flat[1:]
+    params = model([(n,) for n in sizes], dtype, 60, odd)
+    o = F.AdamW(params, **HYPER, state_bits=bits, master_weights=master, max_norm=100.0, seed=77)
+    check_step(o, params, dtype)
+    check_step(o, params, dtype)
