@@ -13,7 +13,24 @@ from . import _lib
 from .language import _whole
 
 _CAPTURE = "AdamW: take a step or load a state before a capture, which would begin with new states at every replay"
+_LEAST, _MOST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 BLOCK = 256                  # elements of a tensor, in row-major order, that share a scale in 8-bit states
+
+
+def _check_group(group):
+    """Refuses what a parameter group's step would be refused for."""
+    lr, betas = group["lr"], group["betas"]
+    if isinstance(lr, torch.Tensor):
+        if lr.numel() != 1 or not lr.is_floating_point():
+            raise ValueError("lr as a tensor must be one floating-point element")
+    elif not 0 <= lr <= _MOST:
+        raise ValueError(f"lr must be at least 0 and finite in 32 bits, got {lr!r}")
+    if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+        raise ValueError(f"betas must be two numbers in [0, 1), got {betas!r}")
+    for name in ("eps", "weight_decay"):
+        if not 0 <= group[name] <= _MOST:
+            raise ValueError(f"{name} must be at least 0 and finite in 32 bits, got {group[name]!r}")
+    _whole(group["seed"], "seed", 0, 2 ** 64 - 1)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -38,25 +55,17 @@ class AdamW(torch.optim.Optimizer):
                  master_weights: bool = True, max_norm: Optional[float] = None, seed: int = 0):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits!r}")
-        if max_norm is not None and not (max_norm > 0 and math.isfinite(max_norm)):
-            raise ValueError(f"max_norm must be positive and finite, got {max_norm!r}")
+        if max_norm is not None and not (max_norm >= _LEAST and math.isfinite(max_norm)):
+            raise ValueError(f"max_norm must be positive (at least 2^-126) and finite, got {max_norm!r}")
         self.state_bits, self.master_weights = int(state_bits), bool(master_weights)
         self.max_norm = None if max_norm is None else float(max_norm)
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, seed=_whole(seed, "seed", 0, 2 ** 64 - 1)))
 
     def add_param_group(self, param_group):
-        group = {**self.defaults, **param_group}
-        lr, betas = group["lr"], group["betas"]
-        if isinstance(lr, torch.Tensor):
-            if lr.numel() != 1 or not lr.is_floating_point():
-                raise ValueError("lr as a tensor must be one floating-point element")
-        elif not (lr >= 0 and math.isfinite(lr)):
-            raise ValueError(f"lr must be at least 0 and finite, got {lr!r}")
-        if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"betas must be two numbers in [0, 1), got {betas!r}")
-        for name in ("eps", "weight_decay"):
-            if not (group[name] >= 0 and math.isfinite(group[name])):
-                raise ValueError(f"{name} must be at least 0 and finite, got {group[name]!r}")
+        if isinstance(param_group, dict):
+            _check_group({**self.defaults, **param_group})
+            if "seed" in param_group:
+                param_group["seed"] = int(param_group["seed"])
         super().add_param_group(param_group)
 
     def __getstate__(self):
@@ -104,12 +113,14 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"{name} of the loaded state has dtype {t.dtype}, expected {dtype}: it is of an optimizer with other state_bits")
                 loaded[k][name] = torch.empty(shape, dtype=dtype, device=p.device).copy_(t)
         for g in state_dict["param_groups"]:
+            _check_group({**self.defaults, **g})
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("loaded state is of an optimizer with amsgrad or maximize, which are not there")
         super().load_state_dict({**state_dict, "state": {}})
         for g in self.param_groups:
             for name, value in self.defaults.items():
                 g.setdefault(name, value)
+            g["seed"] = int(g["seed"])
         for k, s in loaded.items():
             self.state[params[k]] = s
             if params[k].is_cuda:

@@ -50,6 +50,26 @@ def test_arguments_refused(bad):
             F.AdamW([dict(params=[torch.zeros(3, requires_grad=True)], **bad)])
 
 
+@pytest.mark.parametrize("bad", [dict(seed=-1), dict(seed=2 ** 64), dict(seed=0.5), dict(lr=1e39), dict(lr=-1.0), dict(eps=1e39), dict(weight_decay=1e39),
+                                 dict(betas=(0.9, 1.0)), dict(betas=(0.9,))])
+def test_groups_are_refused_when_they_come(bad):
+    """A group's own values, and those of a loaded state: what is there stays."""
+    a, b = torch.zeros(3, requires_grad=True), torch.zeros(4, requires_grad=True)
+    o = F.AdamW([a], lr=0.5, seed=3)
+    with pytest.raises(ValueError):
+        o.add_param_group(dict(params=[b], **bad))
+    assert len(o.param_groups) == 1
+    saved = o.state_dict()
+    state = {"step": 3, "exp_avg": torch.zeros(3), "exp_avg_sq": torch.zeros(3)}
+    with pytest.raises(ValueError):
+        o.load_state_dict({"state": {0: state}, "param_groups": [{**saved["param_groups"][0], **bad}]})
+    assert not o.state and o.param_groups[0]["lr"] == 0.5 and o.param_groups[0]["seed"] == 3
+    o.add_param_group(dict(params=[b], seed=4.0))
+    assert [repr(g["seed"]) for g in o.param_groups] == ["3", "4"]
+    with pytest.raises(ValueError, match="max_norm"):
+        F.AdamW([a], max_norm=1e-50)
+
+
 def test_cpu_parameters_are_refused_and_none_is_fine():
     p = torch.zeros(3, requires_grad=True)
     o = F.AdamW([p])
