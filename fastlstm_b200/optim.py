@@ -90,9 +90,18 @@ class AdamW(torch.optim.Optimizer):
                          for name, (shape, dtype) in self._format(p).items()}
         return self.state[p]
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes copies in the types that this optimizer keeps.  Masters that the state does not have are the parameters."""
+        state_dict = dict(state_dict)
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        self._load(state_dict)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
+
+    @torch.no_grad()
+    def _load(self, state_dict):
         ids = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = dict(zip(ids, chain.from_iterable(g["params"] for g in self.param_groups)))
         loaded = {}
@@ -116,7 +125,13 @@ class AdamW(torch.optim.Optimizer):
             _check_group({**self.defaults, **g})
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("loaded state is of an optimizer with amsgrad or maximize, which are not there")
-        super().load_state_dict({**state_dict, "state": {}})
+        # (torch would cast states to the parameters' types; hooks run around all of this)
+        hooks = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = type(hooks[0])(), type(hooks[1])()
+        try:
+            super().load_state_dict({**state_dict, "state": {}})
+        finally:
+            self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = hooks
         for g in self.param_groups:
             for name, value in self.defaults.items():
                 g.setdefault(name, value)

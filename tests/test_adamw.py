@@ -70,6 +70,31 @@ def test_groups_are_refused_when_they_come(bad):
         F.AdamW([a], max_norm=1e-50)
 
 
+def test_load_hooks_see_and_change_the_whole_state():
+    """What a hook in front returns is what is checked and loaded; a hook behind sees the final state."""
+    p = torch.zeros(5, requires_grad=True)
+    o = F.AdamW([p])
+    groups = o.state_dict()["param_groups"]
+    old = {"m": torch.full((5,), 7.0), "exp_avg_sq": torch.ones(5), "step": 2}
+    seen = []
+
+    def convert(optimizer, d):
+        assert optimizer is o and list(d["state"]) == [0]
+        return {**d, "state": {k: {"exp_avg": s["m"], "exp_avg_sq": s["exp_avg_sq"], "step": 9} for k, s in d["state"].items()}}
+    first = o.register_load_state_dict_pre_hook(convert)
+    o.register_load_state_dict_pre_hook(lambda optimizer, d: seen.append(d["state"][0]["step"]))
+    o.register_load_state_dict_post_hook(lambda optimizer: seen.append((int(o.state[p]["step"]), float(o.state[p]["exp_avg"][0]))))
+    given = {"state": {0: old}, "param_groups": groups}
+    o.load_state_dict(given)
+    assert seen == [9, (9, 7.0)] and list(given["state"][0]) == ["m", "exp_avg_sq", "step"]
+    first.remove()
+    with pytest.raises(ValueError, match="exp_avg"):
+        o.load_state_dict(given)
+    assert len(seen) == 3 and int(o.state[p]["step"]) == 9       # (refused: no hook behind)
+    o.load_state_dict(o.state_dict())                            # (hooks are still there)
+    assert seen[3:] == [9, (9, 7.0)]
+
+
 def test_cpu_parameters_are_refused_and_none_is_fine():
     p = torch.zeros(3, requires_grad=True)
     o = F.AdamW([p])
