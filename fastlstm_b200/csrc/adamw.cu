@@ -14,6 +14,7 @@
 // within 2 % on average.  The chance is a function of seed, step, tensor and element: a run repeats bit by bit.  u is never rounded to
 // 0, which would divide by it.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -146,7 +147,7 @@ __device__ __forceinline__ float max_abs(float m, float v) {      // NaN stays
 }
 // The largest of a warp's magnitudes: their bits have their order, and NaN comes last.
 __device__ __forceinline__ float warp_most(float most) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most))); }
-__device__ __forceinline__ float reciprocal_fast(float x) {      // to 2^-23
+__device__ __forceinline__ float reciprocal_fast(float x) {      // to 2^-23; of 0, or at least 2^-126
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
@@ -692,7 +693,7 @@ extern "C" {
 
 int blstm_adamw(const blstm_adamw_desc* d, void* stream) {
   if (!d || !valid_dtype(d->dtype) || (d->bits != 32 && d->bits != 8) || d->items < 0 || (d->items && !d->item) || !(d->beta1 >= 0 && d->beta1 < 1) ||
-      !(d->beta2 >= 0 && d->beta2 < 1) || !(d->eps >= 0 && std::isfinite((float)d->eps)) || !std::isfinite((float)d->weight_decay) ||
+      !(d->beta2 >= 0 && d->beta2 < 1) || !(d->eps == 0 || d->eps >= FLT_MIN) || !std::isfinite((float)d->eps) || !std::isfinite((float)d->weight_decay) ||
       (!d->lr_at && !std::isfinite((float)d->lr)) || !aligned(4, d->lr_at, d->factor, d->ticket) || !d->ticket)
     return BLSTM_E_INVALID_ARG;
   const size_t e = dtype_bytes(d->dtype), se = d->bits == 32 ? 4 : 1;

@@ -2,6 +2,8 @@
 // step over a layer's four tensors took 31 us where Python collected them.)
 #include "host_language.h"
 
+#include <cfloat>
+
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -176,6 +178,7 @@ std::optional<Tensor> adamw_step(const py::list& groups, const py::dict& state, 
       if (!(beta >= 0 && beta < 1)) throw wrong("betas must be in [0, 1), got " + std::to_string(beta));
     d.beta1 = betas.first; d.beta2 = betas.second;
     d.eps = number_of(group, k_eps, 0);
+    if (d.eps > 0 && d.eps < FLT_MIN) throw wrong("eps must be 0 or at least 2^-126");
     d.weight_decay = number_of(group, k_decay, -HUGE_VAL);
     d.seed = cast<uint64_t>(group, k_seed, "a whole number in [0, 2^64)");
     if (norm) d.factor = static_cast<const float*>(ptr(*norm)) + 1;

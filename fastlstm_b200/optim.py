@@ -30,6 +30,8 @@ def _check_group(group):
     for name in ("eps", "weight_decay"):
         if not 0 <= group[name] <= _MOST:
             raise ValueError(f"{name} must be at least 0 and finite in 32 bits, got {group[name]!r}")
+    if 0 < group["eps"] < _LEAST:
+        raise ValueError(f"eps must be 0 or at least 2^-126 (its reciprocal is held in 32 bits), got {group['eps']!r}")
     _whole(group["seed"], "seed", 0, 2 ** 64 - 1)
 
 

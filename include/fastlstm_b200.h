@@ -359,7 +359,7 @@ typedef struct blstm_adamw_desc {
   int32_t dtype, bits;           /* of param and grad; 32 or 8, of the states                          */
   int32_t items, reserved;
   const blstm_adamw_item* item;  /* HOST memory, read during the call                                  */
-  double lr, beta1, beta2, eps, weight_decay;
+  double lr, beta1, beta2, eps, weight_decay;      /* eps: 0, or at least 2^-126                       */
   uint64_t seed;
   const float* lr_at;            /* lr in device memory, read when the kernel runs, or NULL            */
   const float* factor;           /* of the gradients, in device memory, or NULL: 1.  NaN: nothing changes, no step counts */

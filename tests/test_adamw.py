@@ -70,6 +70,18 @@ def test_groups_are_refused_when_they_come(bad):
         F.AdamW([a], max_norm=1e-50)
 
 
+def test_eps_whose_reciprocal_is_infinite_is_refused():
+    """Below 2^-126 a weight without a gradient would move by 0 times infinity."""
+    p = torch.zeros(3, requires_grad=True)
+    for eps in (1e-40, 1e-300, 2.0 ** -126 * 0.999):
+        with pytest.raises(ValueError, match="eps"):
+            F.AdamW([p], eps=eps)
+        d, _ = _desc(eps=eps)
+        assert _lib.load().blstm_adamw(d, None) == 1
+    F.AdamW([p], eps=2.0 ** -126)
+    F.AdamW([p], eps=0)
+
+
 def test_load_hooks_see_and_change_the_whole_state():
     """What a hook in front returns is what is checked and loaded; a hook behind sees the final state."""
     p = torch.zeros(5, requires_grad=True)

@@ -440,6 +440,21 @@ def test_refusals():
     F.AdamW([empty], max_norm=1.0).step()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_least_eps(bits):
+    """2^-126: a weight whose gradient has always been 0 only decays."""
+    p = torch.randn(600, generator=gen(70), device="cuda").requires_grad_()
+    p.grad = torch.randn(600, generator=gen(71), device="cuda")
+    p.grad[:256] = 0
+    before = p.detach()[:256].clone()
+    o = F.AdamW([p], lr=0.01, weight_decay=0.0, eps=2.0 ** -126, state_bits=bits)
+    o.step()
+    assert torch.equal(p.detach()[:256], before) and p.detach().isfinite().all()
+    o.param_groups[0]["eps"] = 1e-40
+    with pytest.raises(ValueError, match="eps"):
+        o.step()
+
+
 def test_offsets_beyond_32_bits():
     """A tensor of more than 2^31 elements (26 GB with its states): its ends are what small tensors' are."""
     n = 2 ** 31 + 2 ** 12 + 5
