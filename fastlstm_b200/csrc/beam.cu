@@ -550,7 +550,8 @@ int blstm_reorder(const blstm_reorder_item* items, int n, const void* parents, i
                           (s.outer > 1 ? (uint64_t)s.outer_stride : 0) | (uint64_t)s.row_stride;
     const int bytes = bits & 1 ? 1 : bits & 2 ? 2 : bits & 4 ? 4 : bits & 8 ? 8 : 16;
     const uint64_t per_row = (uint64_t)s.inner_bytes / bytes, rows = (uint64_t)(batch * width);
-    if (per_row > UINT32_MAX || (uint64_t)s.outer > (1ull << 48) / rows / per_row) return BLSTM_E_TOO_LARGE;
+    // (the kernel goes up to two parts of 32 lanes past a row's end in 32 bits)
+    if (per_row > UINT32_MAX - 64 * kRowPieces || (uint64_t)s.outer > (1ull << 48) / rows / per_row) return BLSTM_E_TOO_LARGE;
     unsigned lanes = 0;
     while (lanes < 5 && (1ull << lanes) < per_row) ++lanes;
     const uint64_t parts = (per_row + (kRowPieces << lanes) - 1) / (kRowPieces << lanes), units = (uint64_t)s.outer * rows * parts;

@@ -415,7 +415,7 @@ int blstm_beam_step(const blstm_beam_desc* d, const void* logits, const float* s
 typedef struct blstm_reorder_item {
   const void* src;               /* [outer, batch*beams] rows of inner_bytes bytes                     */
   void* dst;                     /* [outer, batch*width, inner_bytes], dense                           */
-  int64_t outer, inner_bytes;
+  int64_t outer, inner_bytes;    /* at most 2^36 bytes and 2^32 - 1025 pieces, of 1 to 16 bytes as everything is a multiple of */
   int64_t outer_stride, row_stride;   /* of src, in bytes                                              */
 } blstm_reorder_item;
 

@@ -96,3 +96,11 @@ def test_reorder_refused():
         assert call(**bad) == 1, bad
     assert lib.blstm_reorder(None, 1, PTR, 64, 2, 3, 4, None) == 1
     assert call(n=0) == 0 and call(outer=0) == 0 and call(batch=0, parents=None) == 0
+
+
+def test_reorder_of_rows_near_2_to_the_32_pieces_is_refused():
+    """The kernel counts a row's pieces, and 512 more at a time, in 32 bits."""
+    lib = _lib.load()
+    for odd in (2 ** 32 - 1, 2 ** 32 - 511, 2 ** 32 + 1):                # in pieces of one byte
+        item = (_lib.ReorderItem * 1)(_lib.ReorderItem(src=PTR, dst=PTR, outer=1, inner_bytes=odd, outer_stride=0, row_stride=odd))
+        assert lib.blstm_reorder(item, 1, PTR, 64, 1, 1, 1, None) == _lib.E_TOO_LARGE
