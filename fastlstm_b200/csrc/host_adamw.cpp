@@ -24,7 +24,7 @@ Tensor dense_grad(const Tensor& g, const Tensor& param) {
   if (g.layout() != at::kStrided) throw wrong("sparse gradients are not there for AdamW");
   beside(g, "a gradient", param);
   same(g, "a gradient", param.scalar_type(), param.sizes());
-  return g.contiguous();
+  return plain(g).contiguous();
 }
 
 float* f32(const Tensor& t, const char* name, const Tensor& param, int64_t n) {
@@ -97,6 +97,7 @@ std::optional<Tensor> adamw_step(const py::list& groups, const py::dict& state, 
       if (!p.grad().defined()) continue;
       on_gpu(p, "a parameter");
       dtype_code(p.scalar_type());
+      if (p.is_neg()) throw wrong("a parameter must not be a lazily negated tensor");
       if (!p.is_contiguous()) throw wrong("a parameter of shape " + shape_str(p.sizes()) + " must be contiguous");
       PyObject* s = PyDict_GetItemWithError(state.ptr(), at.ptr());
       py::object made;

@@ -49,7 +49,7 @@ py::tuple beam_step(const Tensor& logits_in, const Tensor& scores_in, std::optio
     without_grad(scores_in, "beam_step");
     const Lead lead(shape);
     at::AutoDispatchBelowADInplaceOrView guard;
-    const Tensor logits = lead.rows(logits_in, d.logits_stride), given = scores_in.contiguous();
+    const Tensor logits = lead.rows(logits_in, d.logits_stride), given = plain(scores_in).contiguous();
     const Tensor ended = finished_in ? finished_in->contiguous() : Tensor(), written = lengths_in ? lengths_in->contiguous() : Tensor();
     Call call(logits.device());
     const int64_t out[2] = {d.batch, width};

@@ -21,7 +21,7 @@ blstm_embed_desc embed_desc(at::ScalarType dt, const Tensor& tokens, const Lead&
 
 Tensor embedding_impl(const Tensor& tokens_in, const Tensor& weight_in, double scale) {
   const Lead lead(tokens_in.sizes());
-  const Tensor weight = weight_in.size(1) > 1 && weight_in.stride(1) != 1 ? weight_in.contiguous() : weight_in;
+  const Tensor weight = weight_in.size(1) > 1 && weight_in.stride(1) != 1 ? weight_in.contiguous() : plain(weight_in);
   blstm_embed_desc d = embed_desc(weight.scalar_type(), tokens_in, lead, weight.size(0), weight.size(1), scale, -1);
   const Tensor tokens = lead.rows(tokens_in, d.token_stride);
   d.row_stride[0] = weight.stride(0);
@@ -100,7 +100,7 @@ Tensor dropout_impl(const Tensor& x_in, const Mask& k) {
   d.shared = -1;
   d.p = k.p; d.seed = k.seed; d.offset = k.offset;
   d.n0 = d.n1 = 1;
-  Tensor x = x_in;
+  Tensor x = plain(x_in);
   if (k.shared < 0 && dims > 3 && !x.is_contiguous()) x = x.flatten(0, dims - 2);     // (a copy where one stride does not do)
   const bool two = (x.dim() == 2 || x.dim() == 3) && !x.is_contiguous() && x.stride(-1) == 1 && x.numel() / x.size(-1) <= INT32_MAX;
   if (!two) x = x.contiguous();
@@ -250,7 +250,7 @@ struct ScoreGrad : public Node {
     Tensor g2, best;
     if (c.top) {
       best = tops.unpack();
-      if (g[2].defined()) g2 = g[2].contiguous();
+      if (g[2].defined()) g2 = plain(g[2]).contiguous();
     }
     auto f32 = [](const Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; };
     check(blstm_token_log_probs_grad(&d, ptr(rows), ptr(given), f32(saved), c.top ? static_cast<const int64_t*>(ptr(best)) : nullptr, f32(g0), s0,

@@ -36,6 +36,9 @@ inline int token_bits(const Tensor& tokens) {
   throw wrong(std::string("tokens have dtype ") + c10::toString(tokens.scalar_type()) + ", expected int64 or int32");
 }
 
+// The numbers themselves where their signs are still to be turned (z.conj().imag).
+inline Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // The leading dimensions of an operator's tensors as [n0, n1].
 struct Lead {
   int64_t dims, n0, n1;
@@ -46,7 +49,7 @@ struct Lead {
   }
   // t with `dims` leading dimensions as one whose rows stride[0..1] reach
   Tensor rows(const Tensor& t, int64_t stride[2]) const {
-    Tensor v = dims > 2 ? t.flatten(0, dims - 1) : t;
+    Tensor v = plain(dims > 2 ? t.flatten(0, dims - 1) : t);
     const int64_t lead = dims > 2 ? 1 : dims;
     if (v.dim() > lead && v.size(-1) > 1 && v.stride(-1) != 1) v = v.contiguous();
     stride[0] = lead == 2 ? v.stride(0) : 0;

@@ -32,7 +32,7 @@ std::array<Tensor, 3> norm_impl(const Tensor& x_in, const Tensor& weight_in, con
   const auto lead_sizes = x_in.sizes().slice(0, x_in.dim() - 1);
   const Lead lead(lead_sizes);
   blstm_norm_desc d = norm_desc(x_in, lead, eps);
-  const Tensor x = lead.rows(x_in, d.x_stride), weight = weight_in.contiguous();
+  const Tensor x = lead.rows(x_in, d.x_stride), weight = plain(weight_in).contiguous();
   const Tensor r = residual ? lead.rows(*residual, d.residual_stride) : Tensor();
   Call call(x.device());
   const Tensor h = residual ? fresh(x_in.sizes(), x.scalar_type(), x) : Tensor();
@@ -68,7 +68,7 @@ struct NormGrad : public Node {
     const Tensor at_h = h_is_output ? h.unpack(getptr()) : h.unpack(), w_in = weight.unpack(), i = rstd.unpack();
     const Lead lead(at_h.sizes().slice(0, at_h.dim() - 1));
     blstm_norm_desc d = norm_desc(at_h, lead, eps);
-    const Tensor rows = lead.rows(at_h, d.x_stride), w = w_in.contiguous(), up = lead.rows(dy, d.dy_stride);
+    const Tensor rows = lead.rows(at_h, d.x_stride), w = plain(w_in).contiguous(), up = lead.rows(dy, d.dy_stride);
     const Tensor ds = dsum.defined() ? lead.rows(dsum, d.residual_stride) : Tensor();
     Call call(rows.device());
     const Tensor dx = fresh(at_h.sizes(), at_h.scalar_type(), at_h);

@@ -350,6 +350,43 @@ def test_calls_at_once():
         assert all(torch.equal(a, b) for a, b in zip(r, want[k % 2]))
 
 
+def test_lazily_negated_inputs():
+    """Numbers whose signs are still to be turned, in tensors that are dense all the same (rows of one element)."""
+    g = gen(21)
+    lazy = lambda *s: torch.view_as_complex(torch.randn(*s, 2, generator=g, device="cuda")).conj().imag
+    x, r, w, up = lazy(5, 1), lazy(5, 1), lazy(1), lazy(5, 1)
+    assert x.is_neg() and w.is_neg() and w.is_contiguous()
+    plain = [t.clone() for t in (x, r, w, up)]
+    assert not plain[0].is_neg()
+
+    def norm(x, r, w, up):
+        x, r, w = (t.detach().requires_grad_() for t in (x, r, w))
+        y, h = F.rms_norm(x, w, residual=r, eps=0.5)
+        q = F.rms_norm_e4m3(x.detach(), w.detach(), residual=r.detach())
+        return [y, h, q.values.float(), q.scales, *torch.autograd.grad((y, h), (x, r, w), (up, up))]
+
+    def others(x, r, w, up):
+        zero = torch.zeros(5, dtype=torch.long, device="cuda")
+        leaf = x.detach().requires_grad_()
+        drop = F.dropout(leaf[:1], 0.0, 1)
+        out = [drop, *torch.autograd.grad(drop, leaf, up[:1]), F.embedding(zero, w[None]), *F.token_log_probs(x.expand(5, 3), zero)[:2]]
+        s = F.token_log_probs(leaf.expand(5, 3), zero, top=1)
+        out += torch.autograd.grad((s.log_probs, s.top_log_probs), leaf, (up[:, 0], up), allow_unused=True)
+        b = F.beam_step(x.view(5, 1, 1), r)
+        out += [b.scores, *b[1:3]]
+        p = w.clone().requires_grad_()
+        p.grad = up[:1, 0]
+        F.AdamW([p]).step()
+        return out + [p.detach()]
+    for f in (norm, others):
+        for a, b in zip(f(x, r, w, up), f(*plain)):
+            assert torch.equal(a, b)
+    p = w.requires_grad_()
+    p.grad = torch.ones(1, device="cuda")
+    with pytest.raises(ValueError, match="negated"):
+        F.AdamW([p]).step()
+
+
 def test_another_stream():
     g = gen(9)
     x, w = rows(g, 513, 640), rows(g, 640)
