@@ -288,6 +288,24 @@ def test_lengths_that_are_none(V, penalty):
         F.beam_step(logits, scores, lengths=lengths, length_penalty=4.5)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("B,n,V,W", [(2, 32, 1, 32), (3, 4, 205, 4), (2, 4, 1025, 4), (3, 10, 2053, 10), (2, 8, 4099, 32), (1, 32, 9001, 32), (700, 3, 64, 3), (2, 3, 131072, 16),
+                                     (5, 1, 20011, 24), (64, 5, 20003, 5)])
+def test_runs_repeat_bit_by_bit(dtype, B, n, V, W):
+    """All of a step's results, also of equal logits, which overflow the candidates' buffer in whatever order they come."""
+    g = gen(B + n + V)
+    logits, scores = make(g, B, n, V, dtype)
+    few = (logits * 0.5).round()
+    finished = torch.rand(B, n, generator=g, device="cuda") < 0.2
+    lengths = torch.randint(1, 30, (B, n), generator=g, device="cuda")
+    for z in (logits, few, torch.zeros_like(logits)):
+        for s in (scores, torch.zeros_like(scores)):
+            first = spoiled(lambda: F.beam_step(z, s, width=W))
+            for _ in range(4):
+                assert all(torch.equal(a, b) for a, b in zip(first[:3], F.beam_step(z, s, width=W)[:3]))
+            spoiled(lambda: F.beam_step(z, s, width=W, end_token=V - 1, finished=finished, lengths=lengths, length_penalty=0.6))
+
+
 def test_captured_and_replayed_and_on_another_stream():
     g = gen(3)
     logits, scores = make(g, 4, 5, 9000)
