@@ -156,8 +156,9 @@ class AdamW(torch.optim.Optimizer):
 
     @property
     def grad_norm(self) -> Optional[torch.Tensor]:
-        """The norm of all gradients in the last step (before they were clipped), where max_norm is set; None before the first."""
-        return None if self.__dict__.get("_norm") is None else self._norm[0]
+        """The norm of all gradients in the last step (before they were clipped), where max_norm is set; None before the first.  A copy: the
+        next step writes its own."""
+        return None if self.__dict__.get("_norm") is None else self._norm[0].clone()
 
     def _step(self, closure=None):
         loss = None

@@ -122,6 +122,18 @@ def test_sizes(dtype, master, bits, max_norm):
     assert ("master" in o.state[params[0]]) == master
 
 
+def test_norms_that_are_kept():
+    """What was asked for after a step stays that step's."""
+    p = torch.zeros(50, device="cuda", requires_grad=True)
+    o = F.AdamW([p], max_norm=1.0)
+    norms = []
+    for k in range(3):
+        p.grad = torch.full((50,), float(k), device="cuda")
+        o.step()
+        norms.append(o.grad_norm)
+    assert [round(float(n) / 50 ** 0.5, 5) for n in norms] == [0, 1, 2]
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_addresses_on_odd_boundaries(bits, dtype):
