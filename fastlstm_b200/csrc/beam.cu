@@ -423,9 +423,10 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------- host
+// (continuations of a sentence are counted in 32 bits)
 static int check_beam(const blstm_beam_desc* d) {
   if (!d || !valid_dtype(d->dtype) || !valid_rows(d->batch, d->beams) || d->beams <= 0 || d->beams > BLSTM_MAX_BEAMS || d->width <= 0 ||
-      d->width > BLSTM_MAX_TOP || d->vocab <= 0 || d->vocab >= INT32_MAX || d->width > d->beams * d->vocab || d->end_token < -1 ||
+      d->width > BLSTM_MAX_TOP || d->vocab <= 0 || d->vocab >= INT32_MAX || d->beams * d->vocab > UINT32_MAX || d->width > d->beams * d->vocab || d->end_token < -1 ||
       d->end_token >= d->vocab || !(d->length_penalty >= 0 && d->length_penalty <= BLSTM_MAX_LENGTH_PENALTY) || d->batch > INT32_MAX / BLSTM_MAX_TOP)
     return BLSTM_E_INVALID_ARG;
   return BLSTM_OK;

@@ -23,6 +23,7 @@ py::tuple beam_step(const Tensor& logits_in, const Tensor& scores_in, std::optio
       throw wrong("expected logits as [batch, hypotheses, vocabulary], got " + shape_str(logits_in.sizes()));
     d.batch = logits_in.size(0); d.beams = logits_in.size(1); d.vocab = logits_in.size(2);
     if (d.beams > BLSTM_MAX_BEAMS) throw wrong("at most " + std::to_string(BLSTM_MAX_BEAMS) + " hypotheses of a sentence");
+    if (d.beams * d.vocab > UINT32_MAX) throw wrong("at most 2^32 - 1 continuations of a sentence");
     const auto shape = logits_in.sizes().slice(0, 2);
     const int64_t width = width_in.value_or(d.beams);
     const int64_t most = std::min<int64_t>(BLSTM_MAX_TOP, d.beams * d.vocab);

@@ -396,7 +396,7 @@ int blstm_grad_norm(const blstm_grad_norm_desc* d, void* stream);
 #define BLSTM_MAX_LENGTH_PENALTY 4
 typedef struct blstm_beam_desc {
   int32_t dtype, width;          /* of logits; hypotheses that are kept, at most BLSTM_MAX_TOP and beams * vocab */
-  int64_t batch, beams, vocab;   /* batch * beams < 2^31, beams <= BLSTM_MAX_BEAMS                     */
+  int64_t batch, beams, vocab;   /* batch * beams < 2^31, beams <= BLSTM_MAX_BEAMS, beams * vocab < 2^32 */
   int64_t logits_stride[2];
   int64_t end_token;             /* or -1                                                              */
   double length_penalty;         /* 0 to BLSTM_MAX_LENGTH_PENALTY; needs lengths where it is not 0     */

@@ -66,6 +66,16 @@ def test_descriptors_refused(change):
     assert lib.blstm_beam_workspace(d) == 0
 
 
+def test_more_continuations_than_are_counted_are_refused():
+    """A sentence's candidates are counted in 32 bits."""
+    lib = _lib.load()
+    for beams, vocab, fits in ((4, 2 ** 30, False), (32, 2 ** 27, False), (3, 2 ** 31 - 2, False), (4, 2 ** 30 - 1, True), (1, 2 ** 31 - 2, True)):
+        d = _desc(_lib.BeamDesc, **{**BEAM, "beams": beams, "vocab": vocab, "logits_stride": (beams * vocab, vocab)})
+        assert (lib.blstm_beam_workspace(d) > 0) == fits
+        if not fits:
+            assert lib.blstm_beam_step(d, *[PTR] * 10, 1 << 30, None) == 1
+
+
 def test_pointers_refused():
     lib, d = _lib.load(), _desc(_lib.BeamDesc, **BEAM)
     need = lib.blstm_beam_workspace(d)
