@@ -38,7 +38,8 @@ __device__ __forceinline__ unsigned e4m3_two(float a, float b) {
   return r;
 }
 
-// What a row is multiplied by, and its scale, from its largest magnitude.  (At most 2^-110 counts as 0: 448 over it would pass the largest
+// What a row is multiplied by, and its scale, from its largest magnitude.  (A product with 448 / most in place of a quotient by the scale for
+// every element: a number within 2^-23 of the border between two of e4m3 may become the other one.  At most 2^-110 counts as 0: 448 over it would pass the largest
 // float soon after, and the scale would lose its bits.)
 __device__ __forceinline__ float row_up(float most) { return most > 0x1p-110f ? 448.f / most : 0.f; }
 __device__ __forceinline__ float row_scale(float most) { return most <= 0x1p-110f ? 0.f : most / 448.f; }
@@ -210,6 +211,8 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G, G < 128 ? (P <= 2 ? 8 : 1) 
   }
 }
 
+// (The sums stay in 32 bits: of 131072 rows a group has some 22, and sums in 64 bits would double the registers that hold them.  fp32, 627 x 301,
+// all outputs together: 1.0e-7 off, where sums in 64 bits are 0.6e-7 off.)
 // The gradient of the weight is added up over a group's rows in registers, over a block's groups in shared memory (a word of padding a
 // piece, so that neighbours meet no bank twice), and over the blocks by sum_parts_kernel.
 template <typename T, int P, int G, bool EDGES>

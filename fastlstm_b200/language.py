@@ -1,10 +1,11 @@
 """The operators around a language model of LSTM layers: tokens in, regularisation between the layers, predictions out.
 
-Each is a call on CUDA tensors (float32, float16 or bfloat16) that runs on the current stream, allocates through torch and
-is differentiable once.  Invalid arguments raise ValueError.  A token outside of the vocabulary is found on the device: its
+Each is a call on CUDA tensors (float32, float16 or bfloat16; reorder_states takes any type) that runs on the current stream
+and allocates through torch.  embedding, dropout, token_log_probs and rms_norm are differentiable once, the others not.  A backward pass
+can be captured as long as no graph from before the capture has the default stream add up its leaves' gradients.  Invalid arguments raise ValueError.  A token outside of the vocabulary is found on the device: its
 embedding or log probability is NaN, its row gives no gradient, and `check_status()` or a later call raises BlstmError.
-What a call does on the host is csrc/host_language.cpp; the kernels are csrc/embedding.cu, csrc/dropout.cu and
-csrc/log_probs.cu."""
+What a call does on the host is csrc/host_language.cpp, csrc/host_norm.cpp and csrc/host_beam.cpp; the kernels are csrc/embedding.cu,
+csrc/dropout.cu, csrc/log_probs.cu, csrc/rms_norm.cu and csrc/beam.cu."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
@@ -78,7 +79,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
     the result is (y, h): what goes into the next layer, and the next one's residual.
 
     h is rounded to the tensors' type before the norm is taken of it.  y and h are dense; all of x, residual and weight are
-    differentiable, the weight's gradient is added up in 32 bits in an order that the sizes and strides fix."""
+    differentiable, the weight's gradient is added up in 32 bits in an order that sizes, strides and alignment fix.  Squares are added up in 32
+    bits too: rows whose squares come to 2^128 or more (magnitudes from 2^63 on) give zeros, and with an eps of 0 those whose squares vanish (up to 2^-75) infinities."""
     return _lib.host().rms_norm(x, weight, residual, float(eps))
 
 

@@ -50,6 +50,7 @@ class AdamW(torch.optim.Optimizer):
     are less than half the distance of two 16-bit numbers are lost.
     max_norm: gradients are multiplied by min(1, max_norm / (norm + 1e-6)), the norm taken over all parameters (on one device) and
     found in `grad_norm`.  Where it is not finite the step does nothing and does not count.
+    eps is 0 or at least 2^-126.  A step that is refused (ValueError) is refused for all groups, before anything changes.
     lr may be a CUDA tensor of one float32, read when the step runs: a captured step can be replayed with another rate.  (Take a
     step, or load a state, before a capture; step counts lie in device memory and go on in replays.)"""
 
@@ -75,7 +76,7 @@ class AdamW(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ state
     def _format(self, p):
-        """The state's tensors as {name: (shape, dtype)}, in the order that the extension takes them."""
+        """The state's tensors as {name: (shape, dtype)}."""
         moment = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
         f = {"exp_avg": (p.shape, moment), "exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root": (p.shape, moment), "step": ((), torch.int64)}
         if self.state_bits == 8:

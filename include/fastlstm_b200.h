@@ -327,7 +327,7 @@ typedef struct blstm_norm_desc {
   int64_t x_stride[2], residual_stride[2], dy_stride[2];
 } blstm_norm_desc;
 
-/* h = round(x + residual), y = round(h i weight), i = 1 / sqrt(mean h^2 + eps).  residual and sum (h) are both given or both NULL
+/* h = round(x + residual), y = round(h i weight), i = 1 / sqrt(mean h^2 + eps), the mean of squares in 32 bits.  residual and sum (h) are both given or both NULL
  * (h = x).  rstd [n0*n1]: i, which the gradient needs, or NULL. */
 int blstm_rms_norm(const blstm_norm_desc* d, const void* x, const void* residual, const void* weight, void* y, void* sum,
                    float* rstd, void* stream);
@@ -338,7 +338,7 @@ int blstm_rms_norm_e4m3(const blstm_norm_desc* d, const void* x, const void* res
                         float* scales, void* sum, void* stream);
 
 /* dx = the gradient of x and of residual alike, from dy and dsum (the gradient of h, or NULL), and dweight [width] (or NULL): added up
- * in 32 bits in an order that the sizes and strides fix, rounded once.  The workspace is 256-byte aligned and not needed without dweight. */
+ * in 32 bits in an order that sizes, strides and alignment fix, rounded once.  The workspace is 256-byte aligned and not needed without dweight. */
 size_t blstm_rms_norm_grad_workspace(const blstm_norm_desc* d);
 int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* dsum, const void* h, const void* weight,
                         const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
