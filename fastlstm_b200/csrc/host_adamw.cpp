@@ -2,6 +2,7 @@
 // step over a layer's four tensors took 31 us where Python collected them.)
 #include "host_language.h"
 
+#include <algorithm>
 #include <cfloat>
 
 #include <torch/csrc/autograd/python_variable.h>
@@ -134,6 +135,14 @@ std::optional<Tensor> adamw_step(const py::list& groups, const py::dict& state, 
     }
   }
   if (calls.empty()) return std::nullopt;
+  // (a launch works on all of its tensors at a time)
+  std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+  for (const auto& [group, b] : calls)
+    for (const Tensor& p : b.params)
+      if (p.numel()) ranges.emplace_back(reinterpret_cast<uintptr_t>(ptr(p)), reinterpret_cast<uintptr_t>(ptr(p)) + p.nbytes());
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t k = 1; k < ranges.size(); ++k)
+    if (ranges[k].first < ranges[k - 1].second) throw wrong("parameters share memory");
   // Everything that can be refused is, before the first launch: groups and types are launched one by one, and a step is taken by all of
   // them or by none.
   auto scratch_of = [&](const Bucket& b) { return scratch(b.params[0].device().index()).cast<std::pair<Tensor, Tensor>>(); };

@@ -50,7 +50,7 @@ class AdamW(torch.optim.Optimizer):
     are less than half the distance of two 16-bit numbers are lost.
     max_norm: gradients are multiplied by min(1, max_norm / (norm + 1e-6)), the norm taken over all parameters (on one device) and
     found in `grad_norm`.  Where it is not finite the step does nothing and does not count.
-    eps is 0 or at least 2^-126.  A step that is refused (ValueError) is refused for all groups, before anything changes.
+    eps is 0 or at least 2^-126; parameters share no memory.  A step that is refused (ValueError) is refused for all groups, before anything changes.
     lr may be a CUDA tensor of one float32, read when the step runs: a captured step can be replayed with another rate.  (Take a
     step, or load a state, before a capture; step counts lie in device memory and go on in replays.)"""
 

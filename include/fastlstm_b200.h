@@ -319,7 +319,8 @@ int blstm_token_log_probs_grad(const blstm_score_desc* d, const void* logits, co
                                const float* g_entropy, const int64_t g_entropy_stride[2], const float* g_top,
                                void* dlogits, const int64_t dlogits_stride[2], void* stream);
 
-/* Root-mean-square norm of a sum.  Strides of x (of h in the gradient), residual (dsum) and dy; y, values, sum and dx are dense. */
+/* Root-mean-square norm of a sum.  Strides of x (of h in the gradient), residual (dsum) and dy; y, values, sum and dx are dense and share no
+ * memory with what is read. */
 typedef struct blstm_norm_desc {
   int32_t dtype;             /* of every tensor but scales, rstd and values                            */
   float eps;                 /* of at least 0                                                          */
@@ -343,7 +344,8 @@ size_t blstm_rms_norm_grad_workspace(const blstm_norm_desc* d);
 int blstm_rms_norm_grad(const blstm_norm_desc* d, const void* dy, const void* dsum, const void* h, const void* weight,
                         const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
 
-/* One tensor of an AdamW step: param, grad and the states have n elements each, dense, in one order. */
+/* One tensor of an AdamW step: param, grad and the states have n elements each, dense, in one order.  What is written (param, states,
+ * master, step) shares no memory with anything else of the step. */
 typedef struct blstm_adamw_item {
   void* param;
   const void* grad;              /* of param's type                                                    */

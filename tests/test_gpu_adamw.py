@@ -528,6 +528,20 @@ def test_a_refused_step_changes_nothing():
         assert not unchanged() and [int(o.state[p]["step"]) for p in params] == [2] * 4
 
 
+def test_parameters_that_share_memory_are_refused():
+    """All tensors of a launch are worked on at a time.  Neighbours in one buffer, and parameters without a gradient, are fine."""
+    flat = torch.zeros(100, device="cuda")
+    a, b, c = (flat[s].detach().requires_grad_() for s in (slice(0, 40), slice(40, 80), slice(79, 100)))
+    o = F.AdamW([a, c, b])
+    a.grad, b.grad = torch.ones(40, device="cuda"), torch.ones(40, device="cuda")
+    o.step()
+    before = flat.clone()
+    c.grad = torch.ones(21, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        o.step()
+    assert torch.equal(flat, before) and int(o.state[a]["step"]) == 1
+
+
 def test_gradient_norm_is_added_up_in_64_bits():
     """Seven small squares behind a large one, each below half a step of 32 bits: summed in 32 bits the norm is 1.6 u too small, in 64 it has the
     one rounding to its own 32 bits."""
