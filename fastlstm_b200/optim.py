@@ -128,6 +128,8 @@ class AdamW(torch.optim.Optimizer):
             _check_group({**self.defaults, **g})
             if g.get("amsgrad") or g.get("maximize"):
                 raise ValueError("loaded state is of an optimizer with amsgrad or maximize, which are not there")
+            if g.get("decoupled_weight_decay") is False and g.get("weight_decay"):
+                raise ValueError("loaded state is of an optimizer that adds weight decay to its gradients")
         # (torch would cast states to the parameters' types; hooks run around all of this)
         hooks = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
         self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = type(hooks[0])(), type(hooks[1])()

@@ -82,6 +82,18 @@ def test_eps_whose_reciprocal_is_infinite_is_refused():
     F.AdamW([p], eps=0)
 
 
+def test_states_of_coupled_weight_decay_are_refused():
+    """torch's Adam adds weight decay to the gradient: its state does not go on here, unless there is none."""
+    p = torch.zeros(3, requires_grad=True)
+    o = F.AdamW([p], lr=0.5)
+    with pytest.raises(ValueError, match="decay"):
+        o.load_state_dict(torch.optim.Adam([p], weight_decay=0.1).state_dict())
+    assert o.param_groups[0]["lr"] == 0.5
+    o.load_state_dict(torch.optim.Adam([p], lr=0.25).state_dict())
+    o.load_state_dict(torch.optim.AdamW([p], lr=0.125, weight_decay=0.1).state_dict())
+    assert o.param_groups[0]["lr"] == 0.125 and o.param_groups[0]["weight_decay"] == 0.1
+
+
 def test_load_hooks_see_and_change_the_whole_state():
     """What a hook in front returns is what is checked and loaded; a hook behind sees the final state."""
     p = torch.zeros(5, requires_grad=True)
